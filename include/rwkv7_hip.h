@@ -29,7 +29,7 @@
 extern "C" {
 #endif
 
-#define RWKV7_ABI_VERSION 11
+#define RWKV7_ABI_VERSION 12
 #define RWKV7_HEAD_SIZE 64
 
 enum {
@@ -460,6 +460,60 @@ int64_t rwkv7_sample_workspace_bytes(int32_t B, int32_t V);
 int rwkv7_sample(const void *logits, int32_t logits_dtype, int64_t ld, int32_t B, int32_t V, const rwkv7_sampling *params,
                  uint32_t *seen, int64_t seen_ld, int32_t update_seen, int64_t *out, float *probs,
                  int64_t probs_ld, void *workspace, int64_t workspace_bytes, void *stream);
+
+/* ---- between a large model and a small one ------------------------------ */
+/* No counterpart in the reference. Logits: dtype codes of rwkv7_sample, row
+ * stride in elements, any alignment of the rows, V <= 65536. */
+
+/* The k largest logits of each row of [N, V] (1 <= k <= min(V, 256)), in
+ * descending order, ties by the lowest id, -0 as 0, NaN behind everything:
+ * val [N, k] of the logits' type, idx i64 [N, k]; and lse f32 [N] = log sum
+ * exp(logits / temperature) over the whole row (NaN if it holds a NaN or +inf,
+ * -inf if it holds nothing else). */
+int rwkv7_top_logits(const void *logits, int32_t logits_dtype, int64_t ld, int32_t N, int32_t V, int32_t k,
+                     double temperature, void *val, int64_t *idx, float *lse, void *stream);
+
+/* Divergence of student distributions q = softmax(logits / temperature) from a
+ * teacher's top logits, and its gradient. A row's teacher is K entries (1 <= K
+ * <= 1024): ids top_idx i64 [N, K], one outside 0 .. V-1 meaning no entry (its
+ * value is not looked at), and logits top_val [N, K] (val_dtype as above).
+ *   lse f32 [N] given, log sum exp(teacher / temperature) over the teacher's
+ *   vocabulary: p_k = exp(top_val_k / temperature - lse), R = 1 - sum p (none
+ *   below 2^-20, nor where every id has an entry), and loss = sum p_k log(p_k / q_k) + R log(R / the student's
+ *   mass outside the row's ids);
+ *   lse NULL: p = softmax of the entries, R = 0.
+ * An id in several entries has the sum of their p. A row without an entry (or
+ * without lse and without mass) has loss 0 and gradient 0 whatever its logits
+ * hold. loss f32 [N] and grad [N, grad_ld] of the logits' type: either may be
+ * NULL, not both. grad = scale * d loss / d logits with scale f32 [N] (NULL:
+ * scale0); rows with scale 0 have gradient 0. grad may not overlap logits. */
+int rwkv7_distill(const void *logits, int32_t logits_dtype, int64_t ld, int32_t N, int32_t V, const void *top_val,
+                  int32_t val_dtype, const int64_t *top_idx, int32_t K, const float *lse, double temperature,
+                  const float *scale, float scale0, float *loss, void *grad, int64_t grad_ld, void *stream);
+
+/* Verifies drafted tokens against a target model (speculative sampling): for
+ * each of B sequences K <= 63 drafted ids tokens i64 [B, K], of which the first
+ * lengths[b] count (i64 [B], clamped to 0 .. K; NULL: all), target logits after
+ * 0 .. K of them (element (b, i, v) at target[b target_b + i target_r + v], of
+ * type logits_dtype), and the draft model's logits for each (likewise, rows
+ * 0 .. K-1; NULL: the draft is deterministic, a distribution of one token).
+ * With p and q the softmax over temperature and draft_temperature, token i is
+ * accepted while uniforms[b, i] q_i(x_i) < p_i(x_i); behind the accepted ones
+ * the token at which the running sum of max(p - q, 0) (p itself behind an
+ * accepted draft, or where that is 0 everywhere) first exceeds uniforms[b, K]
+ * times its whole. temperature <= 0: accepted while it is the target's argmax
+ * (uniforms and draft are not read), then the argmax. draft_temperature <= 0:
+ * as draft NULL. uniforms f32 [B, K + 1] in [0, 1). Sums in 64 bits. NaN logits
+ * count as -inf; ids outside 0 .. V-1 are rejected; with nothing left to draw
+ * from the token is 0. out i64 [B, K + 1]: the accepted tokens, the next one,
+ * then -1; accepted i64 [B]: how many were. B (2 K + 1) <= 65535. workspace:
+ * rwkv7_verify_workspace_bytes(B, K, V) bytes (need not be cleared), one per
+ * call in flight. */
+int64_t rwkv7_verify_workspace_bytes(int32_t B, int32_t K, int32_t V);
+int rwkv7_verify(const void *target, int64_t target_b, int64_t target_r, const void *draft, int64_t draft_b,
+                 int64_t draft_r, int32_t logits_dtype, const int64_t *tokens, const float *uniforms,
+                 const int64_t *lengths, int32_t B, int32_t K, int32_t V, double temperature, double draft_temperature,
+                 int64_t *out, int64_t *accepted, void *workspace, int64_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

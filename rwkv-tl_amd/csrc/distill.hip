@@ -1,0 +1,309 @@
+// Distillation from a teacher's top logits: the divergence of a student's
+// distribution from them, and its gradient, one workgroup per row.
+//
+// Student: q_j = exp(a z_j - L), L = log sum_j exp(a z_j), a = 1 / temperature.
+// Teacher: entries k < K of ids i_k and logits t_k; one whose id is outside
+// 0 .. V-1 is absent. I is the set of ids present.
+//   lse given (Lt, over the teacher's whole vocabulary): p_k = exp(a t_k - Lt),
+//     P = sum p_k, and R = 1 - P is the teacher's mass outside I (0 below
+//     2^-20, which an f32 Lt cannot tell from none, and 0 where I is the whole
+//     vocabulary), held against the student's own mass there, 1 - Q = sum_{j not
+//     in I} q_j.
+//   no lse: p = softmax of a t over the present entries; P = 1, R = 0.
+//   loss = sum_k p_k (log p_k - log q_{i_k}) + R (log R - log(1 - Q))
+//   d loss / d z_j = a ((P + R) q_j - sum_{k: i_k = j} p_k)      j in I
+//                  = a q_j (P + R - R / (1 - Q))                  else
+// A row without a present entry (or, without lse, without mass) has loss 0 and
+// gradient 0, whatever its logits hold. NaN elsewhere makes its row NaN, as in a
+// log-softmax.
+//
+// 1 - Q is never formed as a difference: the row's elements in I are taken out
+// (a bitmap of the vocabulary in LDS marks them) before the sum, which is about
+// their own largest, and I enters through the entries. The row stays in registers between the sum and the
+// gradient, so a pass reads the logits once and writes the gradient once; the
+// entries' own gradients are stored over it after a barrier.
+#include "logits_rows.h"
+#include "rwkv7_kernels.h"
+
+namespace rwkv7 {
+namespace {
+
+constexpr int kDistMaxK = kRowMaxThreads;
+constexpr double kLeastRest = 1.0 / 1048576.0;
+constexpr double kLn2 = 0.69314718055994531, kLog2E = 1.4426950408889634;
+
+struct DistillArgs {
+  const void *logits;
+  int64_t ld;
+  int V, K;
+  ExpScale sc;
+  double a;
+  const void *top_val;
+  int val_fmt;
+  const int64_t *top_idx;
+  const float *lse;    // null: softmax over the entries
+  const float *scale;  // upstream gradient of each row, null: scale0
+  float scale0;
+  float *loss;         // null: not wanted
+  void *grad;          // null: not wanted
+  int64_t grad_ld;
+};
+
+struct DistillLds {
+  uint32_t bits[kRowMaxV / 32];
+  int idx[kDistMaxK];
+  float p[kDistMaxK];
+  // per wave: the largest logit and the sum about it of the row's rest and of
+  // the entries; the teacher's reference, mass, and mass-weighted difference of
+  // its logarithms about that and the student's about mtop
+  float mrest[kMaxWaves], rest[kMaxWaves], mtop[kMaxWaves], top[kMaxWaves];
+  double tref[kMaxWaves], tw[kMaxWaves], ta[kMaxWaves];
+  bool whole;  // every id of the vocabulary has an entry
+};
+
+template <int FMT, int THREADS>
+RWKV7_DEV void zero_row(char *dst, int V) {
+  const float zero[kRowChunk] = {};
+#pragma unroll 1
+  for (uint32_t b = threadIdx.x; b < (uint32_t)V / kRowChunk; b += THREADS) store_chunk<FMT>(dst, b, zero);
+  if (threadIdx.x < V % kRowChunk) store_logit<FMT>(dst, V / kRowChunk * kRowChunk + threadIdx.x, 0.f);
+}
+
+// The waves' parts joined, one a lane, by every wave for itself. Logarithms and
+// the teacher's references are to base 2.
+struct Joined {
+  float m, mrest;       // largest logit of the row, and without the entries' ids
+  double S, Srest;      // sums about them
+  double in_all;        // what a sum about mrest counts in one about m
+  double W, tref;       // the teacher's mass about its reference
+  double P, rest_t;
+  bool mass;
+};
+template <int WAVES>
+RWKV7_DEV Joined join(const DistillArgs &g, const DistillLds &s, int lane, double lse) {
+  Joined j;
+  const float mr = lane < WAVES ? s.mrest[lane] : -kInf, mt = lane < WAVES ? s.mtop[lane] : -kInf;
+  j.mrest = wave_max(mr);
+  const float mtop = wave_max(mt);
+  j.m = fmaxf(j.mrest, mtop);
+  j.Srest = wave_sum_d(lane < WAVES ? (double)s.rest[lane] * g.sc.part(mr, j.mrest) : 0.0);
+  const double Stop = wave_sum_d(lane < WAVES ? (double)s.top[lane] * g.sc.part(mt, mtop) : 0.0);
+  j.in_all = g.sc.part(j.mrest, j.m);
+  j.S = j.Srest * j.in_all + Stop * g.sc.part(mtop, j.m);
+  if (!(j.m > -kInf)) j.S = __builtin_nan("");  // no finite logit at all
+  const int tws = (g.K + kWave - 1) / kWave;
+  double W = lane < tws ? s.tw[lane] : 0.0;
+  j.tref = lse;
+  if (!g.lse) {
+    const double tr = lane < tws ? s.tref[lane] : -__builtin_inf();
+    j.tref = wave_max_d(tr);
+    W *= tr > -__builtin_inf() ? exp2_d(tr - j.tref) : 0.0;
+  }
+  j.W = wave_sum_d(W);
+  j.P = j.W, j.rest_t = 0.0;
+  if (g.lse) {
+    j.rest_t = 1.0 - j.W;
+    if (j.rest_t < kLeastRest || s.whole) j.rest_t = 0.0;
+  } else {
+    j.P = j.W == j.W ? 1.0 : j.W;
+  }
+  j.mass = g.lse || j.W != 0.0;  // false: every present entry is -inf
+  return j;
+}
+
+RWKV7_DEV void put_loss(const DistillArgs &g, const DistillLds &s, const Joined &j, int lane, double lse, int64_t row) {
+  const int tws = (g.K + kWave - 1) / kWave;
+  // sum p (log p - log q), in log q = k (z - m) - log S, without log S
+  double A = 0.0;
+  if (lane < tws) {
+    const double tr = s.tref[lane], f = g.lse ? 1.0 : tr > -__builtin_inf() ? exp2_d(tr - j.tref) : 0.0;
+    const double up = (g.lse ? 0.0 : tr - j.tref) - g.sc.k * ((double)ExpScale::ref(s.mtop[lane]) - (double)j.m);
+    A = s.tw[lane] != 0.0 ? f * (s.ta[lane] + s.tw[lane] * up) : 0.0;
+  }
+  A = wave_sum_d(A);
+  const double S = log2_d(j.S);
+  double loss;
+  if (g.lse) {
+    loss = A + j.W * S;
+    if (j.rest_t > 0.0)
+      loss += j.rest_t * (log2_d(j.rest_t) - ((g.sc.k * ((double)j.mrest - (double)j.m) + log2_d(j.Srest)) - S));
+  } else {
+    loss = j.mass ? A * rcp_d(j.W) - log2_d(j.W) + S : 0.0;
+  }
+  if (lane == 0) g.loss[row] = (float)(kLn2 * loss);
+}
+
+template <int FMT, int THREADS, bool LOSS, bool GRAD>
+__global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : 8) void distill_kernel(DistillArgs g) {
+  __shared__ DistillLds s;
+  constexpr int kWaves = THREADS / kWave;
+  const int t = threadIdx.x, lane = t & 63, wv = t >> 6, V = g.V;
+  const uint32_t n8 = (uint32_t)V / kRowChunk;
+  const int64_t row = blockIdx.x;
+  const char *src = static_cast<const char *>(g.logits) + row * g.ld * kLogitBytes<FMT>;
+  char *dst = GRAD ? static_cast<char *>(g.grad) + row * g.grad_ld * kLogitBytes<FMT> : nullptr;
+  const float up = GRAD ? (g.scale ? g.scale[row] : g.scale0) : 0.f;
+
+  // the teacher's entry of this thread
+  const int64_t id64 = t < g.K ? g.top_idx[row * g.K + t] : -1;
+  const bool there = id64 >= 0 && id64 < V;
+  const int id = there ? (int)id64 : -1;
+#pragma unroll 1
+  for (int i = t; i < (V + 31) / 32; i += THREADS) s.bits[i] = 0u;
+  const bool some = __syncthreads_or(there);
+  if (!some) {
+    if (LOSS && t == 0) g.loss[row] = 0.f;
+    if (GRAD) zero_row<FMT, THREADS>(dst, V);
+    return;
+  }
+  Chunk<FMT> x[kRowChunks];
+#pragma unroll
+  for (int c = 0; c < kRowChunks; ++c) x[c].load(src, c * THREADS + t, n8);
+  const int tail = t < V % kRowChunk ? (int)n8 * kRowChunk + t : -1;  // this thread's logit behind the eights
+  float xt = tail >= 0 ? load_logit<FMT>(src, tail) : -kInf;
+  const float tv = there ? load_logit_rt(g.top_val, row * g.K + t, g.val_fmt) : -kInf;
+  const float zv = there ? load_logit<FMT>(src, id) : -kInf;
+  const double lse = g.lse ? (double)g.lse[row] * kLog2E : 0.0;
+
+  // mark the ids; `first`: this entry stands for its id
+  bool first = there;
+  if (there) first = !(atomicOr(&s.bits[id >> 5], 1u << (id & 31)) & (1u << (id & 31)));
+  const bool twice = __syncthreads_or(there && !first);
+  if (twice) {  // the same id in several entries: the lowest stands for it
+    s.idx[t] = id;
+    __syncthreads();
+    first = there;
+#pragma unroll 1
+    for (int k = 0; k < t; ++k) first = first && s.idx[k] != id;
+  }
+  if (g.K >= V) {  // (else some id is left over)
+    const bool whole = __syncthreads_count(first) == V;
+    if (t == 0) s.whole = whole;
+  } else if (t == 0) {
+    s.whole = false;
+  }
+
+  // this thread's part of the row without the entries' ids
+  if (tail >= 0 && ((s.bits[tail >> 5] >> (tail & 31)) & 1u)) xt = -kInf;
+  float m = xt;
+#pragma unroll
+  for (int c = 0; c < kRowChunks; ++c) {
+    const uint32_t b = c * THREADS + t;
+    const uint32_t marked = b < n8 ? reinterpret_cast<const uint8_t *>(s.bits)[b] : 0u;
+    if (marked) x[c].remove(marked);
+    float f[kRowChunk];
+    x[c].get(f);
+#pragma unroll
+    for (int e = 0; e < kRowChunk; ++e) m = fmaxf(m, f[e]);
+  }
+  m = wave_max(m);
+  const float R = ExpScale::ref(m), mtop = wave_max(zv);
+  float rest = g.sc.e(xt, R);
+#pragma unroll
+  for (int c = 0; c < kRowChunks; ++c) {
+    float f[kRowChunk];
+    x[c].get(f);
+    float q[kRowChunk];
+#pragma unroll
+    for (int e = 0; e < kRowChunk; ++e) q[e] = g.sc.e(f[e], R);
+    rest += ((q[0] + q[1]) + (q[2] + q[3])) + ((q[4] + q[5]) + (q[6] + q[7]));
+  }
+  const float own = there ? g.sc.e(zv, ExpScale::ref(mtop)) : 0.f;  // exp of the entry's student logit
+  const float2 sums = wave_sum2(rest, first ? own : 0.f);
+
+  // the teacher's entries, about its lse or the wave's largest, in 64 bits and
+  // powers of two
+  const double k2 = g.sc.k;
+  double tref = lse, w = 0.0;
+  if (wv * kWave < g.K) {
+    if (!g.lse) tref = k2 * (double)wave_max(tv);
+    const double y = k2 * (double)tv - tref;  // (NaN stays NaN)
+    w = there && tv != -kInf ? (y == y ? exp2_d(y) : y) : 0.0;
+    const double ta = w != 0.0 ? w * ((k2 * (double)tv - tref) - k2 * ((double)zv - (double)ExpScale::ref(mtop))) : 0.0;
+    const double ws = wave_sum_d(w), as = wave_sum_d(ta);
+    if (lane == 0) s.tref[wv] = tref, s.tw[wv] = ws, s.ta[wv] = as;
+  }
+  if (lane == 0) s.mrest[wv] = m, s.rest[wv] = sums.x, s.mtop[wv] = mtop, s.top[wv] = sums.y;
+  __syncthreads();
+
+  const Joined j = join<kWaves>(g, s, lane, lse);
+  if (!GRAD) {
+    if (wv == 0) put_loss(g, s, j, lane, lse, row);
+    return;
+  }
+
+  // d loss / d z, scaled: f_rest e for the rest, f_top e - ua p for the entries
+  const double ua = j.mass ? (double)up * g.a : 0.0;
+  if (ua == 0.0) {  // a row that counts for nothing: zeros, not 0 * NaN
+    zero_row<FMT, THREADS>(dst, V);
+    if (LOSS && wv == 0) put_loss(g, s, j, lane, lse, row);
+    return;
+  }
+  const double all = ua * (j.P + j.rest_t) * rcp_d(j.S);
+  const float f_top = (float)all;
+  const float f_rest = (float)(all * j.in_all - (j.rest_t > 0.0 && j.Srest > 0.0 ? ua * j.rest_t * rcp_d(j.Srest) : 0.0));
+  float pk = (float)(ua * (g.lse ? w : w * exp2_d(tref - j.tref) * rcp_d(j.W)));
+  const float mrest = ExpScale::ref(j.mrest);
+#pragma unroll
+  for (int c = 0; c < kRowChunks; ++c) {
+    float f[kRowChunk];
+    x[c].get(f);
+#pragma unroll
+    for (int e = 0; e < kRowChunk; ++e) f[e] = f_rest * g.sc.e(f[e], mrest);
+    const uint32_t b = c * THREADS + t;
+    if (b < n8) store_chunk<FMT>(dst, b, f);
+  }
+  if (tail >= 0) store_logit<FMT>(dst, tail, f_rest * g.sc.e(xt, mrest));
+  if (twice) {
+    s.p[t] = there ? pk : 0.f;
+    __syncthreads();
+    double sum = 0.0;
+#pragma unroll 1
+    for (int k = 0; first && k < g.K; ++k) sum += s.idx[k] == id ? (double)s.p[k] : 0.0;
+    pk = (float)sum;
+  }
+  __syncthreads();  // the row's own stores come before the entries'
+  if (first) store_logit<FMT>(dst, id, f_top * g.sc.e(zv, j.m) - pk);
+  // joined once more, so that nothing of it is held beside the row
+  if (LOSS && wv == 0) put_loss(g, s, join<kWaves>(g, s, lane, lse), lane, lse, row);
+}
+
+template <int FMT, int THREADS>
+void launch_t(const DistillArgs &g, int N, hipStream_t st) {
+  if (g.grad && g.loss) distill_kernel<FMT, THREADS, true, true><<<N, THREADS, 0, st>>>(g);
+  else if (g.grad) distill_kernel<FMT, THREADS, false, true><<<N, THREADS, 0, st>>>(g);
+  else distill_kernel<FMT, THREADS, true, false><<<N, THREADS, 0, st>>>(g);
+}
+
+template <int FMT>
+void launch_f(const DistillArgs &g, int N, hipStream_t st) {
+  // one entry a thread
+  const int T = row_threads(g.V) > g.K ? row_threads(g.V) : g.K <= 256 ? 256 : g.K <= 512 ? 512 : 1024;
+  if (T == 256) launch_t<FMT, 256>(g, N, st);
+  else if (T == 512) launch_t<FMT, 512>(g, N, st);
+  else launch_t<FMT, 1024>(g, N, st);
+}
+
+}  // namespace
+}  // namespace rwkv7
+
+extern "C" int rwkv7_distill(const void *logits, int32_t logits_dtype, int64_t ld, int32_t N, int32_t V,
+                             const void *top_val, int32_t val_dtype, const int64_t *top_idx, int32_t K, const float *lse,
+                             double temperature, const float *scale, float scale0, float *loss, void *grad,
+                             int64_t grad_ld, void *stream) {
+  using namespace rwkv7;
+  if (!logits || !top_val || !top_idx || (!loss && !grad)) return RWKV7_EINVAL;
+  if (logits_dtype < 0 || logits_dtype > 2 || val_dtype < 0 || val_dtype > 2) return RWKV7_EINVAL;
+  if (!(temperature > 0.0) || temperature > 1e30 || temperature < 1e-30) return RWKV7_EINVAL;
+  if (N < 1 || V < 1 || V > kRowMaxV || K < 1 || K > kDistMaxK || ld < V || (grad && grad_ld < V)) return RWKV7_ESHAPE;
+  const double a = 1.0 / temperature;
+  const DistillArgs g = {logits, ld, V, K, ExpScale::of(a), a, top_val, val_dtype, top_idx, lse, scale, scale0, loss, grad, grad_ld};
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  switch (logits_dtype) {
+    case 0: launch_f<0>(g, N, st); break;
+    case 1: launch_f<1>(g, N, st); break;
+    default: launch_f<2>(g, N, st); break;
+  }
+  RWKV7_CHECK_LAUNCH();
+  return RWKV7_OK;
+}

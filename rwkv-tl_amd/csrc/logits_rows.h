@@ -1,0 +1,205 @@
+// Rows of up to 65536 logits held in the registers of one workgroup, and the
+// order and wave reductions that the operators on such rows share.
+#pragma once
+
+#include "rwkv7_common.h"
+
+namespace rwkv7 {
+
+typedef unsigned long long u64;
+
+constexpr float kInf = __builtin_inff();
+constexpr int kRowChunk = 8;                         // logits a thread loads at a time
+constexpr int kRowChunks = 8;                        // such chunks per thread
+constexpr int kRowE = kRowChunk * kRowChunks;        // logits per thread
+constexpr int kRowMaxThreads = 1024;
+constexpr int kRowMaxV = kRowMaxThreads * kRowE;     // 65536
+constexpr int kMaxWaves = kRowMaxThreads / kWave;
+
+// Threads of a workgroup for rows of V logits: the fewest of 256, 512, 1024
+// that hold them, so that short rows leave room for more workgroups per CU.
+inline int row_threads(int V) { return V <= 256 * kRowE ? 256 : V <= 512 * kRowE ? 512 : 1024; }
+
+// Bytes per logit: FMT 0 half, 1 f32, 2 bfloat16.
+template <int FMT>
+constexpr int kLogitBytes = FMT == 1 ? 4 : 2;
+inline int logit_bytes(int fmt) { return fmt == 1 ? 4 : 2; }
+
+template <int FMT>
+RWKV7_DEV float load_logit(const void *row, int64_t i) {
+  if constexpr (FMT == 1) return static_cast<const float *>(row)[i];
+  else return F16T<FMT == 2>::to_f(static_cast<const uint16_t *>(row)[i]);
+}
+
+RWKV7_DEV float load_logit_rt(const void *p, int64_t i, int fmt) {
+  return fmt == 1 ? static_cast<const float *>(p)[i] : u16_to_f(static_cast<const uint16_t *>(p)[i], fmt == 2);
+}
+
+template <int FMT>
+RWKV7_DEV void store_logit(void *row, int64_t i, float v) {
+  if constexpr (FMT == 1) static_cast<float *>(row)[i] = v;
+  else static_cast<uint16_t *>(row)[i] = F16T<FMT == 2>::from_f(v);
+}
+
+// Eight logits as they lie in memory: 16 bytes, or 32 in f32. Rows may start
+// at any element (the copies become 16-byte accesses, which need no alignment
+// here). A row is its whole eights, eight b on thread b % threads, and the up to
+// seven logits behind them, one each on the first threads.
+template <int FMT>
+struct Chunk {
+  static constexpr bool F32 = FMT == 1;
+  static constexpr int kWords = F32 ? 8 : 4;
+  uint32_t w[kWords];
+
+  RWKV7_DEV void fill_absent() {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[i] = F32 ? 0xff800000u : FMT == 2 ? 0xff80ff80u : 0xfc00fc00u;  // -inf
+  }
+  // the b-th eight of a row with n8 whole ones, -inf past them
+  RWKV7_DEV void load(const void *row, uint32_t b, uint32_t n8) {
+    fill_absent();
+    if (b < n8) __builtin_memcpy(w, static_cast<const char *>(row) + b * (uint32_t)(kRowChunk * kLogitBytes<FMT>), sizeof w);
+  }
+  // The eight as f32. The compiler would otherwise keep a row's unpacked values
+  // from one pass to the next, which the registers of the larger workgroups do
+  // not hold: each pass unpacks an opaque copy.
+  RWKV7_DEV void get(float (&f)[kRowChunk]) {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) asm volatile("" : "+v"(w[i]));
+    if constexpr (F32) {
+#pragma unroll
+      for (int e = 0; e < kRowChunk; ++e) f[e] = __uint_as_float(w[e]);
+    } else {
+      F16T<FMT == 2>::to_f8(make_uint4(w[0], w[1], w[2], w[3]), f);
+    }
+  }
+  // the logits whose bit is set in `bits` become -inf
+  RWKV7_DEV void remove(uint32_t bits) {
+    if constexpr (F32) {
+#pragma unroll
+      for (int e = 0; e < kRowChunk; ++e)
+        if ((bits >> e) & 1u) w[e] = 0xff800000u;
+    } else {
+      constexpr uint32_t ninf = FMT == 2 ? 0xff80u : 0xfc00u;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if ((bits >> (2 * i)) & 1u) w[i] = (w[i] & 0xffff0000u) | ninf;
+        if ((bits >> (2 * i + 1)) & 1u) w[i] = (w[i] & 0x0000ffffu) | (ninf << 16);
+      }
+    }
+  }
+};
+
+// Eight values as the b-th eight of a row.
+template <int FMT>
+RWKV7_DEV void store_chunk(void *row, uint32_t b, const float (&f)[kRowChunk]) {
+  char *p = static_cast<char *>(row) + b * (uint32_t)(kRowChunk * kLogitBytes<FMT>);
+  if constexpr (FMT == 1) {
+    __builtin_memcpy(p, f, 32);
+  } else {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      w[i] = (uint32_t)F16T<FMT == 2>::from_f(f[2 * i]) | ((uint32_t)F16T<FMT == 2>::from_f(f[2 * i + 1]) << 16);
+    __builtin_memcpy(p, w, 16);
+  }
+}
+
+// Sums and maxima of doubles over the wave by lane permutes and readlanes, as
+// common's float ones: no LDS and no address registers; the result is uniform.
+template <int CTRL>
+RWKV7_DEV double dpp_d(double v) {
+  const u64 u = __builtin_bit_cast(u64, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, 0xF, 0xF, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, 0xF, 0xF, false);
+  return __builtin_bit_cast(double, (u64)lo | ((u64)hi << 32));
+}
+RWKV7_DEV double lane_value_d(double v, int lane) {
+  const u64 u = __builtin_bit_cast(u64, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, lane);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), lane);
+  return __builtin_bit_cast(double, (u64)lo | ((u64)hi << 32));
+}
+RWKV7_DEV double wave_sum_d(double v) {
+  v += dpp_d<kDppXor1>(v);
+  v += dpp_d<kDppXor2>(v);
+  v += dpp_d<kDppHalfMirror>(v);
+  v += dpp_d<kDppMirror>(v);
+  return (lane_value_d(v, 0) + lane_value_d(v, 16)) + (lane_value_d(v, 32) + lane_value_d(v, 48));
+}
+RWKV7_DEV double wave_max_d(double v) {
+  v = fmax(v, dpp_d<kDppXor1>(v));
+  v = fmax(v, dpp_d<kDppXor2>(v));
+  v = fmax(v, dpp_d<kDppHalfMirror>(v));
+  v = fmax(v, dpp_d<kDppMirror>(v));
+  return fmax(fmax(lane_value_d(v, 0), lane_value_d(v, 16)), fmax(lane_value_d(v, 32), lane_value_d(v, 48)));
+}
+RWKV7_DEV float wave_max(float v) {
+  v = fmaxf(v, dpp<kDppXor1>(v));
+  v = fmaxf(v, dpp<kDppXor2>(v));
+  v = fmaxf(v, dpp<kDppHalfMirror>(v));
+  v = fmaxf(v, dpp<kDppMirror>(v));
+  return fmaxf(fmaxf(lane_value(v, 0), lane_value(v, 16)), fmaxf(lane_value(v, 32), lane_value(v, 48)));
+}
+
+// 2^y in 64 bits, y clamped to -2000 from below (0 there; NaN too): y = n + f, |f|
+// <= 1/2, 2^f by its Taylor polynomial of degree 11, whose remainder is below
+// (ln 2 / 2)^12 / 12! = 6.3e-15. A few registers, where the library's exp takes
+// more than a row in registers leaves.
+RWKV7_DEV double exp2_d(double y) {
+  y = fmax(y, -2000.0);
+  const double n = rint(y), f = y - n;
+  double p = 4.44553827187081e-10;
+  p = fma(p, f, 7.054911620801121e-09);
+  p = fma(p, f, 1.0178086009239696e-07);
+  p = fma(p, f, 1.3215486790144305e-06);
+  p = fma(p, f, 1.5252733804059838e-05);
+  p = fma(p, f, 0.00015403530393381606);
+  p = fma(p, f, 0.0013333558146428441);
+  p = fma(p, f, 0.009618129107628477);
+  p = fma(p, f, 0.055504108664821576);
+  p = fma(p, f, 0.2402265069591007);
+  p = fma(p, f, 0.6931471805599453);
+  p = fma(p, f, 1.0);
+  return ldexp(p, (int)n);
+}
+// 1 / x in 64 bits: the hardware's estimate and two Newton steps (0 -> inf).
+RWKV7_DEV double rcp_d(double x) {
+  double y = __builtin_amdgcn_rcp(x);
+  const double e = fma(-x, y, 1.0);
+  if (fabs(e) < 1.0) {  // (x is neither 0 nor infinite)
+    y = fma(y, e, y);
+    y = fma(y, fma(-x, y, 1.0), y);
+  }
+  return y;
+}
+// log2 in 64 bits (0 -> -inf, inf -> inf): the float logarithm of the mantissa and one
+// Newton step of 2^y = x (its error of 1e-7 squared).
+RWKV7_DEV double log2_d(double x) {
+  int ex;
+  const double f = frexp(x, &ex);
+  const double y = (double)__builtin_amdgcn_logf((float)f);
+  return fabs(y) < 2.0 ? (double)ex + (y + (f * exp2_d(-y) - 1.0) * 1.4426950408889634) : y;
+}
+
+// exp(a x) over a row as powers of two about its largest logit, 2^((x - m) kf):
+// a row of any size, the types' lowest values included, has a sum of 1 or more.
+struct ExpScale {
+  float kf;    // a log2(e) in float
+  double k;    // the same in 64 bits
+  static ExpScale of(double a) {
+    const double k = a * 1.4426950408889634;
+    return {(float)k, k};
+  }
+  // m: -inf for none, which any finite reference serves
+  static RWKV7_DEV float ref(float m) { return m > -kInf ? m : 0.f; }
+  RWKV7_DEV float e(float x, float m) const { return __builtin_amdgcn_exp2f((x - m) * kf); }
+  // the share of a part about m in a sum about a larger one (0 for none)
+  RWKV7_DEV double part(float m, float larger) const {
+    return m > -kInf ? exp2_d(((double)m - (double)larger) * k) : 0.0;
+  }
+  // log2 of sum exp(a x) when the sum about m is S
+  RWKV7_DEV double log2z(double S, float m) const { return (double)m * k + log2_d(S); }
+};
+
+}  // namespace rwkv7

@@ -9,6 +9,8 @@ Drop-in for the GPU path of yuyi2439/rwkv-tl:
 * ``make_rwkv7`` -- ``demo.make_rwkv7``
 * ``kernels`` -- the operator-level API of ``rwkv_tl.kernels.fp16``
 * ``sample_logits`` -- ``demo.sampling.sample_logits`` (one HIP kernel launch)
+* ``verify_draft`` / ``kernels.top_logits`` / ``kernels.distill_loss`` -- operators between
+  a large model and a small one (``logits.py``; no counterpart in the reference)
 * ``operators`` -- ``torch.ops.rwkv_tl.*`` (``rwkv_tl.operators``), registered on import
 * ``tokenizer.Tokenizer`` -- ``rwkv_tl.tokenizer.Tokenizer``
 """
@@ -20,6 +22,7 @@ import torch
 from . import operators  # noqa: F401  (registers torch.ops.rwkv_tl.*, as src/rwkv_tl/__init__.py:10 does)
 from .checkpoint import SHAPES, ModelShape, make_random_state_dict
 from .hip_graph import HIPGraph, make_graph_cls, wrap_model
+from .logits import verify_draft
 from .model import RWKV7Model
 from .rwkv7_hip import RWKV7HIP, RWKV7HIPBF16, RWKV7HIPInt8
 from .sampling import sample_logits
@@ -41,6 +44,7 @@ __all__ = [
     "make_random_state_dict",
     "make_rwkv7",
     "sample_logits",
+    "verify_draft",
     "wrap_model",
 ]
 

@@ -8,6 +8,7 @@ fallback: if the library is missing, every entry point raises.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 from pathlib import Path
@@ -15,7 +16,7 @@ from pathlib import Path
 import torch  # noqa: F401  (must be imported before the HIP library)
 
 LIB_NAME = "librwkv7_hip.so"
-ABI_VERSION = 11
+ABI_VERSION = 12
 
 # rwkv7_model.flags
 MODEL_MULTI_LAUNCH_DECODE = 1
@@ -67,6 +68,10 @@ SYMBOLS = (
     "rwkv7_gn_rkrk",
     "rwkv7_sample_workspace_bytes",
     "rwkv7_sample",
+    "rwkv7_top_logits",
+    "rwkv7_distill",
+    "rwkv7_verify_workspace_bytes",
+    "rwkv7_verify",
 )
 
 
@@ -159,7 +164,7 @@ _LIB: ctypes.CDLL | None = None
 
 
 def _declare(lib: ctypes.CDLL) -> None:
-    vp, i32, i64 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64
+    vp, i32, i64, f64 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_double
     sig = {
         "rwkv7_abi_version": (ctypes.c_int, []),
         "rwkv7_strerror": (ctypes.c_char_p, [ctypes.c_int]),
@@ -196,6 +201,12 @@ def _declare(lib: ctypes.CDLL) -> None:
         "rwkv7_sample_workspace_bytes": (i64, [i32, i32]),
         "rwkv7_sample": (ctypes.c_int, [vp, i32, i64, i32, i32, ctypes.POINTER(Sampling), vp, i64, i32, vp, vp, i64,
                                         vp, i64, vp]),
+        "rwkv7_top_logits": (ctypes.c_int, [vp, i32, i64, i32, i32, i32, f64, vp, vp, vp, vp]),
+        "rwkv7_distill": (ctypes.c_int, [vp, i32, i64, i32, i32, vp, i32, vp, i32, vp, f64, vp, ctypes.c_float, vp, vp,
+                                         i64, vp]),
+        "rwkv7_verify_workspace_bytes": (i64, [i32, i32, i32]),
+        "rwkv7_verify": (ctypes.c_int, [vp, i64, i64, vp, i64, i64, i32, vp, vp, vp, i32, i32, i32, f64, f64, vp, vp, vp,
+                                        i64, vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
@@ -232,6 +243,15 @@ def check(rc: int, what: str) -> None:
 
 def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
+
+
+_HERE = contextlib.nullcontext()
+
+
+def device_of(t: torch.Tensor):
+    """A context in which ``t``'s device is the current one, and so are its
+    stream for ``stream_handle`` and the launches."""
+    return _HERE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
 def stream_handle() -> int:

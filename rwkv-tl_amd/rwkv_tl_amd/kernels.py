@@ -24,6 +24,8 @@ example ``dplr.py:258-267``) are not reproduced.
   (``gates.py:315-357``), ``fused_rank_gemv`` (``gates.py:254-285``),
   ``fused_l2norm_neg_kk_a`` (``dplr.py:229-235``), ``fused_gn_rkrk``
   (``dplr.py:237-254``).
+* Between a large model and a small one (``logits.py``): ``top_logits``,
+  ``distill_loss``, ``distill_loss_grad``, ``distill_loss_backward``.
 """
 
 from __future__ import annotations
@@ -34,6 +36,7 @@ import torch
 from torch import Tensor
 
 from . import _lib
+from .logits import distill_loss, distill_loss_backward, distill_loss_grad, top_logits  # noqa: F401
 
 N = 64
 

@@ -1,0 +1,255 @@
+"""Operators between a large model and a small one of the same vocabulary, on
+rows of logits (no counterpart in the reference).
+
+* ``top_logits``: what a teacher hands on of each row: its largest logits, their
+  token ids, and the row's log-sum-exp.
+* ``distill_loss`` / ``distill_loss_grad``: the divergence of a student's
+  distribution from a teacher's top logits, alone or with its gradient in the
+  same pass. ``torch.ops.rwkv_tl.distill_loss`` is the differentiable form.
+* ``verify_draft``: drafted tokens against the target model's probabilities,
+  from given random numbers (speculative sampling).
+
+Logits are float16, bfloat16 or float32 on the GPU, of up to ``MAX_VOCAB``
+tokens; rows may lie at any stride. Nothing waits for the host, so the calls can
+be captured in a HIP graph. Each call allocates what it returns, and
+``verify_draft`` its workspace.
+"""
+
+from __future__ import annotations
+
+import math
+
+import torch
+from torch import Tensor
+
+from . import _lib
+
+MAX_VOCAB = 65536
+MAX_TOP = 256  # largest k of top_logits
+MAX_ENTRIES = 1024  # teacher entries per row of distill_loss
+MAX_DRAFT = 63  # drafted tokens per sequence of verify_draft
+
+LOGIT_DTYPES = {torch.float16: 0, torch.float32: 1, torch.bfloat16: 2}
+
+
+def _need(cond: bool, msg: str) -> None:
+    if not cond:
+        raise ValueError(msg)
+
+
+def _check_logits(x: Tensor, name: str) -> None:
+    _need(isinstance(x, Tensor), f"{name} must be a tensor")
+    _need(x.is_cuda, f"{name} on {x.device}; the HIP kernels need a ROCm device")
+    _need(x.dtype in LOGIT_DTYPES, f"{name} must be float16, bfloat16 or float32, got {x.dtype}")
+    _need(x.ndim >= 1 and 1 <= x.shape[-1] <= MAX_VOCAB, f"{name}: a vocabulary of 1..{MAX_VOCAB}, got {tuple(x.shape)}")
+
+
+def _rows(x: Tensor) -> Tensor:
+    """``[..., V]`` as ``[N, V]`` with adjacent columns (a copy only where no view is one)."""
+    x = x.reshape(-1, x.shape[-1])
+    return x if x.stride(1) == 1 or x.shape[1] == 1 and x.stride(0) >= 1 else x.contiguous()
+
+
+def _ld(x: Tensor) -> int:
+    """Row stride of ``[N, V]``; of a single row any that covers it."""
+    return max(x.stride(0), x.shape[1]) if x.shape[0] == 1 else x.stride(0)
+
+
+def _dense(x: Tensor) -> Tensor:
+    """Rows that do not overlap (an expanded row is copied)."""
+    return x if x.shape[0] <= 1 or x.stride(0) >= x.shape[1] else x.contiguous()
+
+
+def _temperature(t: float) -> float:
+    t = float(t)
+    _need(1e-30 <= t <= 1e30, f"temperature must be positive and finite, got {t}")
+    return t
+
+
+def _same_device(ref: Tensor, **others: Tensor | None) -> None:
+    for name, t in others.items():
+        if t is not None:
+            _need(t.device == ref.device, f"{name} on {t.device}, the logits on {ref.device}")
+
+
+def top_logits(logits: Tensor, k: int, *, temperature: float = 1.0) -> tuple[Tensor, Tensor, Tensor]:
+    """The ``k`` largest of each row of ``logits`` ``[..., V]``, 1 <= k <= min(V, 256).
+
+    Returns ``values [..., k]`` (the logits' dtype, descending; ties by the lowest
+    id, NaN last), ``indices [..., k]`` int64, and ``lse [...]`` float32, the log
+    of the sum of ``exp(logits / temperature)`` over the whole row: a teacher's
+    answers as ``distill_loss`` takes them."""
+    _check_logits(logits, "logits")
+    V = logits.shape[-1]
+    _need(isinstance(k, int) and 1 <= k <= min(V, MAX_TOP), f"k must be in 1..{min(V, MAX_TOP)}, got {k}")
+    temperature = _temperature(temperature)
+    lead = logits.shape[:-1]
+    x = _dense(_rows(logits))
+    N = x.shape[0]
+    with _lib.device_of(x):
+        val = torch.empty(*lead, k, dtype=x.dtype, device=x.device)
+        idx = torch.empty(*lead, k, dtype=torch.int64, device=x.device)
+        lse = torch.empty(lead, dtype=torch.float32, device=x.device)
+        if N:
+            rc = _lib.load().rwkv7_top_logits(
+                x.data_ptr(), LOGIT_DTYPES[x.dtype], _ld(x), N, V, k, temperature, val.data_ptr(), idx.data_ptr(),
+                lse.data_ptr(), _lib.stream_handle(),
+            )
+            _lib.check(rc, "rwkv7_top_logits")
+    return val, idx, lse
+
+
+def _distill(logits, top_val, top_idx, lse, temperature, scale, want_loss: bool, want_grad: bool):
+    _check_logits(logits, "logits")
+    lead, V = logits.shape[:-1], logits.shape[-1]
+    _need(top_val.ndim >= 1 and top_val.shape[:-1] == lead and top_idx.shape == top_val.shape,
+          f"top_val and top_idx must be [{', '.join(map(str, (*lead, 'K')))}], got {tuple(top_val.shape)} and "
+          f"{tuple(top_idx.shape)}")
+    K = top_val.shape[-1]
+    _need(K <= MAX_ENTRIES, f"at most {MAX_ENTRIES} teacher entries per row, got {K}")
+    _need(top_val.dtype in LOGIT_DTYPES, f"top_val must be float16, bfloat16 or float32, got {top_val.dtype}")
+    _need(top_idx.dtype == torch.int64, f"top_idx must be int64, got {top_idx.dtype}")
+    _need(lse is None or (lse.shape == lead and lse.dtype == torch.float32), f"lse must be float32 {tuple(lead)}")
+    rowwise = isinstance(scale, Tensor)
+    _need(not rowwise or (scale.shape == lead and scale.dtype == torch.float32), f"scale must be float32 {tuple(lead)}")
+    _same_device(logits, top_val=top_val, top_idx=top_idx, lse=lse, scale=scale if rowwise else None)
+    temperature = _temperature(temperature)
+    x = _dense(_rows(logits))
+    N = x.shape[0]
+    with _lib.device_of(x):
+        loss = torch.empty(lead, dtype=torch.float32, device=x.device) if want_loss else None
+        grad = torch.empty(logits.shape, dtype=x.dtype, device=x.device) if want_grad else None
+        if N and not K:  # no teacher at all
+            for t in (loss, grad):
+                if t is not None:
+                    t.zero_()
+        elif N:
+            tv, ti = top_val.contiguous(), top_idx.contiguous()
+            ls = None if lse is None else lse.contiguous()
+            sc = scale.contiguous() if rowwise else None
+            rc = _lib.load().rwkv7_distill(
+                x.data_ptr(), LOGIT_DTYPES[x.dtype], _ld(x), N, V, tv.data_ptr(), LOGIT_DTYPES[tv.dtype], ti.data_ptr(),
+                K, _lib.ptr(ls), temperature, _lib.ptr(sc), 1.0 if rowwise else float(scale), _lib.ptr(loss),
+                _lib.ptr(grad), V, _lib.stream_handle(),
+            )
+            _lib.check(rc, "rwkv7_distill")
+    return loss, grad
+
+
+def distill_loss(logits: Tensor, top_val: Tensor, top_idx: Tensor, lse: Tensor | None = None, *,
+                 temperature: float = 1.0) -> Tensor:
+    """Divergence of the student's ``softmax(logits / temperature)`` from a
+    teacher's top logits: float32 ``[...]``, a loss per row of ``logits [..., V]``.
+
+    ``top_val [..., K]`` (any of the three dtypes) and ``top_idx [..., K]`` int64
+    are the teacher's entries, K <= 1024; an id outside ``0..V-1`` (say -1) means
+    no entry, so rows may have fewer, and a row without any has loss 0 and
+    gradient 0 whatever its logits hold (a padded position). With ``lse [...]``
+    float32, the teacher's log-sum-exp over its whole vocabulary at the same
+    temperature, ``p_k = exp(top_val_k / temperature - lse)`` and the mass that
+    this leaves (if 2^-20 or more) is held against the student's mass outside the row's ids; without
+    it, ``p`` is the softmax of the entries. There is no factor ``temperature ** 2``.
+
+    Without autograd; ``torch.ops.rwkv_tl.distill_loss`` is the differentiable form."""
+    return _distill(logits, top_val, top_idx, lse, temperature, 1.0, True, False)[0]
+
+
+def distill_loss_grad(logits: Tensor, top_val: Tensor, top_idx: Tensor, lse: Tensor | None = None, *,
+                      temperature: float = 1.0, scale: Tensor | float = 1.0) -> tuple[Tensor, Tensor]:
+    """``distill_loss`` and ``scale`` times its gradient to ``logits`` in one pass
+    over them: ``(loss [...] float32, grad [..., V] of the logits' dtype)``.
+    ``scale``: a number, or float32 ``[...]`` (each row's weight in the loss and a
+    loss scale; a row with 0 has gradient 0). For ``logits.backward(grad)``."""
+    return _distill(logits, top_val, top_idx, lse, temperature, scale, True, True)
+
+
+def distill_loss_backward(grad_loss: Tensor, logits: Tensor, top_val: Tensor, top_idx: Tensor, lse: Tensor | None,
+                          temperature: float) -> Tensor:
+    """Gradient of ``distill_loss`` to ``logits`` under ``grad_loss`` float32 ``[...]``."""
+    return _distill(logits, top_val, top_idx, lse, temperature, grad_loss, False, True)[1]
+
+
+def _strides(x: Tensor, V: int) -> Tensor:
+    """``[B, R, V]`` with adjacent columns and rows that do not overlap."""
+    ok = (x.stride(2) == 1 or V == 1) and (x.shape[1] <= 1 or x.stride(1) >= V) and x.stride(0) >= 0
+    return x if ok else x.contiguous()
+
+
+def verify_draft(
+    target_logits: Tensor,
+    draft_tokens: Tensor,
+    uniforms: Tensor | None,
+    draft_logits: Tensor | None = None,
+    *,
+    temperature: float | None = None,
+    draft_temperature: float | None = None,
+    lengths: Tensor | None = None,
+) -> tuple[Tensor, Tensor]:
+    """Keep the drafted tokens that the target model lets pass, and draw the next.
+
+    ``target_logits [B, K + 1, V]``: the target's logits after 0..K of the drafted
+    tokens; ``draft_tokens [B, K]`` int64, K <= 63; ``uniforms [B, K + 1]`` float32
+    in ``[0, 1)`` (K for the tokens, one for the draw); ``draft_logits [B, K, V]``:
+    the logits the drafts were drawn from at ``draft_temperature`` (default:
+    ``temperature``), of the target's dtype, or None for drafts without a draw
+    (greedy ones, looked-up ones; ``draft_temperature <= 0`` is the same);
+    ``lengths [B]`` int64: how many of each sequence's drafts count (None: all).
+    Without the dimension B for a single sequence.
+
+    Returns ``tokens [B, K + 1]`` int64 (the accepted ones, the next one, -1 behind
+    it) and ``accepted [B]`` int64. The tokens are distributed as the target's own
+    at ``temperature``; with ``temperature`` None or <= 0 they are its greedy ones
+    and ``uniforms`` is not read. NaN logits count as -inf; ids outside ``0..V-1``
+    are rejected."""
+    _check_logits(target_logits, "target_logits")
+    single = target_logits.ndim == 2
+    up = (lambda t: None if t is None else t.unsqueeze(0)) if single else (lambda t: t)
+    target, tokens, draft = up(target_logits), up(draft_tokens), up(draft_logits)
+    uniforms, lengths = up(uniforms), up(lengths)
+    _need(target.ndim == 3 and target.shape[1] >= 1, f"target_logits must be [B, K + 1, V], got {tuple(target_logits.shape)}")
+    B, K, V = target.shape[0], target.shape[1] - 1, target.shape[2]
+    _need(K <= MAX_DRAFT, f"at most {MAX_DRAFT} drafted tokens, got {K}")
+    _need(B * (2 * K + 1) <= 65535, f"a batch of {B} with {K} drafts is too large: at most {65535 // (2 * K + 1)}")
+    _need(tokens.shape == (B, K) and tokens.dtype == torch.int64,
+          f"draft_tokens must be int64 [{B}, {K}], got {tokens.dtype} {tuple(tokens.shape)}")
+    temperature = 0.0 if temperature is None else float(temperature)
+    greedy = temperature <= 0
+    if not greedy:
+        _temperature(temperature)
+        _need(uniforms is not None, "uniforms are needed unless the temperature is None or <= 0")
+    draft_temperature = temperature if draft_temperature is None else float(draft_temperature)
+    _need(not math.isnan(draft_temperature), "draft_temperature is NaN")
+    if uniforms is not None:
+        _need(uniforms.shape == (B, K + 1) and uniforms.dtype == torch.float32,
+              f"uniforms must be float32 [{B}, {K + 1}], got {uniforms.dtype} {tuple(uniforms.shape)}")
+    if draft is not None:
+        _check_logits(draft, "draft_logits")
+        _need(draft.shape == (B, K, V) and draft.dtype == target.dtype,
+              f"draft_logits must be {target.dtype} [{B}, {K}, {V}], got {draft.dtype} {tuple(draft.shape)}")
+        if not greedy and draft_temperature > 0:
+            _temperature(draft_temperature)
+        else:
+            draft = None
+    if lengths is not None:
+        _need(lengths.shape == (B,) and lengths.dtype == torch.int64, f"lengths must be int64 [{B}]")
+    _same_device(target, draft_tokens=tokens, uniforms=uniforms, draft_logits=draft, lengths=lengths)
+    with _lib.device_of(target):
+        out = torch.empty(B, K + 1, dtype=torch.int64, device=target.device)
+        accepted = torch.empty(B, dtype=torch.int64, device=target.device)
+        if B:
+            lib = _lib.load()
+            t = _strides(target, V)
+            d = None if draft is None or K == 0 else _strides(draft, V)
+            tok = tokens.contiguous()
+            u = None if greedy else uniforms.contiguous()
+            n = None if lengths is None else lengths.contiguous()
+            nb = lib.rwkv7_verify_workspace_bytes(B, K, V)
+            ws = torch.empty(nb, dtype=torch.uint8, device=target.device)
+            rc = lib.rwkv7_verify(
+                t.data_ptr(), t.stride(0), t.stride(1) if K else V, _lib.ptr(d), 0 if d is None else d.stride(0),
+                V if d is None or K == 1 else d.stride(1), LOGIT_DTYPES[t.dtype], tok.data_ptr() if K else None,
+                _lib.ptr(u), _lib.ptr(n), B, K, V, temperature, draft_temperature, out.data_ptr(), accepted.data_ptr(),
+                ws.data_ptr(), nb, _lib.stream_handle(),
+            )
+            _lib.check(rc, "rwkv7_verify")
+    return (out[0], accepted[0]) if single else (out, accepted)

@@ -127,6 +127,53 @@ TRAIN_OPS: dict[str, tuple[str, Callable, Callable]] = {
 }
 
 
+# Operators between a large model and a small one (no counterpart in the
+# reference): a teacher's top logits, the divergence of a student from them.
+# ``distill_loss`` is differentiable to ``logits`` (not to the teacher, and once).
+def _top_meta(logits, k, temperature=1.0):
+    lead = logits.shape[:-1]
+    return (logits.new_empty(*lead, k), logits.new_empty(*lead, k, dtype=torch.int64),
+            logits.new_empty(lead, dtype=torch.float32))
+
+
+LOGITS_OPS: dict[str, tuple[str, Callable, Callable]] = {
+    "top_logits": (
+        "(Tensor logits, int k, float temperature=1.0) -> (Tensor, Tensor, Tensor)",
+        lambda logits, k, temperature=1.0: K.top_logits(logits, k, temperature=temperature),
+        _top_meta,
+    ),
+    "distill_loss": (
+        "(Tensor logits, Tensor top_val, Tensor top_idx, Tensor? lse=None, float temperature=1.0) -> Tensor",
+        lambda logits, top_val, top_idx, lse=None, temperature=1.0: K.distill_loss(
+            logits, top_val, top_idx, lse, temperature=temperature),
+        lambda logits, *_: logits.new_empty(logits.shape[:-1], dtype=torch.float32),
+    ),
+    "distill_loss_backward": (
+        "(Tensor grad_loss, Tensor logits, Tensor top_val, Tensor top_idx, Tensor? lse, float temperature) -> Tensor",
+        K.distill_loss_backward,
+        lambda grad_loss, logits, *_: torch.empty(logits.shape, dtype=logits.dtype, device=logits.device),
+    ),
+}
+
+
+def _distill_setup(ctx, inputs, output) -> None:
+    logits, top_val, top_idx, lse, temperature = inputs
+    if top_val.requires_grad or (lse is not None and lse.requires_grad):
+        raise ValueError("distill_loss has no gradient to the teacher: detach top_val and lse")
+    ctx.save_for_backward(logits, top_val, top_idx, lse)
+    ctx.temperature = temperature
+
+
+def _distill_backward(ctx, grad_loss):
+    logits, top_val, top_idx, lse = ctx.saved_tensors
+    grad = torch.ops.rwkv_tl.distill_loss_backward(grad_loss, logits, top_val, top_idx, lse, ctx.temperature)
+    return grad, None, None, None, None
+
+
+def _distill_backward_twice(ctx, *_):
+    raise NotImplementedError("distill_loss has no second derivative")
+
+
 def _dplr_seq_setup(ctx, inputs, output) -> None:
     ctx.save_for_backward(*inputs)
 
@@ -146,7 +193,7 @@ def register() -> None:
     global _registered
     if _registered:
         return
-    for name, (schema, cuda, meta) in {**OPS, **TRAIN_OPS}.items():
+    for name, (schema, cuda, meta) in {**OPS, **TRAIN_OPS, **LOGITS_OPS}.items():
         qual = f"{NAMESPACE}::{name}"
         torch.library.define(qual, schema)
         torch.library.impl(qual, "CUDA")(cuda)
@@ -154,6 +201,8 @@ def register() -> None:
     torch.library.register_autograd(
         f"{NAMESPACE}::fused_dplr_seq", _dplr_seq_backward, setup_context=_dplr_seq_setup
     )
+    torch.library.register_autograd(f"{NAMESPACE}::distill_loss", _distill_backward, setup_context=_distill_setup)
+    torch.library.register_autograd(f"{NAMESPACE}::distill_loss_backward", _distill_backward_twice)
     _registered = True
 
 
