@@ -83,26 +83,26 @@ template <int WAVES>
 RWKV7_DEV Joined join(const DistillArgs &g, const DistillLds &s, int lane, double lse) {
   Joined j;
   const float mr = lane < WAVES ? s.mrest[lane] : -kInf, mt = lane < WAVES ? s.mtop[lane] : -kInf;
-  j.mrest = wave_max(mr);
+  j.mrest = uniform_f(wave_max(mr));
   const float mtop = wave_max(mt);
-  j.m = fmaxf(j.mrest, mtop);
-  j.Srest = wave_sum_d(lane < WAVES ? (double)s.rest[lane] * g.sc.part(mr, j.mrest) : 0.0);
+  j.m = uniform_f(fmaxf(j.mrest, mtop));
+  j.Srest = uniform_d(wave_sum_d(lane < WAVES ? (double)s.rest[lane] * g.sc.part(mr, j.mrest) : 0.0));
   const double Stop = wave_sum_d(lane < WAVES ? (double)s.top[lane] * g.sc.part(mt, mtop) : 0.0);
-  j.in_all = g.sc.part(j.mrest, j.m);
-  j.S = j.Srest * j.in_all + Stop * g.sc.part(mtop, j.m);
+  j.in_all = uniform_d(g.sc.part(j.mrest, j.m));
+  j.S = uniform_d(j.Srest * j.in_all + Stop * g.sc.part(mtop, j.m));
   if (!(j.m > -kInf)) j.S = __builtin_nan("");  // no finite logit at all
   const int tws = (g.K + kWave - 1) / kWave;
   double W = lane < tws ? s.tw[lane] : 0.0;
   j.tref = lse;
   if (!g.lse) {
     const double tr = lane < tws ? s.tref[lane] : -__builtin_inf();
-    j.tref = wave_max_d(tr);
+    j.tref = uniform_d(wave_max_d(tr));
     W *= tr > -__builtin_inf() ? exp2_d(tr - j.tref) : 0.0;
   }
-  j.W = wave_sum_d(W);
+  j.W = uniform_d(wave_sum_d(W));
   j.P = j.W, j.rest_t = 0.0;
   if (g.lse) {
-    j.rest_t = 1.0 - j.W;
+    j.rest_t = uniform_d(1.0 - j.W);
     if (j.rest_t < kLeastRest || s.whole) j.rest_t = 0.0;
   } else {
     j.P = j.W == j.W ? 1.0 : j.W;
@@ -163,7 +163,7 @@ __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : 8) void distill_kernel(Dist
   float xt = tail >= 0 ? load_logit<FMT>(src, tail) : -kInf;
   const float tv = there ? load_logit_rt(g.top_val, row * g.K + t, g.val_fmt) : -kInf;
   const float zv = there ? load_logit<FMT>(src, id) : -kInf;
-  const double lse = g.lse ? (double)g.lse[row] * kLog2E : 0.0;
+  const double lse = uniform_d(g.lse ? (double)g.lse[row] * kLog2E : 0.0);
 
   // mark the ids; `first`: this entry stands for its id
   bool first = there;
@@ -233,17 +233,17 @@ __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : 8) void distill_kernel(Dist
   }
 
   // d loss / d z, scaled: f_rest e for the rest, f_top e - ua p for the entries
-  const double ua = j.mass ? (double)up * g.a : 0.0;
+  const double ua = uniform_d(j.mass ? (double)up * g.a : 0.0);
   if (ua == 0.0) {  // a row that counts for nothing: zeros, not 0 * NaN
     zero_row<FMT, THREADS>(dst, V);
     if (LOSS && wv == 0) put_loss(g, s, j, lane, lse, row);
     return;
   }
   const double all = ua * (j.P + j.rest_t) * rcp_d(j.S);
-  const float f_top = (float)all;
-  const float f_rest = (float)(all * j.in_all - (j.rest_t > 0.0 && j.Srest > 0.0 ? ua * j.rest_t * rcp_d(j.Srest) : 0.0));
+  const float f_top = uniform_f((float)all);
+  const float f_rest = uniform_f((float)(all * j.in_all - (j.rest_t > 0.0 && j.Srest > 0.0 ? ua * j.rest_t * rcp_d(j.Srest) : 0.0)));
   float pk = (float)(ua * (g.lse ? w : w * exp2_d(tref - j.tref) * rcp_d(j.W)));
-  const float mrest = ExpScale::ref(j.mrest);
+  const float mrest = uniform_f(ExpScale::ref(j.mrest));
 #pragma unroll
   for (int c = 0; c < kRowChunks; ++c) {
     float f[kRowChunk];

@@ -120,6 +120,9 @@ RWKV7_DEV double lane_value_d(double v, int lane) {
   const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), lane);
   return __builtin_bit_cast(double, (u64)lo | ((u64)hi << 32));
 }
+// A value that every lane holds, kept in scalar registers.
+RWKV7_DEV double uniform_d(double v) { return lane_value_d(v, 0); }
+RWKV7_DEV float uniform_f(float v) { return lane_value(v, 0); }
 RWKV7_DEV double wave_sum_d(double v) {
   v += dpp_d<kDppXor1>(v);
   v += dpp_d<kDppXor2>(v);
@@ -142,24 +145,21 @@ RWKV7_DEV float wave_max(float v) {
   return fmaxf(fmaxf(lane_value(v, 0), lane_value(v, 16)), fmaxf(lane_value(v, 32), lane_value(v, 48)));
 }
 
-// 2^y in 64 bits, y clamped to -2000 from below (0 there; NaN too): y = n + f, |f|
-// <= 1/2, 2^f by its Taylor polynomial of degree 11, whose remainder is below
-// (ln 2 / 2)^12 / 12! = 6.3e-15. A few registers, where the library's exp takes
-// more than a row in registers leaves.
+// 2^y in 64 bits to 1.1e-12, y clamped to -2000 from below (0 there; NaN too): y
+// = n + f, |f| <= 1/2, 2^f by the polynomial of degree 8 that interpolates it at
+// the Chebyshev points. Fewer instructions and registers than the library's exp,
+// and nearer than any sum here needs.
 RWKV7_DEV double exp2_d(double y) {
   y = fmax(y, -2000.0);
   const double n = rint(y), f = y - n;
-  double p = 4.44553827187081e-10;
-  p = fma(p, f, 7.054911620801121e-09);
-  p = fma(p, f, 1.0178086009239696e-07);
-  p = fma(p, f, 1.3215486790144305e-06);
-  p = fma(p, f, 1.5252733804059838e-05);
-  p = fma(p, f, 0.00015403530393381606);
-  p = fma(p, f, 0.0013333558146428441);
-  p = fma(p, f, 0.009618129107628477);
-  p = fma(p, f, 0.055504108664821576);
-  p = fma(p, f, 0.2402265069591007);
-  p = fma(p, f, 0.6931471805599453);
+  double p = 1.3255224883682684e-06;
+  p = fma(p, f, 1.5310079402211905e-05);
+  p = fma(p, f, 0.00015403455852430636);
+  p = fma(p, f, 0.0013333450568000708);
+  p = fma(p, f, 0.00961812915940259);
+  p = fma(p, f, 0.055504109412059334);
+  p = fma(p, f, 0.2402265069581299);
+  p = fma(p, f, 0.6931471805459335);
   p = fma(p, f, 1.0);
   return ldexp(p, (int)n);
 }

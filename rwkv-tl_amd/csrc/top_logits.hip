@@ -9,11 +9,13 @@
 // Selection. Each wave finds the r-th largest of its lanes' maxima, r = ceil(k /
 // waves), by ballots; the least of them over the waves is a floor that k logits
 // of the row reach, and few more: each wave has r lanes with a logit from
-// there up. The logits from the floor up are gathered in LDS and ranked by
-// counting, for each, those that come before it. Where more than kCandMax pass
-// (long ties; rows shorter than the workgroup's lanes do not reach that many),
-// the k-th largest is found exactly, key bit by key bit over the whole row, and
-// the last id that a tie admits likewise, so that just k are gathered.
+// there up. (From r = 17 of four maxima a lane; where a mask leaves a wave without
+// r of them, by the waves that have 64.) The logits from the floor up are gathered
+// in LDS, dealt to 256 bins of equal key ranges, and ranked by the bins before
+// theirs and by comparison within their own. Where more than kCandMax pass (long
+// ties), the k-th largest is found exactly by passes over the row that count keys
+// by eight bits, and the last id that a tie admits likewise, so that just k are
+// gathered.
 #include "logits_rows.h"
 #include "rwkv7_kernels.h"
 
@@ -33,12 +35,18 @@ struct TopArgs {
   float *lse;
 };
 
+constexpr int kBins = 256;
+constexpr int kGroups = 4;      // maxima a lane keeps: of its chunks c, c % 4
+constexpr int kFloorLow = 8;    // lowest bit of a floor that is decided: to 2^-15 of a value
+
 struct TopLds {
   u64 cand[kCandMax];
+  uint16_t dealt[kCandMax];
   float m[kMaxWaves], sum[kMaxWaves];
   uint32_t floor[kMaxWaves];
-  int count[kMaxWaves];
-  int n;
+  int some[kMaxWaves];
+  int bin[kBins], at[kBins];  // of each bin: its logits, and where its next one goes
+  int n, digit, above;
 };
 
 // Order-preserving key of a logit: 1 for NaN, which comes behind -inf; 0 is none.
@@ -47,9 +55,87 @@ RWKV7_DEV uint32_t top_key(float x) {
   const uint32_t k = u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
   return x == x ? k : 1u;
 }
+RWKV7_DEV float top_key_inv(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
+
+// The r-th largest of the N keys that each lane of the wave holds, rounded down
+// to bit kFloorLow; 0 when fewer than r are not 0.
+template <int N>
+RWKV7_DEV uint32_t rth_key(const uint32_t (&key)[N], int r) {
+  uint32_t fl = 0;
+#pragma unroll 1
+  for (int bit = 31; bit >= kFloorLow; --bit) {
+    const uint32_t c = fl | (1u << bit);
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) n += __popcll(__ballot(key[i] >= c));
+    if (n >= r) fl = c;
+  }
+  return fl;
+}
+
+// Exclusive prefix over s.bin into s.at, by wave 0.
+RWKV7_DEV void scan_bins(TopLds &s) {
+  const int lane = threadIdx.x;
+  if (lane >= kWave) return;
+  int c[kBins / kWave], own = 0;
+#pragma unroll
+  for (int e = 0; e < kBins / kWave; ++e) own += c[e] = s.bin[kBins / kWave * lane + e];
+  int inc = own;
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) {
+    const int o = __shfl_up(inc, d);
+    if (lane >= d) inc += o;
+  }
+  int at = inc - own;
+#pragma unroll
+  for (int e = 0; e < kBins / kWave; ++e) {
+    s.at[kBins / kWave * lane + e] = at;
+    at += c[e];
+  }
+}
+
+// f(key, id) for every logit of the row, from memory: the way of the long ties,
+// of which nothing is held in registers beside the row.
+template <int FMT, int THREADS, class F>
+RWKV7_DEV void each_logit(const char *src, int V, F f) {
+  const uint32_t n8 = (uint32_t)V / kRowChunk;
+#pragma unroll 1
+  for (uint32_t b = threadIdx.x; b < n8; b += THREADS) {
+    Chunk<FMT> x;
+    x.load(src, b, n8);
+    float v[kRowChunk];
+    x.get(v);
+#pragma unroll
+    for (int e = 0; e < kRowChunk; ++e) f(top_key(v[e]), (int)b * kRowChunk + e);
+  }
+  const int tail = (int)n8 * kRowChunk + threadIdx.x;
+  if (threadIdx.x < kRowChunk && tail < V) f(top_key(load_logit<FMT>(src, tail)), tail);
+}
+
+// One digit of a radix selection: digit(key, id) is 0 .. 255, lowest first, or -1
+// for what the digits before ruled out. Of the digits, the one that holds the
+// `need`-th is returned, and need less those before it.
+template <int FMT, int THREADS, class D>
+RWKV7_DEV int select_digit(const char *src, int V, int &need, TopLds &s, D digit) {
+  const int t = threadIdx.x;
+  __syncthreads();
+  if (t < kBins) s.bin[t] = 0;
+  __syncthreads();
+  each_logit<FMT, THREADS>(src, V, [&](uint32_t key, int id) {
+    const int d = digit(key, id);
+    if (d >= 0) atomicAdd(&s.bin[d], 1);
+  });
+  __syncthreads();
+  scan_bins(s);
+  __syncthreads();
+  if (t < kBins && s.at[t] < need && need <= s.at[t] + s.bin[t]) s.digit = t, s.above = s.at[t];
+  __syncthreads();
+  need -= s.above;
+  return s.digit;
+}
 
 template <int FMT, int THREADS>
-__global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : 8) void top_kernel(TopArgs g) {
+__global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : THREADS == 256 ? 7 : 8) void top_kernel(TopArgs g) {
   __shared__ TopLds s;
   constexpr int kWaves = THREADS / kWave;
   const int t = threadIdx.x, lane = t & 63, wv = t >> 6, V = g.V, k = g.k;
@@ -62,26 +148,37 @@ __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : 8) void top_kernel(TopArgs 
   const int tail = t < V % kRowChunk ? (int)n8 * kRowChunk + t : -1;
   const float xt = tail >= 0 ? load_logit<FMT>(src, tail) : -kInf;
   if (t == 0) s.n = 0;
+  if (t < kBins) s.bin[t] = 0;
 
-  // the lane's largest (-inf also for none: a floor may be too low, never too high)
-  float m = xt;
-#pragma unroll
-  for (int c = 0; c < kRowChunks; ++c) {
-    float f[kRowChunk];
-    x[c].get(f);
-#pragma unroll
-    for (int e = 0; e < kRowChunk; ++e) m = fmaxf(m, f[e]);
-  }
+  // the lane's largest, by groups of chunks (-inf also for none: a floor may be
+  // too low, never too high)
+  float m = -kInf;
+  uint32_t own[kGroups];
   {
-    const uint32_t own = m > -kInf ? top_key(m) : 0u;
-    const int r = (k + kWaves - 1) / kWaves;
-    uint32_t fl = 0;
-#pragma unroll 1
-    for (int bit = 31; bit >= 8; --bit) {  // (to 2^-15 of a value)
-      const uint32_t c = fl | (1u << bit);
-      if (__popcll(__ballot(own >= c)) >= r) fl = c;
+    float mg[kGroups] = {xt, -kInf, -kInf, -kInf};
+#pragma unroll
+    for (int c = 0; c < kRowChunks; ++c) {
+      float f[kRowChunk];
+      x[c].get(f);
+#pragma unroll
+      for (int e = 0; e < kRowChunk; ++e) mg[c % kGroups] = fmaxf(mg[c % kGroups], f[e]);
     }
-    if (lane == 0) s.floor[wv] = fl;
+#pragma unroll
+    for (int i = 0; i < kGroups; ++i) {
+      own[i] = mg[i] > -kInf ? top_key(mg[i]) : 0u;
+      m = fmaxf(m, mg[i]);
+    }
+  }
+  auto wave_floor = [&](int r) {
+    const uint32_t lo = own[0] > own[1] ? own[0] : own[1], hi = own[2] > own[3] ? own[2] : own[3], one[1] = {lo > hi ? lo : hi};
+    return r > 16 ? rth_key(own, r) : rth_key(one, r);
+  };
+  {
+    const uint32_t fl = wave_floor((k + kWaves - 1) / kWaves);
+    int some = 0;
+#pragma unroll
+    for (int i = 0; i < kGroups; ++i) some += __popcll(__ballot(own[i] != 0u));
+    if (lane == 0) s.floor[wv] = fl, s.some[wv] = some;
   }
   m = wave_max(m);
   const float R = ExpScale::ref(m);
@@ -100,77 +197,91 @@ __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : 8) void top_kernel(TopArgs 
   __syncthreads();
 
   uint32_t fl = s.floor[0];
+  int full = 0;  // waves with 64 maxima or more
 #pragma unroll
-  for (int w = 1; w < kWaves; ++w) fl = min(fl, s.floor[w]);
+  for (int w = 0; w < kWaves; ++w) fl = min(fl, s.floor[w]), full += s.some[w] >= kWave;
+  if (fl == 0u && k <= full * kWave) {  // (block-uniform)
+    const uint32_t f = s.some[wv] >= kWave ? rth_key(own, (k + full - 1) / full) : ~0u;
+    __syncthreads();
+    if (lane == 0) s.floor[wv] = f;
+    __syncthreads();
+    fl = ~0u;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) fl = min(fl, s.floor[w]);
+  }
 
-  // f(key, id) for every logit that this thread holds
-  auto each = [&](auto f) {
-#pragma unroll
-    for (int c = 0; c < kRowChunks; ++c) {
-      const uint32_t b = c * THREADS + t;
-      float v[kRowChunk];
-      x[c].get(v);
-      if (b < n8) {
-#pragma unroll
-        for (int e = 0; e < kRowChunk; ++e) f(top_key(v[e]), (int)(b * kRowChunk + e));
-      }
-    }
-    if (tail >= 0) f(top_key(xt), tail);
-  };
   auto gather = [&](uint32_t key, int id) {
     const int slot = atomicAdd(&s.n, 1);
     if (slot < kCandMax) s.cand[slot] = ((u64)key << 32) | (uint32_t)~id;
   };
-  each([&](uint32_t key, int id) {
-    if (key >= fl) gather(key, id);
-  });
+  if (fl) {
+    // by value: one comparison a logit, and no more where none of a wave's passes
+    const float least = top_key_inv(fl);
+#pragma unroll
+    for (int c = 0; c < kRowChunks; ++c) {
+      float v[kRowChunk];
+      x[c].get(v);
+#pragma unroll
+      for (int e = 0; e < kRowChunk; ++e)
+        if (v[e] >= least) gather(top_key(v[e]), (c * THREADS + t) * kRowChunk + e);
+    }
+    if (tail >= 0 && xt >= least) gather(top_key(xt), tail);
+  } else if (V <= kCandMax) {
+    each_logit<FMT, THREADS>(src, V, gather);
+  } else if (t == 0) {
+    s.n = kCandMax + 1;
+  }
   __syncthreads();
   int n = s.n;
   if (n > kCandMax) {  // block-uniform
-    auto count = [&](int own) {  // over the workgroup
-      float c = wave_sum((float)own);  // (exact: at most 65 x 1024)
-      __syncthreads();
-      if (lane == 0) s.count[wv] = (int)c;
-      __syncthreads();
-      int all = 0;
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) all += s.count[w];
-      return all;
-    };
     uint32_t kth = 0;
-    int above = 0;  // logits with a key over kth
+    int need = k;
 #pragma unroll 1
-    for (int bit = 31; bit >= 0; --bit) {
-      const uint32_t c = kth | (1u << bit);
-      int own = 0;
-      each([&](uint32_t key, int) { own += key >= c; });
-      const int all = count(own);
-      if (all >= k) kth = c;
-      else above = all;
-    }
-    int last = 0;  // the lowest bound so that k - above ties have ids up to it
+    for (int sh = 24; sh >= 0; sh -= 8)
+      kth |= (uint32_t)(255 - select_digit<FMT, THREADS>(src, V, need, s, [&](uint32_t key, int) {
+               return ((key ^ kth) >> sh) >> 8 ? -1 : 255 - (int)((key >> sh) & 255u);
+             })) << sh;
+    int last = 0;  // the id of the need-th logit with that key
 #pragma unroll 1
-    for (int bit = 15; bit >= 0; --bit) {
-      const int c = last + (1 << bit);  // are there enough below c?
-      int own = 0;
-      each([&](uint32_t key, int id) { own += key == kth && id < c; });
-      if (count(own) < k - above) last = c;
-    }
-    __syncthreads();
+    for (int sh = 8; sh >= 0; sh -= 8)
+      last |= select_digit<FMT, THREADS>(src, V, need, s, [&](uint32_t key, int id) {
+                return key != kth || ((id ^ last) >> sh) >> 8 ? -1 : (id >> sh) & 255;
+              }) << sh;
     if (t == 0) s.n = 0;
+    if (t < kBins) s.bin[t] = 0;
     __syncthreads();
-    each([&](uint32_t key, int id) {
+    each_logit<FMT, THREADS>(src, V, [&](uint32_t key, int id) {
       if (key > kth || (key == kth && id <= last)) gather(key, id);
     });
     __syncthreads();
-    n = s.n;
+    n = k;
   }
 
+  // keys from `low` up, in bins of 2^shift, the highest first
+  float mm = s.m[0];
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) mm = fmaxf(mm, s.m[w]);
+  const uint32_t low = fl, range = max(top_key(mm), 1u) - low;
+  const int shift = max(0, 24 - __clz((int)(range | 1u)));
+  auto bin_of = [&](u64 c) { return kBins - 1 - (int)(((uint32_t)(c >> 32) - low) >> shift); };
+#pragma unroll 1
+  for (int i = t; i < n; i += THREADS) atomicAdd(&s.bin[bin_of(s.cand[i])], 1);
+  __syncthreads();
+  scan_bins(s);
+  __syncthreads();
+#pragma unroll 1
   for (int i = t; i < n; i += THREADS) {
-    const u64 own = s.cand[i];
-    int rank = 0;
-#pragma unroll 4
-    for (int j = 0; j < n; ++j) rank += s.cand[j] > own;
+    s.dealt[atomicAdd(&s.at[bin_of(s.cand[i])], 1)] = (uint16_t)i;
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int i = t; i < n; i += THREADS) {
+    const u64 own = s.cand[s.dealt[i]];
+    const int bin = bin_of(own), end = s.at[bin], first = end - s.bin[bin];
+    if (first >= k) continue;
+    int rank = first;
+#pragma unroll 1
+    for (int j = first; j < end; ++j) rank += s.cand[s.dealt[j]] > own;
     if (rank < k) {
       const int id = (int)~(uint32_t)own;
       g.idx[row * k + rank] = id;
@@ -179,7 +290,7 @@ __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : 8) void top_kernel(TopArgs 
     }
   }
   if (wv == 0) {
-    const float mw = lane < kWaves ? s.m[lane] : -kInf, mm = wave_max(mw);
+    const float mw = lane < kWaves ? s.m[lane] : -kInf;
     const double S = wave_sum_d(lane < kWaves ? (double)s.sum[lane] * g.sc.part(mw, mm) : 0.0);
     // (S is 0 where there is nothing but -inf)
     if (lane == 0) g.lse[row] = S == 0.0 ? -kInf : (float)(0.69314718055994531 * g.sc.log2z(S, mm));
