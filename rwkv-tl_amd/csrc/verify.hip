@@ -23,12 +23,13 @@
 // draw from.
 //
 // verify_stats_kernel: a slice of a row per workgroup: its largest logit and the
-//   sum of the exponentials about it (greedy: largest logit and its first id).
+//   sum of the exponentials about it, for target rows also of each 512 logits
+//   (greedy: largest logit and its first id).
 // verify_rest_kernel: a slice of each sequence's decisive row: every workgroup
 //   joins the sums of its sequence's rows and decides how many tokens are
-//   accepted; the slice's sum of max(p - q, 0).
-// verify_draw_kernel: one workgroup per sequence: decides again, finds the slice
-//   in which the sum crosses, and in it the token.
+//   accepted; the sums of max(p - q, 0) over each 512 logits of the slice.
+// verify_draw_kernel: one wave per sequence: finds the 512 in which the running
+//   sum crosses, and in them the token.
 #include "logits_rows.h"
 #include "rwkv7_kernels.h"
 
@@ -36,11 +37,23 @@ namespace rwkv7 {
 namespace {
 
 constexpr int kVerThreads = 256;
+constexpr int kVerWaves = kVerThreads / kWave;
 constexpr int kVerChunks = 4;
-constexpr int kVerE = kVerChunks * kRowChunk;       // logits per thread of a slice
-constexpr int kSlice = kVerThreads * kVerE;         // 8192
-constexpr int kMaxSlices = kRowMaxV / kSlice;       // 8
-constexpr int kVerMaxK = kWave - 1;                 // a lane per drafted token and one for the row behind them
+constexpr int kSlice = kVerThreads * kVerChunks * kRowChunk;  // 8192 logits
+constexpr int kMaxSlices = kRowMaxV / kSlice;                 // 8
+constexpr int kBlocks = kVerChunks * kVerWaves;               // of 512 logits in a slice, in order
+constexpr int kDrawE = 3;                                     // block sums per lane of the draw
+constexpr int kVerMaxK = kWave - 1;                           // a lane per drafted token and one for the row behind them
+static_assert(kMaxSlices * kBlocks + 1 <= kDrawE * kWave, "the draw's wave holds every block's sum, and the last logits'");
+
+// What is known of a sequence once its rows are summed.
+struct Decision {
+  int n, rejected;  // accepted tokens; whether the next was drafted and rejected
+  int x;            // the rejected token of a one-hot draft, else -1
+  float mp, mq;     // largest logits of the row behind the accepted tokens, of target and draft
+  float pad;
+  double ip, iq;    // 1 / sum of its exponentials, 0 for an empty row or none
+};
 
 struct VerifyArgs {
   const void *target, *draft;  // draft null: one-hot
@@ -52,30 +65,24 @@ struct VerifyArgs {
   double kt, kd;               // log2(e) / temperature of target and draft; kt <= 0: greedy
   int64_t *out, *accepted;
   // workspace
-  float *m;                    // [rows][G] largest logit; rows: B (K + 1) of the target, B K of the draft
   double *sum;                 // [rows][G] sum of exponentials about m (greedy: first id of the largest)
-  double *rest;                // [B][G] sums of max(p - q, 0)
+  double *block;               // [B (K + 1)][G kBlocks + 1] the same by blocks; last: the logits behind the eights
+  double *rest;                // [B][G kBlocks + 1] sums of max(p - q, 0)
+  Decision *dec;               // [B]
+  float *m;                    // [rows][G] largest logit; rows: B (K + 1) of the target, B K of the draft
 };
 
-// 2^(k (x - m)): 1 at the largest logit (also +inf), 0 for -inf and NaN.
-RWKV7_DEV double weight(float x, float m, double k) {
-  return x == m ? (m > -kInf ? 1.0 : 0.0) : exp2_d(((double)x - (double)m) * k);
-}
-
-// Joined sums of the slices of one row.
-struct RowSum {
-  float m;
-  double S;
+// The exponentials of a row about its largest logit m: 2^(k (x - m)). 1 at the
+// largest, also at +inf; 0 for -inf and NaN.
+struct Weight {
+  float m;         // NaN: nothing is the largest
+  double ref, k;
+  RWKV7_DEV Weight(float largest, double k_)
+      : m(largest > -kInf ? largest : __builtin_nanf("")), ref(largest > -kInf ? (double)largest : 0.0), k(k_) {}
+  // (the difference first: k x - k m would lose it at the types' lowest values)
+  RWKV7_DEV double finite(float x) const { return exp2_d(((double)x - ref) * k); }  // no +inf in the row
+  RWKV7_DEV double operator()(float x) const { return x == m ? 1.0 : finite(x); }
 };
-RWKV7_DEV RowSum join_row(const VerifyArgs &a, int64_t r, double k) {
-  RowSum j = {-kInf, 0.0};
-  for (int s = 0; s < a.G; ++s) j.m = fmaxf(j.m, a.m[r * a.G + s]);
-  for (int s = 0; s < a.G; ++s) {
-    const float ms = a.m[r * a.G + s];
-    j.S += a.sum[r * a.G + s] * weight(ms, j.m, k);
-  }
-  return j;
-}
 
 RWKV7_DEV int drafted(const VerifyArgs &a, int b) {
   if (!a.len) return a.K;
@@ -94,14 +101,12 @@ RWKV7_DEV const void *draft_row(const VerifyArgs &a, int b, int i) {
 
 template <int FMT, bool GREEDY>
 __global__ __launch_bounds__(kVerThreads) void verify_stats_kernel(VerifyArgs a) {
-  __shared__ float s_m[kVerThreads / kWave];
-  __shared__ double s_sum[kVerThreads / kWave];
+  __shared__ float s_m[kVerWaves];
+  __shared__ double s_sum[kVerWaves];
   const int t = threadIdx.x, lane = t & 63, wv = t >> 6, V = a.V, g = blockIdx.x;
-  const int64_t r = blockIdx.y;
-  const int64_t nt = (int64_t)a.B * (a.K + 1);
+  const int r = blockIdx.y, nt = a.B * (a.K + 1);
   const bool tgt = r < nt;
-  const int per = tgt ? a.K + 1 : a.K;
-  const int b = (int)((tgt ? r : r - nt) / per), i = (int)((tgt ? r : r - nt) % per);
+  const int per = tgt ? a.K + 1 : a.K, rr = tgt ? r : r - nt, b = rr / per, i = rr - b * per;
   const int len = drafted(a, b);
   if (i >= (tgt ? len + 1 : len)) return;  // a row that no decision looks at
   const void *row = tgt ? target_row<FMT>(a, b, i) : draft_row<FMT>(a, b, i);
@@ -111,7 +116,7 @@ __global__ __launch_bounds__(kVerThreads) void verify_stats_kernel(VerifyArgs a)
   for (int c = 0; c < kVerChunks; ++c) x[c].load(row, (g * kVerChunks + c) * kVerThreads + t, n8);
   const int tail = g == a.G - 1 && t < V % kRowChunk ? (int)n8 * kRowChunk + t : -1;
   const float xt = tail >= 0 ? load_logit<FMT>(row, tail) : -kInf;
-  float m = fmaxf(xt, -kInf);
+  float m = fmaxf(xt, -kInf);  // (NaN loses)
 #pragma unroll
   for (int c = 0; c < kVerChunks; ++c) {
     float f[kRowChunk];
@@ -123,7 +128,7 @@ __global__ __launch_bounds__(kVerThreads) void verify_stats_kernel(VerifyArgs a)
   if (lane == 0) s_m[wv] = m;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kVerThreads / kWave; ++w) m = fmaxf(m, s_m[w]);
+  for (int w = 0; w < kVerWaves; ++w) m = fmaxf(m, s_m[w]);
   double sum = 0.0;
   if (GREEDY) {
     int at = V;  // first id of the largest
@@ -139,200 +144,268 @@ __global__ __launch_bounds__(kVerThreads) void verify_stats_kernel(VerifyArgs a)
     if (m == -kInf) at = V;  // nothing but -inf and NaN
     sum = -wave_max_d(-(double)at);
   } else {
-    const double k = tgt ? a.kt : a.kd;
-    sum = tail >= 0 ? weight(xt, m, k) : 0.0;
+    const Weight w(m, tgt ? a.kt : a.kd);
+    double *block = tgt ? a.block + (int64_t)r * (a.G * kBlocks + 1) + g * kBlocks : nullptr;
+    auto add = [&](auto weight) {
 #pragma unroll
-    for (int c = 0; c < kVerChunks; ++c) {
-      float f[kRowChunk];
-      x[c].get(f);
+      for (int c = 0; c < kVerChunks; ++c) {
+        float f[kRowChunk];
+        x[c].get(f);
+        double q = 0.0, p = 0.0;
 #pragma unroll
-      for (int e = 0; e < kRowChunk; ++e) sum += weight(f[e], m, k);
-    }
-    sum = wave_sum_d(sum);
+        for (int e = 0; e < kRowChunk; e += 2) q += weight(f[e]), p += weight(f[e + 1]);
+        q = wave_sum_d(q + p);
+        if (block && lane == 0) block[c * kVerWaves + wv] = q;
+        sum += q;
+      }
+      if (g == a.G - 1 && wv == 0) {  // the logits behind the eights
+        const double q = wave_sum_d(tail >= 0 ? weight(xt) : 0.0);
+        if (block && lane == 0) block[kBlocks] = q;
+        sum += q;
+      }
+    };
+    if (m < kInf) add([&](float v) { return w.finite(v); });
+    else add([&](float v) { return w(v); });
   }
   if (lane == 0) s_sum[wv] = sum;
   __syncthreads();
   if (t == 0) {
 #pragma unroll
-    for (int w = 1; w < kVerThreads / kWave; ++w) sum = GREEDY ? fmin(sum, s_sum[w]) : sum + s_sum[w];
-    a.m[r * a.G + g] = m;
-    a.sum[r * a.G + g] = sum;
+    for (int w = 1; w < kVerWaves; ++w) sum = GREEDY ? fmin(sum, s_sum[w]) : sum + s_sum[w];
+    a.m[(int64_t)r * a.G + g] = m;
+    a.sum[(int64_t)r * a.G + g] = sum;
   }
 }
 
-// What wave 0 finds out about sequence b: the accepted tokens, and about the row
-// behind them.
-struct Decision {
-  int n, rejected;      // accepted tokens; whether the next was drafted and rejected
-  float mp, mq;
-  double ip, iq;        // 1 / sum of the row's exponentials, 0 for an empty row; iq 0 without a draft row
-  int x;                // the rejected token of a one-hot draft, else -1
+struct DecideLds {
+  float m[2][kWave];
+  double S[2][kWave];
+  Decision d;
 };
 
+// How many of sequence b's tokens are accepted, by a workgroup: the rows' sums
+// joined, a thread per slice, then a lane per drafted token.
 template <int FMT>
-RWKV7_DEV void decide(const VerifyArgs &a, int b, Decision *d) {
-  const int lane = threadIdx.x;
-  if (lane >= kWave) return;
-  const int len = drafted(a, b);
-  RowSum p = {-kInf, 0.0}, q = {-kInf, 0.0};
-  bool ok = false;
-  if (lane <= len) p = join_row(a, (int64_t)b * (a.K + 1) + lane, a.kt);
-  if (lane < len) {
-    const int64_t x = a.tok[(int64_t)b * a.K + lane];
-    const bool in = x >= 0 && x < a.V;
-    const double px = in && p.S > 0.0 ? weight(load_logit<FMT>(target_row<FMT>(a, b, lane), x), p.m, a.kt) / p.S : 0.0;
-    double qx = 1.0;
-    if (a.draft) {
-      q = join_row(a, (int64_t)a.B * (a.K + 1) + (int64_t)b * a.K + lane, a.kd);
-      qx = in && q.S > 0.0 ? weight(load_logit<FMT>(draft_row<FMT>(a, b, lane), x), q.m, a.kd) / q.S : 0.0;
-    }
-    ok = px > 0.0 && (double)a.u[(int64_t)b * (a.K + 1) + lane] * qx < px;
-  }
-  const u64 bad = ~__ballot(ok);  // (lane len is never ok)
-  const int n = __ffsll(bad) - 1;
-  if (lane == n) {
-    d->n = n;
-    d->rejected = n < len;
-    d->mp = p.m, d->mq = q.m;
-    d->ip = p.S > 0.0 ? 1.0 / p.S : 0.0;
-    d->iq = q.S > 0.0 ? 1.0 / q.S : 0.0;
-    d->x = -1;
-    if (n < len && !a.draft) {
-      const int64_t x = a.tok[(int64_t)b * a.K + n];
-      if (x >= 0 && x < a.V) d->x = (int)x;
+RWKV7_DEV void decide(const VerifyArgs &a, int b, DecideLds &s) {
+  const int t = threadIdx.x, len = drafted(a, b);
+  // the drafted tokens' logits, wanted below
+  float zp = -kInf, zq = -kInf, u = 0.f;
+  int64_t x = -1;
+  if (t < len) {
+    x = a.tok[(int64_t)b * a.K + t];
+    u = a.u[(int64_t)b * (a.K + 1) + t];
+    if (x >= 0 && x < a.V) {
+      zp = load_logit<FMT>(target_row<FMT>(a, b, t), x);
+      if (a.draft) zq = load_logit<FMT>(draft_row<FMT>(a, b, t), x);
+    } else {
+      x = -1;
     }
   }
+  for (int which = 0; which < (a.draft ? 2 : 1); ++which) {
+    const int rows = which ? len : len + 1;
+    const int64_t r0 = which ? (int64_t)a.B * (a.K + 1) + (int64_t)b * a.K : (int64_t)b * (a.K + 1);
+    const double k = which ? a.kd : a.kt;
+    for (int i = t; i < rows * kMaxSlices; i += kVerThreads) {  // (whole groups of eight lanes)
+      const int row = i / kMaxSlices, g = i % kMaxSlices;
+      const int64_t at = (r0 + row) * a.G + g;
+      const float mg = g < a.G ? a.m[at] : -kInf;
+      float m = mg;
+      m = fmaxf(m, dpp<kDppXor1>(m));
+      m = fmaxf(m, dpp<kDppXor2>(m));
+      m = fmaxf(m, dpp<kDppHalfMirror>(m));
+      double S = g < a.G && mg > -kInf ? a.sum[at] * Weight(m, k)(mg) : 0.0;
+      S += dpp_d<kDppXor1>(S);
+      S += dpp_d<kDppXor2>(S);
+      S += dpp_d<kDppHalfMirror>(S);
+      if (g == 0) s.m[which][row] = m, s.S[which][row] = S;
+    }
+  }
+  __syncthreads();
+  if (t < kWave) {
+    bool ok = false;
+    if (t < len && x >= 0) {
+      const double Sp = s.S[0][t], Sq = a.draft ? s.S[1][t] : 0.0;
+      const double px = Sp > 0.0 ? Weight(s.m[0][t], a.kt)(zp) / Sp : 0.0;
+      const double qx = !a.draft ? 1.0 : Sq > 0.0 ? Weight(s.m[1][t], a.kd)(zq) / Sq : 0.0;
+      ok = px > 0.0 && (double)u * qx < px;
+    }
+    const int n = __ffsll((u64)~__ballot(ok)) - 1;  // (lane len is never ok)
+    if (t == n) {
+      const bool rejected = n < len;
+      Decision d;
+      d.n = n, d.rejected = rejected;
+      d.x = rejected && !a.draft ? (int)x : -1;
+      d.mp = s.m[0][n];
+      d.ip = s.S[0][n] > 0.0 ? 1.0 / s.S[0][n] : 0.0;
+      const bool soft = rejected && a.draft;
+      d.mq = soft ? s.m[1][n] : 0.f;
+      d.iq = soft && s.S[1][n] > 0.0 ? 1.0 / s.S[1][n] : 0.0;
+      d.pad = 0.f;
+      s.d = d;
+    }
+  }
+  __syncthreads();
 }
 
 // max(p - q, 0) of one logit; id: its index.
-RWKV7_DEV double residual(const VerifyArgs &a, const Decision &d, float xp, float xq, int id) {
-  double r = weight(xp, d.mp, a.kt) * d.ip;
-  if (a.draft) r = fmax(r - weight(xq, d.mq, a.kd) * d.iq, 0.0);
-  return id == d.x ? 0.0 : r;
-}
+struct Residual {
+  Weight p, q;
+  double ip, iq;
+  int x;
+  bool soft;
+  RWKV7_DEV Residual(const VerifyArgs &a, const Decision &d, bool from_p)
+      : p(d.mp, a.kt), q(d.mq, a.kd), ip(d.ip), iq(d.iq), x(from_p ? -1 : d.x), soft(!from_p && d.rejected && a.draft) {}
+  RWKV7_DEV double operator()(float xp, float xq, int id) const {
+    double r = p(xp) * ip;
+    if (soft) r = fmax(r - q(xq) * iq, 0.0);
+    return id == x ? 0.0 : r;
+  }
+};
 
 template <int FMT>
 __global__ __launch_bounds__(kVerThreads) void verify_rest_kernel(VerifyArgs a) {
-  __shared__ Decision s_d;
-  __shared__ double s_sum[kVerThreads / kWave];
+  __shared__ DecideLds s;
   const int t = threadIdx.x, lane = t & 63, wv = t >> 6, V = a.V, g = blockIdx.x, b = blockIdx.y;
-  decide<FMT>(a, b, &s_d);
-  __syncthreads();
-  const Decision d = s_d;
+  decide<FMT>(a, b, s);
+  const Decision d = s.d;
+  if (g == 0 && t == 0) a.dec[b] = d;
   if (!d.rejected) return;
   const void *pr = target_row<FMT>(a, b, d.n), *qr = a.draft ? draft_row<FMT>(a, b, d.n) : pr;
   const uint32_t n8 = (uint32_t)V / kRowChunk;
-  double sum = 0.0;
+  const Residual res(a, d, false);
+  double *block = a.rest + (int64_t)b * (a.G * kBlocks + 1) + g * kBlocks;
+  Chunk<FMT> xp[kVerChunks], xq[kVerChunks];
+#pragma unroll
+  for (int c = 0; c < kVerChunks; ++c) {
+    xp[c].load(pr, (g * kVerChunks + c) * kVerThreads + t, n8);
+    xq[c].load(qr, (g * kVerChunks + c) * kVerThreads + t, n8);
+  }
 #pragma unroll 1
   for (int c = 0; c < kVerChunks; ++c) {
-    const uint32_t e8 = (g * kVerChunks + c) * kVerThreads + t;
-    if (e8 >= n8) break;
+    float fp[kRowChunk], fq[kRowChunk];
+    xp[0].get(fp);
+    xq[0].get(fq);
+#pragma unroll
+    for (int i = 0; i + 1 < kVerChunks; ++i) xp[i] = xp[i + 1], xq[i] = xq[i + 1];  // (registers have no index)
+    const int i0 = ((g * kVerChunks + c) * kVerThreads + t) * kRowChunk;
+    double sum = 0.0;
+#pragma unroll
+    for (int e = 0; e < kRowChunk; ++e) sum += res(fp[e], fq[e], i0 + e);
+    sum = wave_sum_d(sum);
+    if (lane == 0) block[c * kVerWaves + wv] = sum;
+  }
+  if (g == a.G - 1 && wv == 0) {
+    const int id = (int)n8 * kRowChunk + t;
+    const double sum = wave_sum_d(id < V ? res(load_logit<FMT>(pr, id), load_logit<FMT>(qr, id), id) : 0.0);
+    if (lane == 0) block[kBlocks] = sum;
+  }
+}
+
+RWKV7_DEV double shfl_up_d(double x, int d) {
+  const u64 v = __builtin_bit_cast(u64, x);
+  const int lo = __shfl_up((int)(uint32_t)v, d), hi = __shfl_up((int)(uint32_t)(v >> 32), d);
+  return __builtin_bit_cast(double, (u64)(uint32_t)lo | ((u64)(uint32_t)hi << 32));
+}
+// Inclusive prefix over the lanes.
+RWKV7_DEV double wave_scan_d(double v) {
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) {
+    const double o = shfl_up_d(v, d);
+    if ((int)threadIdx.x >= d) v += o;
+  }
+  return v;
+}
+
+template <int FMT>
+__global__ __launch_bounds__(kWave) void verify_draw_kernel(VerifyArgs a) {
+  const int lane = threadIdx.x, V = a.V, b = blockIdx.x, blocks = a.G * kBlocks + 1;
+  const uint32_t n8 = (uint32_t)V / kRowChunk;
+  const Decision d = a.dec[b];
+  const double u = (double)a.u[(int64_t)b * (a.K + 1) + a.K];
+  const int64_t r = (int64_t)b * (a.K + 1) + d.n;
+  // this lane's block sums of what is drawn from: p - q, or p itself
+  double w[kDrawE];
+  bool from_p = !d.rejected;
+  if (d.rejected) {
+#pragma unroll
+    for (int e = 0; e < kDrawE; ++e) w[e] = kDrawE * lane + e < blocks ? a.rest[(int64_t)b * blocks + kDrawE * lane + e] : 0.0;
+    from_p = !(wave_sum_d((w[0] + w[1]) + w[2]) > 0.0);
+  }
+  if (from_p) {
+    const Weight weight(d.mp, a.kt);
+#pragma unroll
+    for (int e = 0; e < kDrawE; ++e) {
+      const int i = kDrawE * lane + e, g = min(i / kBlocks, a.G - 1);
+      w[e] = i < blocks ? a.block[r * blocks + i] * (weight(a.m[r * a.G + g]) * d.ip) : 0.0;
+    }
+  }
+  double own = (w[0] + w[1]) + w[2];
+  double inc = wave_scan_d(own);
+  const double goal = u * lane_value_d(inc, kWave - 1);
+  // the first block in which the running sum exceeds the goal; none (u >= 1, or
+  // rounding): the last one with any weight
+  u64 over = __ballot(own > 0.0 && inc > goal);
+  const u64 some = __ballot(own > 0.0);
+  const bool none = over == 0;
+  int token = 0;  // with nothing to draw from
+  if (some) {
+    const int who = none ? 63 - __clzll(some) : __ffsll(over) - 1;
+    double base = inc - own;
+    int e0 = -1;
+#pragma unroll
+    for (int e = 0; e < kDrawE; ++e) {
+      const bool stop = none ? w[e] > 0.0 : e0 < 0 && w[e] > 0.0 && base + w[e] > goal;
+      if (stop) e0 = e;
+      else if (e0 < 0) base += w[e];
+    }
+    if (e0 < 0) {  // (by rounding the running sum may end just below the goal)
+#pragma unroll
+      for (int e = 0; e < kDrawE; ++e)
+        if (w[e] > 0.0) e0 = e;
+    }
+    const int blk = __builtin_amdgcn_readlane(kDrawE * lane + e0, who);
+    base = lane_value_d(base, who);
+    // its logits, eight a lane (behind the eights: one)
+    const bool last = blk == blocks - 1;
+    const int g = blk / kBlocks, c = blk % kBlocks / kVerWaves, wv = blk % kVerWaves;
+    const uint32_t e8 = last ? n8 : (g * kVerChunks + c) * kVerThreads + wv * kWave + lane;
+    const void *pr = target_row<FMT>(a, b, d.n);
+    const Residual res(a, d, from_p);
+    const void *qr = res.soft ? draft_row<FMT>(a, b, d.n) : pr;
     Chunk<FMT> xp, xq;
     xp.load(pr, e8, n8);
     xq.load(qr, e8, n8);
     float fp[kRowChunk], fq[kRowChunk];
     xp.get(fp);
     xq.get(fq);
+    int i0 = (int)e8 * kRowChunk;
+    if (last) {
+      i0 += lane;
+      fp[0] = i0 < V ? load_logit<FMT>(pr, i0) : -kInf;
+      fq[0] = i0 < V ? load_logit<FMT>(qr, i0) : -kInf;
+    }
+    double v[kRowChunk];
+    own = 0.0;
 #pragma unroll
-    for (int e = 0; e < kRowChunk; ++e) sum += residual(a, d, fp[e], fq[e], (int)e8 * kRowChunk + e);
-  }
-  if (g == a.G - 1 && t < V % kRowChunk) {
-    const int id = (int)n8 * kRowChunk + t;
-    sum += residual(a, d, load_logit<FMT>(pr, id), load_logit<FMT>(qr, id), id);
-  }
-  sum = wave_sum_d(sum);
-  if (lane == 0) s_sum[wv] = sum;
-  __syncthreads();
-  if (t == 0) {
-#pragma unroll
-    for (int w = 1; w < kVerThreads / kWave; ++w) sum += s_sum[w];
-    a.rest[(int64_t)b * a.G + g] = sum;
-  }
-}
-
-template <int FMT>
-__global__ __launch_bounds__(kVerThreads) void verify_draw_kernel(VerifyArgs a) {
-  __shared__ Decision s_d;
-  __shared__ double s_slice[kMaxSlices + 1], s_wave[kVerThreads / kWave];
-  __shared__ int s_first, s_last;
-  const int t = threadIdx.x, lane = t & 63, wv = t >> 6, V = a.V, b = blockIdx.x;
-  decide<FMT>(a, b, &s_d);
-  __syncthreads();
-  const Decision d = s_d;
-  const int64_t r = (int64_t)b * (a.K + 1) + d.n;
-  // the slices' sums of what is drawn from: p - q, or p itself
-  bool from_p = !d.rejected;
-  if (t < a.G && d.rejected) s_slice[t] = a.rest[(int64_t)b * a.G + t];
-  __syncthreads();
-  if (d.rejected) {
-    double all = 0.0;
-    for (int s = 0; s < a.G; ++s) all += s_slice[s];
-    from_p = !(all > 0.0);
-    __syncthreads();
-  }
-  if (from_p && t < a.G) s_slice[t] = a.sum[r * a.G + t] * weight(a.m[r * a.G + t], d.mp, a.kt) * d.ip;
-  if (t == 0) s_first = V, s_last = -1;
-  __syncthreads();
-  double all = 0.0;
-  for (int s = 0; s < a.G; ++s) all += s_slice[s];
-  const double goal = (double)a.u[(int64_t)b * (a.K + 1) + a.K] * all;
-  // the first slice in which the inclusive sum exceeds the goal; none (u >= 1, or
-  // rounding): the last one with any weight
-  int g = -1, with = 0;
-  double before = 0.0, base = 0.0;
-  for (int s = 0; s < a.G; ++s) {
-    if (s_slice[s] > 0.0) with = s;
-    if (g < 0 && before + s_slice[s] > goal) g = s, base = before;
-    before += s_slice[s];
-  }
-  const bool none = g < 0;
-  if (none) g = with;
-  // its logits, 32 consecutive ones a thread (and the row's last few)
-  const void *pr = target_row<FMT>(a, b, d.n), *qr = a.draft && d.rejected ? draft_row<FMT>(a, b, d.n) : pr;
-  const int i0 = g * kSlice + t * kVerE;
-  auto at = [&](int id) {
-    const float xp = load_logit<FMT>(pr, id);
-    return from_p ? weight(xp, d.mp, a.kt) * d.ip : residual(a, d, xp, load_logit<FMT>(qr, id), id);
-  };
-  double own = 0.0;
-  int last = -1;
-#pragma unroll 4
-  for (int e = 0; e < kVerE; ++e) {
-    const int id = i0 + e;
-    if (id >= V) break;
-    const double w = at(id);
-    own += w;
-    if (w > 0.0) last = id;
-  }
-  // inclusive sums over the threads
-  double inc = own;
-#pragma unroll
-  for (int s = 1; s < kWave; s <<= 1) {
-    const u64 v = __builtin_bit_cast(u64, inc);
-    const int lo = __shfl_up((int)(uint32_t)v, s), hi = __shfl_up((int)(uint32_t)(v >> 32), s);
-    if (lane >= s) inc += __builtin_bit_cast(double, (u64)(uint32_t)lo | ((u64)(uint32_t)hi << 32));
-  }
-  if (lane == kWave - 1) s_wave[wv] = inc;
-  __syncthreads();
-  for (int w = 0; w < wv; ++w) base += s_wave[w];
-  if (last >= 0) atomicMax(&s_last, last);
-  if (!none && own > 0.0 && base + inc > goal) {
+    for (int e = 0; e < kRowChunk; ++e) own += v[e] = res(fp[e], fq[e], i0 + e);
+    inc = wave_scan_d(own);
+    over = none ? 0 : __ballot(own > 0.0 && base + inc > goal);
+    const u64 here = __ballot(own > 0.0);  // (0 only where all of the block's weights are below 2^-1074)
+    const int lane2 = over ? __ffsll(over) - 1 : here ? 63 - __clzll(here) : 0;
     double acc = base + (inc - own);
-    int found = last;  // (by rounding, the running sum may end just below the goal)
-    for (int e = 0; e < kVerE && i0 + e < V; ++e) {
-      const double w = at(i0 + e);
-      acc += w;
-      if (w > 0.0 && acc > goal) {
-        found = i0 + e;
-        break;
+    int at = -1, back = 0;
+#pragma unroll
+    for (int e = 0; e < kRowChunk; ++e) {
+      acc += v[e];
+      if (v[e] > 0.0) {
+        back = e;
+        if (at < 0 && over && acc > goal) at = e;
       }
     }
-    atomicMin(&s_first, found);
+    token = __builtin_amdgcn_readlane(i0 + (at < 0 ? back : at), lane2);
   }
-  __syncthreads();
-  const int next = s_first < V ? s_first : s_last >= 0 ? s_last : 0;
-  if (t <= a.K) a.out[(int64_t)b * (a.K + 1) + t] = t < d.n ? a.tok[(int64_t)b * a.K + t] : t == d.n ? next : -1;
-  if (t == 0) a.accepted[b] = d.n;
+  if (lane <= a.K) a.out[(int64_t)b * (a.K + 1) + lane] = lane < d.n ? a.tok[(int64_t)b * a.K + lane] : lane == d.n ? token : -1;
+  if (lane == 0) a.accepted[b] = d.n;
 }
 
 // Greedy: one wave per sequence, a lane per drafted token.
@@ -342,15 +415,18 @@ __global__ __launch_bounds__(kWave) void verify_greedy_kernel(VerifyArgs a) {
   if (lane <= len) {
     const int64_t r = (int64_t)b * (a.K + 1) + lane;
     float m = -kInf;
-    for (int s = 0; s < a.G; ++s) {
-      const float v = a.m[r * a.G + s];
-      if (v > m) m = v, best = (int)a.sum[r * a.G + s];
+#pragma unroll
+    for (int s = 0; s < kMaxSlices; ++s) {
+      const int64_t at = r * a.G + min(s, a.G - 1);
+      const float v = a.m[at];
+      const int id = (int)a.sum[at];
+      if (v > m) m = v, best = id;
     }
     if (best >= a.V) best = 0;
   }
   const int64_t x = lane < a.K ? a.tok[(int64_t)b * a.K + lane] : -1;
   const bool ok = lane < len && x == best;
-  const int n = __ffsll(~__ballot(ok)) - 1;
+  const int n = __ffsll((u64)~__ballot(ok)) - 1;
   if (lane <= a.K) a.out[(int64_t)b * (a.K + 1) + lane] = lane < n ? x : lane == n ? best : -1;
   if (lane == 0) a.accepted[b] = n;
 }
@@ -370,16 +446,31 @@ int launch_verify(const VerifyArgs &a, hipStream_t st) {
   }
   verify_stats_kernel<FMT, false><<<grid, kVerThreads, 0, st>>>(a);
   RWKV7_CHECK_LAUNCH();
-  if (a.K > 0) {
-    verify_rest_kernel<FMT><<<dim3(a.G, a.B), kVerThreads, 0, st>>>(a);
-    RWKV7_CHECK_LAUNCH();
-  }
-  verify_draw_kernel<FMT><<<a.B, kVerThreads, 0, st>>>(a);
+  verify_rest_kernel<FMT><<<dim3(a.G, a.B), kVerThreads, 0, st>>>(a);
+  RWKV7_CHECK_LAUNCH();
+  verify_draw_kernel<FMT><<<a.B, kWave, 0, st>>>(a);
   RWKV7_CHECK_LAUNCH();
   return RWKV7_OK;
 }
 
 int64_t al256(int64_t x) { return (x + 255) / 256 * 256; }
+
+// The workspace's parts in a's pointers; returns its size.
+int64_t verify_ws(VerifyArgs &a, char *p) {
+  const int64_t rows = (int64_t)a.B * (2 * a.K + 1), blocks = a.G * kBlocks + 1;
+  char *const p0 = p;
+  auto take = [&](int64_t bytes) {
+    char *q = p;
+    p += al256(bytes);
+    return q;
+  };
+  a.sum = reinterpret_cast<double *>(take(rows * a.G * 8));
+  a.block = reinterpret_cast<double *>(take((int64_t)a.B * (a.K + 1) * blocks * 8));
+  a.rest = reinterpret_cast<double *>(take(a.B * blocks * 8));
+  a.dec = reinterpret_cast<Decision *>(take((int64_t)a.B * sizeof(Decision)));
+  a.m = reinterpret_cast<float *>(take(rows * a.G * 4));
+  return p - p0;
+}
 
 }  // namespace
 }  // namespace rwkv7
@@ -387,8 +478,9 @@ int64_t al256(int64_t x) { return (x + 255) / 256 * 256; }
 extern "C" int64_t rwkv7_verify_workspace_bytes(int32_t B, int32_t K, int32_t V) {
   using namespace rwkv7;
   if (B < 1 || K < 0 || K > kVerMaxK || V < 1 || V > kRowMaxV) return 0;
-  const int64_t rg = (int64_t)B * (2 * K + 1) * slices(V);
-  return al256(rg * 4) + al256(rg * 8) + al256((int64_t)B * slices(V) * 8);
+  VerifyArgs a;
+  a.B = B, a.K = K, a.G = slices(V);
+  return verify_ws(a, nullptr);
 }
 
 extern "C" int rwkv7_verify(const void *target, int64_t target_b, int64_t target_r, const void *draft, int64_t draft_b,
@@ -408,20 +500,15 @@ extern "C" int rwkv7_verify(const void *target, int64_t target_b, int64_t target
   if (target_r < V || target_b < 0 || (soft && (draft_r < V || draft_b < 0))) return RWKV7_ESHAPE;
   if (workspace_bytes < rwkv7_verify_workspace_bytes(B, K, V)) return RWKV7_EWORKSPACE;
   constexpr double kLog2E = 1.4426950408889634;
-  const int G = slices(V);
-  const int64_t rg = (int64_t)B * (2 * K + 1) * G;
-  char *w = static_cast<char *>(workspace);
   VerifyArgs a;
   a.target = target, a.draft = soft ? draft : nullptr;
   a.tb = target_b, a.tr = target_r, a.db = draft_b, a.dr = draft_r;
   a.tok = tokens, a.u = uniforms, a.len = lengths;
-  a.B = B, a.K = K, a.V = V, a.G = G;
+  a.B = B, a.K = K, a.V = V, a.G = slices(V);
   a.kt = greedy ? 0.0 : kLog2E / temperature;
   a.kd = soft ? kLog2E / draft_temperature : 0.0;
   a.out = out, a.accepted = accepted;
-  a.m = reinterpret_cast<float *>(w);
-  a.sum = reinterpret_cast<double *>(w + al256(rg * 4));
-  a.rest = reinterpret_cast<double *>(w + al256(rg * 4) + al256(rg * 8));
+  verify_ws(a, static_cast<char *>(workspace));
   const hipStream_t st = static_cast<hipStream_t>(stream);
   switch (logits_dtype) {
     case 0: return launch_verify<0>(a, st);

@@ -18,6 +18,7 @@ be captured in a HIP graph. Each call allocates what it returns, and
 from __future__ import annotations
 
 import math
+from collections.abc import Callable
 
 import torch
 from torch import Tensor
@@ -32,16 +33,17 @@ MAX_DRAFT = 63  # drafted tokens per sequence of verify_draft
 LOGIT_DTYPES = {torch.float16: 0, torch.float32: 1, torch.bfloat16: 2}
 
 
-def _need(cond: bool, msg: str) -> None:
+def _need(cond: bool, msg: str | Callable[[], str]) -> None:
+    """``msg``: a text, or what makes it (formed only where the check fails)."""
     if not cond:
-        raise ValueError(msg)
+        raise ValueError(msg if isinstance(msg, str) else msg())
 
 
 def _check_logits(x: Tensor, name: str) -> None:
-    _need(isinstance(x, Tensor), f"{name} must be a tensor")
-    _need(x.is_cuda, f"{name} on {x.device}; the HIP kernels need a ROCm device")
-    _need(x.dtype in LOGIT_DTYPES, f"{name} must be float16, bfloat16 or float32, got {x.dtype}")
-    _need(x.ndim >= 1 and 1 <= x.shape[-1] <= MAX_VOCAB, f"{name}: a vocabulary of 1..{MAX_VOCAB}, got {tuple(x.shape)}")
+    _need(isinstance(x, Tensor), lambda: f"{name} must be a tensor")
+    _need(x.is_cuda, lambda: f"{name} on {x.device}; the HIP kernels need a ROCm device")
+    _need(x.dtype in LOGIT_DTYPES, lambda: f"{name} must be float16, bfloat16 or float32, got {x.dtype}")
+    _need(x.ndim >= 1 and 1 <= x.shape[-1] <= MAX_VOCAB, lambda: f"{name}: a vocabulary of 1..{MAX_VOCAB}, got {tuple(x.shape)}")
 
 
 def _rows(x: Tensor) -> Tensor:
@@ -62,14 +64,14 @@ def _dense(x: Tensor) -> Tensor:
 
 def _temperature(t: float) -> float:
     t = float(t)
-    _need(1e-30 <= t <= 1e30, f"temperature must be positive and finite, got {t}")
+    _need(1e-30 <= t <= 1e30, lambda: f"temperature must be positive and finite, got {t}")
     return t
 
 
 def _same_device(ref: Tensor, **others: Tensor | None) -> None:
     for name, t in others.items():
         if t is not None:
-            _need(t.device == ref.device, f"{name} on {t.device}, the logits on {ref.device}")
+            _need(t.device == ref.device, lambda: f"{name} on {t.device}, the logits on {ref.device}")
 
 
 def top_logits(logits: Tensor, k: int, *, temperature: float = 1.0) -> tuple[Tensor, Tensor, Tensor]:
@@ -81,7 +83,7 @@ def top_logits(logits: Tensor, k: int, *, temperature: float = 1.0) -> tuple[Ten
     answers as ``distill_loss`` takes them."""
     _check_logits(logits, "logits")
     V = logits.shape[-1]
-    _need(isinstance(k, int) and 1 <= k <= min(V, MAX_TOP), f"k must be in 1..{min(V, MAX_TOP)}, got {k}")
+    _need(isinstance(k, int) and 1 <= k <= min(V, MAX_TOP), lambda: f"k must be in 1..{min(V, MAX_TOP)}, got {k}")
     temperature = _temperature(temperature)
     lead = logits.shape[:-1]
     x = _dense(_rows(logits))
@@ -103,15 +105,15 @@ def _distill(logits, top_val, top_idx, lse, temperature, scale, want_loss: bool,
     _check_logits(logits, "logits")
     lead, V = logits.shape[:-1], logits.shape[-1]
     _need(top_val.ndim >= 1 and top_val.shape[:-1] == lead and top_idx.shape == top_val.shape,
-          f"top_val and top_idx must be [{', '.join(map(str, (*lead, 'K')))}], got {tuple(top_val.shape)} and "
+          lambda: f"top_val and top_idx must be [{', '.join(map(str, (*lead, 'K')))}], got {tuple(top_val.shape)} and "
           f"{tuple(top_idx.shape)}")
     K = top_val.shape[-1]
-    _need(K <= MAX_ENTRIES, f"at most {MAX_ENTRIES} teacher entries per row, got {K}")
-    _need(top_val.dtype in LOGIT_DTYPES, f"top_val must be float16, bfloat16 or float32, got {top_val.dtype}")
-    _need(top_idx.dtype == torch.int64, f"top_idx must be int64, got {top_idx.dtype}")
-    _need(lse is None or (lse.shape == lead and lse.dtype == torch.float32), f"lse must be float32 {tuple(lead)}")
+    _need(K <= MAX_ENTRIES, lambda: f"at most {MAX_ENTRIES} teacher entries per row, got {K}")
+    _need(top_val.dtype in LOGIT_DTYPES, lambda: f"top_val must be float16, bfloat16 or float32, got {top_val.dtype}")
+    _need(top_idx.dtype == torch.int64, lambda: f"top_idx must be int64, got {top_idx.dtype}")
+    _need(lse is None or (lse.shape == lead and lse.dtype == torch.float32), lambda: f"lse must be float32 {tuple(lead)}")
     rowwise = isinstance(scale, Tensor)
-    _need(not rowwise or (scale.shape == lead and scale.dtype == torch.float32), f"scale must be float32 {tuple(lead)}")
+    _need(not rowwise or (scale.shape == lead and scale.dtype == torch.float32), lambda: f"scale must be float32 {tuple(lead)}")
     _same_device(logits, top_val=top_val, top_idx=top_idx, lse=lse, scale=scale if rowwise else None)
     temperature = _temperature(temperature)
     x = _dense(_rows(logits))
@@ -206,12 +208,12 @@ def verify_draft(
     up = (lambda t: None if t is None else t.unsqueeze(0)) if single else (lambda t: t)
     target, tokens, draft = up(target_logits), up(draft_tokens), up(draft_logits)
     uniforms, lengths = up(uniforms), up(lengths)
-    _need(target.ndim == 3 and target.shape[1] >= 1, f"target_logits must be [B, K + 1, V], got {tuple(target_logits.shape)}")
+    _need(target.ndim == 3 and target.shape[1] >= 1, lambda: f"target_logits must be [B, K + 1, V], got {tuple(target_logits.shape)}")
     B, K, V = target.shape[0], target.shape[1] - 1, target.shape[2]
-    _need(K <= MAX_DRAFT, f"at most {MAX_DRAFT} drafted tokens, got {K}")
-    _need(B * (2 * K + 1) <= 65535, f"a batch of {B} with {K} drafts is too large: at most {65535 // (2 * K + 1)}")
+    _need(K <= MAX_DRAFT, lambda: f"at most {MAX_DRAFT} drafted tokens, got {K}")
+    _need(B * (2 * K + 1) <= 65535, lambda: f"a batch of {B} with {K} drafts is too large: at most {65535 // (2 * K + 1)}")
     _need(tokens.shape == (B, K) and tokens.dtype == torch.int64,
-          f"draft_tokens must be int64 [{B}, {K}], got {tokens.dtype} {tuple(tokens.shape)}")
+          lambda: f"draft_tokens must be int64 [{B}, {K}], got {tokens.dtype} {tuple(tokens.shape)}")
     temperature = 0.0 if temperature is None else float(temperature)
     greedy = temperature <= 0
     if not greedy:
@@ -221,17 +223,17 @@ def verify_draft(
     _need(not math.isnan(draft_temperature), "draft_temperature is NaN")
     if uniforms is not None:
         _need(uniforms.shape == (B, K + 1) and uniforms.dtype == torch.float32,
-              f"uniforms must be float32 [{B}, {K + 1}], got {uniforms.dtype} {tuple(uniforms.shape)}")
+              lambda: f"uniforms must be float32 [{B}, {K + 1}], got {uniforms.dtype} {tuple(uniforms.shape)}")
     if draft is not None:
         _check_logits(draft, "draft_logits")
         _need(draft.shape == (B, K, V) and draft.dtype == target.dtype,
-              f"draft_logits must be {target.dtype} [{B}, {K}, {V}], got {draft.dtype} {tuple(draft.shape)}")
+              lambda: f"draft_logits must be {target.dtype} [{B}, {K}, {V}], got {draft.dtype} {tuple(draft.shape)}")
         if not greedy and draft_temperature > 0:
             _temperature(draft_temperature)
         else:
             draft = None
     if lengths is not None:
-        _need(lengths.shape == (B,) and lengths.dtype == torch.int64, f"lengths must be int64 [{B}]")
+        _need(lengths.shape == (B,) and lengths.dtype == torch.int64, lambda: f"lengths must be int64 [{B}]")
     _same_device(target, draft_tokens=tokens, uniforms=uniforms, draft_logits=draft, lengths=lengths)
     with _lib.device_of(target):
         out = torch.empty(B, K + 1, dtype=torch.int64, device=target.device)
