@@ -249,9 +249,14 @@ _HERE = contextlib.nullcontext()
 
 
 def device_of(t: torch.Tensor):
-    """A context in which ``t``'s device is the current one, and so are its
-    stream for ``stream_handle`` and the launches."""
-    return _HERE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+    """A context in which ``t``'s device is the current one (launches go there)."""
+    i = t.get_device()
+    return _HERE if i == torch._C._cuda_getDevice() else torch.cuda.device(i)
+
+
+def stream_of(t: torch.Tensor) -> int:
+    """The current torch stream of ``t``'s device as a hipStream_t."""
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
 def stream_handle() -> int:

@@ -39,27 +39,27 @@ def _need(cond: bool, msg: str | Callable[[], str]) -> None:
         raise ValueError(msg if isinstance(msg, str) else msg())
 
 
-def _check_logits(x: Tensor, name: str) -> None:
+def _check_logits(x: Tensor, name: str) -> int:
+    """The logits' dtype code."""
     _need(isinstance(x, Tensor), lambda: f"{name} must be a tensor")
     _need(x.is_cuda, lambda: f"{name} on {x.device}; the HIP kernels need a ROCm device")
-    _need(x.dtype in LOGIT_DTYPES, lambda: f"{name} must be float16, bfloat16 or float32, got {x.dtype}")
+    code = LOGIT_DTYPES.get(x.dtype)
+    _need(code is not None, lambda: f"{name} must be float16, bfloat16 or float32, got {x.dtype}")
     _need(x.ndim >= 1 and 1 <= x.shape[-1] <= MAX_VOCAB, lambda: f"{name}: a vocabulary of 1..{MAX_VOCAB}, got {tuple(x.shape)}")
+    return code
 
 
-def _rows(x: Tensor) -> Tensor:
-    """``[..., V]`` as ``[N, V]`` with adjacent columns (a copy only where no view is one)."""
-    x = x.reshape(-1, x.shape[-1])
-    return x if x.stride(1) == 1 or x.shape[1] == 1 and x.stride(0) >= 1 else x.contiguous()
-
-
-def _ld(x: Tensor) -> int:
-    """Row stride of ``[N, V]``; of a single row any that covers it."""
-    return max(x.stride(0), x.shape[1]) if x.shape[0] == 1 else x.stride(0)
-
-
-def _dense(x: Tensor) -> Tensor:
-    """Rows that do not overlap (an expanded row is copied)."""
-    return x if x.shape[0] <= 1 or x.stride(0) >= x.shape[1] else x.contiguous()
+def _rows(x: Tensor) -> tuple[Tensor, int, int]:
+    """``[..., V]`` as rows of adjacent columns that do not overlap: what holds them
+    (a copy only where no view is one), their number and their stride."""
+    V = x.shape[-1]
+    if x.is_contiguous():
+        return x, x.numel() // V, V
+    x = x.reshape(-1, V)
+    N = x.shape[0]
+    if (x.stride(1) != 1 and V > 1) or (N > 1 and x.stride(0) < V):
+        x = x.contiguous()
+    return x, N, x.stride(0) if N > 1 else V
 
 
 def _temperature(t: float) -> float:
@@ -68,10 +68,11 @@ def _temperature(t: float) -> float:
     return t
 
 
-def _same_device(ref: Tensor, **others: Tensor | None) -> None:
-    for name, t in others.items():
-        if t is not None:
-            _need(t.device == ref.device, lambda: f"{name} on {t.device}, the logits on {ref.device}")
+def _same_device(ref: Tensor, *others: Tensor | None) -> None:
+    i = ref.get_device()
+    for t in others:
+        if t is not None and t.get_device() != i:
+            raise ValueError(f"tensors on {ref.device} and on {t.device}")
 
 
 def top_logits(logits: Tensor, k: int, *, temperature: float = 1.0) -> tuple[Tensor, Tensor, Tensor]:
@@ -81,46 +82,45 @@ def top_logits(logits: Tensor, k: int, *, temperature: float = 1.0) -> tuple[Ten
     id, NaN last), ``indices [..., k]`` int64, and ``lse [...]`` float32, the log
     of the sum of ``exp(logits / temperature)`` over the whole row: a teacher's
     answers as ``distill_loss`` takes them."""
-    _check_logits(logits, "logits")
+    code = _check_logits(logits, "logits")
     V = logits.shape[-1]
     _need(isinstance(k, int) and 1 <= k <= min(V, MAX_TOP), lambda: f"k must be in 1..{min(V, MAX_TOP)}, got {k}")
     temperature = _temperature(temperature)
     lead = logits.shape[:-1]
-    x = _dense(_rows(logits))
-    N = x.shape[0]
-    with _lib.device_of(x):
-        val = torch.empty(*lead, k, dtype=x.dtype, device=x.device)
-        idx = torch.empty(*lead, k, dtype=torch.int64, device=x.device)
+    with _lib.device_of(logits):
+        x, N, ld = _rows(logits)
+        val = torch.empty((*lead, k), dtype=x.dtype, device=x.device)
+        idx = torch.empty((*lead, k), dtype=torch.int64, device=x.device)
         lse = torch.empty(lead, dtype=torch.float32, device=x.device)
         if N:
             rc = _lib.load().rwkv7_top_logits(
-                x.data_ptr(), LOGIT_DTYPES[x.dtype], _ld(x), N, V, k, temperature, val.data_ptr(), idx.data_ptr(),
-                lse.data_ptr(), _lib.stream_handle(),
+                x.data_ptr(), code, ld, N, V, k, temperature, val.data_ptr(), idx.data_ptr(), lse.data_ptr(), _lib.stream_of(x)
             )
             _lib.check(rc, "rwkv7_top_logits")
     return val, idx, lse
 
 
 def _distill(logits, top_val, top_idx, lse, temperature, scale, want_loss: bool, want_grad: bool):
-    _check_logits(logits, "logits")
-    lead, V = logits.shape[:-1], logits.shape[-1]
-    _need(top_val.ndim >= 1 and top_val.shape[:-1] == lead and top_idx.shape == top_val.shape,
-          lambda: f"top_val and top_idx must be [{', '.join(map(str, (*lead, 'K')))}], got {tuple(top_val.shape)} and "
-          f"{tuple(top_idx.shape)}")
-    K = top_val.shape[-1]
+    code = _check_logits(logits, "logits")
+    shape = logits.shape
+    lead, V = shape[:-1], shape[-1]
+    ts = top_val.shape
+    _need(ts[:-1] == lead and top_idx.shape == ts and len(ts) == len(shape),
+          lambda: f"top_val and top_idx must be [{', '.join(map(str, (*lead, 'K')))}], got {tuple(ts)} and {tuple(top_idx.shape)}")
+    K = ts[-1]
     _need(K <= MAX_ENTRIES, lambda: f"at most {MAX_ENTRIES} teacher entries per row, got {K}")
-    _need(top_val.dtype in LOGIT_DTYPES, lambda: f"top_val must be float16, bfloat16 or float32, got {top_val.dtype}")
-    _need(top_idx.dtype == torch.int64, lambda: f"top_idx must be int64, got {top_idx.dtype}")
-    _need(lse is None or (lse.shape == lead and lse.dtype == torch.float32), lambda: f"lse must be float32 {tuple(lead)}")
+    tcode = LOGIT_DTYPES.get(top_val.dtype)
+    _need(tcode is not None, lambda: f"top_val must be float16, bfloat16 or float32, got {top_val.dtype}")
+    _need(top_idx.dtype is torch.int64, lambda: f"top_idx must be int64, got {top_idx.dtype}")
+    _need(lse is None or (lse.shape == lead and lse.dtype is torch.float32), lambda: f"lse must be float32 {tuple(lead)}")
     rowwise = isinstance(scale, Tensor)
-    _need(not rowwise or (scale.shape == lead and scale.dtype == torch.float32), lambda: f"scale must be float32 {tuple(lead)}")
-    _same_device(logits, top_val=top_val, top_idx=top_idx, lse=lse, scale=scale if rowwise else None)
+    _need(not rowwise or (scale.shape == lead and scale.dtype is torch.float32), lambda: f"scale must be float32 {tuple(lead)}")
+    _same_device(logits, top_val, top_idx, lse, scale if rowwise else None)
     temperature = _temperature(temperature)
-    x = _dense(_rows(logits))
-    N = x.shape[0]
-    with _lib.device_of(x):
+    with _lib.device_of(logits):
+        x, N, ld = _rows(logits)
         loss = torch.empty(lead, dtype=torch.float32, device=x.device) if want_loss else None
-        grad = torch.empty(logits.shape, dtype=x.dtype, device=x.device) if want_grad else None
+        grad = torch.empty(shape, dtype=x.dtype, device=x.device) if want_grad else None
         if N and not K:  # no teacher at all
             for t in (loss, grad):
                 if t is not None:
@@ -130,9 +130,8 @@ def _distill(logits, top_val, top_idx, lse, temperature, scale, want_loss: bool,
             ls = None if lse is None else lse.contiguous()
             sc = scale.contiguous() if rowwise else None
             rc = _lib.load().rwkv7_distill(
-                x.data_ptr(), LOGIT_DTYPES[x.dtype], _ld(x), N, V, tv.data_ptr(), LOGIT_DTYPES[tv.dtype], ti.data_ptr(),
-                K, _lib.ptr(ls), temperature, _lib.ptr(sc), 1.0 if rowwise else float(scale), _lib.ptr(loss),
-                _lib.ptr(grad), V, _lib.stream_handle(),
+                x.data_ptr(), code, ld, N, V, tv.data_ptr(), tcode, ti.data_ptr(), K, _lib.ptr(ls), temperature,
+                _lib.ptr(sc), 1.0 if rowwise else float(scale), _lib.ptr(loss), _lib.ptr(grad), V, _lib.stream_of(x),
             )
             _lib.check(rc, "rwkv7_distill")
     return loss, grad
@@ -203,7 +202,7 @@ def verify_draft(
     at ``temperature``; with ``temperature`` None or <= 0 they are its greedy ones
     and ``uniforms`` is not read. NaN logits count as -inf; ids outside ``0..V-1``
     are rejected."""
-    _check_logits(target_logits, "target_logits")
+    code = _check_logits(target_logits, "target_logits")
     single = target_logits.ndim == 2
     up = (lambda t: None if t is None else t.unsqueeze(0)) if single else (lambda t: t)
     target, tokens, draft = up(target_logits), up(draft_tokens), up(draft_logits)
@@ -234,7 +233,7 @@ def verify_draft(
             draft = None
     if lengths is not None:
         _need(lengths.shape == (B,) and lengths.dtype == torch.int64, lambda: f"lengths must be int64 [{B}]")
-    _same_device(target, draft_tokens=tokens, uniforms=uniforms, draft_logits=draft, lengths=lengths)
+    _same_device(target, tokens, None if greedy else uniforms, draft, lengths)
     with _lib.device_of(target):
         out = torch.empty(B, K + 1, dtype=torch.int64, device=target.device)
         accepted = torch.empty(B, dtype=torch.int64, device=target.device)
@@ -249,9 +248,9 @@ def verify_draft(
             ws = torch.empty(nb, dtype=torch.uint8, device=target.device)
             rc = lib.rwkv7_verify(
                 t.data_ptr(), t.stride(0), t.stride(1) if K else V, _lib.ptr(d), 0 if d is None else d.stride(0),
-                V if d is None or K == 1 else d.stride(1), LOGIT_DTYPES[t.dtype], tok.data_ptr() if K else None,
+                V if d is None or K == 1 else d.stride(1), code, tok.data_ptr() if K else None,
                 _lib.ptr(u), _lib.ptr(n), B, K, V, temperature, draft_temperature, out.data_ptr(), accepted.data_ptr(),
-                ws.data_ptr(), nb, _lib.stream_handle(),
+                ws.data_ptr(), nb, _lib.stream_of(t),
             )
             _lib.check(rc, "rwkv7_verify")
     return (out[0], accepted[0]) if single else (out, accepted)

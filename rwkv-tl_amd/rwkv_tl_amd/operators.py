@@ -156,22 +156,41 @@ LOGITS_OPS: dict[str, tuple[str, Callable, Callable]] = {
 }
 
 
-def _distill_setup(ctx, inputs, output) -> None:
-    logits, top_val, top_idx, lse, temperature = inputs
-    if top_val.requires_grad or (lse is not None and lse.requires_grad):
-        raise ValueError("distill_loss has no gradient to the teacher: detach top_val and lse")
-    ctx.save_for_backward(logits, top_val, top_idx, lse)
-    ctx.temperature = temperature
+class _DistillLoss(torch.autograd.Function):
+    """The Autograd kernel of ``distill_loss``. (torch.library.register_autograd
+    makes one like it that takes 28 us more of a call's host time.)"""
+
+    @staticmethod
+    def forward(ctx, logits, top_val, top_idx, lse, temperature):
+        if ctx.needs_input_grad[1] or ctx.needs_input_grad[3]:
+            raise ValueError("distill_loss has no gradient to the teacher: detach top_val and lse")
+        ctx.save_for_backward(logits, top_val, top_idx, lse)
+        ctx.temperature = temperature
+        with torch._C._AutoDispatchBelowAutograd():
+            return torch.ops.rwkv_tl.distill_loss(logits, top_val, top_idx, lse, temperature)
+
+    @staticmethod
+    def backward(ctx, grad_loss):
+        args = (grad_loss, *ctx.saved_tensors, ctx.temperature)
+        # a plain backward pass calls the kernel; tracing, and a gradient that is to
+        # be differentiated, go through the operator
+        plain = type(grad_loss) is Tensor and grad_loss.is_cuda and not torch.is_grad_enabled()
+        return (K.distill_loss_backward if plain else torch.ops.rwkv_tl.distill_loss_backward)(*args), None, None, None, None
 
 
-def _distill_backward(ctx, grad_loss):
-    logits, top_val, top_idx, lse = ctx.saved_tensors
-    grad = torch.ops.rwkv_tl.distill_loss_backward(grad_loss, logits, top_val, top_idx, lse, ctx.temperature)
-    return grad, None, None, None, None
+class _DistillLossBackward(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, *args):
+        with torch._C._AutoDispatchBelowAutograd():
+            return torch.ops.rwkv_tl.distill_loss_backward(*args)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise NotImplementedError("distill_loss has no second derivative")
 
 
-def _distill_backward_twice(ctx, *_):
-    raise NotImplementedError("distill_loss has no second derivative")
+def _distill_autograd(logits, top_val, top_idx, lse=None, temperature=1.0):
+    return _DistillLoss.apply(logits, top_val, top_idx, lse, temperature)
 
 
 def _dplr_seq_setup(ctx, inputs, output) -> None:
@@ -201,8 +220,8 @@ def register() -> None:
     torch.library.register_autograd(
         f"{NAMESPACE}::fused_dplr_seq", _dplr_seq_backward, setup_context=_dplr_seq_setup
     )
-    torch.library.register_autograd(f"{NAMESPACE}::distill_loss", _distill_backward, setup_context=_distill_setup)
-    torch.library.register_autograd(f"{NAMESPACE}::distill_loss_backward", _distill_backward_twice)
+    torch.library.impl(f"{NAMESPACE}::distill_loss", "Autograd")(_distill_autograd)
+    torch.library.impl(f"{NAMESPACE}::distill_loss_backward", "Autograd")(_DistillLossBackward.apply)
     _registered = True
 
 
