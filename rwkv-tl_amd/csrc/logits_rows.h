@@ -145,13 +145,11 @@ RWKV7_DEV float wave_max(float v) {
   return fmaxf(fmaxf(lane_value(v, 0), lane_value(v, 16)), fmaxf(lane_value(v, 32), lane_value(v, 48)));
 }
 
-// 2^y in 64 bits to 1.1e-12, y clamped to -2000 from below (0 there; NaN too): y
-// = n + f, |f| <= 1/2, 2^f by the polynomial of degree 8 that interpolates it at
-// the Chebyshev points. Fewer instructions and registers than the library's exp,
-// and nearer than any sum here needs.
-RWKV7_DEV double exp2_d(double y) {
-  y = fmax(y, -2000.0);
-  const double n = rint(y), f = y - n;
+// 2^f for |f| <= 1/2 in 64 bits, to 1.1e-12: the polynomial of degree 8 that
+// interpolates it at the Chebyshev points. exp2_d: 2^y, y clamped to -2000 from
+// below (0 there; NaN too). Fewer instructions and registers than the library's
+// exp, and nearer than any sum here needs.
+RWKV7_DEV double exp2_frac(double f) {
   double p = 1.3255224883682684e-06;
   p = fma(p, f, 1.5310079402211905e-05);
   p = fma(p, f, 0.00015403455852430636);
@@ -161,7 +159,12 @@ RWKV7_DEV double exp2_d(double y) {
   p = fma(p, f, 0.2402265069581299);
   p = fma(p, f, 0.6931471805459335);
   p = fma(p, f, 1.0);
-  return ldexp(p, (int)n);
+  return p;
+}
+RWKV7_DEV double exp2_d(double y) {
+  y = fmax(y, -2000.0);
+  const double n = rint(y);
+  return ldexp(exp2_frac(y - n), (int)n);
 }
 // 1 / x in 64 bits: the hardware's estimate and two Newton steps (0 -> inf).
 RWKV7_DEV double rcp_d(double x) {

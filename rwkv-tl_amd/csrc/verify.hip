@@ -25,9 +25,9 @@
 // verify_stats_kernel: a slice of a row per workgroup: its largest logit and the
 //   sum of the exponentials about it, for target rows also of each 512 logits
 //   (greedy: largest logit and its first id).
-// verify_rest_kernel: a slice of each sequence's decisive row: every workgroup
+// verify_rest_kernel: 2048 logits of each sequence's decisive row: every workgroup
 //   joins the sums of its sequence's rows and decides how many tokens are
-//   accepted; the sums of max(p - q, 0) over each 512 logits of the slice.
+//   accepted; the sums of max(p - q, 0) over each 512 of its logits.
 // verify_draw_kernel: one wave per sequence: finds the 512 in which the running
 //   sum crosses, and in them the token.
 #include "logits_rows.h"
@@ -80,8 +80,27 @@ struct Weight {
   RWKV7_DEV Weight(float largest, double k_)
       : m(largest > -kInf ? largest : __builtin_nanf("")), ref(largest > -kInf ? (double)largest : 0.0), k(k_) {}
   // (the difference first: k x - k m would lose it at the types' lowest values)
-  RWKV7_DEV double finite(float x) const { return exp2_d(((double)x - ref) * k); }  // no +inf in the row
-  RWKV7_DEV double operator()(float x) const { return x == m ? 1.0 : finite(x); }
+  RWKV7_DEV double operator()(float x) const { return x == m ? 1.0 : exp2_d(((double)x - ref) * k); }
+};
+
+// The same in bulk, for rows whose largest logit is of ordinary size (so that the
+// rounding of `least` is less than one in y): the power's
+// whole part is added to the exponent's bits as it stands in the low word of y +
+// 1.5 2^52, in place of a rounding, a conversion and a scaling. Below 2^-1000 it
+// stays there instead of 0: sums under kNothing have nothing in them.
+constexpr double kNothing = 0x1p-900;
+struct BulkWeight {
+  float least;
+  double ref, k;
+  static RWKV7_DEV bool serves(float m, double k) { return fabs((double)m) * k <= 0x1p20 && k >= 0x1p-60; }
+  RWKV7_DEV BulkWeight(float m, double k_) : least((float)((double)m - 1000.0 / k_)), ref(m), k(k_) {}
+  RWKV7_DEV double operator()(float x) const {
+    const double d = (double)fmaxf(x, least) - ref, magic = 0x1.8p52;
+    const double t = fma(d, k, magic), f = fma(d, k, magic - t);
+    const u64 p = __builtin_bit_cast(u64, exp2_frac(f));
+    const uint32_t n = (uint32_t)__builtin_bit_cast(u64, t);
+    return __builtin_bit_cast(double, p + ((u64)(n << 20) << 32));
+  }
 };
 
 RWKV7_DEV int drafted(const VerifyArgs &a, int b) {
@@ -164,8 +183,8 @@ __global__ __launch_bounds__(kVerThreads) void verify_stats_kernel(VerifyArgs a)
         sum += q;
       }
     };
-    if (m < kInf) add([&](float v) { return w.finite(v); });
-    else add([&](float v) { return w(v); });
+    if (BulkWeight::serves(m, w.k)) add(BulkWeight(m, w.k));
+    else add(w);
   }
   if (lane == 0) s_sum[wv] = sum;
   __syncthreads();
@@ -187,11 +206,12 @@ struct DecideLds {
 // joined, a thread per slice, then a lane per drafted token.
 template <int FMT>
 RWKV7_DEV void decide(const VerifyArgs &a, int b, DecideLds &s) {
-  const int t = threadIdx.x, len = drafted(a, b);
-  // the drafted tokens' logits, wanted below
+  const int t = threadIdx.x;
+  // Every row's sums and every token, also those that the length leaves out
+  // (their sums are not written): no load here waits for the length.
   float zp = -kInf, zq = -kInf, u = 0.f;
   int64_t x = -1;
-  if (t < len) {
+  if (t < a.K) {
     x = a.tok[(int64_t)b * a.K + t];
     u = a.u[(int64_t)b * (a.K + 1) + t];
     if (x >= 0 && x < a.V) {
@@ -201,24 +221,21 @@ RWKV7_DEV void decide(const VerifyArgs &a, int b, DecideLds &s) {
       x = -1;
     }
   }
-  for (int which = 0; which < (a.draft ? 2 : 1); ++which) {
-    const int rows = which ? len : len + 1;
-    const int64_t r0 = which ? (int64_t)a.B * (a.K + 1) + (int64_t)b * a.K : (int64_t)b * (a.K + 1);
-    const double k = which ? a.kd : a.kt;
-    for (int i = t; i < rows * kMaxSlices; i += kVerThreads) {  // (whole groups of eight lanes)
-      const int row = i / kMaxSlices, g = i % kMaxSlices;
-      const int64_t at = (r0 + row) * a.G + g;
-      const float mg = g < a.G ? a.m[at] : -kInf;
-      float m = mg;
-      m = fmaxf(m, dpp<kDppXor1>(m));
-      m = fmaxf(m, dpp<kDppXor2>(m));
-      m = fmaxf(m, dpp<kDppHalfMirror>(m));
-      double S = g < a.G && mg > -kInf ? a.sum[at] * Weight(m, k)(mg) : 0.0;
-      S += dpp_d<kDppXor1>(S);
-      S += dpp_d<kDppXor2>(S);
-      S += dpp_d<kDppHalfMirror>(S);
-      if (g == 0) s.m[which][row] = m, s.S[which][row] = S;
-    }
+  const int len = drafted(a, b), rows = 2 * a.K + 1;
+  for (int i = t; i < (a.draft ? rows : a.K + 1) * kMaxSlices; i += kVerThreads) {  // (whole groups of eight lanes)
+    const int r = i / kMaxSlices, g = i % kMaxSlices, which = r > a.K, row = which ? r - a.K - 1 : r;
+    const int64_t at = (which ? (int64_t)a.B * (a.K + 1) + (int64_t)b * a.K + row : (int64_t)b * (a.K + 1) + row) * a.G + g;
+    const float mg = g < a.G ? a.m[at] : -kInf;
+    const double sum = g < a.G ? a.sum[at] : 0.0;
+    float m = mg;
+    m = fmaxf(m, dpp<kDppXor1>(m));
+    m = fmaxf(m, dpp<kDppXor2>(m));
+    m = fmaxf(m, dpp<kDppHalfMirror>(m));
+    double S = mg > -kInf ? sum * Weight(m, which ? a.kd : a.kt)(mg) : 0.0;
+    S += dpp_d<kDppXor1>(S);
+    S += dpp_d<kDppXor2>(S);
+    S += dpp_d<kDppHalfMirror>(S);
+    if (g == 0) s.m[which][row] = m, s.S[which][row] = S;
   }
   __syncthreads();
   if (t < kWave) {
@@ -271,33 +288,24 @@ __global__ __launch_bounds__(kVerThreads) void verify_rest_kernel(VerifyArgs a) 
   if (g == 0 && t == 0) a.dec[b] = d;
   if (!d.rejected) return;
   const void *pr = target_row<FMT>(a, b, d.n), *qr = a.draft ? draft_row<FMT>(a, b, d.n) : pr;
-  const uint32_t n8 = (uint32_t)V / kRowChunk;
+  const uint32_t n8 = (uint32_t)V / kRowChunk, e8 = g * kVerThreads + t;
   const Residual res(a, d, false);
-  double *block = a.rest + (int64_t)b * (a.G * kBlocks + 1) + g * kBlocks;
-  Chunk<FMT> xp[kVerChunks], xq[kVerChunks];
+  double *block = a.rest + (int64_t)b * (a.G * kBlocks + 1);
+  Chunk<FMT> xp, xq;
+  xp.load(pr, e8, n8);
+  xq.load(qr, e8, n8);
+  float fp[kRowChunk], fq[kRowChunk];
+  xp.get(fp);
+  xq.get(fq);
+  double sum = 0.0;
 #pragma unroll
-  for (int c = 0; c < kVerChunks; ++c) {
-    xp[c].load(pr, (g * kVerChunks + c) * kVerThreads + t, n8);
-    xq[c].load(qr, (g * kVerChunks + c) * kVerThreads + t, n8);
-  }
-#pragma unroll 1
-  for (int c = 0; c < kVerChunks; ++c) {
-    float fp[kRowChunk], fq[kRowChunk];
-    xp[0].get(fp);
-    xq[0].get(fq);
-#pragma unroll
-    for (int i = 0; i + 1 < kVerChunks; ++i) xp[i] = xp[i + 1], xq[i] = xq[i + 1];  // (registers have no index)
-    const int i0 = ((g * kVerChunks + c) * kVerThreads + t) * kRowChunk;
-    double sum = 0.0;
-#pragma unroll
-    for (int e = 0; e < kRowChunk; ++e) sum += res(fp[e], fq[e], i0 + e);
-    sum = wave_sum_d(sum);
-    if (lane == 0) block[c * kVerWaves + wv] = sum;
-  }
-  if (g == a.G - 1 && wv == 0) {
+  for (int e = 0; e < kRowChunk; ++e) sum += res(fp[e], fq[e], (int)e8 * kRowChunk + e);
+  sum = wave_sum_d(sum);
+  if (lane == 0) block[g * kVerWaves + wv] = sum;
+  if (g == a.G * kVerChunks - 1 && wv == 0) {  // the logits behind the eights
     const int id = (int)n8 * kRowChunk + t;
-    const double sum = wave_sum_d(id < V ? res(load_logit<FMT>(pr, id), load_logit<FMT>(qr, id), id) : 0.0);
-    if (lane == 0) block[kBlocks] = sum;
+    sum = wave_sum_d(id < V ? res(load_logit<FMT>(pr, id), load_logit<FMT>(qr, id), id) : 0.0);
+    if (lane == 0) block[a.G * kBlocks] = sum;
   }
 }
 
@@ -336,7 +344,8 @@ __global__ __launch_bounds__(kWave) void verify_draw_kernel(VerifyArgs a) {
 #pragma unroll
     for (int e = 0; e < kDrawE; ++e) {
       const int i = kDrawE * lane + e, g = min(i / kBlocks, a.G - 1);
-      w[e] = i < blocks ? a.block[r * blocks + i] * (weight(a.m[r * a.G + g]) * d.ip) : 0.0;
+      const double sum = i < blocks ? a.block[r * blocks + i] : 0.0;
+      w[e] = sum > kNothing ? sum * (weight(a.m[r * a.G + g]) * d.ip) : 0.0;
     }
   }
   double own = (w[0] + w[1]) + w[2];
@@ -446,7 +455,7 @@ int launch_verify(const VerifyArgs &a, hipStream_t st) {
   }
   verify_stats_kernel<FMT, false><<<grid, kVerThreads, 0, st>>>(a);
   RWKV7_CHECK_LAUNCH();
-  verify_rest_kernel<FMT><<<dim3(a.G, a.B), kVerThreads, 0, st>>>(a);
+  verify_rest_kernel<FMT><<<dim3(a.G * kVerChunks, a.B), kVerThreads, 0, st>>>(a);
   RWKV7_CHECK_LAUNCH();
   verify_draw_kernel<FMT><<<a.B, kWave, 0, st>>>(a);
   RWKV7_CHECK_LAUNCH();
