@@ -18,7 +18,7 @@
 // log-softmax.
 //
 // 1 - Q is never formed as a difference: the row's elements in I are taken out
-// (a bitmap of the vocabulary in LDS marks them) before the sum, which is about
+// (each thread has a word in LDS that marks them) before the sum, which is about
 // their own largest, and I enters through the entries. The row stays in registers between the sum and the
 // gradient, so a pass reads the logits once and writes the gradient once; the
 // entries' own gradients are stored over it after a barrier.
@@ -49,8 +49,18 @@ struct DistillArgs {
   int64_t grad_ld;
 };
 
+struct Joined {
+  float m, mrest;       // largest logit of the row, and without the entries' ids
+  double S, Srest;      // sums about them
+  double in_all;        // what a sum about mrest counts in one about m
+  double W, tref;       // the teacher's mass about its reference
+  double P, rest_t;
+  bool mass;
+};
+
 struct DistillLds {
-  uint32_t bits[kRowMaxV / 32];
+  u64 mine[kRowMaxThreads];  // of each thread's logits, bit 8 c + e for chunk c: those with an entry
+  uint32_t tail;             // of the logits behind the eights
   int idx[kDistMaxK];
   float p[kDistMaxK];
   // per wave: the largest logit and the sum about it of the row's rest and of
@@ -59,6 +69,8 @@ struct DistillLds {
   float mrest[kMaxWaves], rest[kMaxWaves], mtop[kMaxWaves], top[kMaxWaves];
   double tref[kMaxWaves], tw[kMaxWaves], ta[kMaxWaves];
   bool whole;  // every id of the vocabulary has an entry
+  Joined j;
+  float f_rest, f_top, ua;
 };
 
 template <int FMT, int THREADS>
@@ -69,16 +81,8 @@ RWKV7_DEV void zero_row(char *dst, int V) {
   if (threadIdx.x < V % kRowChunk) store_logit<FMT>(dst, V / kRowChunk * kRowChunk + threadIdx.x, 0.f);
 }
 
-// The waves' parts joined, one a lane, by every wave for itself. Logarithms and
-// the teacher's references are to base 2.
-struct Joined {
-  float m, mrest;       // largest logit of the row, and without the entries' ids
-  double S, Srest;      // sums about them
-  double in_all;        // what a sum about mrest counts in one about m
-  double W, tref;       // the teacher's mass about its reference
-  double P, rest_t;
-  bool mass;
-};
+// The waves' parts joined by one wave, one a lane. Logarithms and the teacher's
+// references are to base 2.
 template <int WAVES>
 RWKV7_DEV Joined join(const DistillArgs &g, const DistillLds &s, int lane, double lse) {
   Joined j;
@@ -121,12 +125,12 @@ RWKV7_DEV void put_loss(const DistillArgs &g, const DistillLds &s, const Joined 
     A = s.tw[lane] != 0.0 ? f * (s.ta[lane] + s.tw[lane] * up) : 0.0;
   }
   A = wave_sum_d(A);
-  const double S = log2_d(j.S);
+  const double S = g.sc.off(j.m) + log2_d(j.S);
   double loss;
   if (g.lse) {
     loss = A + j.W * S;
     if (j.rest_t > 0.0)
-      loss += j.rest_t * (log2_d(j.rest_t) - ((g.sc.k * ((double)j.mrest - (double)j.m) + log2_d(j.Srest)) - S));
+      loss += j.rest_t * (log2_d(j.rest_t) - (g.sc.k * ((double)j.mrest - (double)j.m) + (g.sc.off(j.mrest) + log2_d(j.Srest)) - S));
   } else {
     loss = j.mass ? A * rcp_d(j.W) - log2_d(j.W) + S : 0.0;
   }
@@ -148,8 +152,8 @@ __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : 8) void distill_kernel(Dist
   const int64_t id64 = t < g.K ? g.top_idx[row * g.K + t] : -1;
   const bool there = id64 >= 0 && id64 < V;
   const int id = there ? (int)id64 : -1;
-#pragma unroll 1
-  for (int i = t; i < (V + 31) / 32; i += THREADS) s.bits[i] = 0u;
+  s.mine[t] = 0;
+  if (t == 0) s.tail = 0u;
   const bool some = __syncthreads_or(there);
   if (!some) {
     if (LOSS && t == 0) g.loss[row] = 0.f;
@@ -157,8 +161,7 @@ __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : 8) void distill_kernel(Dist
     return;
   }
   Chunk<FMT> x[kRowChunks];
-#pragma unroll
-  for (int c = 0; c < kRowChunks; ++c) x[c].load(src, c * THREADS + t, n8);
+  load_row<THREADS>(x, src, n8);
   const int tail = t < V % kRowChunk ? (int)n8 * kRowChunk + t : -1;  // this thread's logit behind the eights
   float xt = tail >= 0 ? load_logit<FMT>(src, tail) : -kInf;
   const float tv = there ? load_logit_rt(g.top_val, row * g.K + t, g.val_fmt) : -kInf;
@@ -167,7 +170,12 @@ __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : 8) void distill_kernel(Dist
 
   // mark the ids; `first`: this entry stands for its id
   bool first = there;
-  if (there) first = !(atomicOr(&s.bits[id >> 5], 1u << (id & 31)) & (1u << (id & 31)));
+  if (there) {
+    const uint32_t b = (uint32_t)id / kRowChunk, bit = b / THREADS * kRowChunk + id % kRowChunk;
+    uint32_t *word = b < n8 ? reinterpret_cast<uint32_t *>(&s.mine[b % THREADS]) + bit / 32 : &s.tail;
+    const uint32_t own = b < n8 ? 1u << bit % 32 : 1u << id % kRowChunk;
+    first = !(atomicOr(word, own) & own);
+  }
   const bool twice = __syncthreads_or(there && !first);
   if (twice) {  // the same id in several entries: the lowest stands for it
     s.idx[t] = id;
@@ -184,38 +192,30 @@ __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : 8) void distill_kernel(Dist
   }
 
   // this thread's part of the row without the entries' ids
-  if (tail >= 0 && ((s.bits[tail >> 5] >> (tail & 31)) & 1u)) xt = -kInf;
-  float m = xt;
+  const u64 mine = s.mine[t];
+  if (mine) {
 #pragma unroll
-  for (int c = 0; c < kRowChunks; ++c) {
-    const uint32_t b = c * THREADS + t;
-    const uint32_t marked = b < n8 ? reinterpret_cast<const uint8_t *>(s.bits)[b] : 0u;
-    if (marked) x[c].remove(marked);
-    float f[kRowChunk];
-    x[c].get(f);
-#pragma unroll
-    for (int e = 0; e < kRowChunk; ++e) m = fmaxf(m, f[e]);
+    for (int c = 0; c < kRowChunks; ++c) x[c].remove((uint32_t)(mine >> (kRowChunk * c)) & 255u);
   }
-  m = wave_max(m);
-  const float R = ExpScale::ref(m), mtop = wave_max(zv);
-  float rest = g.sc.e(xt, R);
+  if (tail >= 0 && (s.tail >> t) & 1u) xt = -kInf;
+  float m;
+  {
+    RowMax<FMT> most;
 #pragma unroll
-  for (int c = 0; c < kRowChunks; ++c) {
-    float f[kRowChunk];
-    x[c].get(f);
-    float q[kRowChunk];
-#pragma unroll
-    for (int e = 0; e < kRowChunk; ++e) q[e] = g.sc.e(f[e], R);
-    rest += ((q[0] + q[1]) + (q[2] + q[3])) + ((q[4] + q[5]) + (q[6] + q[7]));
+    for (int c = 0; c < kRowChunks; ++c) most.add(x[c]);
+    m = wave_max(fmaxf(most.value(), xt));
   }
-  const float own = there ? g.sc.e(zv, ExpScale::ref(mtop)) : 0.f;  // exp of the entry's student logit
+  opaque_row(x);
+  const bool entries = wv * kWave < g.K;  // this wave has entries
+  const float mtop = entries ? wave_max(zv) : -kInf, rest = sum_row(x, xt, g.sc, m);
+  const float own = there ? g.sc.e(zv, mtop) : 0.f;  // exp of the entry's student logit
   const float2 sums = wave_sum2(rest, first ? own : 0.f);
 
   // the teacher's entries, about its lse or the wave's largest, in 64 bits and
   // powers of two
   const double k2 = g.sc.k;
   double tref = lse, w = 0.0;
-  if (wv * kWave < g.K) {
+  if (entries) {
     if (!g.lse) tref = k2 * (double)wave_max(tv);
     const double y = k2 * (double)tv - tref;  // (NaN stays NaN)
     w = there && tv != -kInf ? (y == y ? exp2_d(y) : y) : 0.0;
@@ -226,34 +226,44 @@ __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : 8) void distill_kernel(Dist
   if (lane == 0) s.mrest[wv] = m, s.rest[wv] = sums.x, s.mtop[wv] = mtop, s.top[wv] = sums.y;
   __syncthreads();
 
-  const Joined j = join<kWaves>(g, s, lane, lse);
-  if (!GRAD) {
-    if (wv == 0) put_loss(g, s, j, lane, lse, row);
-    return;
+  if (wv == 0) {
+    const Joined j = join<kWaves>(g, s, lane, lse);
+    if (!GRAD) {
+      put_loss(g, s, j, lane, lse, row);
+      return;
+    }
+    // d loss / d z, scaled: f_rest e for the rest, f_top e - ua p for the entries
+    const double ua = j.mass ? (double)up * g.a : 0.0, all = ua * (j.P + j.rest_t) * rcp_d(j.S);
+    if (lane == 0) {
+      s.j = j;
+      s.ua = (float)ua;
+      s.f_top = (float)all;
+      s.f_rest = (float)(all * j.in_all - (j.rest_t > 0.0 && j.Srest > 0.0 ? ua * j.rest_t * rcp_d(j.Srest) : 0.0));
+    }
   }
-
-  // d loss / d z, scaled: f_rest e for the rest, f_top e - ua p for the entries
-  const double ua = uniform_d(j.mass ? (double)up * g.a : 0.0);
-  if (ua == 0.0) {  // a row that counts for nothing: zeros, not 0 * NaN
+  if (!GRAD) return;
+  __syncthreads();
+  const float ua = uniform_f(s.ua), f_rest = uniform_f(s.f_rest);
+  if (ua == 0.f) {  // a row that counts for nothing: zeros, not 0 * NaN
     zero_row<FMT, THREADS>(dst, V);
-    if (LOSS && wv == 0) put_loss(g, s, j, lane, lse, row);
+    if (LOSS && wv == 0) put_loss(g, s, s.j, lane, lse, row);
     return;
   }
-  const double all = ua * (j.P + j.rest_t) * rcp_d(j.S);
-  const float f_top = uniform_f((float)all);
-  const float f_rest = uniform_f((float)(all * j.in_all - (j.rest_t > 0.0 && j.Srest > 0.0 ? ua * j.rest_t * rcp_d(j.Srest) : 0.0)));
-  float pk = (float)(ua * (g.lse ? w : w * exp2_d(tref - j.tref) * rcp_d(j.W)));
-  const float mrest = uniform_f(ExpScale::ref(j.mrest));
+  float pk = entries ? ua * (float)(g.lse ? w : w * exp2_d(tref - s.j.tref) * rcp_d(s.j.W)) : 0.f;
+  opaque_row(x);
+  g.sc.with(s.j.mrest, [&](auto e2, auto far) {
 #pragma unroll
-  for (int c = 0; c < kRowChunks; ++c) {
-    float f[kRowChunk];
-    x[c].get(f);
+    for (int c = 0; c < kRowChunks; ++c) {
+      float f[kRowChunk];
+      x[c].template get<decltype(far)::value>(f);
 #pragma unroll
-    for (int e = 0; e < kRowChunk; ++e) f[e] = f_rest * g.sc.e(f[e], mrest);
-    const uint32_t b = c * THREADS + t;
-    if (b < n8) store_chunk<FMT>(dst, b, f);
-  }
-  if (tail >= 0) store_logit<FMT>(dst, tail, f_rest * g.sc.e(xt, mrest));
+      for (int e = 0; e < kRowChunk; ++e) f[e] = f_rest * e2(f[e]);
+      const uint32_t b = c * THREADS + t;
+      if ((c + 1) * THREADS <= n8) store_chunk<FMT>(dst, b, f);
+      else if (b < n8) store_chunk<FMT>(dst, b, f);
+    }
+    if (tail >= 0) store_logit<FMT>(dst, tail, f_rest * e2(xt));
+  });
   if (twice) {
     s.p[t] = there ? pk : 0.f;
     __syncthreads();
@@ -263,9 +273,8 @@ __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : 8) void distill_kernel(Dist
     pk = (float)sum;
   }
   __syncthreads();  // the row's own stores come before the entries'
-  if (first) store_logit<FMT>(dst, id, f_top * g.sc.e(zv, j.m) - pk);
-  // joined once more, so that nothing of it is held beside the row
-  if (LOSS && wv == 0) put_loss(g, s, join<kWaves>(g, s, lane, lse), lane, lse, row);
+  if (first) store_logit<FMT>(dst, id, s.f_top * g.sc.e(zv, s.j.m) - pk);
+  if (LOSS && wv == 0) put_loss(g, s, s.j, lane, lse, row);
 }
 
 template <int FMT, int THREADS>

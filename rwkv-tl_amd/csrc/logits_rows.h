@@ -55,20 +55,34 @@ struct Chunk {
 #pragma unroll
     for (int i = 0; i < kWords; ++i) w[i] = F32 ? 0xff800000u : FMT == 2 ? 0xff80ff80u : 0xfc00fc00u;  // -inf
   }
+  RWKV7_DEV void load_whole(const void *row, uint32_t b) {
+    __builtin_memcpy(w, static_cast<const char *>(row) + b * (uint32_t)(kRowChunk * kLogitBytes<FMT>), sizeof w);
+  }
   // the b-th eight of a row with n8 whole ones, -inf past them
   RWKV7_DEV void load(const void *row, uint32_t b, uint32_t n8) {
     fill_absent();
-    if (b < n8) __builtin_memcpy(w, static_cast<const char *>(row) + b * (uint32_t)(kRowChunk * kLogitBytes<FMT>), sizeof w);
+    if (b < n8) load_whole(row, b);
   }
-  // The eight as f32. The compiler would otherwise keep a row's unpacked values
-  // from one pass to the next, which the registers of the larger workgroups do
-  // not hold: each pass unpacks an opaque copy.
-  RWKV7_DEV void get(float (&f)[kRowChunk]) {
+  // The compiler would otherwise keep a row's unpacked values from one pass to the
+  // next, which the registers of the larger workgroups do not hold: between two
+  // passes the chunks are made opaque.
+  RWKV7_DEV void opaque() {
 #pragma unroll
     for (int i = 0; i < kWords; ++i) asm volatile("" : "+v"(w[i]));
+  }
+  // the eight as f32. FAR: by byte permutes, for the far arm of ExpScale::with: code
+  // that both arms had alike would be moved before the branch, a row's worth.
+  template <bool FAR = false>
+  RWKV7_DEV void get(float (&f)[kRowChunk]) const {
     if constexpr (F32) {
 #pragma unroll
       for (int e = 0; e < kRowChunk; ++e) f[e] = __uint_as_float(w[e]);
+    } else if constexpr (FAR && FMT == 2) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        f[2 * i] = __uint_as_float(__builtin_amdgcn_perm(w[i], 0u, 0x05040c0cu));
+        f[2 * i + 1] = __uint_as_float(__builtin_amdgcn_perm(w[i], 0u, 0x07060c0cu));
+      }
     } else {
       F16T<FMT == 2>::to_f8(make_uint4(w[0], w[1], w[2], w[3]), f);
     }
@@ -89,6 +103,44 @@ struct Chunk {
     }
   }
 };
+
+// The largest of some chunks' logits, NaN left out: halves in pairs.
+template <int FMT>
+struct RowMax {
+  float m = -kInf;
+  RWKV7_DEV void add(const Chunk<FMT> &x) {
+    float f[kRowChunk];
+    x.get(f);
+#pragma unroll
+    for (int e = 0; e < kRowChunk; ++e) m = fmaxf(m, f[e]);
+  }
+  RWKV7_DEV float value() const { return m; }
+};
+template <>
+struct RowMax<0> {
+  half2v m = {(_Float16)-kInf, (_Float16)-kInf};
+  RWKV7_DEV void add(const Chunk<0> &x) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(half2v, x.w[i]));
+  }
+  RWKV7_DEV float value() const { return fmaxf((float)m[0], (float)m[1]); }
+};
+
+// A workgroup's row: whole eights without a comparison where all threads have one.
+template <int THREADS, int FMT>
+RWKV7_DEV void load_row(Chunk<FMT> (&x)[kRowChunks], const void *row, uint32_t n8) {
+#pragma unroll
+  for (int c = 0; c < kRowChunks; ++c) {
+    const uint32_t b = c * THREADS + threadIdx.x;
+    if ((c + 1) * THREADS <= n8) x[c].load_whole(row, b);
+    else x[c].load(row, b, n8);
+  }
+}
+template <int FMT>
+RWKV7_DEV void opaque_row(Chunk<FMT> (&x)[kRowChunks]) {
+#pragma unroll
+  for (int c = 0; c < kRowChunks; ++c) x[c].opaque();
+}
 
 // Eight values as the b-th eight of a row.
 template <int FMT>
@@ -185,8 +237,17 @@ RWKV7_DEV double log2_d(double x) {
   return fabs(y) < 2.0 ? (double)ex + (y + (f * exp2_d(-y) - 1.0) * 1.4426950408889634) : y;
 }
 
-// exp(a x) over a row as powers of two about its largest logit, 2^((x - m) kf):
-// a row of any size, the types' lowest values included, has a sum of 1 or more.
+template <bool B>
+struct BoolConst {
+  static constexpr bool value = B;
+};
+
+// exp(a x) over a row as powers of two about its largest logit m. Near 0 (|m kf|
+// up to 2^20) about R, the float nearest to m kf: 2^(x kf - R), one fma an
+// element; what R and kf lack of m k is common to the row and made up for by off()
+// and in log2z(). Farther away R's rounding would be more than the logits'
+// differences, and the difference is taken first: 2^((x - m) kf). So a row of any
+// size, the types' lowest values included, has a sum of about 1 or more.
 struct ExpScale {
   float kf;    // a log2(e) in float
   double k;    // the same in 64 bits
@@ -196,13 +257,53 @@ struct ExpScale {
   }
   // m: -inf for none, which any finite reference serves
   static RWKV7_DEV float ref(float m) { return m > -kInf ? m : 0.f; }
-  RWKV7_DEV float e(float x, float m) const { return __builtin_amdgcn_exp2f((x - m) * kf); }
+  RWKV7_DEV bool near(float m) const { return fabsf(ref(m) * kf) <= 1048576.f; }
+  RWKV7_DEV float e_near(float x, float R) const { return __builtin_amdgcn_exp2f(fmaf(x, kf, -R)); }
+  RWKV7_DEV float e_far(float x, float m) const { return __builtin_amdgcn_exp2f((x - m) * kf); }
+  RWKV7_DEV float e(float x, float m) const {
+    m = ref(m);
+    return near(m) ? e_near(x, m * kf) : e_far(x, m);
+  }
+  // body(f, far), f(x) = e(x, m), with the choice made once (m wave-uniform)
+  template <class Body>
+  RWKV7_DEV void with(float m, Body body) const {
+    m = uniform_f(ref(m));
+    if (near(m)) {
+      const float R = m * kf;
+      body([&](float x) { return e_near(x, R); }, BoolConst<false>());
+    } else {
+      body([&](float x) { return e_far(x, m); }, BoolConst<true>());
+    }
+  }
+  // what a sum about m has over one about m exactly, as a power of two
+  RWKV7_DEV double off(float m) const {
+    m = ref(m);
+    return near(m) ? (double)(m * kf) - (double)m * (double)kf : 0.0;
+  }
   // the share of a part about m in a sum about a larger one (0 for none)
   RWKV7_DEV double part(float m, float larger) const {
-    return m > -kInf ? exp2_d(((double)m - (double)larger) * k) : 0.0;
+    return m > -kInf ? exp2_d(((double)m - (double)larger) * (double)kf + (off(m) - off(larger))) : 0.0;
   }
   // log2 of sum exp(a x) when the sum about m is S
-  RWKV7_DEV double log2z(double S, float m) const { return (double)m * k + log2_d(S); }
+  RWKV7_DEV double log2z(double S, float m) const { return (double)m * k + off(m) + log2_d(S); }
 };
+
+// Sum of exp(a x) about m over a thread's chunks.
+template <int FMT>
+RWKV7_DEV float sum_row(const Chunk<FMT> (&x)[kRowChunks], float tail, const ExpScale &sc, float m) {
+  float sum;
+  sc.with(m, [&](auto e2, auto far) {
+    sum = e2(tail);
+#pragma unroll
+    for (int c = 0; c < kRowChunks; ++c) {
+      float f[kRowChunk], q[kRowChunk];
+      x[c].template get<decltype(far)::value>(f);
+#pragma unroll
+      for (int e = 0; e < kRowChunk; ++e) q[e] = e2(f[e]);
+      sum += ((q[0] + q[1]) + (q[2] + q[3])) + ((q[4] + q[5]) + (q[6] + q[7]));
+    }
+  });
+  return sum;
+}
 
 }  // namespace rwkv7

@@ -143,8 +143,7 @@ __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : THREADS == 256 ? 7 : 8) voi
   const int64_t row = blockIdx.x;
   const char *src = static_cast<const char *>(g.logits) + row * g.ld * kLogitBytes<FMT>;
   Chunk<FMT> x[kRowChunks];
-#pragma unroll
-  for (int c = 0; c < kRowChunks; ++c) x[c].load(src, c * THREADS + t, n8);
+  load_row<THREADS>(x, src, n8);
   const int tail = t < V % kRowChunk ? (int)n8 * kRowChunk + t : -1;
   const float xt = tail >= 0 ? load_logit<FMT>(src, tail) : -kInf;
   if (t == 0) s.n = 0;
@@ -155,20 +154,17 @@ __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : THREADS == 256 ? 7 : 8) voi
   float m = -kInf;
   uint32_t own[kGroups];
   {
-    float mg[kGroups] = {xt, -kInf, -kInf, -kInf};
+    RowMax<FMT> most[kGroups];
 #pragma unroll
-    for (int c = 0; c < kRowChunks; ++c) {
-      float f[kRowChunk];
-      x[c].get(f);
-#pragma unroll
-      for (int e = 0; e < kRowChunk; ++e) mg[c % kGroups] = fmaxf(mg[c % kGroups], f[e]);
-    }
+    for (int c = 0; c < kRowChunks; ++c) most[c % kGroups].add(x[c]);
 #pragma unroll
     for (int i = 0; i < kGroups; ++i) {
-      own[i] = mg[i] > -kInf ? top_key(mg[i]) : 0u;
-      m = fmaxf(m, mg[i]);
+      const float mg = i == 0 ? fmaxf(most[0].value(), xt) : most[i].value();
+      own[i] = mg > -kInf ? top_key(mg) : 0u;
+      m = fmaxf(m, mg);
     }
   }
+  opaque_row(x);
   auto wave_floor = [&](int r) {
     const uint32_t lo = own[0] > own[1] ? own[0] : own[1], hi = own[2] > own[3] ? own[2] : own[3], one[1] = {lo > hi ? lo : hi};
     return r > 16 ? rth_key(own, r) : rth_key(one, r);
@@ -181,33 +177,29 @@ __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : THREADS == 256 ? 7 : 8) voi
     if (lane == 0) s.floor[wv] = fl, s.some[wv] = some;
   }
   m = wave_max(m);
-  const float R = ExpScale::ref(m);
-  float sum = g.sc.e(xt, R);
-#pragma unroll
-  for (int c = 0; c < kRowChunks; ++c) {
-    float f[kRowChunk];
-    x[c].get(f);
-    float q[kRowChunk];
-#pragma unroll
-    for (int e = 0; e < kRowChunk; ++e) q[e] = g.sc.e(f[e], R);
-    sum += ((q[0] + q[1]) + (q[2] + q[3])) + ((q[4] + q[5]) + (q[6] + q[7]));
-  }
-  sum = wave_sum(sum);
+  const float sum = wave_sum(sum_row(x, xt, g.sc, m));
+  opaque_row(x);
   if (lane == 0) s.m[wv] = m, s.sum[wv] = sum;
   __syncthreads();
 
-  uint32_t fl = s.floor[0];
-  int full = 0;  // waves with 64 maxima or more
+  // the least floor, and the waves with 64 maxima or more, one a lane
+  auto least_floor = [&]() {
+    uint32_t f = lane < kWaves ? s.floor[lane] : ~0u;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) fl = min(fl, s.floor[w]), full += s.some[w] >= kWave;
+    for (int d = 1; d < kMaxWaves; d <<= 1) {
+      const uint32_t o = (uint32_t)__shfl_xor((int)f, d);
+      f = o < f ? o : f;
+    }
+    return (uint32_t)__builtin_amdgcn_readfirstlane((int)f);
+  };
+  uint32_t fl = least_floor();
+  const int full = __popcll(__ballot(lane < kWaves && s.some[lane] >= kWave));
   if (fl == 0u && k <= full * kWave) {  // (block-uniform)
     const uint32_t f = s.some[wv] >= kWave ? rth_key(own, (k + full - 1) / full) : ~0u;
     __syncthreads();
     if (lane == 0) s.floor[wv] = f;
     __syncthreads();
-    fl = ~0u;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) fl = min(fl, s.floor[w]);
+    fl = least_floor();
   }
 
   auto gather = [&](uint32_t key, int id) {
@@ -258,9 +250,7 @@ __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : THREADS == 256 ? 7 : 8) voi
   }
 
   // keys from `low` up, in bins of 2^shift, the highest first
-  float mm = s.m[0];
-#pragma unroll
-  for (int w = 1; w < kWaves; ++w) mm = fmaxf(mm, s.m[w]);
+  const float mm = wave_max(lane < kWaves ? s.m[lane] : -kInf);
   const uint32_t low = fl, range = max(top_key(mm), 1u) - low;
   const int shift = max(0, 24 - __clz((int)(range | 1u)));
   auto bin_of = [&](u64 c) { return kBins - 1 - (int)(((uint32_t)(c >> 32) - low) >> shift); };

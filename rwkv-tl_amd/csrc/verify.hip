@@ -22,9 +22,9 @@
 // drafted token is rejected, and the next token falls to 0 if nothing is left to
 // draw from.
 //
-// verify_stats_kernel: a slice of a row per workgroup: its largest logit and the
-//   sum of the exponentials about it, for target rows also of each 512 logits
-//   (greedy: largest logit and its first id).
+// verify_stats_kernel: a slice of a row per workgroup: the sum of its
+//   exponentials, about 0 or its largest logit, for target rows also of each 512
+//   logits (greedy: largest logit and its first id).
 // verify_rest_kernel: 2048 logits of each sequence's decisive row: every workgroup
 //   joins the sums of its sequence's rows and decides how many tokens are
 //   accepted; the sums of max(p - q, 0) over each 512 of its logits.
@@ -50,9 +50,9 @@ static_assert(kMaxSlices * kBlocks + 1 <= kDrawE * kWave, "the draw's wave holds
 struct Decision {
   int n, rejected;  // accepted tokens; whether the next was drafted and rejected
   int x;            // the rejected token of a one-hot draft, else -1
-  float mp, mq;     // largest logits of the row behind the accepted tokens, of target and draft
+  float mp, mq;     // what the sums of the row behind the accepted tokens are about, of target and draft
   float pad;
-  double ip, iq;    // 1 / sum of its exponentials, 0 for an empty row or none
+  double ip, iq;    // 1 / those sums, 0 for an empty row or none
 };
 
 struct VerifyArgs {
@@ -69,13 +69,14 @@ struct VerifyArgs {
   double *block;               // [B (K + 1)][G kBlocks + 1] the same by blocks; last: the logits behind the eights
   double *rest;                // [B][G kBlocks + 1] sums of max(p - q, 0)
   Decision *dec;               // [B]
-  float *m;                    // [rows][G] largest logit; rows: B (K + 1) of the target, B K of the draft
+  float *m;                    // [rows][G] what a slice's sums are about: 0 or its largest logit (greedy: that); rows: B
+                               // (K + 1) of the target, B K of the draft
 };
 
-// The exponentials of a row about its largest logit m: 2^(k (x - m)). 1 at the
-// largest, also at +inf; 0 for -inf and NaN.
+// The exponentials of a row about m, 0 or its largest logit: 2^(k (x - m)), 1 at m,
+// also at +inf; 0 for -inf and NaN.
 struct Weight {
-  float m;         // NaN: nothing is the largest
+  float m;         // NaN: the row is empty
   double ref, k;
   RWKV7_DEV Weight(float largest, double k_)
       : m(largest > -kInf ? largest : __builtin_nanf("")), ref(largest > -kInf ? (double)largest : 0.0), k(k_) {}
@@ -83,19 +84,19 @@ struct Weight {
   RWKV7_DEV double operator()(float x) const { return x == m ? 1.0 : exp2_d(((double)x - ref) * k); }
 };
 
-// The same in bulk, for rows whose largest logit is of ordinary size (so that the
-// rounding of `least` is less than one in y): the power's
-// whole part is added to the exponent's bits as it stands in the low word of y +
-// 1.5 2^52, in place of a rounding, a conversion and a scaling. Below 2^-1000 it
-// stays there instead of 0: sums under kNothing have nothing in them.
-constexpr double kNothing = 0x1p-900;
+// The same in bulk, about 0: 2^(k x), which 64 bits hold for |k x| up to 1000, so
+// that a slice needs no pass for its largest. The power's whole part is added to
+// the exponent's bits as it stands in the low word of k x + 1.5 2^52. Logits
+// outside the range are moved to its ends: a sum over kMuch may hold some from
+// above, one under kNothing holds nothing else than some from below, and either
+// slice is summed again about its largest.
+constexpr double kNothing = 0x1p-900, kMuch = 0x1p999;
 struct BulkWeight {
-  float least;
-  double ref, k;
-  static RWKV7_DEV bool serves(float m, double k) { return fabs((double)m) * k <= 0x1p20 && k >= 0x1p-60; }
-  RWKV7_DEV BulkWeight(float m, double k_) : least((float)((double)m - 1000.0 / k_)), ref(m), k(k_) {}
+  float lo, hi;
+  double k;
+  RWKV7_DEV explicit BulkWeight(double k_) : lo((float)(-1000.0 / k_)), hi((float)(1000.0 / k_)), k(k_) {}
   RWKV7_DEV double operator()(float x) const {
-    const double d = (double)fmaxf(x, least) - ref, magic = 0x1.8p52;
+    const double d = (double)__builtin_amdgcn_fmed3f(x, lo, hi), magic = 0x1.8p52;  // (NaN: lo)
     const double t = fma(d, k, magic), f = fma(d, k, magic - t);
     const u64 p = __builtin_bit_cast(u64, exp2_frac(f));
     const uint32_t n = (uint32_t)__builtin_bit_cast(u64, t);
@@ -135,21 +136,19 @@ __global__ __launch_bounds__(kVerThreads) void verify_stats_kernel(VerifyArgs a)
   for (int c = 0; c < kVerChunks; ++c) x[c].load(row, (g * kVerChunks + c) * kVerThreads + t, n8);
   const int tail = g == a.G - 1 && t < V % kRowChunk ? (int)n8 * kRowChunk + t : -1;
   const float xt = tail >= 0 ? load_logit<FMT>(row, tail) : -kInf;
-  float m = fmaxf(xt, -kInf);  // (NaN loses)
+  auto largest = [&]() {  // of the slice (NaN loses)
+    RowMax<FMT> most;
 #pragma unroll
-  for (int c = 0; c < kVerChunks; ++c) {
-    float f[kRowChunk];
-    x[c].get(f);
+    for (int c = 0; c < kVerChunks; ++c) most.add(x[c]);
+    float m = wave_max(fmaxf(most.value(), xt));
+    if (lane == 0) s_m[wv] = m;
+    __syncthreads();
 #pragma unroll
-    for (int e = 0; e < kRowChunk; ++e) m = fmaxf(m, f[e]);
-  }
-  m = wave_max(m);
-  if (lane == 0) s_m[wv] = m;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kVerWaves; ++w) m = fmaxf(m, s_m[w]);
-  double sum = 0.0;
+    for (int w = 0; w < kVerWaves; ++w) m = fmaxf(m, s_m[w]);
+    return m;
+  };
   if (GREEDY) {
+    const float m = largest();
     int at = V;  // first id of the largest
 #pragma unroll
     for (int c = kVerChunks - 1; c >= 0; --c) {
@@ -161,36 +160,48 @@ __global__ __launch_bounds__(kVerThreads) void verify_stats_kernel(VerifyArgs a)
     }
     if (at == V && tail >= 0 && xt == m) at = tail;
     if (m == -kInf) at = V;  // nothing but -inf and NaN
-    sum = -wave_max_d(-(double)at);
-  } else {
-    const Weight w(m, tgt ? a.kt : a.kd);
-    double *block = tgt ? a.block + (int64_t)r * (a.G * kBlocks + 1) + g * kBlocks : nullptr;
-    auto add = [&](auto weight) {
-#pragma unroll
-      for (int c = 0; c < kVerChunks; ++c) {
-        float f[kRowChunk];
-        x[c].get(f);
-        double q = 0.0, p = 0.0;
-#pragma unroll
-        for (int e = 0; e < kRowChunk; e += 2) q += weight(f[e]), p += weight(f[e + 1]);
-        q = wave_sum_d(q + p);
-        if (block && lane == 0) block[c * kVerWaves + wv] = q;
-        sum += q;
-      }
-      if (g == a.G - 1 && wv == 0) {  // the logits behind the eights
-        const double q = wave_sum_d(tail >= 0 ? weight(xt) : 0.0);
-        if (block && lane == 0) block[kBlocks] = q;
-        sum += q;
-      }
-    };
-    if (BulkWeight::serves(m, w.k)) add(BulkWeight(m, w.k));
-    else add(w);
+    const double first = -wave_max_d(-(double)at);
+    if (lane == 0) s_sum[wv] = first;
+    __syncthreads();
+    if (t == 0) {
+      a.m[(int64_t)r * a.G + g] = m;
+      a.sum[(int64_t)r * a.G + g] = fmin(fmin(s_sum[0], s_sum[1]), fmin(s_sum[2], s_sum[3]));
+    }
+    return;
   }
-  if (lane == 0) s_sum[wv] = sum;
-  __syncthreads();
-  if (t == 0) {
+  const double k = tgt ? a.kt : a.kd;
+  double *block = tgt ? a.block + (int64_t)r * (a.G * kBlocks + 1) + g * kBlocks : nullptr;
+  auto total = [&](auto weight) {  // of the slice, with its blocks' sums put down
+    double sum = 0.0;
 #pragma unroll
-    for (int w = 1; w < kVerWaves; ++w) sum = GREEDY ? fmin(sum, s_sum[w]) : sum + s_sum[w];
+    for (int c = 0; c < kVerChunks; ++c) {
+      float f[kRowChunk];
+      x[c].get(f);
+      double q = 0.0, p = 0.0;
+#pragma unroll
+      for (int e = 0; e < kRowChunk; e += 2) q += weight(f[e]), p += weight(f[e + 1]);
+      q = wave_sum_d(q + p);
+      if (block && lane == 0) block[c * kVerWaves + wv] = q;
+      sum += q;
+    }
+    if (g == a.G - 1 && wv == 0) {  // the logits behind the eights
+      const double q = wave_sum_d(tail >= 0 ? weight(xt) : 0.0);
+      if (block && lane == 0) block[kBlocks] = q;
+      sum += q;
+    }
+    if (lane == 0) s_sum[wv] = sum;
+    __syncthreads();
+    return (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
+  };
+  float m = 0.f;
+  double sum = total(BulkWeight(k));
+  if (!(sum > kNothing && sum < kMuch)) {  // (the same in every thread)
+    m = largest();
+#pragma unroll
+    for (int c = 0; c < kVerChunks; ++c) x[c].opaque();
+    sum = total(Weight(m, k));
+  }
+  if (t == 0) {
     a.m[(int64_t)r * a.G + g] = m;
     a.sum[(int64_t)r * a.G + g] = sum;
   }

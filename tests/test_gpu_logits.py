@@ -38,7 +38,8 @@ def _gen(*key):
 
 
 def _lse_close(got, want):
-    got = got.double().cpu()
+    got, stored = got.double().cpu(), want.float()
+    want = torch.where(stored.isinf(), stored.double(), want)  # past float32's range
     fine = want.isfinite()
     assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got[~fine & ~want.isnan()], want[~fine & ~want.isnan()])
     assert ((got - want).abs()[fine] <= 56 * U + U * want.abs()[fine]).all()
@@ -258,25 +259,48 @@ def test_distill_same_id_in_several_entries(cuda, dtype, rest, V, k):
     assert all(torch.equal(r[0], runs[0][0]) and torch.equal(r[1], runs[0][1]) for r in runs)
 
 
+@pytest.mark.parametrize("dtype", [H, B16, F], ids=str)
+@pytest.mark.parametrize("T", [1.0, 0.04])
 @pytest.mark.parametrize("rest", [False, True])
-def test_distill_masked_vocabularies(cuda, rest):
+def test_distill_masked_vocabularies(cuda, dtype, T, rest):
     g = _gen(13, rest)
-    z, val, idx, lse = _case(g, 6, 2001, 20, F, 1.0, rest)
+    low = torch.finfo(dtype).min
+    z, val, idx, lse = _case(g, 9, 2001, 20, F, T, rest)
     away = torch.ones(2001, dtype=torch.bool)
     away[idx[0]] = False
     z[0, away] = torch.where(torch.rand(int(away.sum()), generator=g) < 0.7, -INF, z[0, away])  # a mask outside the entries
     val[1, 5:] = -INF                                    # the teacher's own mask
     z[1, idx[1, 5:]] = -INF                              # under which the student's -inf costs nothing
-    z[2, torch.randint(0, 2001, (900,), generator=g)] = torch.finfo(F).min / 2
+    z[2, torch.randint(0, 2001, (900,), generator=g)] = low / 2
     z[2, idx[2]] = 0.0
     z[3] -= 30000.0                                      # far from 0
     z[4] *= 40.0
     z[5] = 0.25                                          # a flat student
-    z = torch.cat([z, torch.full((2, 2001), torch.finfo(F).min)])  # masks of the type's lowest value: a row of nothing
-    z[7, idx[1]] = torch.linspace(-2.0, 2.0, 20)         # else, and one outside the entries
-    val, idx = torch.cat([val, val[4:5], val[1:2]]), torch.cat([idx, idx[4:5], idx[1:2]])
-    lse = None if lse is None else torch.cat([lse, lse[4:5], lse[1:2]])
-    _check_distill(cuda, z, val, idx, lse)
+    z[6] = low                                           # masks of the type's lowest value: a row of nothing else,
+    val[7], idx[7] = val[1], idx[1]
+    z[7] = low                                           # and one outside the entries
+    z[7, idx[7]] = torch.linspace(-2.0, 2.0, 20)
+    z[8] = -low                                          # and of its highest, but for one
+    z[8, 77] = -low / 2
+    if lse is not None:
+        lse[7] = lse[1]
+    _check_distill(cuda, z.to(dtype), val, idx, lse, T)
+
+
+@pytest.mark.parametrize("dtype", [H, B16, F], ids=str)
+def test_top_logits_far_from_zero(cuda, dtype):
+    g = _gen(41)
+    low = torch.finfo(dtype).min
+    x = torch.randn(6, 3001, generator=g)
+    x[0] = low
+    x[1] = -low
+    x[1, 5] = -low / 2
+    x[2, 100:] = low
+    x[3] += 30000.0
+    x[4] *= 500.0
+    x[5, ::2] = low
+    for T in (1.0, 0.02, 50.0):
+        _check_top(x.to(dtype).to(cuda), 40, T)
 
 
 def test_distill_infinite_and_nan_rows(cuda):
@@ -475,6 +499,29 @@ def test_verify_infinities_and_foreign_ids(cuda):
     tok[5, 0], tok[6, 1], tok[7, 0] = -1, 2000, 2**40
     for T, Td in ((1.0, 1.0), (1.0, 0.0), (0.0, 0.0)):
         _check_verify(cuda, target, tok, u, draft, T, Td)
+
+
+@pytest.mark.parametrize("dtype", [H, B16, F], ids=str)
+@pytest.mark.parametrize("T", [1.0, 0.01, 100.0])
+def test_verify_far_from_zero(cuda, dtype, T):
+    """Rows, and parts of rows, whose exponentials about 0 are past 64 bits on either side."""
+    g = _gen(26)
+    target, tok, u, draft = _drafts(g, 9, 2, 20003, F, T)
+    low = torch.finfo(dtype).min
+    target[0] -= 30000.0
+    draft[0] += 30000.0
+    target[1, :, :9000] = low
+    draft[1, :, 9000:] = low
+    target[2] *= 700.0
+    target[3, :, 5] = -low
+    draft[4] = low
+    target[5] = low
+    target[6, :, 100:] = -INF
+    target[7, :, 8192:16384] -= 2000.0
+    draft[7, :, :8192] += 1500.0
+    target[8, :, 8192:] = NAN
+    _check_verify(cuda, target.to(dtype), tok, u, draft.to(dtype), T, T)
+    _check_verify(cuda, target.to(dtype), tok, u, None, T, 0.0)
 
 
 def test_verify_greedy_ties_take_the_lowest_id(cuda):
