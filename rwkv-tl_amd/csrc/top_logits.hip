@@ -37,7 +37,9 @@ struct TopArgs {
 
 constexpr int kBins = 256;
 constexpr int kGroups = 4;      // maxima a lane keeps: of its chunks c, c % 4
-constexpr int kFloorLow = 8;    // lowest bit of a floor that is decided: to 2^-15 of a value
+// Lowest bit of a floor that is decided: the formats' last, f32's to 2^-15 of a value.
+template <int FMT>
+constexpr int kFloorLow = FMT == 2 ? 16 : FMT == 0 ? 13 : 8;
 
 struct TopLds {
   u64 cand[kCandMax];
@@ -58,12 +60,12 @@ RWKV7_DEV uint32_t top_key(float x) {
 RWKV7_DEV float top_key_inv(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
 // The r-th largest of the N keys that each lane of the wave holds, rounded down
-// to bit kFloorLow; 0 when fewer than r are not 0.
-template <int N>
+// to bit LOW; 0 when fewer than r are not 0.
+template <int LOW, int N>
 RWKV7_DEV uint32_t rth_key(const uint32_t (&key)[N], int r) {
   uint32_t fl = 0;
 #pragma unroll 1
-  for (int bit = 31; bit >= kFloorLow; --bit) {
+  for (int bit = 31; bit >= LOW; --bit) {
     const uint32_t c = fl | (1u << bit);
     int n = 0;
 #pragma unroll
@@ -94,7 +96,7 @@ RWKV7_DEV void scan_bins(TopLds &s) {
   }
 }
 
-// f(key, id) for every logit of the row, from memory: the way of the long ties,
+// f(logit, id) for every logit of the row, from memory: the way of the long ties,
 // of which nothing is held in registers beside the row.
 template <int FMT, int THREADS, class F>
 RWKV7_DEV void each_logit(const char *src, int V, F f) {
@@ -106,10 +108,10 @@ RWKV7_DEV void each_logit(const char *src, int V, F f) {
     float v[kRowChunk];
     x.get(v);
 #pragma unroll
-    for (int e = 0; e < kRowChunk; ++e) f(top_key(v[e]), (int)b * kRowChunk + e);
+    for (int e = 0; e < kRowChunk; ++e) f(v[e], (int)b * kRowChunk + e);
   }
   const int tail = (int)n8 * kRowChunk + threadIdx.x;
-  if (threadIdx.x < kRowChunk && tail < V) f(top_key(load_logit<FMT>(src, tail)), tail);
+  if (threadIdx.x < kRowChunk && tail < V) f(load_logit<FMT>(src, tail), tail);
 }
 
 // One digit of a radix selection: digit(key, id) is 0 .. 255, lowest first, or -1
@@ -121,8 +123,8 @@ RWKV7_DEV int select_digit(const char *src, int V, int &need, TopLds &s, D digit
   __syncthreads();
   if (t < kBins) s.bin[t] = 0;
   __syncthreads();
-  each_logit<FMT, THREADS>(src, V, [&](uint32_t key, int id) {
-    const int d = digit(key, id);
+  each_logit<FMT, THREADS>(src, V, [&](float v, int id) {
+    const int d = digit(top_key(v), id);
     if (d >= 0) atomicAdd(&s.bin[d], 1);
   });
   __syncthreads();
@@ -167,7 +169,7 @@ __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : THREADS == 256 ? 7 : 8) voi
   opaque_row(x);
   auto wave_floor = [&](int r) {
     const uint32_t lo = own[0] > own[1] ? own[0] : own[1], hi = own[2] > own[3] ? own[2] : own[3], one[1] = {lo > hi ? lo : hi};
-    return r > 16 ? rth_key(own, r) : rth_key(one, r);
+    return r > 16 ? rth_key<kFloorLow<FMT>>(own, r) : rth_key<kFloorLow<FMT>>(one, r);
   };
   {
     const uint32_t fl = wave_floor((k + kWaves - 1) / kWaves);
@@ -195,16 +197,21 @@ __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : THREADS == 256 ? 7 : 8) voi
   uint32_t fl = least_floor();
   const int full = __popcll(__ballot(lane < kWaves && s.some[lane] >= kWave));
   if (fl == 0u && k <= full * kWave) {  // (block-uniform)
-    const uint32_t f = s.some[wv] >= kWave ? rth_key(own, (k + full - 1) / full) : ~0u;
+    const uint32_t f = s.some[wv] >= kWave ? rth_key<kFloorLow<FMT>>(own, (k + full - 1) / full) : ~0u;
     __syncthreads();
     if (lane == 0) s.floor[wv] = f;
     __syncthreads();
     fl = least_floor();
   }
 
-  auto gather = [&](uint32_t key, int id) {
-    const int slot = atomicAdd(&s.n, 1);
-    if (slot < kCandMax) s.cand[slot] = ((u64)key << 32) | (uint32_t)~id;
+  // (The counter's place is opaque: the compiler would otherwise join the lanes'
+  // additions first, in twenty instructions for the one or two that there are.)
+  int zero = 0;
+  asm volatile("" : "+v"(zero));
+  int *const next = &s.n + zero;
+  auto gather = [&](float v, int id) {
+    const int slot = atomicAdd(next, 1);
+    if (slot < kCandMax) s.cand[slot] = ((u64)__float_as_uint(v) << 32) | (uint32_t)~id;
   };
   if (fl) {
     // by value: one comparison a logit, and no more where none of a wave's passes
@@ -215,9 +222,9 @@ __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : THREADS == 256 ? 7 : 8) voi
       x[c].get(v);
 #pragma unroll
       for (int e = 0; e < kRowChunk; ++e)
-        if (v[e] >= least) gather(top_key(v[e]), (c * THREADS + t) * kRowChunk + e);
+        if (v[e] >= least) gather(v[e], (c * THREADS + t) * kRowChunk + e);
     }
-    if (tail >= 0 && xt >= least) gather(top_key(xt), tail);
+    if (tail >= 0 && xt >= least) gather(xt, tail);
   } else if (V <= kCandMax) {
     each_logit<FMT, THREADS>(src, V, gather);
   } else if (t == 0) {
@@ -242,8 +249,9 @@ __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : THREADS == 256 ? 7 : 8) voi
     if (t == 0) s.n = 0;
     if (t < kBins) s.bin[t] = 0;
     __syncthreads();
-    each_logit<FMT, THREADS>(src, V, [&](uint32_t key, int id) {
-      if (key > kth || (key == kth && id <= last)) gather(key, id);
+    each_logit<FMT, THREADS>(src, V, [&](float v, int id) {
+      const uint32_t key = top_key(v);
+      if (key > kth || (key == kth && id <= last)) gather(v, id);
     });
     __syncthreads();
     n = k;
@@ -255,7 +263,11 @@ __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : THREADS == 256 ? 7 : 8) voi
   const int shift = max(0, 24 - __clz((int)(range | 1u)));
   auto bin_of = [&](u64 c) { return kBins - 1 - (int)(((uint32_t)(c >> 32) - low) >> shift); };
 #pragma unroll 1
-  for (int i = t; i < n; i += THREADS) atomicAdd(&s.bin[bin_of(s.cand[i])], 1);
+  for (int i = t; i < n; i += THREADS) {  // (from here on by their keys)
+    const u64 c = s.cand[i], own = ((u64)top_key(__uint_as_float((uint32_t)(c >> 32))) << 32) | (uint32_t)c;
+    s.cand[i] = own;
+    atomicAdd(&s.bin[bin_of(own)], 1);
+  }
   __syncthreads();
   scan_bins(s);
   __syncthreads();

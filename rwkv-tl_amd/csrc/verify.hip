@@ -275,7 +275,13 @@ RWKV7_DEV void decide(const VerifyArgs &a, int b, DecideLds &s) {
   __syncthreads();
 }
 
-// max(p - q, 0) of one logit; id: its index.
+// max(p - q, 0); both products rounded, so that equal rows leave nothing.
+RWKV7_DEV double over(double wp, double ip, double wq, double iq) {
+#pragma clang fp contract(off)
+  return fmax(wp * ip - wq * iq, 0.0);
+}
+
+// The same of one logit from the exponentials; id: its index.
 struct Residual {
   Weight p, q;
   double ip, iq;
@@ -284,8 +290,7 @@ struct Residual {
   RWKV7_DEV Residual(const VerifyArgs &a, const Decision &d, bool from_p)
       : p(d.mp, a.kt), q(d.mq, a.kd), ip(d.ip), iq(d.iq), x(from_p ? -1 : d.x), soft(!from_p && d.rejected && a.draft) {}
   RWKV7_DEV double operator()(float xp, float xq, int id) const {
-    double r = p(xp) * ip;
-    if (soft) r = fmax(r - q(xq) * iq, 0.0);
+    const double r = soft ? over(p(xp), ip, q(xq), iq) : p(xp) * ip;
     return id == x ? 0.0 : r;
   }
 };
@@ -309,8 +314,17 @@ __global__ __launch_bounds__(kVerThreads) void verify_rest_kernel(VerifyArgs a) 
   xp.get(fp);
   xq.get(fq);
   double sum = 0.0;
+  if (d.mp == 0.f && d.mq == 0.f) {
+    const BulkWeight p(a.kt), q(a.kd);
 #pragma unroll
-  for (int e = 0; e < kRowChunk; ++e) sum += res(fp[e], fq[e], (int)e8 * kRowChunk + e);
+    for (int e = 0; e < kRowChunk; ++e) {
+      const double r = res.soft ? over(p(fp[e]), d.ip, q(fq[e]), d.iq) : p(fp[e]) * d.ip;
+      sum += (int)e8 * kRowChunk + e == d.x ? 0.0 : r;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < kRowChunk; ++e) sum += res(fp[e], fq[e], (int)e8 * kRowChunk + e);
+  }
   sum = wave_sum_d(sum);
   if (lane == 0) block[g * kVerWaves + wv] = sum;
   if (g == a.G * kVerChunks - 1 && wv == 0) {  // the logits behind the eights
@@ -347,7 +361,10 @@ __global__ __launch_bounds__(kWave) void verify_draw_kernel(VerifyArgs a) {
   bool from_p = !d.rejected;
   if (d.rejected) {
 #pragma unroll
-    for (int e = 0; e < kDrawE; ++e) w[e] = kDrawE * lane + e < blocks ? a.rest[(int64_t)b * blocks + kDrawE * lane + e] : 0.0;
+    for (int e = 0; e < kDrawE; ++e) {
+      w[e] = kDrawE * lane + e < blocks ? a.rest[(int64_t)b * blocks + kDrawE * lane + e] : 0.0;
+      if (!(w[e] > kNothing)) w[e] = 0.0;
+    }
     from_p = !(wave_sum_d((w[0] + w[1]) + w[2]) > 0.0);
   }
   if (from_p) {

@@ -461,6 +461,10 @@ def test_verify_identical_models_accept_everything(cuda):
     target, tok, u, _ = _drafts(g, 30, 5, 3001, B16, 1.0, 0.0)
     out, n = verify_draft(target.to(cuda), tok.to(cuda), u.to(cuda), target[:, :5].contiguous().to(cuda), temperature=1.0)
     assert (n == 5).all() and torch.equal(out[:, :5].cpu(), tok)
+    # even a u of 1, which rejects, leaves no residue of p - q to draw from: p itself
+    one = torch.ones_like(u)
+    one[:, 5] = u[:, 5]
+    _check_verify(cuda, target, tok, one, target[:, :5].contiguous(), 1.0, 1.0)
 
 
 def test_verify_borders(cuda):
