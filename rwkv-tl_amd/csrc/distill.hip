@@ -61,16 +61,17 @@ struct Joined {
 struct DistillLds {
   u64 mine[kRowMaxThreads];  // of each thread's logits, bit 8 c + e for chunk c: those with an entry
   uint32_t tail;             // of the logits behind the eights
-  int idx[kDistMaxK];
-  float p[kDistMaxK];
+  int idx[kDistMaxK];        // of each thread's entry, -1 for none
+  float z[kDistMaxK];        // its student logit
   // per wave: the largest logit and the sum about it of the row's rest and of
   // the entries; the teacher's reference, mass, and mass-weighted difference of
   // its logarithms about that and the student's about mtop
-  float mrest[kMaxWaves], rest[kMaxWaves], mtop[kMaxWaves], top[kMaxWaves];
-  double tref[kMaxWaves], tw[kMaxWaves], ta[kMaxWaves];
+  float mrest[kMaxWaves], rest[kMaxWaves], mtop[kMaxWaves];
+  double top[kMaxWaves], tref[kMaxWaves], tw[kMaxWaves], ta[kMaxWaves];
   bool whole;  // every id of the vocabulary has an entry
   Joined j;
-  float f_rest, f_top, ua;
+  float f_rest;
+  double f_top, ua;
 };
 
 template <int FMT, int THREADS>
@@ -91,9 +92,9 @@ RWKV7_DEV Joined join(const DistillArgs &g, const DistillLds &s, int lane, doubl
   const float mtop = wave_max(mt);
   j.m = uniform_f(fmaxf(j.mrest, mtop));
   j.Srest = uniform_d(wave_sum_d(lane < WAVES ? (double)s.rest[lane] * g.sc.part(mr, j.mrest) : 0.0));
-  const double Stop = wave_sum_d(lane < WAVES ? (double)s.top[lane] * g.sc.part(mt, mtop) : 0.0);
-  j.in_all = uniform_d(g.sc.part(j.mrest, j.m));
-  j.S = uniform_d(j.Srest * j.in_all + Stop * g.sc.part(mtop, j.m));
+  const double Stop = wave_sum_d(lane < WAVES ? s.top[lane] * g.sc.shift(mt, mtop) : 0.0);
+  j.in_all = uniform_d(g.sc.part_of_exact(j.mrest, j.m));
+  j.S = uniform_d(j.Srest * j.in_all + Stop * g.sc.shift(mtop, j.m));
   if (!(j.m > -kInf)) j.S = __builtin_nan("");  // no finite logit at all
   const int tws = (g.K + kWave - 1) / kWave;
   double W = lane < tws ? s.tw[lane] : 0.0;
@@ -125,7 +126,7 @@ RWKV7_DEV void put_loss(const DistillArgs &g, const DistillLds &s, const Joined 
     A = s.tw[lane] != 0.0 ? f * (s.ta[lane] + s.tw[lane] * up) : 0.0;
   }
   A = wave_sum_d(A);
-  const double S = g.sc.off(j.m) + log2_d(j.S);
+  const double S = log2_d(j.S);
   double loss;
   if (g.lse) {
     loss = A + j.W * S;
@@ -168,7 +169,10 @@ __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : 8) void distill_kernel(Dist
   const float zv = there ? load_logit<FMT>(src, id) : -kInf;
   const double lse = uniform_d(g.lse ? (double)g.lse[row] * kLog2E : 0.0);
 
-  // mark the ids; `first`: this entry stands for its id
+  // mark the ids; `first`: this entry stands for its id. (Id and logit wait in LDS
+  // for the gradient: nothing is held beside the row.)
+  s.idx[t] = id;
+  if (GRAD) s.z[t] = zv;
   bool first = there;
   if (there) {
     const uint32_t b = (uint32_t)id / kRowChunk, bit = b / THREADS * kRowChunk + id % kRowChunk;
@@ -178,7 +182,6 @@ __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : 8) void distill_kernel(Dist
   }
   const bool twice = __syncthreads_or(there && !first);
   if (twice) {  // the same id in several entries: the lowest stands for it
-    s.idx[t] = id;
     __syncthreads();
     first = there;
 #pragma unroll 1
@@ -208,22 +211,26 @@ __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : 8) void distill_kernel(Dist
   opaque_row(x);
   const bool entries = wv * kWave < g.K;  // this wave has entries
   const float mtop = entries ? wave_max(zv) : -kInf, rest = sum_row(x, xt, g.sc, m);
-  const float own = there ? g.sc.e(zv, mtop) : 0.f;  // exp of the entry's student logit
-  const float2 sums = wave_sum2(rest, first ? own : 0.f);
+  const float sum = wave_sum(rest);
 
-  // the teacher's entries, about its lse or the wave's largest, in 64 bits and
-  // powers of two
+  // the entries in 64 bits and powers of two: the student's about their largest,
+  // the teacher's about its lse or the wave's largest (a gradient's q - p is what
+  // is left of the two)
   const double k2 = g.sc.k;
   double tref = lse, w = 0.0;
   if (entries) {
+    const double zk = k2 * ((double)zv - (double)ExpScale::ref(mtop));  // (NaN stays NaN)
+    const double top = wave_sum_d(first ? zk == zk ? exp2_d(zk) : zk : 0.0);
     if (!g.lse) tref = k2 * (double)wave_max(tv);
     const double y = k2 * (double)tv - tref;  // (NaN stays NaN)
     w = there && tv != -kInf ? (y == y ? exp2_d(y) : y) : 0.0;
-    const double ta = w != 0.0 ? w * ((k2 * (double)tv - tref) - k2 * ((double)zv - (double)ExpScale::ref(mtop))) : 0.0;
+    const double ta = w != 0.0 ? w * (y - zk) : 0.0;
     const double ws = wave_sum_d(w), as = wave_sum_d(ta);
-    if (lane == 0) s.tref[wv] = tref, s.tw[wv] = ws, s.ta[wv] = as;
+    if (lane == 0) s.tref[wv] = tref, s.tw[wv] = ws, s.ta[wv] = as, s.top[wv] = top;
+    if (GRAD) s.mine[t] = __builtin_bit_cast(u64, w);  // (the marks are used up)
   }
-  if (lane == 0) s.mrest[wv] = m, s.rest[wv] = sums.x, s.mtop[wv] = mtop, s.top[wv] = sums.y;
+  if (lane == 0) s.mrest[wv] = m, s.rest[wv] = sum, s.mtop[wv] = mtop;
+  if (!entries && lane == 0) s.top[wv] = 0.0;
   __syncthreads();
 
   if (wv == 0) {
@@ -236,45 +243,51 @@ __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : 8) void distill_kernel(Dist
     const double ua = j.mass ? (double)up * g.a : 0.0, all = ua * (j.P + j.rest_t) * rcp_d(j.S);
     if (lane == 0) {
       s.j = j;
-      s.ua = (float)ua;
-      s.f_top = (float)all;
+      s.ua = ua;
+      s.f_top = all;
       s.f_rest = (float)(all * j.in_all - (j.rest_t > 0.0 && j.Srest > 0.0 ? ua * j.rest_t * rcp_d(j.Srest) : 0.0));
     }
   }
   if (!GRAD) return;
   __syncthreads();
-  const float ua = uniform_f(s.ua), f_rest = uniform_f(s.f_rest);
-  if (ua == 0.f) {  // a row that counts for nothing: zeros, not 0 * NaN
+  if (s.ua == 0.0) {  // a row that counts for nothing: zeros, not 0 * NaN
     zero_row<FMT, THREADS>(dst, V);
-    if (LOSS && wv == 0) put_loss(g, s, s.j, lane, lse, row);
-    return;
-  }
-  float pk = entries ? ua * (float)(g.lse ? w : w * exp2_d(tref - s.j.tref) * rcp_d(s.j.W)) : 0.f;
-  opaque_row(x);
-  g.sc.with(s.j.mrest, [&](auto e2, auto far) {
+  } else {
+    const float f_rest = uniform_f(s.f_rest);
+    opaque_row(x);
+    g.sc.with(s.j.mrest, [&](auto e2, auto far) {
 #pragma unroll
-    for (int c = 0; c < kRowChunks; ++c) {
-      float f[kRowChunk];
-      x[c].template get<decltype(far)::value>(f);
+      for (int c = 0; c < kRowChunks; ++c) {
+        float f[kRowChunk];
+        x[c].template get<decltype(far)::value>(f);
 #pragma unroll
-      for (int e = 0; e < kRowChunk; ++e) f[e] = f_rest * e2(f[e]);
-      const uint32_t b = c * THREADS + t;
-      if ((c + 1) * THREADS <= n8) store_chunk<FMT>(dst, b, f);
-      else if (b < n8) store_chunk<FMT>(dst, b, f);
+        for (int e = 0; e < kRowChunk; ++e) f[e] = f_rest * e2(f[e]);
+        const uint32_t b = c * THREADS + t;
+        if ((c + 1) * THREADS <= n8) store_chunk<FMT>(dst, b, f);
+        else if (b < n8) store_chunk<FMT>(dst, b, f);
+      }
+      if (t < V % kRowChunk) store_logit<FMT>(dst, (int)n8 * kRowChunk + t, f_rest * e2(xt));
+    });
+    double pk = 0.0;
+    if (wv * kWave < g.K) {
+      pk = __builtin_bit_cast(double, s.mine[t]);
+      if (!g.lse) pk *= exp2_d(s.tref[wv] - s.j.tref) * rcp_d(s.j.W);
     }
-    if (tail >= 0) store_logit<FMT>(dst, tail, f_rest * e2(xt));
-  });
-  if (twice) {
-    s.p[t] = there ? pk : 0.f;
-    __syncthreads();
-    double sum = 0.0;
+    if (twice) {
+      s.mine[t] = __builtin_bit_cast(u64, s.idx[t] >= 0 ? pk : 0.0);
+      __syncthreads();
+      double sum = 0.0;
 #pragma unroll 1
-    for (int k = 0; first && k < g.K; ++k) sum += s.idx[k] == id ? (double)s.p[k] : 0.0;
-    pk = (float)sum;
+      for (int k = 0; first && k < g.K; ++k) sum += s.idx[k] == s.idx[t] ? __builtin_bit_cast(double, s.mine[k]) : 0.0;
+      pk = sum;
+    }
+    __syncthreads();  // the row's own stores come before the entries'
+    if (first) {
+      const double zk = g.sc.k * ((double)s.z[t] - (double)s.j.m);  // (NaN stays NaN)
+      store_logit<FMT>(dst, s.idx[t], (float)(s.f_top * (zk == zk ? exp2_d(zk) : zk) - s.ua * pk));
+    }
   }
-  __syncthreads();  // the row's own stores come before the entries'
-  if (first) store_logit<FMT>(dst, id, s.f_top * g.sc.e(zv, s.j.m) - pk);
-  if (LOSS && wv == 0) put_loss(g, s, s.j, lane, lse, row);
+  if (LOSS && wv == 0) put_loss(g, s, s.j, lane, g.lse ? (double)g.lse[row] * kLog2E : 0.0, row);
 }
 
 template <int FMT, int THREADS>

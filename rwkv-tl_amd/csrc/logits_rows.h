@@ -280,10 +280,13 @@ struct ExpScale {
     m = ref(m);
     return near(m) ? (double)(m * kf) - (double)m * (double)kf : 0.0;
   }
-  // the share of a part about m in a sum about a larger one (0 for none)
-  RWKV7_DEV double part(float m, float larger) const {
-    return m > -kInf ? exp2_d(((double)m - (double)larger) * (double)kf + (off(m) - off(larger))) : 0.0;
+  // what a sum about m (0 for none) counts in one about a larger one, both exactly
+  RWKV7_DEV double shift(float m, float larger) const {
+    return m > -kInf ? exp2_d(((double)m - (double)larger) * k) : 0.0;
   }
+  // the same of sums of e(), and of one of those in an exact one
+  RWKV7_DEV double part(float m, float larger) const { return shift(m, larger) * exp2_d(off(m) - off(larger)); }
+  RWKV7_DEV double part_of_exact(float m, float larger) const { return shift(m, larger) * exp2_d(off(m)); }
   // log2 of sum exp(a x) when the sum about m is S
   RWKV7_DEV double log2z(double S, float m) const { return (double)m * k + off(m) + log2_d(S); }
 };
