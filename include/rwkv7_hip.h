@@ -241,6 +241,13 @@ int rwkv7_prefill(const rwkv7_model *model, const rwkv7_state *state,
                   const int64_t *tokens, int32_t seq_len, void *workspace,
                   int64_t workspace_bytes, void *stream);
 
+/* rwkv7_prefill with the logits after every token: logits f16 [B, T, V] (bf16
+ * for a bf16 model), row (b, t) those after tokens[b, 0 .. t]. For what looks at
+ * a whole sequence: a teacher's answers, drafted tokens to verify. The same
+ * workspace. seq_len 1 is rwkv7_decode. No counterpart in the reference. */
+int rwkv7_prefill_logits(const rwkv7_model *model, const rwkv7_state *state, const int64_t *tokens, int32_t seq_len,
+                         void *logits, void *workspace, int64_t workspace_bytes, void *stream);
+
 /* ---- operator level ---------------------------------------------------- */
 
 /* Every operator below that takes 16-bit operands takes them in one format

@@ -312,10 +312,14 @@ static int decode_one(const rwkv7_model &m, const rwkv7_state &s, const int64_t 
 // activations are rounded to the model's 16-bit format.
 static bool batch_a32(const rwkv7_dims &d, int M) { return M < gemm_big_min_rows(d.n_ffn > d.n_embd ? d.n_ffn : d.n_embd); }
 
+// Rows of one head GEMM of a step with logits of every row: few enough that the
+// GEMMs' offsets stay in 32 bits at any vocabulary here.
+constexpr int kHeadRows = 1024;
+
 // B sequences x T tokens through the MFMA GEMM path; logits (optional) of the
-// last token of each sequence.
+// last token of each sequence, or of every row.
 static int run_batched(const rwkv7_model &m, const rwkv7_state &s, const int64_t *tok, int T,
-                       void *logits, char *ws, hipStream_t st) {
+                       void *logits, bool all_rows, char *ws, hipStream_t st) {
   const rwkv7_dims &d = m.dims;
   const int B = s.batch;
   const int C = d.n_embd, F = d.n_ffn, H = d.n_head, SR = sum_ranks(d);
@@ -550,20 +554,29 @@ static int run_batched(const rwkv7_model &m, const rwkv7_state &s, const int64_t
     RWKV7_TRY(ffn_value(gv));
   }
   if (logits) {
-    // B rows: the head GEMM always takes f32 A (B is far below the large-M path)
+    // The head GEMM always takes f32 A. B rows in their own buffer; all M rows,
+    // 16 at a time in order, in the layers' operand buffer, which is done with
+    // (all of them before the first GEMM, whose scratch holds the last FFN
+    // value's slices).
     const float *lo = static_cast<const float *>(m.ln_out);
-    const bool hf = m.head_frag && B > kA32SkinnyMaxM;
-    RWKV7_TRY(launch_ln_rows(x, 1, lo, lo + C, w.headin, hf ? 2 : 1, B, C, T, T - 1, bf, st, w.part, nparts, MC));
-    GemmProb gh = {static_cast<const uint16_t *>(w.headin), static_cast<const uint16_t *>(m.head), logits, C, C,
-                   d.vocab, d.vocab, C, GEPI_F16};
-    if (m.head_frag) {
-      gh.Wf = static_cast<const uint16_t *>(m.head_frag);
-      gh.nksf = (C + 31) / 32;
+    const int R = all_rows ? M : B;
+    const bool hf = m.head_frag && R > kA32SkinnyMaxM;
+    char *hin = static_cast<char *>(all_rows ? w.xmix : w.headin);
+    RWKV7_TRY(launch_ln_rows(x, 1, lo, lo + C, hin, hf ? 2 : 1, R, C, all_rows ? 1 : T, all_rows ? 0 : T - 1, bf, st, w.part, nparts, MC));
+    for (int r = 0; r < R;) {
+      const int rows = R - r > kHeadRows + kHeadRows / 2 ? kHeadRows : R - r;  // (no short last one)
+      GemmProb gh = {reinterpret_cast<const uint16_t *>(hin + (int64_t)r * C * 4), static_cast<const uint16_t *>(m.head),
+                     static_cast<uint16_t *>(logits) + (int64_t)r * d.vocab, C, C, d.vocab, d.vocab, C, GEPI_F16};
+      if (m.head_frag) {
+        gh.Wf = static_cast<const uint16_t *>(m.head_frag);
+        gh.nksf = (C + 31) / 32;
+      }
+      gh.bf = bf;
+      gh.a32 = 1;
+      if (hf) RWKV7_TRY(launch_gemm_frag(&gh, 1, rows, st));
+      else RWKV7_TRY(launch_gemm_group(&gh, 1, rows, st, w.part, ctr));
+      r += rows;
     }
-    gh.bf = bf;
-    gh.a32 = 1;
-    if (hf) return launch_gemm_frag(&gh, 1, B, st);
-    RWKV7_TRY(launch_gemm_group(&gh, 1, B, st, w.part, ctr));
   }
   return RWKV7_OK;
 }
@@ -591,13 +604,13 @@ static bool use_persistent_decode(const rwkv7_model &m, int batch, bool logits) 
 // decode has its own kernel above.
 static bool use_rows_kernel(const rwkv7_model &m, int batch, int T) { return rows_usable(m, batch, T); }
 
-static int run_rows(const rwkv7_model &m, const rwkv7_state &s, const int64_t *tok, int T, void *logits, char *ws,
-                    hipStream_t st) {
+static int run_rows(const rwkv7_model &m, const rwkv7_state &s, const int64_t *tok, int T, void *logits, bool all_rows,
+                    char *ws, hipStream_t st) {
   rwkv7_layer_layout lay;
   layout_of(m.dims, &lay);
   // the aborted-launch counter shared with the batch-1 kernel (workspace byte 32)
-  return launch_rows_mk(m, lay, s, tok, T, logits, rows_exchange(m.dims, ws), reinterpret_cast<unsigned *>(ws + 32),
-                        st);
+  return launch_rows_mk(m, lay, s, tok, T, logits, all_rows, rows_exchange(m.dims, ws),
+                        reinterpret_cast<unsigned *>(ws + 32), st);
 }
 
 }  // namespace rwkv7
@@ -679,8 +692,8 @@ int rwkv7_decode(const rwkv7_model *model, const rwkv7_state *state, const int64
     return decode_one(*model, *state, tokens, logits, static_cast<char *>(workspace), st);
   }
   if (use_rows_kernel(*model, state->batch, 1))
-    return run_rows(*model, *state, tokens, 1, logits, static_cast<char *>(workspace), st);
-  return run_batched(*model, *state, tokens, 1, logits, static_cast<char *>(workspace), st);
+    return run_rows(*model, *state, tokens, 1, logits, false, static_cast<char *>(workspace), st);
+  return run_batched(*model, *state, tokens, 1, logits, false, static_cast<char *>(workspace), st);
 }
 
 int rwkv7_workspace_errors(const void *workspace, int64_t workspace_bytes, uint32_t *count, void *stream) {
@@ -695,17 +708,28 @@ int rwkv7_workspace_errors(const void *workspace, int64_t workspace_bytes, uint3
   return RWKV7_OK;
 }
 
-int rwkv7_prefill(const rwkv7_model *model, const rwkv7_state *state, const int64_t *tokens, int32_t seq_len,
-                  void *workspace, int64_t workspace_bytes, void *stream) {
+static int prefill_step(const rwkv7_model *model, const rwkv7_state *state, const int64_t *tokens, int32_t seq_len,
+                        void *logits, void *workspace, int64_t workspace_bytes, void *stream) {
   RWKV7_TRY(check_model_state(model, state));
   if (!tokens || !workspace) return RWKV7_EINVAL;
   if (seq_len < 1) return RWKV7_ESHAPE;
   if (workspace_bytes < rwkv7_workspace_bytes(&model->dims, state->batch, seq_len)) return RWKV7_EWORKSPACE;
+  const hipStream_t st = static_cast<hipStream_t>(stream);
   if (use_rows_kernel(*model, state->batch, seq_len))
-    return run_rows(*model, *state, tokens, seq_len, nullptr, static_cast<char *>(workspace),
-                    static_cast<hipStream_t>(stream));
-  return run_batched(*model, *state, tokens, seq_len, nullptr, static_cast<char *>(workspace),
-                     static_cast<hipStream_t>(stream));
+    return run_rows(*model, *state, tokens, seq_len, logits, true, static_cast<char *>(workspace), st);
+  return run_batched(*model, *state, tokens, seq_len, logits, true, static_cast<char *>(workspace), st);
+}
+
+int rwkv7_prefill(const rwkv7_model *model, const rwkv7_state *state, const int64_t *tokens, int32_t seq_len,
+                  void *workspace, int64_t workspace_bytes, void *stream) {
+  return prefill_step(model, state, tokens, seq_len, nullptr, workspace, workspace_bytes, stream);
+}
+
+int rwkv7_prefill_logits(const rwkv7_model *model, const rwkv7_state *state, const int64_t *tokens, int32_t seq_len,
+                         void *logits, void *workspace, int64_t workspace_bytes, void *stream) {
+  if (!logits) return RWKV7_EINVAL;
+  if (seq_len == 1) return rwkv7_decode(model, state, tokens, logits, workspace, workspace_bytes, stream);
+  return prefill_step(model, state, tokens, seq_len, logits, workspace, workspace_bytes, stream);
 }
 
 // The scan instance for the operand formats of an operator-level call: 16-bit

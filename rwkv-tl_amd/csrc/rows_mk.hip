@@ -93,8 +93,9 @@ struct RkArgs {
   float *rnn;
   uint16_t *cmix_x;
   const int64_t *tok;
-  uint16_t *logits;  // [B, V] or null
+  uint16_t *logits;  // of hT'th row each of hB: every sequence's last token, or every row; or null
   int B, T, M, G;
+  int hB, hT;
   unsigned *sync, *started, *errors;
   unsigned *fl[5];   // per-stage flags: P2 units, P3 blocks, P4 blocks, P5 blocks (fl[0] unused: P1 hands off tagged words)
   uint64_t *proj;    // [M, 3C + SR] f32 as tagged words
@@ -896,8 +897,9 @@ __global__ __launch_bounds__(kRT) void rows_mk_kernel(RkArgs a) {
   const bool done = wait_flags(cx, a.fl[4], nP5, cx.tag(L - 1, 4), ident);
   if (slice_owner && done) store_shift_slice(a, s.shs2, a.cmix_x, L - 1, 16 * g);
   if (a.logits) {
-    const int B = a.B, T = a.T;
-    // LN_out of each sequence's last token into A rows 0..B-1
+    const int B = a.hB, T = a.hT;
+    // LN_out of the rows that have logits (each sequence's last token, or all)
+    // into A rows 0..B-1
     const __amdgpu_buffer_rsrc_t rx = rrsrc(a.x, (int64_t)a.M * C * 4);
     const int n = B * C / 4;
     floatx4 v[8];
@@ -1024,7 +1026,7 @@ bool rows_usable(const rwkv7_model &m, int B, int T) {
 }
 
 int launch_rows_mk(const rwkv7_model &m, const rwkv7_layer_layout &lay, const rwkv7_state &s, const int64_t *tok,
-                   int T, void *logits, char *xreg, unsigned *errors, hipStream_t st) {
+                   int T, void *logits, bool all_rows, char *xreg, unsigned *errors, hipStream_t st) {
   if (!rows_usable(m, s.batch, T)) return RWKV7_ESHAPE;
   const rwkv7_dims &d = m.dims;
   RkArgs a;
@@ -1060,6 +1062,8 @@ int launch_rows_mk(const rwkv7_model &m, const rwkv7_layer_layout &lay, const rw
   a.B = s.batch;
   a.T = T;
   a.M = s.batch * T;
+  a.hB = all_rows ? a.M : a.B;
+  a.hT = all_rows ? 1 : T;
   a.G = mk_cus();
   const int64_t C = a.C, F = a.F, H = a.H, SR = a.SR, M = 16;
   auto al = [](int64_t x) { return (x + 255) & ~int64_t(255); };

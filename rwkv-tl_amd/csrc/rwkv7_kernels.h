@@ -296,6 +296,6 @@ int64_t rows_exchange_bytes(const rwkv7_dims &d);
 // on the current device at once
 bool rows_usable(const rwkv7_model &m, int B, int T);
 int launch_rows_mk(const rwkv7_model &m, const rwkv7_layer_layout &lay, const rwkv7_state &s, const int64_t *tok,
-                   int T, void *logits, char *xreg, unsigned *errors, hipStream_t st);
+                   int T, void *logits, bool all_rows, char *xreg, unsigned *errors, hipStream_t st);
 
 }  // namespace rwkv7

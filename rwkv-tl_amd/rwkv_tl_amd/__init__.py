@@ -10,7 +10,8 @@ Drop-in for the GPU path of yuyi2439/rwkv-tl:
 * ``kernels`` -- the operator-level API of ``rwkv_tl.kernels.fp16``
 * ``sample_logits`` -- ``demo.sampling.sample_logits`` (one HIP kernel launch)
 * ``verify_draft`` / ``kernels.top_logits`` / ``kernels.distill_loss`` -- operators between
-  a large model and a small one (``logits.py``; no counterpart in the reference)
+  a large model and a small one (``logits.py``; no counterpart in the reference);
+  ``generate_speculative`` drafts with one model and verifies with the other
 * ``operators`` -- ``torch.ops.rwkv_tl.*`` (``rwkv_tl.operators``), registered on import
 * ``tokenizer.Tokenizer`` -- ``rwkv_tl.tokenizer.Tokenizer``
 """
@@ -26,6 +27,7 @@ from .logits import verify_draft
 from .model import RWKV7Model
 from .rwkv7_hip import RWKV7HIP, RWKV7HIPBF16, RWKV7HIPInt8
 from .sampling import sample_logits
+from .speculative import generate_speculative
 from .state import State
 from .weight import LNWeight, RWKV7Weight
 
@@ -40,6 +42,7 @@ __all__ = [
     "RWKV7Weight",
     "SHAPES",
     "State",
+    "generate_speculative",
     "make_graph_cls",
     "make_random_state_dict",
     "make_rwkv7",

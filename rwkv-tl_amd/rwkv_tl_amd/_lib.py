@@ -45,6 +45,7 @@ SYMBOLS = (
     "rwkv7_decode",
     "rwkv7_decode_noalloc",
     "rwkv7_prefill",
+    "rwkv7_prefill_logits",
     "rwkv7_wkv7",
     "rwkv7_wkv7_chunked_workspace_bytes",
     "rwkv7_wkv7_chunked",
@@ -177,6 +178,7 @@ def _declare(lib: ctypes.CDLL) -> None:
         "rwkv7_decode": (ctypes.c_int, [ctypes.POINTER(Model), ctypes.POINTER(StateDesc), vp, vp, vp, i64, vp]),
         "rwkv7_decode_noalloc": (ctypes.c_int, [ctypes.POINTER(Model), ctypes.POINTER(StateDesc), vp, vp, vp]),
         "rwkv7_prefill": (ctypes.c_int, [ctypes.POINTER(Model), ctypes.POINTER(StateDesc), vp, i32, vp, i64, vp]),
+        "rwkv7_prefill_logits": (ctypes.c_int, [ctypes.POINTER(Model), ctypes.POINTER(StateDesc), vp, i32, vp, vp, i64, vp]),
         "rwkv7_wkv7": (ctypes.c_int, [vp, vp, vp, i32, vp, vp, vp, vp, vp, i32, i32, i32, i32, vp]),
         "rwkv7_wkv7_chunked_workspace_bytes": (ctypes.c_int64, [i32, i32, i32]),
         "rwkv7_wkv7_chunked": (ctypes.c_int, [vp, vp, vp, i32, vp, vp, vp, vp, vp, i32, i32, i32, i32, vp, i64, vp]),

@@ -212,6 +212,17 @@ class RWKV7HIP(RWKV7Model):
         )
         _lib.check(rc, "rwkv7_prefill")
 
+    def prefill_logits_into(self, tok: Tensor, S: State, logits: Tensor) -> None:
+        """Prefill ``tok`` int64 [B, T] on device into ``S``; ``logits`` [B, T, V] of the model's dtype."""
+        B, T = tok.shape
+        ws = self.workspace(B, T)
+        sd = self._desc(S)
+        rc = self._lib.rwkv7_prefill_logits(
+            ctypes.byref(self.dev.desc), ctypes.byref(sd), tok.data_ptr(), T, logits.data_ptr(), ws.data_ptr(),
+            ws.numel(), _lib.stream_handle(),
+        )
+        _lib.check(rc, "rwkv7_prefill_logits")
+
     # ------------------------------------------------------------------ #
     # RWKV7Model interface
     # ------------------------------------------------------------------ #
@@ -232,6 +243,16 @@ class RWKV7HIP(RWKV7Model):
 
     def prefill(self, tokens: Tensor, S: State) -> State:
         """Consume ``tokens`` (``[T]``, or ``[B, T]`` for a batched state) in place."""
+        return self._prefill(tokens, S, False)[1]
+
+    def prefill_logits(self, tokens: Tensor, S: State) -> tuple[Tensor, State]:
+        """``prefill`` with the logits after every token: ``[T, V]`` (``[B, T, V]``
+        for a batched state). What a teacher hands on to a student
+        (``kernels.top_logits``), and what drafted tokens are verified with
+        (``verify_draft``)."""
+        return self._prefill(tokens, S, True)
+
+    def _prefill(self, tokens: Tensor, S: State, with_logits: bool) -> tuple[Tensor | None, State]:
         self._check_state(S)
         tokens = torch.as_tensor(tokens)
         if tokens.numel() == 0:
@@ -248,12 +269,16 @@ class RWKV7HIP(RWKV7Model):
             shape = (1, tokens.shape[0])
         tok = self._tokens(tokens, shape)
         run, shadow = self._arena_state(S)
-        self.prefill_into(tok, run)
+        logits = torch.empty(*shape, self.V, dtype=self.kernel_dtype, device=self.w.device) if with_logits else None
+        if logits is None:
+            self.prefill_into(tok, run)
+        else:
+            self.prefill_logits_into(tok, run, logits)
         if shadow:
             _copy_into(S, run)
         if self.check_errors:
             self.raise_if_aborted()
-        return S
+        return (logits[0] if logits is not None and not batched else logits), S
 
 
 def _copy_into(dst, src: State) -> None:
