@@ -50,7 +50,7 @@ struct DistillArgs {
 };
 
 struct Joined {
-  float m, mrest;       // largest logit of the row, and without the entries' ids
+  float m, mrest;       // what the row's sum is about, and that without the entries' ids
   double S, Srest;      // sums about them
   double in_all;        // what a sum about mrest counts in one about m
   double W, tref;       // the teacher's mass about its reference
@@ -63,9 +63,10 @@ struct DistillLds {
   uint32_t tail;             // of the logits behind the eights
   int idx[kDistMaxK];        // of each thread's entry, -1 for none
   float z[kDistMaxK];        // its student logit
-  // per wave: the largest logit and the sum about it of the row's rest and of
-  // the entries; the teacher's reference, mass, and mass-weighted difference of
-  // its logarithms about that and the student's about mtop
+  // per wave: of the row's rest a logit and the sum about it, of the entries the
+  // largest and the sum about that; the teacher's reference, mass, and
+  // mass-weighted difference of its logarithms about that and the student's about
+  // mtop
   float mrest[kMaxWaves], rest[kMaxWaves], mtop[kMaxWaves];
   double top[kMaxWaves], tref[kMaxWaves], tw[kMaxWaves], ta[kMaxWaves];
   bool whole;  // every id of the vocabulary has an entry
@@ -196,22 +197,14 @@ __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : 8) void distill_kernel(Dist
 
   // this thread's part of the row without the entries' ids
   const u64 mine = s.mine[t];
-  if (mine) {
-#pragma unroll
-    for (int c = 0; c < kRowChunks; ++c) x[c].remove((uint32_t)(mine >> (kRowChunk * c)) & 255u);
-  }
   if (tail >= 0 && (s.tail >> t) & 1u) xt = -kInf;
-  float m;
-  {
-    RowMax<FMT> most;
-#pragma unroll
-    for (int c = 0; c < kRowChunks; ++c) most.add(x[c]);
-    m = wave_max(fmaxf(most.value(), xt));
-  }
-  opaque_row(x);
   const bool entries = wv * kWave < g.K;  // this wave has entries
-  const float mtop = entries ? wave_max(zv) : -kInf, rest = sum_row(x, xt, g.sc, m);
-  const float sum = wave_sum(rest);
+  const float mtop = entries ? wave_max(zv) : -kInf;
+  float m;
+  const float sum = sum_row<THREADS, false>(x, src, n8, xt, g.sc, m, [&](int c, Chunk<FMT> &y) {
+    const uint32_t marked = (uint32_t)(mine >> (kRowChunk * c)) & 255u;
+    if (marked) y.remove(marked);
+  });
 
   // the entries in 64 bits and powers of two: the student's about their largest,
   // the teacher's about its lse or the wave's largest (a gradient's q - p is what
@@ -254,7 +247,6 @@ __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : 8) void distill_kernel(Dist
     zero_row<FMT, THREADS>(dst, V);
   } else {
     const float f_rest = uniform_f(s.f_rest);
-    opaque_row(x);
     g.sc.with(s.j.mrest, [&](auto e2, auto far) {
 #pragma unroll
       for (int c = 0; c < kRowChunks; ++c) {

@@ -291,21 +291,58 @@ struct ExpScale {
   RWKV7_DEV double log2z(double S, float m) const { return (double)m * k + off(m) + log2_d(S); }
 };
 
-// Sum of exp(a x) about m over a thread's chunks.
-template <int FMT>
-RWKV7_DEV float sum_row(const Chunk<FMT> (&x)[kRowChunks], float tail, const ExpScale &sc, float m) {
-  float sum;
-  sc.with(m, [&](auto e2, auto far) {
-    sum = e2(tail);
+// Sum of exp(a x) over a wave's chunks, each handed to see(c, chunk) first, about a
+// logit of its own finding, m: the largest of the wave's first chunks, so that the
+// others are summed as they arrive and no pass goes before for the largest of
+// all. That is at least m, and the sum 1 or more; where it runs over (a logit 69 a
+// units above m), where the first chunks hold nothing, and far from 0, it is formed
+// again about the largest: from memory, a chunk at a time, which is rare and holds
+// nothing beside the row. KNOWN: m is the wave's largest already.
+template <int THREADS, bool KNOWN, int FMT, class See>
+RWKV7_DEV float sum_row(Chunk<FMT> (&x)[kRowChunks], const void *src, uint32_t n8, float tail, const ExpScale &sc, float &m,
+                        See see) {
+  see(0, x[0]);
+  if (!KNOWN) {
+    RowMax<FMT> first;
+    first.add(x[0]);
+    m = wave_max(first.value());
+  }
+  const bool good = m > -kInf && sc.near(m);
+  const float R = uniform_f(good ? m * sc.kf : 0.f);
+  float sum = sc.e_near(tail, R);
 #pragma unroll
-    for (int c = 0; c < kRowChunks; ++c) {
-      float f[kRowChunk], q[kRowChunk];
-      x[c].template get<decltype(far)::value>(f);
+  for (int c = 0; c < kRowChunks; ++c) {
+    if (c > 0) see(c, x[c]);
+    float f[kRowChunk], q[kRowChunk];
+    x[c].get(f);
 #pragma unroll
-      for (int e = 0; e < kRowChunk; ++e) q[e] = e2(f[e]);
-      sum += ((q[0] + q[1]) + (q[2] + q[3])) + ((q[4] + q[5]) + (q[6] + q[7]));
-    }
-  });
+    for (int e = 0; e < kRowChunk; ++e) q[e] = sc.e_near(f[e], R);
+    sum += ((q[0] + q[1]) + (q[2] + q[3])) + ((q[4] + q[5]) + (q[6] + q[7]));
+  }
+  sum = wave_sum(sum);
+  opaque_row(x);
+  if (!(good && sum >= 0.5f && sum < 0x1p100f)) {  // (wave-uniform)
+    auto each = [&](auto f) {
+#pragma unroll 1
+      for (int c = 0; c < kRowChunks; ++c) {
+        Chunk<FMT> y;
+        y.load(src, c * THREADS + threadIdx.x, n8);
+        see(c, y);
+        f(y);
+      }
+    };
+    RowMax<FMT> most;
+    each([&](const Chunk<FMT> &y) { most.add(y); });
+    m = wave_max(fmaxf(most.value(), tail));
+    sum = sc.e(tail, m);
+    each([&](const Chunk<FMT> &y) {
+      float f[kRowChunk];
+      y.get(f);
+#pragma unroll
+      for (int e = 0; e < kRowChunk; ++e) sum += sc.e(f[e], m);
+    });
+    sum = wave_sum(sum);
+  }
   return sum;
 }
 

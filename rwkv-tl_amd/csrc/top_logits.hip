@@ -153,8 +153,8 @@ __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : THREADS == 256 ? 7 : 8) voi
 
   // the lane's largest, by groups of chunks (-inf also for none: a floor may be
   // too low, never too high)
-  float m = -kInf;
   uint32_t own[kGroups];
+  float m = -kInf;
   {
     RowMax<FMT> most[kGroups];
 #pragma unroll
@@ -179,8 +179,7 @@ __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : THREADS == 256 ? 7 : 8) voi
     if (lane == 0) s.floor[wv] = fl, s.some[wv] = some;
   }
   m = wave_max(m);
-  const float sum = wave_sum(sum_row(x, xt, g.sc, m));
-  opaque_row(x);
+  const float sum = sum_row<THREADS, true>(x, src, n8, xt, g.sc, m, [](int, Chunk<FMT> &) {});
   if (lane == 0) s.m[wv] = m, s.sum[wv] = sum;
   __syncthreads();
 

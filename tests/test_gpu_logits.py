@@ -303,6 +303,26 @@ def test_top_logits_far_from_zero(cuda, dtype):
         _check_top(x.to(dtype).to(cuda), 40, T)
 
 
+@pytest.mark.parametrize("dtype", [H, B16, F], ids=str)
+@pytest.mark.parametrize("V", [20003, 65536])
+def test_distill_rows_whose_first_logits_say_little(cuda, dtype, V):
+    """A wave's sum is about the largest of its first 512 logits: rows that rise by hundreds behind them, whose first ones
+    are masked, or the highest by hundreds."""
+    g = _gen(43, V)
+    z, val, idx, lse = _case(g, 5, V, 20, F, 1.0, True)
+    z[0, V // 2:] += 300.0
+    z[1, V - 3:] += 90.0
+    z[2, :V // 4] = -INF
+    z[2, idx[2]] = 0.0
+    z[3, :V // 4] += 500.0
+    z[4, :V - 100] = torch.finfo(dtype).min
+    z[4, idx[4]] = 0.0
+    _check_distill(cuda, z.to(dtype), val, idx, lse)
+    x = z.clone()
+    x[4, ::7] = -INF
+    _check_top(x.to(dtype).to(cuda), 30)
+
+
 def test_distill_infinite_and_nan_rows(cuda):
     z = torch.zeros(6, 40)
     val, idx = torch.zeros(6, 3), torch.tensor([[1, 2, 3]]).repeat(6, 1)
