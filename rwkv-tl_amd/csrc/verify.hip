@@ -25,11 +25,13 @@
 // verify_stats_kernel: a slice of a row per workgroup: the sum of its
 //   exponentials, about 0 or its largest logit, for target rows also of each 512
 //   logits (greedy: largest logit and its first id).
-// verify_rest_kernel: 2048 logits of each sequence's decisive row: every workgroup
+// verify_draw_kernel: 2048 logits of each sequence's decisive row: every workgroup
 //   joins the sums of its sequence's rows and decides how many tokens are
-//   accepted; the sums of max(p - q, 0) over each 512 of its logits.
-// verify_draw_kernel: one wave per sequence: finds the 512 in which the running
-//   sum crosses, and in them the token.
+//   accepted; the sums of max(p - q, 0) over each 512 of its logits; the last
+//   workgroup of a sequence to finish (the only one that stays, where all tokens
+//   are accepted) finds the 512 in which the running sum crosses, and in them the
+//   token, by one wave. (As a launch of its own this draw took 3 us more of a call's
+//   chain and 2 of its host time.)
 #include "logits_rows.h"
 #include "rwkv7_kernels.h"
 
@@ -51,7 +53,6 @@ struct Decision {
   int n, rejected;  // accepted tokens; whether the next was drafted and rejected
   int x;            // the rejected token of a one-hot draft, else -1
   float mp, mq;     // what the sums of the row behind the accepted tokens are about, of target and draft
-  float pad;
   double ip, iq;    // 1 / those sums, 0 for an empty row or none
 };
 
@@ -68,7 +69,7 @@ struct VerifyArgs {
   double *sum;                 // [rows][G] sum of exponentials about m (greedy: first id of the largest)
   double *block;               // [B (K + 1)][G kBlocks + 1] the same by blocks; last: the logits behind the eights
   double *rest;                // [B][G kBlocks + 1] sums of max(p - q, 0)
-  Decision *dec;               // [B]
+  int *done;                   // [B] workgroups that have stored theirs
   float *m;                    // [rows][G] what a slice's sums are about: 0 or its largest logit (greedy: that); rows: B
                                // (K + 1) of the target, B K of the draft
 };
@@ -128,6 +129,7 @@ __global__ __launch_bounds__(kVerThreads) void verify_stats_kernel(VerifyArgs a)
   const bool tgt = r < nt;
   const int per = tgt ? a.K + 1 : a.K, rr = tgt ? r : r - nt, b = rr / per, i = rr - b * per;
   const int len = drafted(a, b);
+  if (tgt && i == 0 && g == 0 && t == 0) a.done[b] = 0;
   if (i >= (tgt ? len + 1 : len)) return;  // a row that no decision looks at
   const void *row = tgt ? target_row<FMT>(a, b, i) : draft_row<FMT>(a, b, i);
   const uint32_t n8 = (uint32_t)V / kRowChunk;
@@ -268,7 +270,6 @@ RWKV7_DEV void decide(const VerifyArgs &a, int b, DecideLds &s) {
       const bool soft = rejected && a.draft;
       d.mq = soft ? s.m[1][n] : 0.f;
       d.iq = soft && s.S[1][n] > 0.0 ? 1.0 / s.S[1][n] : 0.0;
-      d.pad = 0.f;
       s.d = d;
     }
   }
@@ -295,45 +296,6 @@ struct Residual {
   }
 };
 
-template <int FMT>
-__global__ __launch_bounds__(kVerThreads) void verify_rest_kernel(VerifyArgs a) {
-  __shared__ DecideLds s;
-  const int t = threadIdx.x, lane = t & 63, wv = t >> 6, V = a.V, g = blockIdx.x, b = blockIdx.y;
-  decide<FMT>(a, b, s);
-  const Decision d = s.d;
-  if (g == 0 && t == 0) a.dec[b] = d;
-  if (!d.rejected) return;
-  const void *pr = target_row<FMT>(a, b, d.n), *qr = a.draft ? draft_row<FMT>(a, b, d.n) : pr;
-  const uint32_t n8 = (uint32_t)V / kRowChunk, e8 = g * kVerThreads + t;
-  const Residual res(a, d, false);
-  double *block = a.rest + (int64_t)b * (a.G * kBlocks + 1);
-  Chunk<FMT> xp, xq;
-  xp.load(pr, e8, n8);
-  xq.load(qr, e8, n8);
-  float fp[kRowChunk], fq[kRowChunk];
-  xp.get(fp);
-  xq.get(fq);
-  double sum = 0.0;
-  if (d.mp == 0.f && d.mq == 0.f) {
-    const BulkWeight p(a.kt), q(a.kd);
-#pragma unroll
-    for (int e = 0; e < kRowChunk; ++e) {
-      const double r = res.soft ? over(p(fp[e]), d.ip, q(fq[e]), d.iq) : p(fp[e]) * d.ip;
-      sum += (int)e8 * kRowChunk + e == d.x ? 0.0 : r;
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < kRowChunk; ++e) sum += res(fp[e], fq[e], (int)e8 * kRowChunk + e);
-  }
-  sum = wave_sum_d(sum);
-  if (lane == 0) block[g * kVerWaves + wv] = sum;
-  if (g == a.G * kVerChunks - 1 && wv == 0) {  // the logits behind the eights
-    const int id = (int)n8 * kRowChunk + t;
-    sum = wave_sum_d(id < V ? res(load_logit<FMT>(pr, id), load_logit<FMT>(qr, id), id) : 0.0);
-    if (lane == 0) block[a.G * kBlocks] = sum;
-  }
-}
-
 RWKV7_DEV double shfl_up_d(double x, int d) {
   const u64 v = __builtin_bit_cast(u64, x);
   const int lo = __shfl_up((int)(uint32_t)v, d), hi = __shfl_up((int)(uint32_t)(v >> 32), d);
@@ -349,11 +311,11 @@ RWKV7_DEV double wave_scan_d(double v) {
   return v;
 }
 
+// The token behind the accepted ones, and the outputs, by one wave.
 template <int FMT>
-__global__ __launch_bounds__(kWave) void verify_draw_kernel(VerifyArgs a) {
-  const int lane = threadIdx.x, V = a.V, b = blockIdx.x, blocks = a.G * kBlocks + 1;
+RWKV7_DEV void draw(const VerifyArgs &a, int b, const Decision &d) {
+  const int lane = threadIdx.x, V = a.V, blocks = a.G * kBlocks + 1;
   const uint32_t n8 = (uint32_t)V / kRowChunk;
-  const Decision d = a.dec[b];
   const double u = (double)a.u[(int64_t)b * (a.K + 1) + a.K];
   const int64_t r = (int64_t)b * (a.K + 1) + d.n;
   // this lane's block sums of what is drawn from: p - q, or p itself
@@ -362,7 +324,10 @@ __global__ __launch_bounds__(kWave) void verify_draw_kernel(VerifyArgs a) {
   if (d.rejected) {
 #pragma unroll
     for (int e = 0; e < kDrawE; ++e) {
-      w[e] = kDrawE * lane + e < blocks ? a.rest[(int64_t)b * blocks + kDrawE * lane + e] : 0.0;
+      // (device-scope, as they were stored: other workgroups' of this launch)
+      w[e] = kDrawE * lane + e < blocks ? __hip_atomic_load(a.rest + (int64_t)b * blocks + kDrawE * lane + e, __ATOMIC_RELAXED,
+                                                            __HIP_MEMORY_SCOPE_AGENT)
+                                        : 0.0;
       if (!(w[e] > kNothing)) w[e] = 0.0;
     }
     from_p = !(wave_sum_d((w[0] + w[1]) + w[2]) > 0.0);
@@ -445,6 +410,56 @@ __global__ __launch_bounds__(kWave) void verify_draw_kernel(VerifyArgs a) {
   if (lane == 0) a.accepted[b] = d.n;
 }
 
+template <int FMT>
+__global__ __launch_bounds__(kVerThreads) void verify_draw_kernel(VerifyArgs a) {
+  __shared__ DecideLds s;
+  __shared__ bool s_last;
+  const int t = threadIdx.x, lane = t & 63, wv = t >> 6, V = a.V, g = blockIdx.x, b = blockIdx.y;
+  decide<FMT>(a, b, s);
+  const Decision d = s.d;
+  if (!d.rejected) {
+    if (g == 0 && wv == 0) draw<FMT>(a, b, d);
+    return;
+  }
+  const void *pr = target_row<FMT>(a, b, d.n), *qr = a.draft ? draft_row<FMT>(a, b, d.n) : pr;
+  const uint32_t n8 = (uint32_t)V / kRowChunk, e8 = g * kVerThreads + t;
+  const Residual res(a, d, false);
+  double *block = a.rest + (int64_t)b * (a.G * kBlocks + 1);
+  Chunk<FMT> xp, xq;
+  xp.load(pr, e8, n8);
+  xq.load(qr, e8, n8);
+  float fp[kRowChunk], fq[kRowChunk];
+  xp.get(fp);
+  xq.get(fq);
+  double sum = 0.0;
+  if (d.mp == 0.f && d.mq == 0.f) {
+    const BulkWeight p(a.kt), q(a.kd);
+#pragma unroll
+    for (int e = 0; e < kRowChunk; ++e) {
+      const double r = res.soft ? over(p(fp[e]), d.ip, q(fq[e]), d.iq) : p(fp[e]) * d.ip;
+      sum += (int)e8 * kRowChunk + e == d.x ? 0.0 : r;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < kRowChunk; ++e) sum += res(fp[e], fq[e], (int)e8 * kRowChunk + e);
+  }
+  sum = wave_sum_d(sum);
+  // stored past the caches of this XCD, acknowledged before the count goes up
+  auto put = [&](int i, double v) { __hip_atomic_store(block + i, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+  if (lane == 0) put(g * kVerWaves + wv, sum);
+  if (g == a.G * kVerChunks - 1 && wv == 0) {  // the logits behind the eights
+    const int id = (int)n8 * kRowChunk + t;
+    sum = wave_sum_d(id < V ? res(load_logit<FMT>(pr, id), load_logit<FMT>(qr, id), id) : 0.0);
+    if (lane == 0) put(a.G * kBlocks, sum);
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (t == 0)
+    s_last = __hip_atomic_fetch_add(a.done + b, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.G * kVerChunks - 1;
+  __syncthreads();
+  if (s_last && wv == 0) draw<FMT>(a, b, d);
+}
+
 // Greedy: one wave per sequence, a lane per drafted token.
 __global__ __launch_bounds__(kWave) void verify_greedy_kernel(VerifyArgs a) {
   const int lane = threadIdx.x, b = blockIdx.x, len = drafted(a, b);
@@ -483,9 +498,7 @@ int launch_verify(const VerifyArgs &a, hipStream_t st) {
   }
   verify_stats_kernel<FMT, false><<<grid, kVerThreads, 0, st>>>(a);
   RWKV7_CHECK_LAUNCH();
-  verify_rest_kernel<FMT><<<dim3(a.G * kVerChunks, a.B), kVerThreads, 0, st>>>(a);
-  RWKV7_CHECK_LAUNCH();
-  verify_draw_kernel<FMT><<<a.B, kWave, 0, st>>>(a);
+  verify_draw_kernel<FMT><<<dim3(a.G * kVerChunks, a.B), kVerThreads, 0, st>>>(a);
   RWKV7_CHECK_LAUNCH();
   return RWKV7_OK;
 }
@@ -504,7 +517,7 @@ int64_t verify_ws(VerifyArgs &a, char *p) {
   a.sum = reinterpret_cast<double *>(take(rows * a.G * 8));
   a.block = reinterpret_cast<double *>(take((int64_t)a.B * (a.K + 1) * blocks * 8));
   a.rest = reinterpret_cast<double *>(take(a.B * blocks * 8));
-  a.dec = reinterpret_cast<Decision *>(take((int64_t)a.B * sizeof(Decision)));
+  a.done = reinterpret_cast<int *>(take((int64_t)a.B * 4));
   a.m = reinterpret_cast<float *>(take(rows * a.G * 4));
   return p - p0;
 }

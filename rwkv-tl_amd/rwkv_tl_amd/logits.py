@@ -19,6 +19,7 @@ from __future__ import annotations
 
 import math
 from collections.abc import Callable
+from functools import lru_cache
 
 import torch
 from torch import Tensor
@@ -176,6 +177,11 @@ def _strides(x: Tensor, V: int) -> Tensor:
     return x if ok else x.contiguous()
 
 
+@lru_cache(maxsize=64)
+def _verify_bytes(B: int, K: int, V: int) -> int:
+    return _lib.load().rwkv7_verify_workspace_bytes(B, K, V)
+
+
 def verify_draft(
     target_logits: Tensor,
     draft_tokens: Tensor,
@@ -244,7 +250,7 @@ def verify_draft(
             tok = tokens.contiguous()
             u = None if greedy else uniforms.contiguous()
             n = None if lengths is None else lengths.contiguous()
-            nb = lib.rwkv7_verify_workspace_bytes(B, K, V)
+            nb = _verify_bytes(B, K, V)
             ws = torch.empty(nb, dtype=torch.uint8, device=target.device)
             rc = lib.rwkv7_verify(
                 t.data_ptr(), t.stride(0), t.stride(1) if K else V, _lib.ptr(d), 0 if d is None else d.stride(0),

@@ -156,6 +156,12 @@ LOGITS_OPS: dict[str, tuple[str, Callable, Callable]] = {
 }
 
 
+def _plain(x: Tensor) -> bool:
+    """Whether a call on ``x`` may go straight to the kernel: no tracing, no
+    dispatch mode that wants to see the operator."""
+    return type(x) is Tensor and x.is_cuda and not torch._C._len_torch_dispatch_stack()
+
+
 class _DistillLoss(torch.autograd.Function):
     """The Autograd kernel of ``distill_loss``. (torch.library.register_autograd
     makes one like it that takes 28 us more of a call's host time.)"""
@@ -166,15 +172,16 @@ class _DistillLoss(torch.autograd.Function):
             raise ValueError("distill_loss has no gradient to the teacher: detach top_val and lse")
         ctx.save_for_backward(logits, top_val, top_idx, lse)
         ctx.temperature = temperature
+        if _plain(logits):
+            return K.distill_loss(logits, top_val, top_idx, lse, temperature=temperature)
         with torch._C._AutoDispatchBelowAutograd():
             return torch.ops.rwkv_tl.distill_loss(logits, top_val, top_idx, lse, temperature)
 
     @staticmethod
     def backward(ctx, grad_loss):
         args = (grad_loss, *ctx.saved_tensors, ctx.temperature)
-        # a plain backward pass calls the kernel; tracing, and a gradient that is to
-        # be differentiated, go through the operator
-        plain = type(grad_loss) is Tensor and grad_loss.is_cuda and not torch.is_grad_enabled()
+        # (a gradient that is to be differentiated goes through the operator, which refuses)
+        plain = _plain(grad_loss) and not torch.is_grad_enabled()
         return (K.distill_loss_backward if plain else torch.ops.rwkv_tl.distill_loss_backward)(*args), None, None, None, None
 
 
