@@ -47,6 +47,7 @@ struct DistillArgs {
   float *loss;         // null: not wanted
   void *grad;          // null: not wanted
   int64_t grad_ld;
+  int64_t row0;
 };
 
 struct Joined {
@@ -145,7 +146,7 @@ __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : 8) void distill_kernel(Dist
   constexpr int kWaves = THREADS / kWave;
   const int t = threadIdx.x, lane = t & 63, wv = t >> 6, V = g.V;
   const uint32_t n8 = (uint32_t)V / kRowChunk;
-  const int64_t row = blockIdx.x;
+  const int64_t row = g.row0 + blockIdx.x;
   const char *src = static_cast<const char *>(g.logits) + row * g.ld * kLogitBytes<FMT>;
   char *dst = GRAD ? static_cast<char *>(g.grad) + row * g.grad_ld * kLogitBytes<FMT> : nullptr;
   const float up = GRAD ? (g.scale ? g.scale[row] : g.scale0) : 0.f;
@@ -311,13 +312,16 @@ extern "C" int rwkv7_distill(const void *logits, int32_t logits_dtype, int64_t l
   if (!(temperature > 0.0) || temperature > 1e30 || temperature < 1e-30) return RWKV7_EINVAL;
   if (N < 1 || V < 1 || V > kRowMaxV || K < 1 || K > kDistMaxK || ld < V || (grad && grad_ld < V)) return RWKV7_ESHAPE;
   const double a = 1.0 / temperature;
-  const DistillArgs g = {logits, ld, V, K, ExpScale::of(a), a, top_val, val_dtype, top_idx, lse, scale, scale0, loss, grad, grad_ld};
+  DistillArgs g = {logits, ld, V, K, ExpScale::of(a), a, top_val, val_dtype, top_idx, lse, scale, scale0, loss, grad, grad_ld, 0};
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  switch (logits_dtype) {
-    case 0: launch_f<0>(g, N, st); break;
-    case 1: launch_f<1>(g, N, st); break;
-    default: launch_f<2>(g, N, st); break;
+  for (; g.row0 < N; g.row0 += kLaunchRows) {
+    const int n = N - g.row0 < kLaunchRows ? (int)(N - g.row0) : kLaunchRows;
+    switch (logits_dtype) {
+      case 0: launch_f<0>(g, n, st); break;
+      case 1: launch_f<1>(g, n, st); break;
+      default: launch_f<2>(g, n, st); break;
+    }
+    RWKV7_CHECK_LAUNCH();
   }
-  RWKV7_CHECK_LAUNCH();
   return RWKV7_OK;
 }

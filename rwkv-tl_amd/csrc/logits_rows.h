@@ -20,6 +20,9 @@ constexpr int kMaxWaves = kRowMaxThreads / kWave;
 // that hold them, so that short rows leave room for more workgroups per CU.
 inline int row_threads(int V) { return V <= 256 * kRowE ? 256 : V <= 512 * kRowE ? 512 : 1024; }
 
+// Rows of one launch, a workgroup each: a grid has fewer than 2^32 threads.
+constexpr int kLaunchRows = 1 << 21;
+
 // Bytes per logit: FMT 0 half, 1 f32, 2 bfloat16.
 template <int FMT>
 constexpr int kLogitBytes = FMT == 1 ? 4 : 2;

@@ -33,6 +33,7 @@ struct TopArgs {
   void *val;
   int64_t *idx;
   float *lse;
+  int64_t row0;
 };
 
 constexpr int kBins = 256;
@@ -142,7 +143,7 @@ __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : THREADS == 256 ? 7 : 8) voi
   constexpr int kWaves = THREADS / kWave;
   const int t = threadIdx.x, lane = t & 63, wv = t >> 6, V = g.V, k = g.k;
   const uint32_t n8 = (uint32_t)V / kRowChunk;
-  const int64_t row = blockIdx.x;
+  const int64_t row = g.row0 + blockIdx.x;
   const char *src = static_cast<const char *>(g.logits) + row * g.ld * kLogitBytes<FMT>;
   Chunk<FMT> x[kRowChunks];
   load_row<THREADS>(x, src, n8);
@@ -316,13 +317,16 @@ extern "C" int rwkv7_top_logits(const void *logits, int32_t logits_dtype, int64_
   if (!logits || !val || !idx || !lse || logits_dtype < 0 || logits_dtype > 2) return RWKV7_EINVAL;
   if (!(temperature >= 1e-30 && temperature <= 1e30)) return RWKV7_EINVAL;
   if (N < 1 || V < 1 || V > kRowMaxV || ld < V || k < 1 || k > V || k > kTopMax) return RWKV7_ESHAPE;
-  const TopArgs g = {logits, ld, V, k, ExpScale::of(1.0 / temperature), val, idx, lse};
+  TopArgs g = {logits, ld, V, k, ExpScale::of(1.0 / temperature), val, idx, lse, 0};
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  switch (logits_dtype) {
-    case 0: launch_top<0>(g, N, st); break;
-    case 1: launch_top<1>(g, N, st); break;
-    default: launch_top<2>(g, N, st); break;
+  for (; g.row0 < N; g.row0 += kLaunchRows) {
+    const int n = N - g.row0 < kLaunchRows ? (int)(N - g.row0) : kLaunchRows;
+    switch (logits_dtype) {
+      case 0: launch_top<0>(g, n, st); break;
+      case 1: launch_top<1>(g, n, st); break;
+      default: launch_top<2>(g, n, st); break;
+    }
+    RWKV7_CHECK_LAUNCH();
   }
-  RWKV7_CHECK_LAUNCH();
   return RWKV7_OK;
 }

@@ -18,7 +18,6 @@ be captured in a HIP graph. Each call allocates what it returns, and
 from __future__ import annotations
 
 import math
-from collections.abc import Callable
 from functools import lru_cache
 
 import torch
@@ -34,19 +33,17 @@ MAX_DRAFT = 63  # drafted tokens per sequence of verify_draft
 LOGIT_DTYPES = {torch.float16: 0, torch.float32: 1, torch.bfloat16: 2}
 
 
-def _need(cond: bool, msg: str | Callable[[], str]) -> None:
-    """``msg``: a text, or what makes it (formed only where the check fails)."""
-    if not cond:
-        raise ValueError(msg if isinstance(msg, str) else msg())
-
-
 def _check_logits(x: Tensor, name: str) -> int:
     """The logits' dtype code."""
-    _need(isinstance(x, Tensor), lambda: f"{name} must be a tensor")
-    _need(x.is_cuda, lambda: f"{name} on {x.device}; the HIP kernels need a ROCm device")
+    if not isinstance(x, Tensor):
+        raise ValueError(f"{name} must be a tensor")
+    if not x.is_cuda:
+        raise ValueError(f"{name} on {x.device}; the HIP kernels need a ROCm device")
     code = LOGIT_DTYPES.get(x.dtype)
-    _need(code is not None, lambda: f"{name} must be float16, bfloat16 or float32, got {x.dtype}")
-    _need(x.ndim >= 1 and 1 <= x.shape[-1] <= MAX_VOCAB, lambda: f"{name}: a vocabulary of 1..{MAX_VOCAB}, got {tuple(x.shape)}")
+    if code is None:
+        raise ValueError(f"{name} must be float16, bfloat16 or float32, got {x.dtype}")
+    if x.ndim < 1 or not 1 <= x.shape[-1] <= MAX_VOCAB:
+        raise ValueError(f"{name}: a vocabulary of 1..{MAX_VOCAB}, got {tuple(x.shape)}")
     return code
 
 
@@ -54,10 +51,12 @@ def _rows(x: Tensor) -> tuple[Tensor, int, int]:
     """``[..., V]`` as rows of adjacent columns that do not overlap: what holds them
     (a copy only where no view is one), their number and their stride."""
     V = x.shape[-1]
+    N = x.numel() // V
+    if N > 2**31 - 1:
+        raise ValueError(f"{N} rows are too many for one call")
     if x.is_contiguous():
-        return x, x.numel() // V, V
-    x = x.reshape(-1, V)
-    N = x.shape[0]
+        return x, N, V
+    x = x.reshape(N, V)
     if (x.stride(1) != 1 and V > 1) or (N > 1 and x.stride(0) < V):
         x = x.contiguous()
     return x, N, x.stride(0) if N > 1 else V
@@ -65,7 +64,8 @@ def _rows(x: Tensor) -> tuple[Tensor, int, int]:
 
 def _temperature(t: float) -> float:
     t = float(t)
-    _need(1e-30 <= t <= 1e30, lambda: f"temperature must be positive and finite, got {t}")
+    if not 1e-30 <= t <= 1e30:  # (NaN neither)
+        raise ValueError(f"temperature must be positive and finite, got {t}")
     return t
 
 
@@ -85,7 +85,8 @@ def top_logits(logits: Tensor, k: int, *, temperature: float = 1.0) -> tuple[Ten
     answers as ``distill_loss`` takes them."""
     code = _check_logits(logits, "logits")
     V = logits.shape[-1]
-    _need(isinstance(k, int) and 1 <= k <= min(V, MAX_TOP), lambda: f"k must be in 1..{min(V, MAX_TOP)}, got {k}")
+    if not isinstance(k, int) or not 1 <= k <= min(V, MAX_TOP):
+        raise ValueError(f"k must be in 1..{min(V, MAX_TOP)}, got {k}")
     temperature = _temperature(temperature)
     lead = logits.shape[:-1]
     with _lib.device_of(logits):
@@ -106,35 +107,40 @@ def _distill(logits, top_val, top_idx, lse, temperature, scale, want_loss: bool,
     shape = logits.shape
     lead, V = shape[:-1], shape[-1]
     ts = top_val.shape
-    _need(ts[:-1] == lead and top_idx.shape == ts and len(ts) == len(shape),
-          lambda: f"top_val and top_idx must be [{', '.join(map(str, (*lead, 'K')))}], got {tuple(ts)} and {tuple(top_idx.shape)}")
+    if ts[:-1] != lead or top_idx.shape != ts or len(ts) != len(shape):
+        raise ValueError(f"top_val and top_idx must be [{', '.join(map(str, (*lead, 'K')))}], got {tuple(ts)} and {tuple(top_idx.shape)}")
     K = ts[-1]
-    _need(K <= MAX_ENTRIES, lambda: f"at most {MAX_ENTRIES} teacher entries per row, got {K}")
+    if K > MAX_ENTRIES:
+        raise ValueError(f"at most {MAX_ENTRIES} teacher entries per row, got {K}")
     tcode = LOGIT_DTYPES.get(top_val.dtype)
-    _need(tcode is not None, lambda: f"top_val must be float16, bfloat16 or float32, got {top_val.dtype}")
-    _need(top_idx.dtype is torch.int64, lambda: f"top_idx must be int64, got {top_idx.dtype}")
-    _need(lse is None or (lse.shape == lead and lse.dtype is torch.float32), lambda: f"lse must be float32 {tuple(lead)}")
-    rowwise = isinstance(scale, Tensor)
-    _need(not rowwise or (scale.shape == lead and scale.dtype is torch.float32), lambda: f"scale must be float32 {tuple(lead)}")
-    _same_device(logits, top_val, top_idx, lse, scale if rowwise else None)
+    if tcode is None:
+        raise ValueError(f"top_val must be float16, bfloat16 or float32, got {top_val.dtype}")
+    if top_idx.dtype is not torch.int64:
+        raise ValueError(f"top_idx must be int64, got {top_idx.dtype}")
+    if lse is not None and (lse.shape != lead or lse.dtype is not torch.float32):
+        raise ValueError(f"lse must be float32 {tuple(lead)}")
+    rows = scale if isinstance(scale, Tensor) else None
+    if rows is not None and (rows.shape != lead or rows.dtype is not torch.float32):
+        raise ValueError(f"scale must be float32 {tuple(lead)}")
+    _same_device(logits, top_val, top_idx, lse, rows)
     temperature = _temperature(temperature)
     with _lib.device_of(logits):
+        loss = torch.empty(lead, dtype=torch.float32, device=logits.device) if want_loss else None
+        grad = torch.empty(shape, dtype=logits.dtype, device=logits.device) if want_grad else None
         x, N, ld = _rows(logits)
-        loss = torch.empty(lead, dtype=torch.float32, device=x.device) if want_loss else None
-        grad = torch.empty(shape, dtype=x.dtype, device=x.device) if want_grad else None
-        if N and not K:  # no teacher at all
-            for t in (loss, grad):
-                if t is not None:
-                    t.zero_()
-        elif N:
+        if N and K:
             tv, ti = top_val.contiguous(), top_idx.contiguous()
             ls = None if lse is None else lse.contiguous()
-            sc = scale.contiguous() if rowwise else None
+            sc = None if rows is None else rows.contiguous()
             rc = _lib.load().rwkv7_distill(
                 x.data_ptr(), code, ld, N, V, tv.data_ptr(), tcode, ti.data_ptr(), K, _lib.ptr(ls), temperature,
-                _lib.ptr(sc), 1.0 if rowwise else float(scale), _lib.ptr(loss), _lib.ptr(grad), V, _lib.stream_of(x),
+                _lib.ptr(sc), 1.0 if rows is not None else float(scale), _lib.ptr(loss), _lib.ptr(grad), V, _lib.stream_of(x),
             )
             _lib.check(rc, "rwkv7_distill")
+        else:
+            for t in (loss, grad):
+                if t is not None:
+                    t.zero_()  # rows without any teacher
     return loss, grad
 
 
@@ -149,8 +155,9 @@ def distill_loss(logits: Tensor, top_val: Tensor, top_idx: Tensor, lse: Tensor |
     gradient 0 whatever its logits hold (a padded position). With ``lse [...]``
     float32, the teacher's log-sum-exp over its whole vocabulary at the same
     temperature, ``p_k = exp(top_val_k / temperature - lse)`` and the mass that
-    this leaves (if 2^-20 or more) is held against the student's mass outside the row's ids; without
-    it, ``p`` is the softmax of the entries. There is no factor ``temperature ** 2``.
+    this leaves (2^-20 or more, of a row that does not list every id) is held against
+    the student's mass outside the row's ids; without it, ``p`` is the softmax of the
+    entries. There is no factor ``temperature ** 2``.
 
     Without autograd; ``torch.ops.rwkv_tl.distill_loss`` is the differentiable form."""
     return _distill(logits, top_val, top_idx, lse, temperature, 1.0, True, False)[0]
@@ -213,32 +220,38 @@ def verify_draft(
     up = (lambda t: None if t is None else t.unsqueeze(0)) if single else (lambda t: t)
     target, tokens, draft = up(target_logits), up(draft_tokens), up(draft_logits)
     uniforms, lengths = up(uniforms), up(lengths)
-    _need(target.ndim == 3 and target.shape[1] >= 1, lambda: f"target_logits must be [B, K + 1, V], got {tuple(target_logits.shape)}")
+    if target.ndim != 3 or target.shape[1] < 1:
+        raise ValueError(f"target_logits must be [B, K + 1, V], got {tuple(target_logits.shape)}")
     B, K, V = target.shape[0], target.shape[1] - 1, target.shape[2]
-    _need(K <= MAX_DRAFT, lambda: f"at most {MAX_DRAFT} drafted tokens, got {K}")
-    _need(B * (2 * K + 1) <= 65535, lambda: f"a batch of {B} with {K} drafts is too large: at most {65535 // (2 * K + 1)}")
-    _need(tokens.shape == (B, K) and tokens.dtype == torch.int64,
-          lambda: f"draft_tokens must be int64 [{B}, {K}], got {tokens.dtype} {tuple(tokens.shape)}")
+    if K > MAX_DRAFT:
+        raise ValueError(f"at most {MAX_DRAFT} drafted tokens, got {K}")
+    if B * (2 * K + 1) > 65535:
+        raise ValueError(f"a batch of {B} with {K} drafts is too large: at most {65535 // (2 * K + 1)}")
+    if tokens.shape != (B, K) or tokens.dtype is not torch.int64:
+        raise ValueError(f"draft_tokens must be int64 [{B}, {K}], got {tokens.dtype} {tuple(tokens.shape)}")
     temperature = 0.0 if temperature is None else float(temperature)
     greedy = temperature <= 0
     if not greedy:
         _temperature(temperature)
-        _need(uniforms is not None, "uniforms are needed unless the temperature is None or <= 0")
+        if uniforms is None:
+            raise ValueError("uniforms are needed unless the temperature is None or <= 0")
     draft_temperature = temperature if draft_temperature is None else float(draft_temperature)
-    _need(not math.isnan(draft_temperature), "draft_temperature is NaN")
+    if math.isnan(draft_temperature):
+        raise ValueError("draft_temperature is NaN")
     if uniforms is not None:
-        _need(uniforms.shape == (B, K + 1) and uniforms.dtype == torch.float32,
-              lambda: f"uniforms must be float32 [{B}, {K + 1}], got {uniforms.dtype} {tuple(uniforms.shape)}")
+        if uniforms.shape != (B, K + 1) or uniforms.dtype is not torch.float32:
+            raise ValueError(f"uniforms must be float32 [{B}, {K + 1}], got {uniforms.dtype} {tuple(uniforms.shape)}")
     if draft is not None:
         _check_logits(draft, "draft_logits")
-        _need(draft.shape == (B, K, V) and draft.dtype == target.dtype,
-              lambda: f"draft_logits must be {target.dtype} [{B}, {K}, {V}], got {draft.dtype} {tuple(draft.shape)}")
+        if draft.shape != (B, K, V) or draft.dtype is not target.dtype:
+            raise ValueError(f"draft_logits must be {target.dtype} [{B}, {K}, {V}], got {draft.dtype} {tuple(draft.shape)}")
         if not greedy and draft_temperature > 0:
             _temperature(draft_temperature)
         else:
             draft = None
     if lengths is not None:
-        _need(lengths.shape == (B,) and lengths.dtype == torch.int64, lambda: f"lengths must be int64 [{B}]")
+        if lengths.shape != (B,) or lengths.dtype is not torch.int64:
+            raise ValueError(f"lengths must be int64 [{B}]")
     _same_device(target, tokens, None if greedy else uniforms, draft, lengths)
     with _lib.device_of(target):
         out = torch.empty(B, K + 1, dtype=torch.int64, device=target.device)

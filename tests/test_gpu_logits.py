@@ -14,7 +14,10 @@ with a < -log q, and half a step of the type it is stored in.
 
 from __future__ import annotations
 
+import math
+
 import pytest
+
 import torch
 
 import rwkv_tl_amd  # noqa: F401
@@ -141,6 +144,24 @@ def test_top_logits_rows_past_2_to_the_31_elements(cuda):
     assert (loss.double() - want).abs().max() < 56 * U + U * want
     assert bool((grad[torch.arange(N, device=cuda), hot].double() + (1 - 2.718281828459045 ** -want)).abs().max() < 1e-3)
     assert bool((grad != 0).sum(-1).min() == grad.shape[1])
+
+
+def test_more_rows_than_a_launch_has(cuda):
+    # Rows of the same logits have the same bits. Rows whose 1.0 stands elsewhere add the same
+    # three numbers in another order, which is a rounding of a sum in 32 bits: (1 + e) + e and
+    # (e + e) + 1, e = 1/exp(1), are half a step apart before they round. They are held to the
+    # formula: lse = log(exp(1) + 2), loss = lse - 1 (no rest: the entry alone is the teacher).
+    N = (1 << 21) + 5
+    x = torch.zeros(N, 3, dtype=H, device=cuda)
+    hot = torch.arange(N, device=cuda) % 3
+    x[torch.arange(N, device=cuda), hot] = 1.0
+    v, i, lse = K.top_logits(x, 1)
+    want = math.log(math.exp(1.0) + 2.0)
+    assert torch.equal(i[:, 0], hot) and bool((v == 1).all())
+    assert torch.equal(lse, lse[hot]) and bool(((lse - want).abs() < 16 * U * want).all())
+    loss, grad = K.distill_loss_grad(x, v, i)
+    assert torch.equal(loss, loss[hot]) and bool(((loss - (want - 1)).abs() < 56 * U).all())
+    assert torch.equal(grad, grad[hot]) and bool((grad != 0).all())
 
 
 def test_top_logits_refusals(cuda):
@@ -389,6 +410,37 @@ def test_distill_autograd(cuda):
     (g1,) = torch.autograd.grad(ops.distill_loss(x, v, i, ls, 2.0).sum(), x, create_graph=True)
     with pytest.raises(NotImplementedError, match="second derivative"):
         g1.float().sum().backward()
+
+
+def test_distill_saved_tensors(cuda):
+    """A saved-tensor hook that brings them back elsewhere, an in-place change that autograd refuses, copies of operands
+    that are not adjacent, and a graph kept for a second backward."""
+    g = _gen(18)
+    z, val, idx, lse = (t.to(cuda) for t in _case(g, 4, 2001, 12, B16, 1.0, True))
+    want = K.distill_loss_grad(z, val, idx, lse)[1]
+    x = z.clone().requires_grad_()
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t.to(cuda)):
+        loss = ops.distill_loss(x, val, idx, lse).sum()
+    loss.backward()
+    assert torch.equal(x.grad, want)
+    x = z.clone().requires_grad_()
+    with torch.autograd.graph.save_on_cpu():
+        loss = ops.distill_loss(x, val.t().contiguous().t(), idx.t().contiguous().t(), lse).sum()
+    loss.backward()
+    assert torch.equal(x.grad, want)
+    x = z.clone().requires_grad_()
+    loss = ops.distill_loss(x, val.t().contiguous().t(), idx, lse).sum()
+    loss.backward(retain_graph=True)
+    loss.backward()
+    assert torch.equal(x.grad, want + want)
+    x, v = z.clone().requires_grad_(), val.clone()
+    loss = ops.distill_loss(x, v, idx, lse).sum()
+    v.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.no_grad():
+        assert torch.equal(ops.distill_loss(x, val, idx, lse), K.distill_loss(z, val, idx, lse))
+    assert not ops.distill_loss(z, val, idx, lse).requires_grad
 
 
 def test_distill_compiles(cuda):
