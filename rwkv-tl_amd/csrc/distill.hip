@@ -18,10 +18,22 @@
 // log-softmax.
 //
 // 1 - Q is never formed as a difference: the row's elements in I are taken out
-// (each thread has a word in LDS that marks them) before the sum, which is about
-// their own largest, and I enters through the entries. The row stays in registers between the sum and the
+// (each thread has a word in LDS that marks them) before the sum, and I enters
+// through the entries. The row stays in registers between the sum and the
 // gradient, so a pass reads the logits once and writes the gradient once; the
 // entries' own gradients are stored over it after a barrier.
+//
+// The row's exponentials are in 32 bits, and so are the sums of a wave; waves are
+// joined, and the entries' exponentials, products and gradients formed, in 64: a
+// listed id's gradient is what is left of q - p, and the loss what is left of terms
+// of both signs (in 32 bits a loss of 331 x 20011 f32 was off by 3.5e-6 of itself,
+// now by 1.2e-7).
+//
+// Measured (kernel, us; a large copy moves 5.05 TB/s here): loss and gradient of 4096
+// x 65536 bf16 215, 5.0 TB/s: the bytes (vector units busy 64 %). Loss of 1021 x
+// 65536 f16 29.5, 4.5 TB/s, and its gradient 49, 5.4 TB/s (in part from the last
+// cache). Few or short rows are a chain of load, sum, join and logarithms: 16 x 65536
+// f16 9.2; 331 x 20011 f32 11.5, gradient 14.8.
 #include "logits_rows.h"
 #include "rwkv7_kernels.h"
 

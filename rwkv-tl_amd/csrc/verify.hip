@@ -14,7 +14,7 @@
 // The sums and the draw are in 64 bits: among 65536 tokens the borders of the
 // cumulative sum lie within 1e-9 of each other in the tail, where f32 sums (1e-7)
 // would draw another token than the one that u stands for. One 64-bit fma costs
-// as much as one 32-bit fma on this machine, so an exponential of ~18 of them
+// as much as one 32-bit fma on this machine, so an exponential of ~19 of them
 // takes about as long as reading its logit.
 //
 // NaN counts as -inf (never drawn, never accepted). A drafted id outside the
@@ -24,14 +24,19 @@
 //
 // verify_stats_kernel: a slice of a row per workgroup: the sum of its
 //   exponentials, about 0 or its largest logit, for target rows also of each 512
-//   logits (greedy: largest logit and its first id).
+//   logits (greedy: largest logit and its first id). 8192 logits a workgroup, so that
+//   one sequence of four drafts already has 72 of them. 96 sequences of 7 drafts
+//   x 65536 bf16 47.5 us (189 MB, 4.0 TB/s): vector instructions, 93 % of it, 14 a logit.
+//   16 x 8 f16 12.7, 1 x 4 4.4.
 // verify_draw_kernel: 2048 logits of each sequence's decisive row: every workgroup
 //   joins the sums of its sequence's rows and decides how many tokens are
 //   accepted; the sums of max(p - q, 0) over each 512 of its logits; the last
 //   workgroup of a sequence to finish (the only one that stays, where all tokens
 //   are accepted) finds the 512 in which the running sum crosses, and in them the
 //   token, by one wave. (As a launch of its own this draw took 3 us more of a call's
-//   chain and 2 of its host time.)
+//   chain and 2 of its host time.) A chain of seven dependent trips to memory and
+//   three prefixes: 9.7 us for one sequence, 12 for 16, 22.5 for 96.
+// verify_greedy_kernel: a wave per sequence, 3.8 us, most of it the launch.
 #include "logits_rows.h"
 #include "rwkv7_kernels.h"
 

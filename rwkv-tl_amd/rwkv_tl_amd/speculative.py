@@ -54,6 +54,8 @@ def generate_speculative(
     if tokens.ndim != 1 or tokens.numel() < 2:
         raise ValueError(f"expected a prompt of two or more token ids, got shape {tuple(tokens.shape)}")
     states = ((model, S, _arenas(model, S)), (draft, S_draft, _arenas(draft, S_draft)))
+    if {a.data_ptr() for a in states[0][2]} & {a.data_ptr() for a in states[1][2]}:
+        raise ValueError("S and S_draft share their tensors")
     for m, s, _ in states:
         m.prefill(tokens[:-1], s)
     greedy = temperature is None or temperature <= 0

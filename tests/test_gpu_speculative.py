@@ -167,6 +167,15 @@ def test_speculative_refusals(cuda):
             bad()
 
 
+def test_speculative_refuses_one_state_for_both_models(cuda):
+    model, _ = _model(cuda)
+    S = model.new_state()
+    before = [a.clone() for a in S.arenas]
+    with pytest.raises(ValueError, match="share"):
+        generate_speculative(model, model, [1, 2], S, S)
+    assert all(torch.equal(a, b) for a, b in zip(S.arenas, before))
+
+
 @pytest.mark.parametrize("cls", [RWKV7HIP, RWKV7HIPBF16])
 def test_distillation_step_from_one_model_to_another(cuda, cls):
     """A teacher's answers to two sequences (the last tokens of one padding), its top logits, and a student's head trained
