@@ -25,6 +25,14 @@ def _arenas(model, S: State) -> list[Tensor]:
     return list(S.arenas)
 
 
+def _advance(model, tokens: Tensor, S: State) -> None:
+    """``S`` on by ``tokens``; one token by the decode kernel (0.4B: 0.32 ms, as a prefill of one 0.73)."""
+    if tokens.numel() == 1:
+        model.decode(tokens, S)
+    else:
+        model.prefill(tokens, S)
+
+
 def generate_speculative(
     model: RWKV7HIP,
     draft: RWKV7HIP,
@@ -57,7 +65,7 @@ def generate_speculative(
     if {a.data_ptr() for a in states[0][2]} & {a.data_ptr() for a in states[1][2]}:
         raise ValueError("S and S_draft share their tensors")
     for m, s, _ in states:
-        m.prefill(tokens[:-1], s)
+        _advance(m, tokens[:-1], s)
     greedy = temperature is None or temperature <= 0
     sampler = Sampler(V, dev, temperature=temperature)
     ids: list[int] = []
@@ -79,9 +87,9 @@ def generate_speculative(
             for (m, s, arenas), old in zip(states, saved):
                 for a, b in zip(arenas, old):
                     a.copy_(b)
-                m.prefill(row[: n_ok + 1], s)
+                _advance(m, row[: n_ok + 1], s)
         else:  # the draft model has not taken its own last token
-            draft.prefill(row[k : k + 1], S_draft)
+            _advance(draft, row[k : k + 1], S_draft)
         ids += new[: n_ok + 1]
         row[:1] = out[n_ok : n_ok + 1]
     for m, _, _ in states:
