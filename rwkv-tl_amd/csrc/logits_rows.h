@@ -172,8 +172,8 @@ RWKV7_DEV void store_chunk(void *row, uint32_t b, const float (&f)[kRowChunk]) {
 template <int CTRL>
 RWKV7_DEV double dpp_d(double v) {
   const u64 u = __builtin_bit_cast(u64, v);
-  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, 0xF, 0xF, false);
-  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, 0xF, 0xF, false);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, 0xF, 0xF, true);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, 0xF, 0xF, true);
   return __builtin_bit_cast(double, (u64)lo | ((u64)hi << 32));
 }
 RWKV7_DEV double lane_value_d(double v, int lane) {

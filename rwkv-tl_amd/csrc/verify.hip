@@ -14,8 +14,8 @@
 // The sums and the draw are in 64 bits: among 65536 tokens the borders of the
 // cumulative sum lie within 1e-9 of each other in the tail, where f32 sums (1e-7)
 // would draw another token than the one that u stands for. One 64-bit fma costs
-// as much as one 32-bit fma on this machine, so an exponential of ~19 of them
-// takes about as long as reading its logit.
+// as much as one 32-bit fma on this machine, so an exponential of 12 of them
+// and 6 others takes about as long as reading its logit.
 //
 // NaN counts as -inf (never drawn, never accepted). A drafted id outside the
 // vocabulary is rejected, a row without a finite logit has no probability: its
@@ -25,17 +25,18 @@
 // verify_stats_kernel: a slice of a row per workgroup: the sum of its
 //   exponentials, about 0 or its largest logit, for target rows also of each 512
 //   logits (greedy: largest logit and its first id). 8192 logits a workgroup, so that
-//   one sequence of four drafts already has 72 of them. 96 sequences of 7 drafts
-//   x 65536 bf16 47.5 us (189 MB, 4.0 TB/s): vector instructions, 93 % of it, 14 a logit.
-//   16 x 8 f16 12.7, 1 x 4 4.4.
-// verify_draw_kernel: 2048 logits of each sequence's decisive row: every workgroup
+//   one sequence of four drafts already has 72 of them. 96 sequences of up to 7
+//   drafts x 65536 bf16, 830 rows that count: 41 us (109 MB, 2.6 TB/s), the vector units busy
+//   86 % of it at 1.86 GHz with 19.6 instructions a logit, 12 of them 64-bit. 16 x 8 f16
+//   10.5, 1 x 4 4.1.
+// verify_draw_kernel: 2048 logits (large batches: 8192) of each sequence's decisive row: every workgroup
 //   joins the sums of its sequence's rows and decides how many tokens are
 //   accepted; the sums of max(p - q, 0) over each 512 of its logits; the last
 //   workgroup of a sequence to finish (the only one that stays, where all tokens
 //   are accepted) finds the 512 in which the running sum crosses, and in them the
 //   token, by one wave. (As a launch of its own this draw took 3 us more of a call's
 //   chain and 2 of its host time.) A chain of seven dependent trips to memory and
-//   three prefixes: 9.7 us for one sequence, 12 for 16, 22.5 for 96.
+//   three prefixes: 9.7 us for one sequence, 11.7 for 16, 19.3 for 96.
 // verify_greedy_kernel: a wave per sequence, 3.8 us, most of it the launch.
 #include "logits_rows.h"
 #include "rwkv7_kernels.h"
@@ -50,6 +51,11 @@ constexpr int kSlice = kVerThreads * kVerChunks * kRowChunk;  // 8192 logits
 constexpr int kMaxSlices = kRowMaxV / kSlice;                 // 8
 constexpr int kBlocks = kVerChunks * kVerWaves;               // of 512 logits in a slice, in order
 constexpr int kDrawE = 3;                                     // block sums per lane of the draw
+// Workgroups of the draw, one per 2048 logits, above which each takes four times as
+// many: all of a sequence's decide the same, which then counts for more than a
+// longer chain. (Calls of 65536 bf16 logits, one / four: 24 x 5 21.7 / 22.5 us, 48 x 5
+// 28.4 / 30.4, 64 x 7 41.9 / 38.9, 96 x 7 56.8 / 55.0.)
+constexpr int kDrawWide = 1792;
 constexpr int kVerMaxK = kWave - 1;                           // a lane per drafted token and one for the row behind them
 static_assert(kMaxSlices * kBlocks + 1 <= kDrawE * kWave, "the draw's wave holds every block's sum, and the last logits'");
 
@@ -69,6 +75,7 @@ struct VerifyArgs {
   const int64_t *len;          // null: K
   int B, K, V, G;              // G slices of a row
   double kt, kd;               // log2(e) / temperature of target and draft; kt <= 0: greedy
+  float endt, endd;            // 1000 / those
   int64_t *out, *accepted;
   // workspace
   double *sum;                 // [rows][G] sum of exponentials about m (greedy: first id of the largest)
@@ -98,17 +105,41 @@ struct Weight {
 // slice is summed again about its largest.
 constexpr double kNothing = 0x1p-900, kMuch = 0x1p999;
 struct BulkWeight {
-  float lo, hi;
+  float end;  // 1000 / k
   double k;
-  RWKV7_DEV explicit BulkWeight(double k_) : lo((float)(-1000.0 / k_)), hi((float)(1000.0 / k_)), k(k_) {}
   RWKV7_DEV double operator()(float x) const {
-    const double d = (double)__builtin_amdgcn_fmed3f(x, lo, hi), magic = 0x1.8p52;  // (NaN: lo)
+    const double d = (double)__builtin_amdgcn_fmed3f(x, -end, end), magic = 0x1.8p52;  // (NaN: -end)
     const double t = fma(d, k, magic), f = fma(d, k, magic - t);
     const u64 p = __builtin_bit_cast(u64, exp2_frac(f));
-    const uint32_t n = (uint32_t)__builtin_bit_cast(u64, t);
-    return __builtin_bit_cast(double, p + ((u64)(n << 20) << 32));
+    uint32_t high = (uint32_t)(p >> 32);
+    // (in assembly: the compiler makes a 64-bit addition of it, with three moves)
+    asm("v_lshl_add_u32 %0, %1, 20, %0" : "+v"(high) : "v"((uint32_t)__builtin_bit_cast(u64, t)));
+    return __builtin_bit_cast(double, (u64)(uint32_t)p | ((u64)high << 32));
   }
 };
+
+// A lane's four values summed over the wave, value l & 3 on lane l: lanes trade
+// halves of the values before they add, 37 instructions for what takes four
+// wave_sum_d 100.
+constexpr int kDppRor4 = 0x124, kDppRor8 = 0x128;  // lane i <- i - 4, i - 8 within each 16
+template <int CTRL>
+RWKV7_DEV double trade_d(double even, double odd, bool is_odd) {
+  return (is_odd ? odd : even) + dpp_d<CTRL>(is_odd ? even : odd);
+}
+RWKV7_DEV double wave_sums_d(const double (&v)[4]) {
+  const int lane = threadIdx.x & (kWave - 1);
+  double q = trade_d<kDppXor2>(trade_d<kDppXor1>(v[0], v[1], lane & 1), trade_d<kDppXor1>(v[2], v[3], lane & 1), lane & 2);
+  q += dpp_d<kDppRor4>(q);
+  q += dpp_d<kDppRor8>(q);
+  auto rows = [&](auto swap) {  // rows of 16, then of 32 lanes
+    const u64 u = __builtin_bit_cast(u64, q);
+    const auto lo = swap((uint32_t)u), hi = swap((uint32_t)(u >> 32));
+    q = __builtin_bit_cast(double, (u64)lo[0] | ((u64)hi[0] << 32)) + __builtin_bit_cast(double, (u64)lo[1] | ((u64)hi[1] << 32));
+  };
+  rows([](uint32_t w) { return __builtin_amdgcn_permlane16_swap(w, w, false, false); });
+  rows([](uint32_t w) { return __builtin_amdgcn_permlane32_swap(w, w, false, false); });
+  return q;
+}
 
 RWKV7_DEV int drafted(const VerifyArgs &a, int b) {
   if (!a.len) return a.K;
@@ -177,9 +208,10 @@ __global__ __launch_bounds__(kVerThreads) void verify_stats_kernel(VerifyArgs a)
     return;
   }
   const double k = tgt ? a.kt : a.kd;
+  const BulkWeight bulk{tgt ? a.endt : a.endd, k};
   double *block = tgt ? a.block + (int64_t)r * (a.G * kBlocks + 1) + g * kBlocks : nullptr;
   auto total = [&](auto weight) {  // of the slice, with its blocks' sums put down
-    double sum = 0.0;
+    double own[kVerChunks];
 #pragma unroll
     for (int c = 0; c < kVerChunks; ++c) {
       float f[kRowChunk];
@@ -187,10 +219,12 @@ __global__ __launch_bounds__(kVerThreads) void verify_stats_kernel(VerifyArgs a)
       double q = 0.0, p = 0.0;
 #pragma unroll
       for (int e = 0; e < kRowChunk; e += 2) q += weight(f[e]), p += weight(f[e + 1]);
-      q = wave_sum_d(q + p);
-      if (block && lane == 0) block[c * kVerWaves + wv] = q;
-      sum += q;
+      own[c] = q + p;
     }
+    double sum = wave_sums_d(own);  // lane c: chunk c's
+    if (block && lane < kVerChunks) block[lane * kVerWaves + wv] = sum;
+    sum += dpp_d<kDppXor1>(sum);
+    sum += dpp_d<kDppXor2>(sum);
     if (g == a.G - 1 && wv == 0) {  // the logits behind the eights
       const double q = wave_sum_d(tail >= 0 ? weight(xt) : 0.0);
       if (block && lane == 0) block[kBlocks] = q;
@@ -201,7 +235,7 @@ __global__ __launch_bounds__(kVerThreads) void verify_stats_kernel(VerifyArgs a)
     return (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
   };
   float m = 0.f;
-  double sum = total(BulkWeight(k));
+  double sum = total(bulk);
   if (!(sum > kNothing && sum < kMuch)) {  // (the same in every thread)
     m = largest();
 #pragma unroll
@@ -415,7 +449,8 @@ RWKV7_DEV void draw(const VerifyArgs &a, int b, const Decision &d) {
   if (lane == 0) a.accepted[b] = d.n;
 }
 
-template <int FMT>
+// CH: chunks of 2048 logits a workgroup.
+template <int FMT, int CH>
 __global__ __launch_bounds__(kVerThreads) void verify_draw_kernel(VerifyArgs a) {
   __shared__ DecideLds s;
   __shared__ bool s_last;
@@ -427,40 +462,56 @@ __global__ __launch_bounds__(kVerThreads) void verify_draw_kernel(VerifyArgs a) 
     return;
   }
   const void *pr = target_row<FMT>(a, b, d.n), *qr = a.draft ? draft_row<FMT>(a, b, d.n) : pr;
-  const uint32_t n8 = (uint32_t)V / kRowChunk, e8 = g * kVerThreads + t;
+  const uint32_t n8 = (uint32_t)V / kRowChunk;
   const Residual res(a, d, false);
   double *block = a.rest + (int64_t)b * (a.G * kBlocks + 1);
-  Chunk<FMT> xp, xq;
-  xp.load(pr, e8, n8);
-  xq.load(qr, e8, n8);
-  float fp[kRowChunk], fq[kRowChunk];
-  xp.get(fp);
-  xq.get(fq);
-  double sum = 0.0;
-  if (d.mp == 0.f && d.mq == 0.f) {
-    const BulkWeight p(a.kt), q(a.kd);
+  Chunk<FMT> xp[CH], xq[CH];
 #pragma unroll
-    for (int e = 0; e < kRowChunk; ++e) {
-      const double r = res.soft ? over(p(fp[e]), d.ip, q(fq[e]), d.iq) : p(fp[e]) * d.ip;
-      sum += (int)e8 * kRowChunk + e == d.x ? 0.0 : r;
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < kRowChunk; ++e) sum += res(fp[e], fq[e], (int)e8 * kRowChunk + e);
+  for (int c = 0; c < CH; ++c) {
+    const uint32_t e8 = (g * CH + c) * kVerThreads + t;
+    xp[c].load(pr, e8, n8);
+    xq[c].load(qr, e8, n8);
   }
-  sum = wave_sum_d(sum);
+  double own[CH];
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const int id = ((g * CH + c) * kVerThreads + t) * kRowChunk;
+    float fp[kRowChunk], fq[kRowChunk];
+    xp[c].get(fp);
+    xq[c].get(fq);
+    double sum = 0.0;
+    if (d.mp == 0.f && d.mq == 0.f) {
+      const BulkWeight p{a.endt, a.kt}, q{a.endd, a.kd};
+#pragma unroll
+      for (int e = 0; e < kRowChunk; ++e) {
+        const double r = res.soft ? over(p(fp[e]), d.ip, q(fq[e]), d.iq) : p(fp[e]) * d.ip;
+        sum += id + e == d.x ? 0.0 : r;
+      }
+    } else {
+#pragma unroll 1
+      for (int e = 0; e < kRowChunk; ++e) sum += res(fp[e], fq[e], id + e);
+    }
+    own[c] = sum;
+  }
   // stored past the caches of this XCD, acknowledged before the count goes up
   auto put = [&](int i, double v) { __hip_atomic_store(block + i, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
-  if (lane == 0) put(g * kVerWaves + wv, sum);
-  if (g == a.G * kVerChunks - 1 && wv == 0) {  // the logits behind the eights
+  if constexpr (CH == kVerChunks) {
+    const double sum = wave_sums_d(own);  // lane c: chunk c's
+    if (lane < CH) put((g * CH + lane) * kVerWaves + wv, sum);
+  } else {
+    static_assert(CH == 1);
+    const double sum = wave_sum_d(own[0]);
+    if (lane == 0) put(g * kVerWaves + wv, sum);
+  }
+  if (g == (int)gridDim.x - 1 && wv == 0) {  // the logits behind the eights
     const int id = (int)n8 * kRowChunk + t;
-    sum = wave_sum_d(id < V ? res(load_logit<FMT>(pr, id), load_logit<FMT>(qr, id), id) : 0.0);
+    const double sum = wave_sum_d(id < V ? res(load_logit<FMT>(pr, id), load_logit<FMT>(qr, id), id) : 0.0);
     if (lane == 0) put(a.G * kBlocks, sum);
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   if (t == 0)
-    s_last = __hip_atomic_fetch_add(a.done + b, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.G * kVerChunks - 1;
+    s_last = __hip_atomic_fetch_add(a.done + b, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (int)gridDim.x - 1;
   __syncthreads();
   if (s_last && wv == 0) draw<FMT>(a, b, d);
 }
@@ -503,7 +554,8 @@ int launch_verify(const VerifyArgs &a, hipStream_t st) {
   }
   verify_stats_kernel<FMT, false><<<grid, kVerThreads, 0, st>>>(a);
   RWKV7_CHECK_LAUNCH();
-  verify_draw_kernel<FMT><<<dim3(a.G * kVerChunks, a.B), kVerThreads, 0, st>>>(a);
+  if (a.B * a.G * kVerChunks > kDrawWide) verify_draw_kernel<FMT, kVerChunks><<<dim3(a.G, a.B), kVerThreads, 0, st>>>(a);
+  else verify_draw_kernel<FMT, 1><<<dim3(a.G * kVerChunks, a.B), kVerThreads, 0, st>>>(a);
   RWKV7_CHECK_LAUNCH();
   return RWKV7_OK;
 }
@@ -562,6 +614,7 @@ extern "C" int rwkv7_verify(const void *target, int64_t target_b, int64_t target
   a.B = B, a.K = K, a.V = V, a.G = slices(V);
   a.kt = greedy ? 0.0 : kLog2E / temperature;
   a.kd = soft ? kLog2E / draft_temperature : 0.0;
+  a.endt = (float)(1000.0 / a.kt), a.endd = (float)(1000.0 / a.kd);  // (0: inf, not read)
   a.out = out, a.accepted = accepted;
   verify_ws(a, static_cast<char *>(workspace));
   const hipStream_t st = static_cast<hipStream_t>(stream);

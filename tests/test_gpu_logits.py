@@ -600,6 +600,26 @@ def test_verify_far_from_zero(cuda, dtype, T):
     _check_verify(cuda, target.to(dtype), tok, u, None, T, 0.0)
 
 
+@pytest.mark.parametrize("dtype", [H, B16, F], ids=str)
+@pytest.mark.parametrize("B,k,V", [(450, 3, 515), (225, 2, 9001), (57, 1, 65535)])
+def test_verify_wide_batches(cuda, dtype, B, k, V):
+    """As many sequences as take more of a decisive row to a workgroup."""
+    for T, Td in ((1.0, 1.0), (0.7, 0.0)):
+        _check_verify(cuda, *_drafts(_gen(27, B, int(Td)), B, k, V, dtype, Td, 1.5), T, Td)
+    target, tok, u, draft = _drafts(_gen(28, B), 9, k, V, dtype, 1.0)
+    low = torch.finfo(dtype).min
+    target[0] *= 700.0
+    target[1, :, V // 2 :] = low
+    draft[2, :, : V // 2] = low
+    draft[3] = low
+    target[4, :, 3:] = -INF
+    target[5] = -INF
+    target[6, :, V // 2 :] = NAN
+    target[7, :, : V // 3] -= 2000.0
+    n = -(-B // 9)
+    _check_verify(cuda, *(t.repeat(n, *[1] * (t.ndim - 1)) for t in (target, tok, u, draft)), 1.0, 1.0)
+
+
 def test_verify_greedy_ties_take_the_lowest_id(cuda):
     target = torch.zeros(3, 3, 20000, dtype=H)
     target[1, :, 9000] = target[1, :, 8000] = target[1, :, 15000] = 1.0
