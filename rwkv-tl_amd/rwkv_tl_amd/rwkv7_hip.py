@@ -249,7 +249,8 @@ class RWKV7HIP(RWKV7Model):
         """``prefill`` with the logits after every token: ``[T, V]`` (``[B, T, V]``
         for a batched state). What a teacher hands on to a student
         (``kernels.top_logits``), and what drafted tokens are verified with
-        (``verify_draft``)."""
+        (``verify_draft``). Of an int8 model: of its 16-bit weights, but for one token
+        of one sequence, which is a ``decode``."""
         return self._prefill(tokens, S, True)
 
     def _prefill(self, tokens: Tensor, S: State, with_logits: bool) -> tuple[Tensor | None, State]:

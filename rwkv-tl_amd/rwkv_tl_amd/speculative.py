@@ -12,7 +12,7 @@ from __future__ import annotations
 import torch
 from torch import Tensor
 
-from .logits import MAX_DRAFT, verify_draft
+from .logits import MAX_DRAFT, _temperature, verify_draft
 from .rwkv7_hip import RWKV7HIP
 from .sampling import Sampler
 from .state import State
@@ -48,7 +48,8 @@ def generate_speculative(
     proposing up to ``n_draft`` tokens at a time, 1 <= n_draft <= 63.
 
     ``S`` and ``S_draft`` are the two models' states before the prompt ``tokens``
-    (two or more). Returns ``(ids, S, S_draft)``; the states hold everything but
+    (two or more). The models may be wrapped in ``HIPGraph``; an int8 one can only
+    draft. Returns ``(ids, S, S_draft)``; the states hold everything but
     the last id, as after ``generate``. The host waits once per round of drafts,
     for the number accepted."""
     dev, V = model.w.device, model.w.head.shape[0]
@@ -58,15 +59,20 @@ def generate_speculative(
         raise ValueError(f"the draft model is {draft.kernel_dtype}, the target {model.kernel_dtype}")
     if not 1 <= n_draft <= MAX_DRAFT:
         raise ValueError(f"n_draft must be in 1..{MAX_DRAFT}, got {n_draft}")
-    tokens = torch.as_tensor(tokens, device=dev)
+    if model.weight_quant is not None:
+        raise ValueError("an int8 model prefills with its 16-bit weights and decodes with the int8 ones: it can draft, not verify")
+    greedy = temperature is None or temperature <= 0
+    if not greedy:
+        _temperature(temperature)
+    tokens = torch.as_tensor(tokens)
     if tokens.ndim != 1 or tokens.numel() < 2:
         raise ValueError(f"expected a prompt of two or more token ids, got shape {tuple(tokens.shape)}")
+    tokens = model._tokens(tokens, tuple(tokens.shape))
     states = ((model, S, _arenas(model, S)), (draft, S_draft, _arenas(draft, S_draft)))
     if {a.data_ptr() for a in states[0][2]} & {a.data_ptr() for a in states[1][2]}:
         raise ValueError("S and S_draft share their tensors")
     for m, s, _ in states:
         _advance(m, tokens[:-1], s)
-    greedy = temperature is None or temperature <= 0
     sampler = Sampler(V, dev, temperature=temperature)
     ids: list[int] = []
     row = torch.empty(n_draft + 1, dtype=torch.int64, device=dev)  # the last token, then the drafts

@@ -9,7 +9,7 @@ import torch
 
 from oracle import logits_ref as LR
 from oracle import rwkv7_ref as R
-from rwkv_tl_amd import RWKV7HIP, RWKV7HIPBF16, HIPGraph, generate_speculative
+from rwkv_tl_amd import RWKV7HIP, RWKV7HIPBF16, RWKV7HIPInt8, HIPGraph, generate_speculative
 from rwkv_tl_amd import kernels as K
 from rwkv_tl_amd.checkpoint import make_random_state_dict
 from rwkv_tl_amd.weight import RWKV7Weight
@@ -165,6 +165,35 @@ def test_speculative_refusals(cuda):
                 lambda: generate_speculative(model, model, [1, 2], S(batch=1), S())):
         with pytest.raises(ValueError):
             bad()
+
+
+@pytest.mark.parametrize("T", [None, 0.9])
+def test_speculative_through_graph_wrappers_and_an_int8_draft(cuda, T):
+    """The same ids as of the bare models (the same kernels run); an int8 copy of the target drafts for it."""
+    model, _ = _model(cuda, scale=8.0)
+    draft, _ = _model(cuda, seed=7, scale=8.0)
+    prompt = _tokens(9, seed=3).tolist()
+
+    def ids(m, d):
+        torch.manual_seed(5)
+        return generate_speculative(m, d, prompt, m.new_state(), d.new_state(), 25, n_draft=4, temperature=T)[0]
+
+    assert ids(HIPGraph(model), HIPGraph(draft)) == ids(model, draft)
+    q, _ = _model(cuda, cls=RWKV7HIPInt8, scale=8.0)
+    got = ids(model, q)
+    assert len(got) == 25
+    with pytest.raises(ValueError, match="int8"):
+        ids(q, model)
+
+
+def test_speculative_refuses_before_it_touches_a_state(cuda):
+    model, _ = _model(cuda)
+    S, Sd = model.new_state(), model.new_state()
+    before = [a.clone() for a in S.arenas]
+    for prompt, T in (([1, 512], None), ([-1, 3], None), ([1.0, 2.0], None), ([1, 2], float("nan")), ([1, 2], 1e-40), ([[1, 2]], None)):
+        with pytest.raises(ValueError):
+            generate_speculative(model, model, prompt, S, Sd, temperature=T)
+    assert all(torch.equal(a, b) for a, b in zip(S.arenas, before))
 
 
 def test_speculative_refuses_one_state_for_both_models(cuda):
