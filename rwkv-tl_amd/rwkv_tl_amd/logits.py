@@ -62,6 +62,11 @@ def _rows(x: Tensor) -> tuple[Tensor, int, int]:
     return x, N, x.stride(0) if N > 1 else V
 
 
+def _empty(shape, dtype: torch.dtype, device: torch.device) -> Tensor:
+    # (sizes one by one: torch.empty takes 1 us more for a torch.Size)
+    return torch.empty(*shape, dtype=dtype, device=device) if shape else torch.empty((), dtype=dtype, device=device)
+
+
 def _temperature(t: float) -> float:
     t = float(t)
     if not 1e-30 <= t <= 1e30:  # (NaN neither)
@@ -91,9 +96,10 @@ def top_logits(logits: Tensor, k: int, *, temperature: float = 1.0) -> tuple[Ten
     lead = logits.shape[:-1]
     with _lib.device_of(logits):
         x, N, ld = _rows(logits)
-        val = torch.empty((*lead, k), dtype=x.dtype, device=x.device)
-        idx = torch.empty((*lead, k), dtype=torch.int64, device=x.device)
-        lse = torch.empty(lead, dtype=torch.float32, device=x.device)
+        dev = x.device
+        val = torch.empty(*lead, k, dtype=x.dtype, device=dev)
+        idx = torch.empty(*lead, k, dtype=torch.int64, device=dev)
+        lse = _empty(lead, torch.float32, dev)
         if N:
             rc = _lib.load().rwkv7_top_logits(
                 x.data_ptr(), code, ld, N, V, k, temperature, val.data_ptr(), idx.data_ptr(), lse.data_ptr(), _lib.stream_of(x)
@@ -125,8 +131,8 @@ def _distill(logits, top_val, top_idx, lse, temperature, scale, want_loss: bool,
     _same_device(logits, top_val, top_idx, lse, rows)
     temperature = _temperature(temperature)
     with _lib.device_of(logits):
-        loss = torch.empty(lead, dtype=torch.float32, device=logits.device) if want_loss else None
-        grad = torch.empty(shape, dtype=logits.dtype, device=logits.device) if want_grad else None
+        loss = _empty(lead, torch.float32, logits.device) if want_loss else None
+        grad = torch.empty(*shape, dtype=logits.dtype, device=logits.device) if want_grad else None
         x, N, ld = _rows(logits)
         if N and K:
             tv, ti = top_val.contiguous(), top_idx.contiguous()
@@ -216,13 +222,15 @@ def verify_draft(
     and ``uniforms`` is not read. NaN logits count as -inf; ids outside ``0..V-1``
     are rejected."""
     code = _check_logits(target_logits, "target_logits")
-    single = target_logits.ndim == 2
-    up = (lambda t: None if t is None else t.unsqueeze(0)) if single else (lambda t: t)
-    target, tokens, draft = up(target_logits), up(draft_tokens), up(draft_logits)
-    uniforms, lengths = up(uniforms), up(lengths)
+    target, tokens, draft = target_logits, draft_tokens, draft_logits
+    single = target.ndim == 2
+    if single:
+        up = lambda t: None if t is None else t.unsqueeze(0)  # noqa: E731
+        target, tokens, draft, uniforms, lengths = up(target), up(tokens), up(draft), up(uniforms), up(lengths)
     if target.ndim != 3 or target.shape[1] < 1:
         raise ValueError(f"target_logits must be [B, K + 1, V], got {tuple(target_logits.shape)}")
-    B, K, V = target.shape[0], target.shape[1] - 1, target.shape[2]
+    B, K, V = target.shape
+    K -= 1
     if K > MAX_DRAFT:
         raise ValueError(f"at most {MAX_DRAFT} drafted tokens, got {K}")
     if B * (2 * K + 1) > 65535:
@@ -254,8 +262,9 @@ def verify_draft(
             raise ValueError(f"lengths must be int64 [{B}]")
     _same_device(target, tokens, None if greedy else uniforms, draft, lengths)
     with _lib.device_of(target):
-        out = torch.empty(B, K + 1, dtype=torch.int64, device=target.device)
-        accepted = torch.empty(B, dtype=torch.int64, device=target.device)
+        dev = target.device
+        out = torch.empty(B, K + 1, dtype=torch.int64, device=dev)
+        accepted = torch.empty(B, dtype=torch.int64, device=dev)
         if B:
             lib = _lib.load()
             t = _strides(target, V)
@@ -264,7 +273,7 @@ def verify_draft(
             u = None if greedy else uniforms.contiguous()
             n = None if lengths is None else lengths.contiguous()
             nb = _verify_bytes(B, K, V)
-            ws = torch.empty(nb, dtype=torch.uint8, device=target.device)
+            ws = torch.empty(nb, dtype=torch.uint8, device=dev)
             rc = lib.rwkv7_verify(
                 t.data_ptr(), t.stride(0), t.stride(1) if K else V, _lib.ptr(d), 0 if d is None else d.stride(0),
                 V if d is None or K == 1 else d.stride(1), code, tok.data_ptr() if K else None,
