@@ -33,7 +33,7 @@
 // x 65536 bf16 215, 5.0 TB/s: the bytes (vector units busy 64 %). Loss of 1021 x
 // 65536 f16 29.5, 4.5 TB/s, and its gradient 49, 5.4 TB/s (in part from the last
 // cache). Few or short rows are a chain of load, sum, join and logarithms: 16 x 65536
-// f16 9.2; 331 x 20011 f32 11.5, gradient 14.8.
+// f16 9.2; 331 x 20011 f32 10.6, gradient 14.5.
 #include "logits_rows.h"
 #include "rwkv7_kernels.h"
 
@@ -214,7 +214,7 @@ __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : 8) void distill_kernel(Dist
   const bool entries = wv * kWave < g.K;  // this wave has entries
   const float mtop = entries ? wave_max(zv) : -kInf;
   float m;
-  const float sum = sum_row<THREADS, false>(x, src, n8, xt, g.sc, m, [&](int c, Chunk<FMT> &y) {
+  const float sum = sum_row<THREADS, false, !GRAD>(x, src, n8, xt, g.sc, m, [&](int c, Chunk<FMT> &y) {
     const uint32_t marked = (uint32_t)(mine >> (kRowChunk * c)) & 255u;
     if (marked) y.remove(marked);
   });
@@ -263,6 +263,7 @@ __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : 8) void distill_kernel(Dist
     g.sc.with(s.j.mrest, [&](auto e2, auto far) {
 #pragma unroll
       for (int c = 0; c < kRowChunks; ++c) {
+        if (c > 0 && c * THREADS >= (int)n8) break;
         float f[kRowChunk];
         x[c].template get<decltype(far)::value>(f);
 #pragma unroll

@@ -22,7 +22,7 @@
 // TB/s: the vector units are busy 91 % of it with 13 instructions a logit (maxima,
 // exponentials, comparisons). 509 x 65536 bf16, k 64, 20, 3.3 TB/s: one round of two
 // rows a CU, each a chain of load, floor, sum, gather and ranking. One row 9.0; 257 x
-// 20011 f32 12.1.
+// 20011 f32 11.6.
 #include "logits_rows.h"
 #include "rwkv7_kernels.h"
 
@@ -187,7 +187,7 @@ __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : THREADS == 256 ? 7 : 8) voi
     if (lane == 0) s.floor[wv] = fl, s.some[wv] = some;
   }
   m = wave_max(m);
-  const float sum = sum_row<THREADS, true>(x, src, n8, xt, g.sc, m, [](int, Chunk<FMT> &) {});
+  const float sum = sum_row<THREADS, true, true>(x, src, n8, xt, g.sc, m, [](int, Chunk<FMT> &) {});
   if (lane == 0) s.m[wv] = m, s.sum[wv] = sum;
   __syncthreads();
 
@@ -225,6 +225,7 @@ __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : THREADS == 256 ? 7 : 8) voi
     const float least = top_key_inv(fl);
 #pragma unroll
     for (int c = 0; c < kRowChunks; ++c) {
+      if (c > 0 && c * THREADS >= (int)n8) break;
       float v[kRowChunk];
       x[c].get(v);
 #pragma unroll
