@@ -735,3 +735,38 @@ def test_graph_replays_match_eager(cuda):
         want = call()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_single_rows_empty_batches_and_broadcast_inputs(cuda):
+    """One row without a batch dimension, batches without rows, and gradients to a row that stands for many."""
+    g = _gen(34)
+    x = torch.randn(3, 2, 777, generator=g).to(B16).to(cuda)
+    val, idx, lse = K.top_logits(x, 9)
+    v1, i1, l1 = K.top_logits(x[1, 1], 9)
+    assert v1.shape == (9,) and l1.shape == () and torch.equal(v1, val[1, 1]) and torch.equal(i1, idx[1, 1]) and torch.equal(l1, lse[1, 1])
+    loss = K.distill_loss(x, val, idx, lse)
+    one, grad = K.distill_loss_grad(x[1, 1], v1, i1, l1)
+    assert loss.shape == (3, 2) and one.shape == () and torch.equal(one, loss[1, 1]) and grad.shape == (777,)
+    for shape in ((0, 777), (3, 0, 777)):
+        e = torch.empty(shape, device=cuda, requires_grad=True)
+        top = K.top_logits(e.detach(), 5)
+        assert top[0].shape == top[1].shape == (*shape[:-1], 5) and top[2].shape == shape[:-1]
+        ops.distill_loss(e, *top, 1.0).sum().backward()
+        assert e.grad.shape == shape
+    # six equal rows: their gradients are added by autograd, in f32: five roundings of a sum below 6
+    w = torch.randn(777, generator=g).to(cuda).requires_grad_()
+    ops.distill_loss(w.expand(3, 2, 777), val, idx, lse).sum().backward()
+    rows = K.distill_loss_grad(w.detach().expand(3, 2, 777), val, idx, lse)[1]
+    assert bool(((w.grad - rows.double().sum((0, 1))).abs() <= 5 * U * rows.double().abs().sum((0, 1))).all())
+    # an entry of one row for all
+    assert torch.equal(K.distill_loss(x, val[:1, :1].expand(3, 2, 9), idx[:1, :1].expand(3, 2, 9)),
+                       K.distill_loss(x, val[:1, :1].repeat(3, 2, 1), idx[:1, :1].repeat(3, 2, 1)))
+    for B in (0, 1):
+        t = torch.randn(B, 4, 777, generator=g).to(cuda)
+        out, n = verify_draft(t, torch.zeros(B, 3, dtype=torch.int64, device=cuda), torch.rand(B, 4, device=cuda), t[:, :3], temperature=1.0)
+        assert out.shape == (B, 4) and n.shape == (B,)
+    t = torch.randn(1, 777, generator=g)
+    u, tok = torch.rand(5, 4, generator=g), torch.randint(0, 777, (5, 3), generator=g)
+    out, n = verify_draft(t.to(cuda).expand(5, 4, 777), tok.to(cuda), u.to(cuda), t.to(cuda).expand(5, 3, 777), temperature=1.0)
+    want, wn = R.verify_draft(t.expand(5, 4, 777).contiguous(), tok, u, t.expand(5, 3, 777).contiguous(), 1.0, 1.0)
+    assert torch.equal(out.cpu(), want) and torch.equal(n.cpu(), wn)
