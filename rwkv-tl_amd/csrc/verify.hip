@@ -101,9 +101,12 @@ struct Weight {
 // that a slice needs no pass for its largest. The power's whole part is added to
 // the exponent's bits as it stands in the low word of k x + 1.5 2^52. Logits
 // outside the range are moved to its ends: a sum over kMuch may hold some from
-// above, one under kNothing holds nothing else than some from below, and either
-// slice is summed again about its largest.
-constexpr double kNothing = 0x1p-900, kMuch = 0x1p999;
+// above, and such a slice is summed again about its largest. One moved up from below
+// counts as 2^-1000, 512 of them as 2^-991: a block's sum under kNothing is taken for
+// nothing. A slice is summed again from kLeast down, far above that, so that a block
+// taken for nothing is at most 2^-500 of its slice. (With one bound for both, 16 blocks
+// of 2^-903 made a slice that stood and of which nothing was drawn.)
+constexpr double kNothing = 0x1p-900, kLeast = 0x1p-400, kMuch = 0x1p999;
 struct BulkWeight {
   float end;  // 1000 / k
   double k;
@@ -236,7 +239,7 @@ __global__ __launch_bounds__(kVerThreads) void verify_stats_kernel(VerifyArgs a)
   };
   float m = 0.f;
   double sum = total(bulk);
-  if (!(sum > kNothing && sum < kMuch)) {  // (the same in every thread)
+  if (!(sum > kLeast && sum < kMuch)) {  // (the same in every thread)
     m = largest();
 #pragma unroll
     for (int c = 0; c < kVerChunks; ++c) x[c].opaque();

@@ -1,0 +1,88 @@
+"""``verify_draft`` over the whole range of its 64-bit exponentials: rows whose sums about 0 come near the range's ends,
+masked tokens at u = 0, and goals that the running sum meets within a rounding. Against float64 on the CPU
+(``oracle.logits_ref``) and whole numbers. Tokens are compared for equality: the kernel's sums are within 1e-11 of
+themselves, a random u meets a border between two of some thousand tokens by that with a chance of 1e-8, and the inputs
+are fixed."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from oracle import logits_ref as R
+from rwkv_tl_amd import verify_draft
+
+pytestmark = pytest.mark.gpu
+H, B16, F = torch.float16, torch.bfloat16, torch.float32
+INF, NAN = float("inf"), float("nan")
+LOG2E = 1.4426950408889634
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def _zipf(g, *shape):
+    return -1.3 * torch.empty(*shape).exponential_(generator=g).log()
+
+
+def _check(cuda, target, tok, u, draft, T, Td):
+    """Equal to the oracle. But behind the rejection of a token drawn from a row almost the target's own the residual
+    max(p - q, 0) is what is left of a cancellation: p and q are known to 2e-12, so of a residual of 1e-3 in all some 9000
+    borders are known to 4e-9 (a u meets one of those with a chance of 4e-5), and of one below that less and less, down to
+    roundings, the oracle's too. Those are left out."""
+    up = lambda t: None if t is None else t.to(cuda)  # noqa: E731
+    out, n = (o.cpu() for o in verify_draft(up(target), up(tok), up(u), up(draft), temperature=T, draft_temperature=Td))
+    want, wn = R.verify_draft(target, tok, u, draft, T, Td)
+    assert torch.equal(n, wn)
+    if draft is not None and Td > 0:
+        p, q = (torch.softmax(x[:, 0].double().nan_to_num(nan=-INF) / t, -1) for x, t in ((target, T), (draft, Td)))
+        vague = (n == 0) & ((p - q).clamp_min(0.0).sum(-1) < 1e-3)
+        out, want = out[~vague], want[~vague]
+    assert torch.equal(out, want)
+
+
+def _shifted(row, shifts, dtype):
+    """``row`` [V], largest 0, moved so that its largest is each of ``shifts``."""
+    return (row + shifts[:, None]).to(dtype)
+
+
+# ---------------------------------------------------------------------------
+# rows whose sum about 0 comes near the lower end of the range
+# ---------------------------------------------------------------------------
+
+# (largest logit) * log2(e) / T: where a slice's sum about 0 is and is not taken, and the range's own end
+SWEEPS = {"-920..-880": torch.arange(-920.0, -879.0), "-600..-560": torch.arange(-600.0, -559.0, 2.0),
+          "-420..-380": torch.arange(-420.0, -379.0), "-1010..-980": torch.arange(-1010.0, -979.0)}
+
+
+@pytest.mark.parametrize("dtype", [H, B16, F], ids=str)
+@pytest.mark.parametrize("sweep", SWEEPS)
+@pytest.mark.parametrize("T", [1.0, 0.1, 0.01])
+def test_rows_near_the_ends_of_the_range(cuda, dtype, sweep, T):
+    at = SWEEPS[sweep] * (T / LOG2E)
+    g = _gen(int(100 * T) + len(sweep))
+    two = torch.full((8192,), -100.0)
+    two[0], two[600] = 0.0, -0.002 * T / 0.01  # two tokens of weight in different blocks of 512
+    for row in (torch.zeros(1000), torch.zeros(8192), two * max(1.0, T), T * _zipf(g, 9001)):
+        row = row - row.max()
+        x = _shifted(row, at, dtype)
+        n, V = x.shape
+        u = torch.rand(n, 2, generator=g)
+        none = torch.zeros(n, 0, dtype=torch.int64)
+        _check(cuda, x[:, None], none, u[:, :1], None, T, 0.0)                       # no drafts
+        tok = torch.randint(0, V, (n, 1), generator=g)
+        both = torch.stack([x, x], 1)
+        _check(cuda, both, tok, u, None, T, 0.0)                                     # drafts without a draw
+        mild = x.float() + T * torch.randn(n, V, generator=g)
+        _check(cuda, both, tok, u, mild.to(dtype)[:, None], T, T)                    # drawn from a row near the target's
+        _check(cuda, both, tok, u, (T * torch.randn(n, 1, V, generator=g)).to(dtype), T, T)  # and from one near 0
+
+
+@pytest.mark.parametrize("dtype", [H, F], ids=str)
+def test_flat_rows_at_every_shift(cuda, dtype):
+    g = _gen(7)
+    at = -torch.arange(600.0, 641.0, 0.5)
+    for V in (1000, 65536):
+        x = _shifted(torch.zeros(V), at, dtype)
+        _check(cuda, x[:, None], torch.zeros(len(at), 0, dtype=torch.int64), torch.rand(len(at), 1, generator=g), None, 1.0, 0.0)
