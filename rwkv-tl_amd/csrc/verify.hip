@@ -101,12 +101,14 @@ struct Weight {
 // that a slice needs no pass for its largest. The power's whole part is added to
 // the exponent's bits as it stands in the low word of k x + 1.5 2^52. Logits
 // outside the range are moved to its ends: a sum over kMuch may hold some from
-// above, and such a slice is summed again about its largest. One moved up from below
-// counts as 2^-1000, 512 of them as 2^-991: a block's sum under kNothing is taken for
-// nothing. A slice is summed again from kLeast down, far above that, so that a block
-// taken for nothing is at most 2^-500 of its slice. (With one bound for both, 16 blocks
-// of 2^-903 made a slice that stood and of which nothing was drawn.)
-constexpr double kNothing = 0x1p-900, kLeast = 0x1p-400, kMuch = 0x1p999;
+// above, and a slice from kLeast down is summed more exactly too: either is summed
+// again about its largest. One moved up from below counts as 2^-1000, 512 of them as
+// 2^-991, which is at most 2^-591 of a row that is summed about 0: a block whose share
+// of what is drawn from is under kNoShare counts for nothing, so that no token is drawn
+// whose logit is -inf or NaN. (Shares, not sums: of a row with a sum of 2^-145, -100 its
+// largest logit, blocks of masked tokens alone were 2^-846 of the whole, more than a
+// bound for sums of 2^-900, and u = 0 fell to their first.)
+constexpr double kLeast = 0x1p-400, kNoShare = 0x1p-580, kMuch = 0x1p999;
 struct BulkWeight {
   float end;  // 1000 / k
   double k;
@@ -370,7 +372,7 @@ RWKV7_DEV void draw(const VerifyArgs &a, int b, const Decision &d) {
       w[e] = kDrawE * lane + e < blocks ? __hip_atomic_load(a.rest + (int64_t)b * blocks + kDrawE * lane + e, __ATOMIC_RELAXED,
                                                             __HIP_MEMORY_SCOPE_AGENT)
                                         : 0.0;
-      if (!(w[e] > kNothing)) w[e] = 0.0;
+      if (!(w[e] > kNoShare)) w[e] = 0.0;
     }
     from_p = !(wave_sum_d((w[0] + w[1]) + w[2]) > 0.0);
   }
@@ -379,8 +381,8 @@ RWKV7_DEV void draw(const VerifyArgs &a, int b, const Decision &d) {
 #pragma unroll
     for (int e = 0; e < kDrawE; ++e) {
       const int i = kDrawE * lane + e, g = min(i / kBlocks, a.G - 1);
-      const double sum = i < blocks ? a.block[r * blocks + i] : 0.0;
-      w[e] = sum > kNothing ? sum * (weight(a.m[r * a.G + g]) * d.ip) : 0.0;
+      w[e] = i < blocks ? a.block[r * blocks + i] * (weight(a.m[r * a.G + g]) * d.ip) : 0.0;
+      if (!(w[e] > kNoShare)) w[e] = 0.0;
     }
   }
   double own = (w[0] + w[1]) + w[2];
@@ -434,7 +436,7 @@ RWKV7_DEV void draw(const VerifyArgs &a, int b, const Decision &d) {
     for (int e = 0; e < kRowChunk; ++e) own += v[e] = res(fp[e], fq[e], i0 + e);
     inc = wave_scan_d(own);
     over = none ? 0 : __ballot(own > 0.0 && base + inc > goal);
-    const u64 here = __ballot(own > 0.0);  // (0 only where all of the block's weights are below 2^-1074)
+    const u64 here = __ballot(own > 0.0);  // (0 only where the block's weight was the roundings of p - q)
     const int lane2 = over ? __ffsll(over) - 1 : here ? 63 - __clzll(here) : 0;
     double acc = base + (inc - own);
     int at = -1, back = 0;

@@ -30,7 +30,7 @@ def _check(cuda, target, tok, u, draft, T, Td):
     """Equal to the oracle. But behind the rejection of a token drawn from a row almost the target's own the residual
     max(p - q, 0) is what is left of a cancellation: p and q are known to 2e-12, so of a residual of 1e-3 in all some 9000
     borders are known to 4e-9 (a u meets one of those with a chance of 4e-5), and of one below that less and less, down to
-    roundings, the oracle's too. Those are left out."""
+    roundings, the oracle's too. There the token needs only be one that the target allows."""
     up = lambda t: None if t is None else t.to(cuda)  # noqa: E731
     out, n = (o.cpu() for o in verify_draft(up(target), up(tok), up(u), up(draft), temperature=T, draft_temperature=Td))
     want, wn = R.verify_draft(target, tok, u, draft, T, Td)
@@ -38,6 +38,7 @@ def _check(cuda, target, tok, u, draft, T, Td):
     if draft is not None and Td > 0:
         p, q = (torch.softmax(x[:, 0].double().nan_to_num(nan=-INF) / t, -1) for x, t in ((target, T), (draft, Td)))
         vague = (n == 0) & ((p - q).clamp_min(0.0).sum(-1) < 1e-3)
+        assert bool((p.gather(1, out[:, :1].clamp_min(0))[:, 0] > 0)[vague].all()) and bool((out[vague, 1] == -1).all())
         out, want = out[~vague], want[~vague]
     assert torch.equal(out, want)
 
@@ -86,3 +87,33 @@ def test_flat_rows_at_every_shift(cuda, dtype):
     for V in (1000, 65536):
         x = _shifted(torch.zeros(V), at, dtype)
         _check(cuda, x[:, None], torch.zeros(len(at), 0, dtype=torch.int64), torch.rand(len(at), 1, generator=g), None, 1.0, 0.0)
+
+# ---------------------------------------------------------------------------
+# masked tokens are never drawn
+# ---------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [H, B16, F], ids=str)
+@pytest.mark.parametrize("mask", [-INF, NAN])
+@pytest.mark.parametrize("T", [1.0, 0.05])
+def test_masked_blocks_are_passed_over_at_u_0(cuda, dtype, mask, T):
+    """u_K = 0 draws the first token with any weight: 512 and 1024 masked ones before it, rows at many distances from 0."""
+    g = _gen(8)
+    at = T * torch.tensor([0.0, 50.0, 500.0, -30.0, -60.0, -64.0, -70.0, -100.0, -120.0, -200.0, -270.0, -280.0, -300.0,
+                           -500.0, -600.0, -620.0, -630.0, -700.0])
+    for V, gone in ((1000, 512), (3000, 1024), (9001, 8192), (20003, 8704)):
+        n = len(at)
+        x = torch.stack([_shifted(T * _zipf(g, V), at, dtype)] * 2, 1)
+        tok = torch.full((n, 1), V - 3)
+        x[:, :, :gone] = mask
+        x[:, 0, V - 3] = (x[:, 0, V - 3].float() - 30.0 * T).to(dtype)  # rejected at the u below
+        u = torch.tensor([[1.0 - 2.0**-24, 0.0]]).repeat(n, 1)
+        _check(cuda, x, tok, u, None, T, 0.0)
+        draft = T * _zipf(g, n, 1, V)
+        draft[:, :, V - 3] = draft.amax(-1) + 20.0 * T
+        for q in (draft, draft.masked_fill(torch.arange(V) < gone, mask), draft + at[:, None, None]):
+            _check(cuda, x, tok, u, q.to(dtype), T, T)
+        u[:, 0] = 0.0  # accepted: the draw from p itself
+        _check(cuda, x, tok, u, draft.to(dtype), T, T)
+        u[:, 1] = 1.0  # (the documented range ends below it: the last token with any weight)
+        _check(cuda, x, tok, u, draft.to(dtype), T, T)
