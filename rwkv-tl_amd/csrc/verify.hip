@@ -431,12 +431,18 @@ RWKV7_DEV void draw(const VerifyArgs &a, int b, const Decision &d) {
       fq[0] = i0 < V ? load_logit<FMT>(qr, i0) : -kInf;
     }
     double v[kRowChunk];
-    own = 0.0;
+    auto weigh = [&](auto of) {
+      own = 0.0;
 #pragma unroll
-    for (int e = 0; e < kRowChunk; ++e) own += v[e] = res(fp[e], fq[e], i0 + e);
+      for (int e = 0; e < kRowChunk; ++e) own += v[e] = of(e);
+      return __ballot(own > 0.0);
+    };
+    u64 here = weigh([&](int e) { return res(fp[e], fq[e], i0 + e); });
+    // Where p and q differ by their last bits, the block's sum, of bulk exponentials, may
+    // be a rounding that these do not have: then by p, so that no masked token is drawn.
+    if (!here) here = weigh([&](int e) { return res.p(fp[e]) * d.ip; });
     inc = wave_scan_d(own);
     over = none ? 0 : __ballot(own > 0.0 && base + inc > goal);
-    const u64 here = __ballot(own > 0.0);  // (0 only where the block's weight was the roundings of p - q)
     const int lane2 = over ? __ffsll(over) - 1 : here ? 63 - __clzll(here) : 0;
     double acc = base + (inc - own);
     int at = -1, back = 0;

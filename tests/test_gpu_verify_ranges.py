@@ -117,3 +117,21 @@ def test_masked_blocks_are_passed_over_at_u_0(cuda, dtype, mask, T):
         _check(cuda, x, tok, u, draft.to(dtype), T, T)
         u[:, 1] = 1.0  # (the documented range ends below it: the last token with any weight)
         _check(cuda, x, tok, u, draft.to(dtype), T, T)
+
+
+def test_a_residual_of_roundings_alone_draws_no_masked_token(cuda):
+    """One token before the others whose p and q are a rounding apart: whether that leaves it any weight is a matter of
+    roundings, but the masked ones around it have none."""
+    n, V = 4000, 1500
+    g = _gen(9)
+    x = torch.full((n, 2, V), -INF)
+    x[:, :, 300] = -6.0 * torch.rand(n, 1, generator=g) - 0.5
+    x[:, :, 600:856] = 0.0
+    x[:, :, 1100] = 0.0
+    q = x[:, :1].clone()
+    q[:, :, 1100], q[:, :, 1200] = -INF, 0.0
+    q[:, 0, 700] = 2.0**-45 * torch.randint(-6, 7, (n,), generator=g)
+    out, acc = verify_draft(x.to(cuda), torch.full((n, 1), 1200, device=cuda), torch.zeros(n, 2, device=cuda), q.to(cuda),
+                            temperature=0.7)
+    assert (acc == 0).all()
+    assert x[:, 0].gather(1, out[:, :1].cpu()).isfinite().all()
