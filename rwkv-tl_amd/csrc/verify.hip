@@ -404,7 +404,10 @@ RWKV7_DEV void draw(const VerifyArgs &a, int b, const Decision &d) {
       if (stop) e0 = e;
       else if (e0 < 0) base += w[e];
     }
-    if (e0 < 0) {  // (by rounding the running sum may end just below the goal)
+    // By rounding the running sum may end just below the goal: then the last token of
+    // the lane's last block with any weight, as where nothing exceeds the goal.
+    const bool end = none || __builtin_amdgcn_readlane(e0, who) < 0;
+    if (e0 < 0) {
 #pragma unroll
       for (int e = 0; e < kDrawE; ++e)
         if (w[e] > 0.0) e0 = e;
@@ -442,7 +445,7 @@ RWKV7_DEV void draw(const VerifyArgs &a, int b, const Decision &d) {
     // be a rounding that these do not have: then by p, so that no masked token is drawn.
     if (!here) here = weigh([&](int e) { return res.p(fp[e]) * d.ip; });
     inc = wave_scan_d(own);
-    over = none ? 0 : __ballot(own > 0.0 && base + inc > goal);
+    over = end ? 0 : __ballot(own > 0.0 && base + inc > goal);
     const int lane2 = over ? __ffsll(over) - 1 : here ? 63 - __clzll(here) : 0;
     double acc = base + (inc - own);
     int at = -1, back = 0;

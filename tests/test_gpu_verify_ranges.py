@@ -135,3 +135,43 @@ def test_a_residual_of_roundings_alone_draws_no_masked_token(cuda):
                             temperature=0.7)
     assert (acc == 0).all()
     assert x[:, 0].gather(1, out[:, :1].cpu()).isfinite().all()
+
+
+# ---------------------------------------------------------------------------
+# goals within a rounding of a border
+# ---------------------------------------------------------------------------
+
+# Sums of blocks of 512 tokens, as multiples of one weight: those of the first lanes of three blocks are a few units more
+# than half of all, so that at u = 0.5 the exact sum passes the goal at the last token of the last of them, while the
+# running sum in 64 bits, from block to block, ends on the goal.
+BLOCK_SUMS = [
+    [1145859633778797, 352630542926771, 973175940787175, 613593555701514, 536808607908891, 881530479136178] + 9 * [450359876023932]
+    + [450359876023937],
+    [759373514701697, 1214240432488022, 128677358106348, 661252096165449, 1158952546121088, 581103048745430] + 9 * [450359899632803]
+    + [450359899632806],
+    [246368824764733, 548419992108399, 854323041859110, 396816985282743, 343466264402641, 358936908495985, 575037014482333,
+     752082123627653, 428147725270595] + 6 * [643371268613455] + [643371268613458],
+    [816075089083930, 362505266396518, 577498043038902, 604518220769384, 81891060324226, 196261183937186, 358973546335445,
+     802100149714336, 703776430349826] + 6 * [643371284278536] + [643371284278536],
+]
+
+
+@pytest.mark.parametrize("case", range(len(BLOCK_SUMS)))
+@pytest.mark.parametrize("dtype", [H, F], ids=str)
+def test_a_goal_that_the_running_sum_just_misses(cuda, case, dtype):
+    """Weights that are powers of two (T = log2(e), whole logits), the largest of each block last."""
+    x = torch.full((1, 1, 8192), -INF)
+    weight = [0] * 8192
+    for b, s in enumerate(BLOCK_SUMS[case]):
+        for j, e in enumerate(e for e in range(53) if s >> e & 1):
+            x[0, 0, 512 * b + 9 * j + 3] = float(e)
+            weight[512 * b + 9 * j + 3] = 1 << e
+    acc, want = 0, None
+    for v, w in enumerate(weight):  # the first whose exact sum exceeds half
+        acc += w
+        if 2 * acc > sum(weight):
+            want = v
+            break
+    out, _ = verify_draft(x.to(dtype).to(cuda), torch.zeros(1, 0, dtype=torch.int64, device=cuda),
+                          torch.full((1, 1), 0.5, device=cuda), temperature=LOG2E)
+    assert out.tolist() == [[want]]
