@@ -490,9 +490,9 @@ int rwkv7_top_logits(const void *logits, int32_t logits_dtype, int64_t ld, int32
  *   loss = sum p_k log(p_k / q_k) + R log(R / the student's mass outside the
  *   row's ids);
  *   lse NULL: p = softmax of the entries, R = 0.
- * An id in several entries has the sum of their p. A row without an entry (or
- * without lse and without mass) has loss 0 and gradient 0 whatever its logits
- * hold. loss f32 [N] and grad [N, grad_ld] of the logits' type: either may be
+ * An id in several entries has the sum of their p. A row without an entry, or
+ * without mass (entries of -inf alone; lse NULL, or -inf), has loss 0 and gradient
+ * 0 whatever its logits hold. loss f32 [N] and grad [N, grad_ld] of the logits' type: either may be
  * NULL, not both. grad = scale * d loss / d logits with scale f32 [N] (NULL:
  * scale0); rows with scale 0 have gradient 0. grad may not overlap logits. */
 int rwkv7_distill(const void *logits, int32_t logits_dtype, int64_t ld, int32_t N, int32_t V, const void *top_val,

@@ -13,9 +13,9 @@
 //   loss = sum_k p_k (log p_k - log q_{i_k}) + R (log R - log(1 - Q))
 //   d loss / d z_j = a ((P + R) q_j - sum_{k: i_k = j} p_k)      j in I
 //                  = a q_j (P + R - R / (1 - Q))                  else
-// A row without a present entry (or, without lse, without mass) has loss 0 and
-// gradient 0, whatever its logits hold. NaN elsewhere makes its row NaN, as in a
-// log-softmax.
+// A row without a present entry or without mass (entries of -inf alone, and no lse or
+// one of -inf: a teacher's row that a mask leaves nothing of) has loss 0 and gradient 0,
+// whatever its logits hold. NaN elsewhere makes its row NaN, as in a log-softmax.
 //
 // 1 - Q is never formed as a difference: the row's elements in I are taken out
 // (each thread has a word in LDS that marks them) before the sum, and I enters
@@ -126,7 +126,7 @@ RWKV7_DEV Joined join(const DistillArgs &g, const DistillLds &s, int lane, doubl
   } else {
     j.P = j.W == j.W ? 1.0 : j.W;
   }
-  j.mass = g.lse || j.W != 0.0;  // false: every present entry is -inf
+  j.mass = (g.lse && lse != -__builtin_inf()) || j.W != 0.0;  // false: every present entry is -inf
   return j;
 }
 
@@ -147,8 +147,9 @@ RWKV7_DEV void put_loss(const DistillArgs &g, const DistillLds &s, const Joined 
     if (j.rest_t > 0.0)
       loss += j.rest_t * (log2_d(j.rest_t) - (g.sc.k * ((double)j.mrest - (double)j.m) + (g.sc.off(j.mrest) + log2_d(j.Srest)) - S));
   } else {
-    loss = j.mass ? A * rcp_d(j.W) - log2_d(j.W) + S : 0.0;
+    loss = A * rcp_d(j.W) - log2_d(j.W) + S;
   }
+  if (!j.mass) loss = 0.0;
   if (lane == 0) g.loss[row] = (float)(kLn2 * loss);
 }
 

@@ -157,8 +157,9 @@ def distill_loss(logits: Tensor, top_val: Tensor, top_idx: Tensor, lse: Tensor |
 
     ``top_val [..., K]`` (any of the three dtypes) and ``top_idx [..., K]`` int64
     are the teacher's entries, K <= 1024; an id outside ``0..V-1`` (say -1) means
-    no entry, so rows may have fewer, and a row without any has loss 0 and
-    gradient 0 whatever its logits hold (a padded position). With ``lse [...]``
+    no entry, so rows may have fewer, and a row without any, or with values of -inf
+    alone (and an ``lse`` of -inf, as ``top_logits`` gives a row that is all masked),
+    has loss 0 and gradient 0 whatever its logits hold (a padded position). With ``lse [...]``
     float32, the teacher's log-sum-exp over its whole vocabulary at the same
     temperature, ``p_k = exp(top_val_k / temperature - lse)`` and the mass that
     this leaves (2^-20 or more, of a row that does not list every id) is held against
