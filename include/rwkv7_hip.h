@@ -486,7 +486,7 @@ int rwkv7_top_logits(const void *logits, int32_t logits_dtype, int64_t ld, int32
  * value is not looked at), and logits top_val [N, K] (val_dtype as above).
  *   lse f32 [N] given, log sum exp(teacher / temperature) over the teacher's
  *   vocabulary: p_k = exp(top_val_k / temperature - lse), R = 1 - sum p (none
- *   below 2^-20, nor where every id has an entry), and
+ *   below half a step of lse, 2^-20 at least, nor where every id has an entry), and
  *   loss = sum p_k log(p_k / q_k) + R log(R / the student's mass outside the
  *   row's ids);
  *   lse NULL: p = softmax of the entries, R = 0.

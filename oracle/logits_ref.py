@@ -3,10 +3,15 @@
 
 from __future__ import annotations
 
+import math
+
 import torch
 from torch import Tensor
 
-LEAST_REST = 2.0**-20
+def least_rest(lse: float) -> float:
+    """A teacher's mass outside its entries below this is none: half a step of ``lse`` as float32 (which rounding it may
+    take from 1), 2^-20 at least."""
+    return max(2.0**-20, math.ldexp(1.0, math.frexp(float(torch.tensor(lse).float()))[1] - 25))
 
 
 def top_logits(logits: Tensor, k: int, temperature: float = 1.0) -> tuple[Tensor, Tensor, Tensor]:
@@ -38,7 +43,7 @@ def distill_loss(logits: Tensor, top_val: Tensor, top_idx: Tensor, lse: Tensor |
         rest = max(0.0, 1.0 - float(p.sum())) if lse is not None else 0.0
         outside = torch.ones(V, dtype=torch.bool)
         outside[ids] = False
-        if rest >= LEAST_REST and bool(outside.any()):
+        if lse is not None and rest >= least_rest(float(lse[r])) and bool(outside.any()):
             # about its own largest logit: far below the row's, the others' differences would be lost
             z = logits[r][outside]
             m = z.detach().max()

@@ -6,7 +6,7 @@
 // 0 .. V-1 is absent. I is the set of ids present.
 //   lse given (Lt, over the teacher's whole vocabulary): p_k = exp(a t_k - Lt),
 //     P = sum p_k, and R = 1 - P is the teacher's mass outside I (0 below
-//     2^-20, which an f32 Lt cannot tell from none, and 0 where I is the whole
+//     least_rest, which an f32 Lt cannot tell from none, and 0 where I is the whole
 //     vocabulary), held against the student's own mass there, 1 - Q = sum_{j not
 //     in I} q_j.
 //   no lse: p = softmax of a t over the present entries; P = 1, R = 0.
@@ -41,7 +41,6 @@ namespace rwkv7 {
 namespace {
 
 constexpr int kDistMaxK = kRowMaxThreads;
-constexpr double kLeastRest = 1.0 / 1048576.0;
 constexpr double kLn2 = 0.69314718055994531, kLog2E = 1.4426950408889634;
 
 struct DistillArgs {
@@ -96,6 +95,17 @@ RWKV7_DEV void zero_row(char *dst, int V) {
   if (threadIdx.x < V % kRowChunk) store_logit<FMT>(dst, V / kRowChunk * kRowChunk + threadIdx.x, 0.f);
 }
 
+// The least mass outside the ids that counts: half a step of the f32 Lt, which rounding
+// alone can take from 1 (P = exp(-half a step) of a teacher whose every logit with
+// any mass is listed), but no less than 2^-20, the half step of 16 <= |Lt| < 32. (With
+// 2^-20 for all, an Lt of 200 made a rest of up to 8e-6, and a student with 1e-30 outside
+// the ids paid 5e-4 for it.) lse: Lt to base 2.
+RWKV7_DEV double least_rest(double lse) {
+  int ex;
+  (void)frexpf((float)(lse * kLn2), &ex);  // (back to Lt itself, exactly)
+  return fmax(0x1p-20, ldexp(1.0, ex - 25));
+}
+
 // The waves' parts joined by one wave, one a lane. Logarithms and the teacher's
 // references are to base 2.
 template <int WAVES>
@@ -122,7 +132,7 @@ RWKV7_DEV Joined join(const DistillArgs &g, const DistillLds &s, int lane, doubl
   j.P = j.W, j.rest_t = 0.0;
   if (g.lse) {
     j.rest_t = uniform_d(1.0 - j.W);
-    if (j.rest_t < kLeastRest || s.whole) j.rest_t = 0.0;
+    if (j.rest_t < least_rest(lse) || s.whole) j.rest_t = 0.0;
   } else {
     j.P = j.W == j.W ? 1.0 : j.W;
   }

@@ -162,8 +162,9 @@ def distill_loss(logits: Tensor, top_val: Tensor, top_idx: Tensor, lse: Tensor |
     has loss 0 and gradient 0 whatever its logits hold (a padded position). With ``lse [...]``
     float32, the teacher's log-sum-exp over its whole vocabulary at the same
     temperature, ``p_k = exp(top_val_k / temperature - lse)`` and the mass that
-    this leaves (2^-20 or more, of a row that does not list every id) is held against
-    the student's mass outside the row's ids; without it, ``p`` is the softmax of the
+    this leaves (2^-20 or more, or half a step of ``lse`` where that is more: beyond
+    +-32; of a row that does not list every id) is held against the student's mass
+    outside the row's ids; without it, ``p`` is the softmax of the
     entries. There is no factor ``temperature ** 2``.
 
     Without autograd; ``torch.ops.rwkv_tl.distill_loss`` is the differentiable form."""

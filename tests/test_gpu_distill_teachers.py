@@ -1,7 +1,9 @@
-"""Teachers at the edges of ``distill_loss``: rows that a mask leaves nothing of. Against float64 on the CPU
-(``oracle.logits_ref``)."""
+"""Teachers at the edges of ``distill_loss``: rows that a mask leaves nothing of, and log-sum-exps far from 0, against
+float64 on the CPU (``oracle.logits_ref``)."""
 
 from __future__ import annotations
+
+import math
 
 import pytest
 import torch
@@ -40,3 +42,45 @@ def test_a_teacher_row_that_a_mask_leaves_nothing_of(cuda, dtype, V, k):
     # a finite entry beside an lse of -inf is no distribution
     val[1, 0] = 0.0
     assert K.distill_loss(torch.zeros(3, V, device=cuda), val, idx, lse)[1].isnan()
+
+
+@pytest.mark.parametrize("at", [100.0, -100.0, 200.3, -1000.7, 60000.0])
+def test_a_rounded_log_sum_exp_leaves_no_mass(cuda, at):
+    """Teachers whose listed logits are all of their mass, far from 0: what rounding their lse to float32 takes from 1 is
+    no rest, however little the student has outside the ids."""
+    g = torch.Generator().manual_seed(int(abs(at)))
+    N, V, k = 64, 500, 12
+    t = (torch.randn(N, k, generator=g) + at).float()
+    idx = torch.stack([torch.randperm(V, generator=g)[:k] for _ in range(N)])
+    lse = torch.logsumexp(t.double(), -1)
+    lse32 = lse.float()
+    assert bool((lse32.double() > lse).any())  # of which P < 1
+    z = torch.full((N, V), -80.0)
+    z.scatter_(1, idx, torch.randn(N, k, generator=g))
+    loss, grad = (x.double().cpu() for x in K.distill_loss_grad(z.to(cuda), t.to(cuda), idx.to(cuda), lse32.to(cuda)))
+    p = (t.double() - lse32.double()[:, None]).exp()  # the teacher that the stored lse gives, without a rest
+    y = torch.log_softmax(z.double(), -1)
+    want = (p * (p.log() - y.gather(1, idx))).sum(-1)
+    assert bool(((loss - want).abs() <= 112 * U + U * want.abs()).all())
+    ref = (y.exp() * p.sum(-1, keepdim=True)).scatter_add(1, idx, -p)
+    # 60 half steps of each term, and 3 of the exponent's size (up to 85)
+    size = (y.exp() * p.sum(-1, keepdim=True)).scatter_add(1, idx, p)
+    assert bool(((grad - ref).abs() <= (60 + 3 * 90) * U * size + U * ref.abs() + 2.0**-125).all())
+    assert torch.allclose(R.distill_loss(z.double(), t, idx, lse32), want, rtol=0, atol=1e-9)
+
+
+def test_a_rest_just_above_half_a_step_counts(cuda):
+    """A teacher's mass outside its ids of twice the cut is held against the student's."""
+    z = torch.tensor([[0.0, 0.0, -3.0, -4.0]]).repeat(2, 1)
+    val, idx = torch.tensor([[200.0], [10.0]]), torch.zeros(2, 1, dtype=torch.int64)
+    lse = torch.tensor([200.0 + 2.0**-16, 10.0 + 2.0**-19])  # half steps of 2^-17 and 2^-21
+    want = R.distill_loss(z.double(), val, idx, lse)
+    q = torch.softmax(z[0].double(), -1)
+    for r in range(2):
+        p = math.exp(float(val[r, 0]) - float(lse[r]))
+        by_hand = p * math.log(p / float(q[0])) + (1 - p) * math.log((1 - p) / float(q[1:].sum()))
+        assert abs(by_hand - float(want[r])) < 1e-10
+    loss = K.distill_loss(z.to(cuda), val.to(cuda), idx.to(cuda), lse.to(cuda)).double().cpu()
+    assert bool(((loss - want).abs() <= 112 * U + U * want.abs()).all())
+    # (without it the first loss would be 1.5e-4 more; the tolerance is 6.7e-6)
+    assert abs(float(want[0]) + math.log(float(q[0]))) > 1e-4
