@@ -158,8 +158,9 @@ LOGITS_OPS: dict[str, tuple[str, Callable, Callable]] = {
 
 def _plain(x: Tensor) -> bool:
     """Whether a call on ``x`` may go straight to the kernel: no tracing, no
-    dispatch mode that wants to see the operator."""
-    return type(x) is Tensor and x.is_cuda and not torch._C._len_torch_dispatch_stack()
+    dispatch mode that wants to see the operator, no batch of tensors in one (that of
+    ``torch.autograd.grad(..., is_grads_batched=True)``, which has no storage)."""
+    return type(x) is Tensor and x.is_cuda and not torch._C._len_torch_dispatch_stack() and torch._C._has_storage(x)
 
 
 class _DistillLoss(torch.autograd.Function):
