@@ -169,8 +169,6 @@ class _DistillLoss(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, top_val, top_idx, lse, temperature):
-        if ctx.needs_input_grad[1] or ctx.needs_input_grad[3]:
-            raise ValueError("distill_loss has no gradient to the teacher: detach top_val and lse")
         ctx.save_for_backward(logits, top_val, top_idx, lse)
         ctx.temperature = temperature
         if _plain(logits):
@@ -198,6 +196,9 @@ class _DistillLossBackward(torch.autograd.Function):
 
 
 def _distill_autograd(logits, top_val, top_idx, lse=None, temperature=1.0):
+    # (here: in forward the grad mode is off, and the flags say the same without it)
+    if (top_val.requires_grad or (lse is not None and lse.requires_grad)) and torch.is_grad_enabled():
+        raise ValueError("distill_loss has no gradient to the teacher: detach top_val and lse")
     return _DistillLoss.apply(logits, top_val, top_idx, lse, temperature)
 
 

@@ -1,5 +1,5 @@
-"""``torch.ops.rwkv_tl.distill_loss`` under autograd's batching, vmap and checkpointing: the same bits as the kernels called
-row by row."""
+"""``torch.ops.rwkv_tl.distill_loss`` under autograd's batching, vmap and checkpointing, the same bits as the kernels called
+row by row; and a teacher that requires gradients."""
 
 from __future__ import annotations
 
@@ -56,3 +56,17 @@ def test_transforms_without_a_rule_are_refused(case):
         torch.func.grad(lambda x: _loss(case)(x).sum())(z)
     with pytest.raises(NotImplementedError, match="jvp"), torch.autograd.forward_ad.dual_level():
         _loss(case)(torch.autograd.forward_ad.make_dual(z, z))
+
+
+def test_a_teacher_that_requires_gradients_without_grad_mode(cuda):
+    """Evaluation inside no_grad of a teacher whose tensors are part of a graph: nothing asks for their gradient."""
+    z = torch.randn(3, 100, generator=torch.Generator().manual_seed(4)).to(cuda)
+    t = torch.randn(3, 100, generator=torch.Generator().manual_seed(5)).to(cuda).requires_grad_()
+    val, idx = t.topk(7)
+    lse = torch.logsumexp(t, -1)
+    want = K.distill_loss(z, val.detach(), idx, lse.detach())
+    for x in (z, z.clone().requires_grad_()):
+        with torch.no_grad():
+            assert torch.equal(ops.distill_loss(x, val, idx, lse), want)
+        with pytest.raises(ValueError, match="no gradient to the teacher"):
+            ops.distill_loss(x, val, idx, lse)
