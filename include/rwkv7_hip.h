@@ -494,7 +494,8 @@ int rwkv7_top_logits(const void *logits, int32_t logits_dtype, int64_t ld, int32
  * without mass (entries of -inf alone; lse NULL, or -inf), has loss 0 and gradient
  * 0 whatever its logits hold. loss f32 [N] and grad [N, grad_ld] of the logits' type: either may be
  * NULL, not both. grad = scale * d loss / d logits with scale f32 [N] (NULL:
- * scale0); rows with scale 0 have gradient 0. grad may not overlap logits. */
+ * scale0); rows with scale 0 have gradient 0, and scale / temperature has to be an
+ * f32 number. grad may not overlap logits. */
 int rwkv7_distill(const void *logits, int32_t logits_dtype, int64_t ld, int32_t N, int32_t V, const void *top_val,
                   int32_t val_dtype, const int64_t *top_idx, int32_t K, const float *lse, double temperature,
                   const float *scale, float scale0, float *loss, void *grad, int64_t grad_ld, void *stream);

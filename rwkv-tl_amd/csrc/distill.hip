@@ -29,11 +29,12 @@
 // of both signs (in 32 bits a loss of 331 x 20011 f32 was off by 3.5e-6 of itself,
 // now by 1.2e-7).
 //
-// Measured (kernel, us; a large copy moves 5.05 TB/s here): loss and gradient of 4096
-// x 65536 bf16 215, 5.0 TB/s: the bytes (vector units busy 64 %). Loss of 1021 x
-// 65536 f16 29.5, 4.5 TB/s, and its gradient 49, 5.4 TB/s (in part from the last
+// Measured (kernel trace, us; a large copy moves 5.05 TB/s here): loss and gradient of
+// 4096 x 65536 bf16 216, 5.0 TB/s: the bytes (vector units busy 64 %). Loss of 1021 x
+// 65536 f16 29.8, 4.5 TB/s, and its gradient 49, 5.4 TB/s (in part from the last
 // cache). Few or short rows are a chain of load, sum, join and logarithms: 16 x 65536
-// f16 9.2; 331 x 20011 f32 10.6, gradient 14.5.
+// f16 9.2; 331 x 20011 f32 10.6, gradient 14.5. Back to back in a graph: 331 x 20011
+// f32 loss 9.0, loss and gradient 16; 2000 x 65536 f32 119 (4.4 TB/s) and 243 (4.3).
 #include "logits_rows.h"
 #include "rwkv7_kernels.h"
 

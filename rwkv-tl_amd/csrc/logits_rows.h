@@ -5,8 +5,9 @@
 // (maximum, sum, selection, gradient). 64 logits a thread is what that needs at
 // 65536 logits and 1024 threads: 32 registers in 16 bits, of the 64 that two such
 // workgroups on a CU leave each thread (f32: 64 of 128, one workgroup). Two matter:
-// one loads while the other computes. With the 27 registers a thread that spilled at
-// first, loss and gradient of 4096 x 65536 bf16 took 302 us; without, 244.
+// one loads while the other computes (loss and gradient of 4096 x 65536 bf16 5.0 TB/s;
+// of 2000 x 65536 f32 4.3). With the 27 registers a thread that spilled at first, loss
+// and gradient of the former took 302 us; without, 244.
 #pragma once
 
 #include "rwkv7_common.h"
@@ -309,8 +310,8 @@ struct ExpScale {
 // units above m), where the first chunks hold nothing, and far from 0, it is formed
 // again about the largest: from memory, a chunk at a time, which is rare and holds
 // nothing beside the row. KNOWN: m is the wave's largest already. SKIP: chunks that no
-// thread has are left out (loss of 331 x 20011 f32 9.9 -> 9.2 us, top logits of 2000 x
-// 20011 bf16 29.8 -> 26.8); where registers are short, in a kernel with a gradient, the
+// thread has are left out (back to back, loss of 331 x 20011 f32 9.9 -> 9.2 us, top
+// logits of 2000 x 20011 bf16 29.8 -> 26.8); where registers are short, in a kernel with a gradient, the
 // branches cost a full row more (loss and gradient of 4096 x 65536 bf16 214 -> 225).
 template <int THREADS, bool KNOWN, bool SKIP, int FMT, class See>
 RWKV7_DEV float sum_row(Chunk<FMT> (&x)[kRowChunks], const void *src, uint32_t n8, float tail, const ExpScale &sc, float &m,

@@ -18,11 +18,12 @@
 // gathered.
 //
 // Why bins: ranked each against all, some 400 candidates took 4.7 us a row. Measured
-// (kernel, us; a large copy moves 5.05 TB/s here): 4096 x 65536 bf16, k 200, 131, 4.1
-// TB/s: the vector units are busy 91 % of it with 13 instructions a logit (maxima,
-// exponentials, comparisons). 509 x 65536 bf16, k 64, 20, 3.3 TB/s: one round of two
-// rows a CU, each a chain of load, floor, sum, gather and ranking. One row 9.0; 257 x
-// 20011 f32 11.6.
+// (kernel trace, us; a large copy moves 5.05 TB/s here): 4096 x 65536 bf16, k 200,
+// 131-139, 3.9-4.1 TB/s: the vector units are busy 91 % of it with 13 instructions a
+// logit (maxima, exponentials, comparisons). 509 x 65536 bf16, k 64, 20, 3.3 TB/s: one
+// round of two rows a CU, each a chain of load, floor, sum, gather and ranking. One row
+// 9.1; 257 x 20011 f32 12.5 (back to back in a graph 9.9); 2000 x 65536 f32, k 64, back
+// to back 125, 4.2 TB/s.
 #include "logits_rows.h"
 #include "rwkv7_kernels.h"
 

@@ -23,21 +23,23 @@
 // draw from.
 //
 // verify_stats_kernel: a slice of a row per workgroup: the sum of its
-//   exponentials, about 0 or its largest logit, for target rows also of each 512
-//   logits (greedy: largest logit and its first id). 8192 logits a workgroup, so that
-//   one sequence of four drafts already has 72 of them. 96 sequences of up to 7
-//   drafts x 65536 bf16, 830 rows that count: 41 us (109 MB, 2.6 TB/s), the vector units busy
-//   86 % of it at 1.86 GHz with 19.6 instructions a logit, 12 of them 64-bit. 16 x 8 f16
-//   10.5, 1 x 4 4.1.
-// verify_draw_kernel: 2048 logits (large batches: 8192) of each sequence's decisive row: every workgroup
-//   joins the sums of its sequence's rows and decides how many tokens are
+//   exponentials, about 0 or (where that comes out far from 1) about its largest
+//   logit, for target rows also of each 512 logits (greedy: largest logit and its
+//   first id). 8192 logits a workgroup, so that one sequence of four drafts already
+//   has 72 of them. 96 sequences of up to 7 drafts x 65536 bf16, 830 rows that count:
+//   41 us (109 MB, 2.6 TB/s), the vector units busy 86 % of it at 1.86 GHz with 19.6
+//   instructions a logit, 12 of them 64-bit. 16 x 8 f16 10.2, 1 x 4 4.1.
+// verify_draw_kernel: 2048 logits (large batches: 8192) of each sequence's decisive
+//   row: every workgroup joins the sums of its sequence's rows and decides how many tokens are
 //   accepted; the sums of max(p - q, 0) over each 512 of its logits; the last
 //   workgroup of a sequence to finish (the only one that stays, where all tokens
 //   are accepted) finds the 512 in which the running sum crosses, and in them the
 //   token, by one wave. (As a launch of its own this draw took 3 us more of a call's
 //   chain and 2 of its host time.) A chain of seven dependent trips to memory and
-//   three prefixes: 9.7 us for one sequence, 11.7 for 16, 19.3 for 96.
-// verify_greedy_kernel: a wave per sequence, 3.8 us, most of it the launch.
+//   three prefixes: 10.0 us for one sequence, 12.0 for 16, 19.3 for 96. Both
+//   kernels back to back in a graph, 1 x 4 / 16 x 8 / 96 x 7: 12.6 / 21.7 / 59 us, and of
+//   drafts without a draw, whose rows are half as many, 11.0 / 19.3 / 39.
+// verify_greedy_kernel: a wave per sequence, 3.6 us, most of it the launch.
 #include "logits_rows.h"
 #include "rwkv7_kernels.h"
 

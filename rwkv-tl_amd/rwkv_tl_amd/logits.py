@@ -176,7 +176,8 @@ def distill_loss_grad(logits: Tensor, top_val: Tensor, top_idx: Tensor, lse: Ten
     """``distill_loss`` and ``scale`` times its gradient to ``logits`` in one pass
     over them: ``(loss [...] float32, grad [..., V] of the logits' dtype)``.
     ``scale``: a number, or float32 ``[...]`` (each row's weight in the loss and a
-    loss scale; a row with 0 has gradient 0). For ``logits.backward(grad)``."""
+    loss scale; a row with 0 has gradient 0); ``scale / temperature`` within float32.
+    For ``logits.backward(grad)``."""
     return _distill(logits, top_val, top_idx, lse, temperature, scale, True, True)
 
 
