@@ -119,6 +119,26 @@ def test_masked_blocks_are_passed_over_at_u_0(cuda, dtype, mask, T):
         _check(cuda, x, tok, u, draft.to(dtype), T, T)
 
 
+def test_masked_blocks_in_wide_batches(cuda):
+    """The same in batches whose decisive rows are dealt 8192 logits to a workgroup."""
+    g = _gen(10)
+    V, gone = 9001, 2048
+    at = torch.tensor([0.0, -60.0, -70.0, -120.0, -270.0, -290.0, -500.0, -630.0, -700.0])
+    x = torch.stack([_shifted(_zipf(g, V), at, F)] * 2, 1)
+    x[:, :, :gone] = -INF
+    x[:, 0, V - 3] -= 30.0
+    draft = _zipf(g, len(at), 1, V)
+    draft[:, :, V - 3] = draft.amax(-1) + 20.0
+    tok = torch.full((len(at), 1), V - 3)
+    for last in (0.0, 0.3, 1.0 - 2.0**-24):
+        u = torch.tensor([[1.0 - 2.0**-24, last]]).repeat(len(at), 1)
+        for q in (None, draft):
+            want = R.verify_draft(x, tok, u, q, 1.0, 0.0 if q is None else 1.0)[0]
+            many = [None if t is None else t.repeat(26, *[1] * (t.ndim - 1)).to(cuda) for t in (x, tok, u, q)]
+            out, n = verify_draft(*many, temperature=1.0)
+            assert bool((n == 0).all()) and torch.equal(out.cpu(), want.repeat(26, 1))
+
+
 def test_a_residual_of_roundings_alone_draws_no_masked_token(cuda):
     """One token before the others whose p and q are a rounding apart: whether that leaves it any weight is a matter of
     roundings, but the masked ones around it have none."""
