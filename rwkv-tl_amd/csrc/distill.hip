@@ -100,15 +100,15 @@ RWKV7_DEV void zero_row(char *dst, int V) {
 // alone can take from 1 (P = exp(-half a step) of a teacher whose every logit with
 // any mass is listed), but no less than 2^-20, the half step of 16 <= |Lt| < 32. (With
 // 2^-20 for all, an Lt of 200 made a rest of up to 8e-6, and a student with 1e-30 outside
-// the ids paid 5e-4 for it.) lse: Lt to base 2.
+// the ids paid 5e-4 for it.)
 RWKV7_DEV double least_rest(double lse) {
   int ex;
-  (void)frexpf((float)(lse * kLn2), &ex);  // (back to Lt itself, exactly)
+  (void)frexpf((float)lse, &ex);
   return fmax(0x1p-20, ldexp(1.0, ex - 25));
 }
 
 // The waves' parts joined by one wave, one a lane. Logarithms and the teacher's
-// references are to base 2.
+// references are to base 2, but lse.
 template <int WAVES>
 RWKV7_DEV Joined join(const DistillArgs &g, const DistillLds &s, int lane, double lse) {
   Joined j;
@@ -123,7 +123,7 @@ RWKV7_DEV Joined join(const DistillArgs &g, const DistillLds &s, int lane, doubl
   if (!(j.m > -kInf)) j.S = __builtin_nan("");  // no finite logit at all
   const int tws = (g.K + kWave - 1) / kWave;
   double W = lane < tws ? s.tw[lane] : 0.0;
-  j.tref = lse;
+  j.tref = 0.0;
   if (!g.lse) {
     const double tr = lane < tws ? s.tref[lane] : -__builtin_inf();
     j.tref = uniform_d(wave_max_d(tr));
@@ -141,7 +141,7 @@ RWKV7_DEV Joined join(const DistillArgs &g, const DistillLds &s, int lane, doubl
   return j;
 }
 
-RWKV7_DEV void put_loss(const DistillArgs &g, const DistillLds &s, const Joined &j, int lane, double lse, int64_t row) {
+RWKV7_DEV void put_loss(const DistillArgs &g, const DistillLds &s, const Joined &j, int lane, int64_t row) {
   const int tws = (g.K + kWave - 1) / kWave;
   // sum p (log p - log q), in log q = k (z - m) - log S, without log S
   double A = 0.0;
@@ -193,7 +193,7 @@ __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : 8) void distill_kernel(Dist
   float xt = tail >= 0 ? load_logit<FMT>(src, tail) : -kInf;
   const float tv = there ? load_logit_rt(g.top_val, row * g.K + t, g.val_fmt) : -kInf;
   const float zv = there ? load_logit<FMT>(src, id) : -kInf;
-  const double lse = uniform_d(g.lse ? (double)g.lse[row] * kLog2E : 0.0);
+  const double lse = uniform_d(g.lse ? (double)g.lse[row] : 0.0);
 
   // mark the ids; `first`: this entry stands for its id. (Id and logit wait in LDS
   // for the gradient: nothing is held beside the row.)
@@ -233,14 +233,22 @@ __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : 8) void distill_kernel(Dist
 
   // the entries in 64 bits and powers of two: the student's about their largest,
   // the teacher's about its lse or the wave's largest (a gradient's q - p is what
-  // is left of the two)
+  // is left of the two). Differences come before the factor: a product less a rounded
+  // one, which the compiler joins in one fma, is what the rounding took, 1e22 at the
+  // lowest value of f32, and a row of that alone had p of 2^1e22.
   const double k2 = g.sc.k;
-  double tref = lse, w = 0.0;
+  double tref = 0.0, w = 0.0;
   if (entries) {
     const double zk = k2 * ((double)zv - (double)ExpScale::ref(mtop));  // (NaN stays NaN)
     const double top = wave_sum_d(first ? zk == zk ? exp2_d(zk) : zk : 0.0);
-    if (!g.lse) tref = k2 * (double)wave_max(tv);
-    const double y = k2 * (double)tv - tref;  // (NaN stays NaN)
+    double y;  // (NaN stays NaN)
+    if (g.lse) {
+      y = kLog2E * (g.a * (double)tv - lse);
+    } else {
+      const double most = (double)wave_max(tv);
+      tref = k2 * most;
+      y = k2 * ((double)tv - most);
+    }
     w = there && tv != -kInf ? (y == y ? exp2_d(y) : y) : 0.0;
     const double ta = w != 0.0 ? w * (y - zk) : 0.0;
     const double ws = wave_sum_d(w), as = wave_sum_d(ta);
@@ -254,7 +262,7 @@ __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : 8) void distill_kernel(Dist
   if (wv == 0) {
     const Joined j = join<kWaves>(g, s, lane, lse);
     if (!GRAD) {
-      put_loss(g, s, j, lane, lse, row);
+      put_loss(g, s, j, lane, row);
       return;
     }
     // d loss / d z, scaled: f_rest e for the rest, f_top e - ua p for the entries
@@ -305,7 +313,7 @@ __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : 8) void distill_kernel(Dist
       store_logit<FMT>(dst, s.idx[t], (float)(s.f_top * (zk == zk ? exp2_d(zk) : zk) - s.ua * pk));
     }
   }
-  if (LOSS && wv == 0) put_loss(g, s, s.j, lane, g.lse ? (double)g.lse[row] * kLog2E : 0.0, row);
+  if (LOSS && wv == 0) put_loss(g, s, s.j, lane, row);
 }
 
 template <int FMT, int THREADS>

@@ -44,6 +44,27 @@ def test_a_teacher_row_that_a_mask_leaves_nothing_of(cuda, dtype, V, k):
     assert K.distill_loss(torch.zeros(3, V, device=cuda), val, idx, lse)[1].isnan()
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32], ids=str)
+@pytest.mark.parametrize("T", [1.0, 0.7, 3.0, 1e-20])
+@pytest.mark.parametrize("V,k", [(1, 1), (40, 5), (3001, 130)])
+def test_a_teacher_row_of_the_lowest_value(cuda, dtype, T, V, k):
+    """Without an lse: the softmax of equal entries, however far from 0 they lie."""
+    g = torch.Generator().manual_seed(V)
+    t = torch.full((2, V), torch.finfo(dtype).min)
+    t[1] *= -1.0
+    z = (T * torch.randn(2, V, generator=g)).float()
+    val, idx, _ = K.top_logits(t.to(dtype).to(cuda), k)
+    loss, grad = (x.double().cpu() for x in K.distill_loss_grad(z.to(cuda), val, idx, temperature=T))
+    y = torch.log_softmax(z.double() / T, -1)
+    want = -math.log(k) - y[:, :k].mean(-1)
+    assert bool(((loss - want).abs() <= 112 * U + U * want.abs()).all())
+    ref = y.exp()
+    size = ref.clone()
+    ref[:, :k] -= 1 / k
+    size[:, :k] += 1 / k
+    assert bool(((grad * T - ref).abs() <= (60 + 3 * 20) * U * size + U * ref.abs() + 2.0**-125 * max(T, 1.0)).all())
+
+
 @pytest.mark.parametrize("at", [100.0, -100.0, 200.3, -1000.7, 60000.0])
 def test_a_rounded_log_sum_exp_leaves_no_mass(cuda, at):
     """Teachers whose listed logits are all of their mass, far from 0: what rounding their lse to float32 takes from 1 is
