@@ -491,8 +491,9 @@ int rwkv7_top_logits(const void *logits, int32_t logits_dtype, int64_t ld, int32
  *   row's ids);
  *   lse NULL: p = softmax of the entries, R = 0.
  * An id in several entries has the sum of their p. A row without an entry, or
- * without mass (entries of -inf alone; lse NULL, or -inf), has loss 0 and gradient
- * 0 whatever its logits hold. loss f32 [N] and grad [N, grad_ld] of the logits' type: either may be
+ * without mass (lse NULL and entries of -inf alone; lse of -2^24 or less, as of a row
+ * masked by -inf or by its type's lowest value), has loss 0 and gradient 0 whatever
+ * its logits hold. loss f32 [N] and grad [N, grad_ld] of the logits' type: either may be
  * NULL, not both. grad = scale * d loss / d logits with scale f32 [N] (NULL:
  * scale0); rows with scale 0 have gradient 0, and scale / temperature has to be an
  * f32 number. grad may not overlap logits. */

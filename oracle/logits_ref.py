@@ -32,7 +32,7 @@ def distill_loss(logits: Tensor, top_val: Tensor, top_idx: Tensor, lse: Tensor |
     for r in range(logits.shape[0]):
         live = (top_idx[r] >= 0) & (top_idx[r] < V)
         ids, t = top_idx[r][live], top_val[r][live].double() / temperature
-        if not len(ids) or (lse is None and bool((t == -torch.inf).all())):
+        if not len(ids) or (bool((t == -torch.inf).all()) if lse is None else float(lse[r]) <= -(2.0**24)):
             out.append(logits[r].detach().new_zeros(()))
             continue
         y = torch.log_softmax(logits[r] / temperature, -1)

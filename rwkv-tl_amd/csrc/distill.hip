@@ -13,9 +13,10 @@
 //   loss = sum_k p_k (log p_k - log q_{i_k}) + R (log R - log(1 - Q))
 //   d loss / d z_j = a ((P + R) q_j - sum_{k: i_k = j} p_k)      j in I
 //                  = a q_j (P + R - R / (1 - Q))                  else
-// A row without a present entry or without mass (entries of -inf alone, and no lse or
-// one of -inf: a teacher's row that a mask leaves nothing of) has loss 0 and gradient 0,
-// whatever its logits hold. NaN elsewhere makes its row NaN, as in a log-softmax.
+// A row without a present entry or without mass (no lse and entries of -inf alone, or an
+// lse of kNoTeacher or less: a teacher's row that a mask leaves nothing of) has loss 0
+// and gradient 0, whatever its logits hold. NaN elsewhere makes its row NaN, as in a
+// log-softmax.
 //
 // 1 - Q is never formed as a difference: the row's elements in I are taken out
 // (each thread has a word in LDS that marks them) before the sum, and I enters
@@ -42,6 +43,10 @@ namespace rwkv7 {
 namespace {
 
 constexpr int kDistMaxK = kRowMaxThreads;
+// Half a step of such an lse is a factor e and more of every p. Rows masked by their
+// type's lowest value have one (bf16, f32: -3e38 / temperature, or -inf where that is past
+// f32), and p as it fell, 0, 1 or infinite.
+constexpr double kNoTeacher = -0x1p24;
 constexpr double kLn2 = 0.69314718055994531, kLog2E = 1.4426950408889634;
 
 struct DistillArgs {
@@ -137,7 +142,7 @@ RWKV7_DEV Joined join(const DistillArgs &g, const DistillLds &s, int lane, doubl
   } else {
     j.P = j.W == j.W ? 1.0 : j.W;
   }
-  j.mass = (g.lse && lse != -__builtin_inf()) || j.W != 0.0;  // false: every present entry is -inf
+  j.mass = g.lse ? !(lse <= kNoTeacher) : j.W != 0.0;  // (NaN: the row's loss is NaN)
   return j;
 }
 

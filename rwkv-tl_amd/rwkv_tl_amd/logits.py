@@ -158,8 +158,8 @@ def distill_loss(logits: Tensor, top_val: Tensor, top_idx: Tensor, lse: Tensor |
     ``top_val [..., K]`` (any of the three dtypes) and ``top_idx [..., K]`` int64
     are the teacher's entries, K <= 1024; an id outside ``0..V-1`` (say -1) means
     no entry, so rows may have fewer, and a row without any, or with values of -inf
-    alone (and an ``lse`` of -inf, as ``top_logits`` gives a row that is all masked),
-    has loss 0 and gradient 0 whatever its logits hold (a padded position). With ``lse [...]``
+    alone, or with an ``lse`` of -2^24 or less (as ``top_logits`` gives of a row that is
+    all masked, by -inf or by the lowest value of bfloat16 or float32), has loss 0 and gradient 0 whatever its logits hold (a padded position). With ``lse [...]``
     float32, the teacher's log-sum-exp over its whole vocabulary at the same
     temperature, ``p_k = exp(top_val_k / temperature - lse)`` and the mass that
     this leaves (2^-20 or more, or half a step of ``lse`` where that is more: beyond

@@ -39,9 +39,6 @@ def test_a_teacher_row_that_a_mask_leaves_nothing_of(cuda, dtype, V, k):
     z[1] = float("nan")
     again = K.distill_loss_grad(z.to(cuda), val, idx, lse)
     assert torch.equal(again[0], loss) and torch.equal(again[1], grad)
-    # a finite entry beside an lse of -inf is no distribution
-    val[1, 0] = 0.0
-    assert K.distill_loss(torch.zeros(3, V, device=cuda), val, idx, lse)[1].isnan()
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32], ids=str)
@@ -63,6 +60,24 @@ def test_a_teacher_row_of_the_lowest_value(cuda, dtype, T, V, k):
     ref[:, :k] -= 1 / k
     size[:, :k] += 1 / k
     assert bool(((grad * T - ref).abs() <= (60 + 3 * 20) * U * size + U * ref.abs() + 2.0**-125 * max(T, 1.0)).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32], ids=str)
+@pytest.mark.parametrize("T", [1.0, 0.7, 1.5, 3.0, 50.0])
+def test_a_teacher_row_of_the_lowest_value_with_its_lse(cuda, dtype, T):
+    """float16's (-65504) has a log-sum-exp that tells its distribution; bfloat16's and float32's, whose half step is 1e30,
+    have not, and such a row has no teacher."""
+    g = torch.Generator().manual_seed(5)
+    V, k = 50, 7
+    t = torch.randn(3, V, generator=g)
+    t[1] = torch.finfo(dtype).min
+    val, idx, lse = K.top_logits(t.to(dtype).to(cuda), k, temperature=T)
+    z = torch.randn(3, V, generator=g)
+    loss, grad = K.distill_loss_grad(z.to(cuda), val, idx, lse, temperature=T)
+    want = R.distill_loss(z.double(), val.cpu(), idx.cpu(), lse.cpu(), T)
+    assert bool(((loss.cpu() - want).abs() <= 112 * U + U * want.abs()).all()) and bool(grad.isfinite().all())
+    assert (float(loss[1]) == 0 and bool((grad[1] == 0).all())) == (dtype != torch.float16)
+    assert bool((grad[0] != 0).all()) and bool((grad[2] != 0).all())
 
 
 @pytest.mark.parametrize("at", [100.0, -100.0, 200.3, -1000.7, 60000.0])
