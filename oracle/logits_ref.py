@@ -35,6 +35,9 @@ def distill_loss(logits: Tensor, top_val: Tensor, top_idx: Tensor, lse: Tensor |
         if not len(ids) or (bool((t == -torch.inf).all()) if lse is None else float(lse[r]) <= -(2.0**24)):
             out.append(logits[r].detach().new_zeros(()))
             continue
+        if lse is not None and bool(lse[r].isnan()):
+            out.append(logits[r].sum() * torch.nan)
+            continue
         y = torch.log_softmax(logits[r] / temperature, -1)
         logp = t - (torch.logsumexp(t, -1) if lse is None else lse[r].double())
         p = logp.exp()

@@ -135,6 +135,7 @@ RWKV7_DEV Joined join(const DistillArgs &g, const DistillLds &s, int lane, doubl
     W *= tr > -__builtin_inf() ? exp2_d(tr - j.tref) : 0.0;
   }
   j.W = uniform_d(wave_sum_d(W));
+  if (lse != lse) j.W = lse;  // (also where all entries are -inf)
   j.P = j.W, j.rest_t = 0.0;
   if (g.lse) {
     j.rest_t = uniform_d(1.0 - j.W);

@@ -41,6 +41,19 @@ def test_a_teacher_row_that_a_mask_leaves_nothing_of(cuda, dtype, V, k):
     assert torch.equal(again[0], loss) and torch.equal(again[1], grad)
 
 
+@pytest.mark.parametrize("other", [float("nan"), INF])
+def test_a_teacher_row_of_a_nan_or_an_infinity(cuda, other):
+    """top_logits gives it an lse of NaN; its entries may all be -inf (NaN comes behind them)."""
+    t = torch.full((2, 300), -INF)
+    t[0], t[1, 250] = torch.randn(300, generator=torch.Generator().manual_seed(1)), other
+    val, idx, lse = K.top_logits(t.to(cuda), 4)
+    assert bool(lse[1].isnan())
+    for z in (torch.zeros(2, 300, dtype=torch.float16), torch.randn(2, 300, generator=torch.Generator().manual_seed(2))):
+        loss, grad = K.distill_loss_grad(z.to(cuda), val, idx, lse)
+        assert torch.equal(K.distill_loss(z.to(cuda), val, idx, lse).isnan(), loss.isnan())
+        assert loss.isnan().tolist() == [False, True] and bool(grad[1].isnan().all()) and bool(grad[0].isfinite().all())
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32], ids=str)
 @pytest.mark.parametrize("T", [1.0, 0.7, 3.0, 1e-20])
 @pytest.mark.parametrize("V,k", [(1, 1), (40, 5), (3001, 130)])
