@@ -29,7 +29,7 @@
 extern "C" {
 #endif
 
-#define RWKV7_ABI_VERSION 12
+#define RWKV7_ABI_VERSION 13
 #define RWKV7_HEAD_SIZE 64
 
 enum {
@@ -524,6 +524,66 @@ int rwkv7_verify(const void *target, int64_t target_b, int64_t target_r, const v
                  int64_t draft_r, int32_t logits_dtype, const int64_t *tokens, const float *uniforms,
                  const int64_t *lengths, int32_t B, int32_t K, int32_t V, double temperature, double draft_temperature,
                  int64_t *out, int64_t *accepted, void *workspace, int64_t workspace_bytes, void *stream);
+
+/* ---- the two ends and the norms of a training step ----------------------- */
+/* No counterpart in the reference. dtype: 0 f16, 1 f32, 2 bf16; rows of adjacent
+ * values at a stride in elements, of any alignment. */
+
+/* out[i, :] = scale * weight[tokens[i], :], N rows of C values; an id outside
+ * 0 .. V-1 (a padded position) gives a row of zeros. weight [V, ldw], out [N, C]
+ * of the same type. N < 2^26 - 3, V <= 2^20, C <= 65536. */
+int rwkv7_embed(const void *weight, int32_t dtype, int64_t ldw, const int64_t *tokens, float scale, void *out,
+                int64_t N, int32_t V, int32_t C, void *stream);
+
+/* Its gradient to the table: grad_weight[v, :] = scale * the sum of the rows i of
+ * grad [N, ldg] with tokens[i] = v, zeros where there is none; every row of
+ * grad_weight [V, C] is written. Sums in 32 bits, the same bits every time. The
+ * workspace is needed (its size not 0) for N > 64; it need not be cleared, and serves
+ * one call in flight. Sizes as rwkv7_embed's. */
+int64_t rwkv7_embed_backward_workspace_bytes(int64_t N, int32_t V, int32_t C);
+int rwkv7_embed_backward(const void *grad, int32_t dtype, int64_t ldg, const int64_t *tokens, float scale,
+                         void *grad_weight, int64_t N, int32_t V, int32_t C, void *workspace, int64_t workspace_bytes,
+                         void *stream);
+
+/* LayerNorm of N rows of C <= 16384 values: y = (x - m) r weight + bias of x's type,
+ * m and r = 1 / sqrt(v + eps) the row's mean and biased deviation, which mean and rstd
+ * f32 [N] receive (both NULL: not wanted). weight and bias [C] of x's type or f32
+ * (weight_dtype). 1e-30 <= eps <= 1e30. Statistics in 32 bits or more. The form
+ * of rwkv7_layernorm that training needs. */
+int rwkv7_layer_norm_forward(const void *x, int32_t dtype, int64_t ldx, const void *weight, const void *bias,
+                             int32_t weight_dtype, double eps, void *y, float *mean, float *rstd, int64_t N, int32_t C,
+                             void *stream);
+
+/* Its gradients from grad_y [N, ldg] of x's type, x and the forward's statistics:
+ * grad_x [N, C] of x's type, grad_weight and grad_bias [C] of the weight's, summed over
+ * the rows in an order that the sizes alone decide. The workspace need not be cleared,
+ * and serves one call in flight. */
+int64_t rwkv7_layer_norm_backward_workspace_bytes(int32_t dtype, int64_t N, int32_t C);
+int rwkv7_layer_norm_backward(const void *grad_y, int64_t ldg, const void *x, int64_t ldx, int32_t dtype,
+                              const void *weight, int32_t weight_dtype, const float *mean, const float *rstd,
+                              void *grad_x, void *grad_weight, void *grad_bias, int64_t N, int32_t C, void *workspace,
+                              int64_t workspace_bytes, void *stream);
+
+/* Of each row of logits [N, V] (types, strides and limits as rwkv7_top_logits), with
+ * q = softmax(logits / temperature): logp f32 [N] = log q of the row's token, tokens
+ * i64 [N], and entropy f32 [N] = -sum q log q; and for k > 0 (k <= min(V, 256)) the k
+ * most likely alternatives, ordered as rwkv7_top_logits', as top_logp f32 [N, k] =
+ * log q and top_idx i64 [N, k]. A token outside 0 .. V-1 makes its row a padded
+ * one: logp and entropy 0, top_logp -inf and top_idx -1, whatever its logits hold. A row of
+ * -inf alone: logp (and top_logp) -inf, entropy 0; one with a NaN or +inf: NaN. */
+int rwkv7_token_logprobs(const void *logits, int32_t logits_dtype, int64_t ld, int32_t N, int32_t V,
+                         const int64_t *tokens, double temperature, int32_t k, float *logp, float *entropy,
+                         float *top_logp, int64_t *top_idx, void *stream);
+
+/* grad [N, V] of the logits' type = scale * d logp / d logits + entropy_scale *
+ * d entropy / d logits, and logp and entropy in the same pass (each may be NULL).
+ * scale and entropy_scale f32 [N] (NULL: scale0, entropy_scale0 for every row),
+ * each / temperature within f32. Padded rows, rows of -inf alone and rows where both
+ * scales are 0 have gradient 0. grad may not overlap logits. */
+int rwkv7_token_logprobs_grad(const void *logits, int32_t logits_dtype, int64_t ld, int32_t N, int32_t V,
+                              const int64_t *tokens, double temperature, const float *scale, float scale0,
+                              const float *entropy_scale, float entropy_scale0, float *logp, float *entropy, void *grad,
+                              void *stream);
 
 #ifdef __cplusplus
 }

@@ -273,6 +273,10 @@ int launch_l2norm(const uint16_t *kk, const uint16_t *a, uint16_t *kn, uint16_t 
 int launch_gn_rkrk(const uint16_t *y, const uint16_t *r, const uint16_t *k, const uint16_t *v, const uint16_t *r_k,
                    const uint16_t *lw, const uint16_t *lb, uint16_t *out, int H, int bf, hipStream_t st);
 
+// rwkv7_token_logprobs with alternatives (top_logits.hip).
+int launch_top_scores(const void *logits, int dtype, int64_t ld, int N, int V, const int64_t *tokens, double temperature, int k,
+                      float *logp, float *entropy, float *top_logp, int64_t *top_idx, hipStream_t st);
+
 // One-token, one-sequence decode as a single persistent kernel (decode_mk.hip).
 int mk_cus();
 bool mk_supported(const rwkv7_dims &d, int G);

@@ -1,0 +1,216 @@
+// Log probabilities of given tokens, the rows' entropies, and the gradient of both,
+// one workgroup per row (with alternatives: top_logits.hip).
+//
+//   q_j = exp(a z_j - L), L = log sum exp(a z), a = 1 / temperature
+//   l = a z_x - L,  H = -sum q log q
+//   d (s l + h H) / d z_j = a (s (1 where j = x) - q_j (s + h (log q_j + H)))
+// x outside 0 .. V-1: a padded row, l = H = 0 and gradient 0 whatever its logits hold. A
+// row of -inf alone: l = -inf, H = 0, gradient 0. NaN or +inf elsewhere: NaN, as in a
+// log-softmax.
+//
+// The row stays in registers: the largest, then the sums about it (logits_score.h), then
+// the gradient, with one read and one write of memory. The token's own gradient is
+// formed in 64 bits (1 - q of a likely token is what is left of a difference) and
+// stored over the row's after a barrier.
+#include "logits_score.h"
+#include "rwkv7_kernels.h"
+
+namespace rwkv7 {
+namespace {
+
+struct TokenArgs {
+  const void *logits;
+  int64_t ld;
+  int V;
+  ExpScale sc;
+  double a;
+  const int64_t *tokens;
+  float *logp, *entropy;  // null: not wanted
+  // gradient only: the rows' upstream gradients, null: the same for all
+  const float *scale, *entropy_scale;
+  float scale0, entropy_scale0;
+  void *grad;
+  int64_t row0;
+};
+
+template <int FMT, int THREADS>
+RWKV7_DEV void zero_grad(char *dst, int V) {
+  const float zero[kRowChunk] = {};
+#pragma unroll 1
+  for (uint32_t b = threadIdx.x; b < (uint32_t)V / kRowChunk; b += THREADS) store_chunk<FMT>(dst, b, zero);
+  if (threadIdx.x < V % kRowChunk) store_logit<FMT>(dst, V / kRowChunk * kRowChunk + threadIdx.x, 0.f);
+}
+
+struct TokenLds {
+  ScoreLds s;
+  float base, slope;  // the gradient is 2^y (base + slope y), with log q = ln 2 y - log total
+};
+
+template <int FMT, int THREADS, bool GRAD>
+__global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : 8) void token_kernel(TokenArgs g) {
+  __shared__ TokenLds s;
+  constexpr int kWaves = THREADS / kWave;
+  const int t = threadIdx.x, lane = t & 63, wv = t >> 6, V = g.V;
+  const uint32_t n8 = (uint32_t)V / kRowChunk;
+  const int64_t row = g.row0 + blockIdx.x;
+  const char *src = static_cast<const char *>(g.logits) + row * g.ld * kLogitBytes<FMT>;
+  char *dst = GRAD ? static_cast<char *>(g.grad) + row * (int64_t)V * kLogitBytes<FMT> : nullptr;
+  const int64_t id = g.tokens[row];
+  float up = 0.f, up_h = 0.f;
+  if (GRAD) {
+    up = g.scale ? g.scale[row] : g.scale0;
+    up_h = g.entropy_scale ? g.entropy_scale[row] : g.entropy_scale0;
+  }
+  if (id < 0 || id >= V) {  // (block-uniform)
+    if (t == 0 && g.logp) g.logp[row] = 0.f;
+    if (t == 0 && g.entropy) g.entropy[row] = 0.f;
+    if (GRAD) zero_grad<FMT, THREADS>(dst, V);
+    return;
+  }
+  if (GRAD && !g.logp && !g.entropy && up == 0.f && up_h == 0.f) {
+    zero_grad<FMT, THREADS>(dst, V);
+    return;
+  }
+
+  Chunk<FMT> x[kRowChunks];
+  load_row<THREADS>(x, src, n8);
+  const int tail = t < V % kRowChunk ? (int)n8 * kRowChunk + t : -1;  // this thread's logit behind the eights
+  const float xt = tail >= 0 ? load_logit<FMT>(src, tail) : -kInf;
+  const float zx = load_logit<FMT>(src, id);
+
+  RowMax<FMT> most;
+#pragma unroll
+  for (int c = 0; c < kRowChunks; ++c) {
+    if (!GRAD && c > 0 && c * THREADS >= (int)n8) break;
+    most.add(x[c]);
+  }
+  const float own = wave_max(fmaxf(most.value(), xt));
+  opaque_row(x);
+  if (lane == 0) s.s.m[wv] = own;
+  __syncthreads();
+  const float M = uniform_f(wave_max(lane < kWaves ? s.s.m[lane] : -kInf));
+
+  float S, T;
+  int n;
+  score_row<THREADS, !GRAD>(x, n8, xt, g.sc, M, own, S, T, n);
+  if (lane == 0) s.s.S[wv] = S, s.s.T[wv] = T, s.s.n[wv] = n;
+  if (GRAD) opaque_row(x);
+  __syncthreads();
+
+  double grad_x = 0.0;
+  bool zero = false;
+  if (wv == 0) {
+    const RowScore r = row_score(join_sums<kWaves>(s.s, g.sc, M, lane));
+    const double lp = log_prob(r, g.a, zx, M);
+    if (lane == 0 && g.logp) g.logp[row] = (float)lp;
+    if (lane == 0 && g.entropy) g.entropy[row] = (float)r.H;
+    if (GRAD) {
+      zero = r.none || (up == 0.f && up_h == 0.f);
+      const double f = g.a * rcp_d(r.total);
+      const double q = lp > -__builtin_inf() ? exp2_d(1.4426950408889634 * lp) : lp == lp ? 0.0 : lp;
+      grad_x = g.a * ((double)up * one_minus_exp(lp) - (q != 0.0 ? q * (double)up_h * (lp + r.H) : 0.0));
+      if (lane == 0) {
+        s.base = zero ? 0.f : (float)(-f * ((double)up + (double)up_h * (r.H - r.log_total)));
+        s.slope = zero ? 0.f : (float)(-f * kLn2 * (double)up_h);
+      }
+    }
+  }
+  if (!GRAD) return;
+  __syncthreads();
+  const float base = uniform_f(s.base), slope = uniform_f(s.slope);
+  if (base == 0.f && slope == 0.f) {  // a row that counts for nothing: zeros, not 0 * NaN
+    zero_grad<FMT, THREADS>(dst, V);
+  } else {
+    const float ref = ExpScale::ref(M);
+    auto put = [&](auto far, auto flat) {
+      constexpr bool kFar = decltype(far)::value, kFlat = decltype(flat)::value;
+      const float R = ref * g.sc.kf;
+      auto one = [&](float v) {
+        const float y = score_arg<kFar>(g.sc, v, ref, R), e = __builtin_amdgcn_exp2f(y);
+        return kFlat ? e * base : e * fmaf(slope, fmaxf(y, -1000.f), base);
+      };
+#pragma unroll
+      for (int c = 0; c < kRowChunks; ++c) {
+        if (c > 0 && c * THREADS >= (int)n8) break;
+        float f[kRowChunk];
+        if (!kFlat) x[c].opaque();
+        x[c].template get<kFar>(f);
+#pragma unroll
+        for (int e = 0; e < kRowChunk; ++e) f[e] = one(f[e]);
+        const uint32_t b = c * THREADS + t;
+        if ((c + 1) * THREADS <= (int)n8) store_chunk<FMT>(dst, b, f);
+        else if (b < n8) store_chunk<FMT>(dst, b, f);
+      }
+      if (tail >= 0) store_logit<FMT>(dst, tail, one(xt));
+    };
+    if (g.sc.near(M)) {
+      if (slope == 0.f) put(BoolConst<false>(), BoolConst<true>());
+      else put(BoolConst<false>(), BoolConst<false>());
+    } else {
+      if (slope == 0.f) put(BoolConst<true>(), BoolConst<true>());
+      else put(BoolConst<true>(), BoolConst<false>());
+    }
+  }
+  __syncthreads();  // the row's own stores come before the token's
+  if (t == 0 && !zero) store_logit<FMT>(dst, id, (float)grad_x);
+}
+
+template <int FMT, int THREADS>
+void launch_t(const TokenArgs &g, int N, hipStream_t st) {
+  if (g.grad) token_kernel<FMT, THREADS, true><<<N, THREADS, 0, st>>>(g);
+  else token_kernel<FMT, THREADS, false><<<N, THREADS, 0, st>>>(g);
+}
+
+template <int FMT>
+void launch_f(const TokenArgs &g, int N, hipStream_t st) {
+  switch (row_threads(g.V)) {
+    case 256: launch_t<FMT, 256>(g, N, st); break;
+    case 512: launch_t<FMT, 512>(g, N, st); break;
+    default: launch_t<FMT, 1024>(g, N, st); break;
+  }
+}
+
+int launch_rows(TokenArgs g, int dtype, int N, hipStream_t st) {
+  for (; g.row0 < N; g.row0 += kLaunchRows) {
+    const int n = N - g.row0 < kLaunchRows ? (int)(N - g.row0) : kLaunchRows;
+    switch (dtype) {
+      case 0: launch_f<0>(g, n, st); break;
+      case 1: launch_f<1>(g, n, st); break;
+      default: launch_f<2>(g, n, st); break;
+    }
+    RWKV7_CHECK_LAUNCH();
+  }
+  return RWKV7_OK;
+}
+
+}  // namespace
+}  // namespace rwkv7
+
+extern "C" int rwkv7_token_logprobs(const void *logits, int32_t logits_dtype, int64_t ld, int32_t N, int32_t V,
+                                    const int64_t *tokens, double temperature, int32_t k, float *logp, float *entropy,
+                                    float *top_logp, int64_t *top_idx, void *stream) {
+  using namespace rwkv7;
+  if (!logits || !tokens || !logp || !entropy || logits_dtype < 0 || logits_dtype > 2) return RWKV7_EINVAL;
+  if (!(temperature >= 1e-30 && temperature <= 1e30)) return RWKV7_EINVAL;
+  if (N < 1 || V < 1 || V > kRowMaxV || ld < V || k < 0) return RWKV7_ESHAPE;
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (k > 0) {
+    if (!top_logp || !top_idx) return RWKV7_EINVAL;
+    return launch_top_scores(logits, logits_dtype, ld, N, V, tokens, temperature, k, logp, entropy, top_logp, top_idx, st);
+  }
+  const double a = 1.0 / temperature;
+  return launch_rows({logits, ld, V, ExpScale::of(a), a, tokens, logp, entropy}, logits_dtype, N, st);
+}
+
+extern "C" int rwkv7_token_logprobs_grad(const void *logits, int32_t logits_dtype, int64_t ld, int32_t N, int32_t V,
+                                         const int64_t *tokens, double temperature, const float *scale, float scale0,
+                                         const float *entropy_scale, float entropy_scale0, float *logp, float *entropy,
+                                         void *grad, void *stream) {
+  using namespace rwkv7;
+  if (!logits || !tokens || !grad || logits_dtype < 0 || logits_dtype > 2) return RWKV7_EINVAL;
+  if (!(temperature >= 1e-30 && temperature <= 1e30)) return RWKV7_EINVAL;
+  if (N < 1 || V < 1 || V > kRowMaxV || ld < V) return RWKV7_ESHAPE;
+  const double a = 1.0 / temperature;
+  return launch_rows({logits, ld, V, ExpScale::of(a), a, tokens, logp, entropy, scale, entropy_scale, scale0, entropy_scale0, grad},
+                     logits_dtype, N, static_cast<hipStream_t>(stream));
+}

@@ -1,6 +1,8 @@
 // The k largest logits of each row, in order, with their ids, and the row's
-// log-sum-exp: what a teacher hands on of its answers. One workgroup per row;
-// the row stays in registers.
+// log-sum-exp: what a teacher hands on of its answers. Or (SCORE) the log probabilities
+// of these and of a given token, and the row's entropy, by the sums of logits_score.h
+// and for the rows that token_logprobs.hip describes; the alternatives of a padded row
+// are -1 and -inf. One workgroup per row; the row stays in registers.
 //
 // Order: descending value (-0 is 0), ties by the lowest id, NaN behind
 // everything. lse = log sum_j exp(a z_j), a = 1 / temperature, NaN if a logit
@@ -24,7 +26,7 @@
 // round of two rows a CU, each a chain of load, floor, sum, gather and ranking. One row
 // 9.1; 257 x 20011 f32 12.5 (back to back in a graph 9.9); 2000 x 65536 f32, k 64, back
 // to back 125, 4.2 TB/s.
-#include "logits_rows.h"
+#include "logits_score.h"
 #include "rwkv7_kernels.h"
 
 namespace rwkv7 {
@@ -42,6 +44,10 @@ struct TopArgs {
   int64_t *idx;
   float *lse;
   int64_t row0;
+  // SCORE (val are floats then)
+  double a;
+  const int64_t *tokens;
+  float *logp, *entropy;
 };
 
 constexpr int kBins = 256;
@@ -145,14 +151,30 @@ RWKV7_DEV int select_digit(const char *src, int V, int &need, TopLds &s, D digit
   return s.digit;
 }
 
-template <int FMT, int THREADS>
+struct NoLds {};
+struct TopScoreLds : ScoreLds {
+  double log_S;
+};
+
+template <int FMT, int THREADS, bool SCORE>
 __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : THREADS == 256 ? 7 : 8) void top_kernel(TopArgs g) {
   __shared__ TopLds s;
+  __shared__ std::conditional_t<SCORE, TopScoreLds, NoLds> sco;
   constexpr int kWaves = THREADS / kWave;
   const int t = threadIdx.x, lane = t & 63, wv = t >> 6, V = g.V, k = g.k;
   const uint32_t n8 = (uint32_t)V / kRowChunk;
   const int64_t row = g.row0 + blockIdx.x;
   const char *src = static_cast<const char *>(g.logits) + row * g.ld * kLogitBytes<FMT>;
+  float zx = 0.f;
+  if constexpr (SCORE) {
+    const int64_t id = g.tokens[row];
+    if (id < 0 || id >= V) {  // (block-uniform; k <= THREADS)
+      if (t == 0) g.logp[row] = 0.f, g.entropy[row] = 0.f;
+      if (t < k) static_cast<float *>(g.val)[row * k + t] = -kInf, g.idx[row * k + t] = -1;
+      return;
+    }
+    zx = load_logit<FMT>(src, id);
+  }
   Chunk<FMT> x[kRowChunks];
   load_row<THREADS>(x, src, n8);
   const int tail = t < V % kRowChunk ? (int)n8 * kRowChunk + t : -1;
@@ -188,9 +210,27 @@ __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : THREADS == 256 ? 7 : 8) voi
     if (lane == 0) s.floor[wv] = fl, s.some[wv] = some;
   }
   m = wave_max(m);
-  const float sum = sum_row<THREADS, true, true>(x, src, n8, xt, g.sc, m, [](int, Chunk<FMT> &) {});
-  if (lane == 0) s.m[wv] = m, s.sum[wv] = sum;
+  if constexpr (SCORE) {
+    if (lane == 0) s.m[wv] = m;
+    __syncthreads();
+    const float M = uniform_f(wave_max(lane < kWaves ? s.m[lane] : -kInf));
+    float S, T;
+    int n;
+    score_row<THREADS, true>(x, n8, xt, g.sc, M, m, S, T, n);
+    opaque_row(x);
+    if (lane == 0) sco.S[wv] = S, sco.T[wv] = T, sco.n[wv] = n;
+  } else {
+    const float sum = sum_row<THREADS, true, true>(x, src, n8, xt, g.sc, m, [](int, Chunk<FMT> &) {});
+    if (lane == 0) s.m[wv] = m, s.sum[wv] = sum;
+  }
   __syncthreads();
+  if constexpr (SCORE) {
+    if (wv == kWaves - 1) {  // (the alternatives read log_S barriers later)
+      const float M = uniform_f(wave_max(lane < kWaves ? s.m[lane] : -kInf));
+      const RowScore r = row_score(join_sums<kWaves>(sco, g.sc, M, lane));
+      if (lane == 0) sco.log_S = r.log_S, g.logp[row] = (float)log_prob(r, g.a, zx, M), g.entropy[row] = (float)r.H;
+    }
+  }
 
   // the least floor, and the waves with 64 maxima or more, one a lane
   auto least_floor = [&]() {
@@ -296,11 +336,14 @@ __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : THREADS == 256 ? 7 : 8) voi
     if (rank < k) {
       const int id = (int)~(uint32_t)own;
       g.idx[row * k + rank] = id;
-      if constexpr (FMT == 1) static_cast<float *>(g.val)[row * k + rank] = reinterpret_cast<const float *>(src)[id];
+      if constexpr (SCORE) {
+        const double z = (double)load_logit<FMT>(src, id) - (double)ExpScale::ref(mm);
+        static_cast<float *>(g.val)[row * k + rank] = (float)(g.a * z - sco.log_S);
+      } else if constexpr (FMT == 1) static_cast<float *>(g.val)[row * k + rank] = reinterpret_cast<const float *>(src)[id];
       else static_cast<uint16_t *>(g.val)[row * k + rank] = reinterpret_cast<const uint16_t *>(src)[id];
     }
   }
-  if (wv == 0) {
+  if (!SCORE && wv == 0) {
     const float mw = lane < kWaves ? s.m[lane] : -kInf;
     const double S = wave_sum_d(lane < kWaves ? (double)s.sum[lane] * g.sc.part(mw, mm) : 0.0);
     // (S is 0 where there is nothing but -inf)
@@ -308,16 +351,38 @@ __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : THREADS == 256 ? 7 : 8) voi
   }
 }
 
-template <int FMT>
-void launch_top(const TopArgs &g, int N, hipStream_t st) {
+template <int FMT, bool SCORE>
+void launch_f(const TopArgs &g, int N, hipStream_t st) {
   switch (row_threads(g.V)) {
-    case 256: top_kernel<FMT, 256><<<N, 256, 0, st>>>(g); break;
-    case 512: top_kernel<FMT, 512><<<N, 512, 0, st>>>(g); break;
-    default: top_kernel<FMT, 1024><<<N, 1024, 0, st>>>(g); break;
+    case 256: top_kernel<FMT, 256, SCORE><<<N, 256, 0, st>>>(g); break;
+    case 512: top_kernel<FMT, 512, SCORE><<<N, 512, 0, st>>>(g); break;
+    default: top_kernel<FMT, 1024, SCORE><<<N, 1024, 0, st>>>(g); break;
   }
 }
 
+template <bool SCORE>
+int launch_top(TopArgs g, int dtype, int N, hipStream_t st) {
+  for (; g.row0 < N; g.row0 += kLaunchRows) {
+    const int n = N - g.row0 < kLaunchRows ? (int)(N - g.row0) : kLaunchRows;
+    switch (dtype) {
+      case 0: launch_f<0, SCORE>(g, n, st); break;
+      case 1: launch_f<1, SCORE>(g, n, st); break;
+      default: launch_f<2, SCORE>(g, n, st); break;
+    }
+    RWKV7_CHECK_LAUNCH();
+  }
+  return RWKV7_OK;
+}
+
 }  // namespace
+
+int launch_top_scores(const void *logits, int dtype, int64_t ld, int N, int V, const int64_t *tokens, double temperature, int k,
+                      float *logp, float *entropy, float *top_logp, int64_t *top_idx, hipStream_t st) {
+  if (k > V || k > kTopMax) return RWKV7_ESHAPE;
+  const double a = 1.0 / temperature;
+  return launch_top<true>({logits, ld, V, k, ExpScale::of(a), top_logp, top_idx, nullptr, 0, a, tokens, logp, entropy}, dtype, N, st);
+}
+
 }  // namespace rwkv7
 
 extern "C" int rwkv7_top_logits(const void *logits, int32_t logits_dtype, int64_t ld, int32_t N, int32_t V, int32_t k,
@@ -326,16 +391,6 @@ extern "C" int rwkv7_top_logits(const void *logits, int32_t logits_dtype, int64_
   if (!logits || !val || !idx || !lse || logits_dtype < 0 || logits_dtype > 2) return RWKV7_EINVAL;
   if (!(temperature >= 1e-30 && temperature <= 1e30)) return RWKV7_EINVAL;
   if (N < 1 || V < 1 || V > kRowMaxV || ld < V || k < 1 || k > V || k > kTopMax) return RWKV7_ESHAPE;
-  TopArgs g = {logits, ld, V, k, ExpScale::of(1.0 / temperature), val, idx, lse, 0};
-  const hipStream_t st = static_cast<hipStream_t>(stream);
-  for (; g.row0 < N; g.row0 += kLaunchRows) {
-    const int n = N - g.row0 < kLaunchRows ? (int)(N - g.row0) : kLaunchRows;
-    switch (logits_dtype) {
-      case 0: launch_top<0>(g, n, st); break;
-      case 1: launch_top<1>(g, n, st); break;
-      default: launch_top<2>(g, n, st); break;
-    }
-    RWKV7_CHECK_LAUNCH();
-  }
-  return RWKV7_OK;
+  return launch_top<false>({logits, ld, V, k, ExpScale::of(1.0 / temperature), val, idx, lse}, logits_dtype, N,
+                           static_cast<hipStream_t>(stream));
 }

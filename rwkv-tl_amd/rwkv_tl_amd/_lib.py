@@ -16,7 +16,7 @@ from pathlib import Path
 import torch  # noqa: F401  (must be imported before the HIP library)
 
 LIB_NAME = "librwkv7_hip.so"
-ABI_VERSION = 12
+ABI_VERSION = 13
 
 # rwkv7_model.flags
 MODEL_MULTI_LAUNCH_DECODE = 1
@@ -73,6 +73,14 @@ SYMBOLS = (
     "rwkv7_distill",
     "rwkv7_verify_workspace_bytes",
     "rwkv7_verify",
+    "rwkv7_embed",
+    "rwkv7_embed_backward_workspace_bytes",
+    "rwkv7_embed_backward",
+    "rwkv7_layer_norm_forward",
+    "rwkv7_layer_norm_backward_workspace_bytes",
+    "rwkv7_layer_norm_backward",
+    "rwkv7_token_logprobs",
+    "rwkv7_token_logprobs_grad",
 )
 
 
@@ -165,7 +173,7 @@ _LIB: ctypes.CDLL | None = None
 
 
 def _declare(lib: ctypes.CDLL) -> None:
-    vp, i32, i64, f64 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_double
+    vp, i32, i64, f32, f64 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_double
     sig = {
         "rwkv7_abi_version": (ctypes.c_int, []),
         "rwkv7_strerror": (ctypes.c_char_p, [ctypes.c_int]),
@@ -209,6 +217,14 @@ def _declare(lib: ctypes.CDLL) -> None:
         "rwkv7_verify_workspace_bytes": (i64, [i32, i32, i32]),
         "rwkv7_verify": (ctypes.c_int, [vp, i64, i64, vp, i64, i64, i32, vp, vp, vp, i32, i32, i32, f64, f64, vp, vp, vp,
                                         i64, vp]),
+        "rwkv7_embed": (ctypes.c_int, [vp, i32, i64, vp, f32, vp, i64, i32, i32, vp]),
+        "rwkv7_embed_backward_workspace_bytes": (i64, [i64, i32, i32]),
+        "rwkv7_embed_backward": (ctypes.c_int, [vp, i32, i64, vp, f32, vp, i64, i32, i32, vp, i64, vp]),
+        "rwkv7_layer_norm_forward": (ctypes.c_int, [vp, i32, i64, vp, vp, i32, f64, vp, vp, vp, i64, i32, vp]),
+        "rwkv7_layer_norm_backward_workspace_bytes": (i64, [i32, i64, i32]),
+        "rwkv7_layer_norm_backward": (ctypes.c_int, [vp, i64, vp, i64, i32, vp, i32, vp, vp, vp, vp, vp, i64, i32, vp, i64, vp]),
+        "rwkv7_token_logprobs": (ctypes.c_int, [vp, i32, i64, i32, i32, vp, f64, i32, vp, vp, vp, vp, vp]),
+        "rwkv7_token_logprobs_grad": (ctypes.c_int, [vp, i32, i64, i32, i32, vp, f64, vp, f32, vp, f32, vp, vp, vp, vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)

@@ -26,6 +26,10 @@ example ``dplr.py:258-267``) are not reproduced.
   (``dplr.py:237-254``).
 * Between a large model and a small one (``logits.py``): ``top_logits``,
   ``distill_loss``, ``distill_loss_grad``, ``distill_loss_backward``.
+* Training, around ``dplr_seq_forward`` / ``dplr_seq_backward``: ``embed`` /
+  ``embed_backward`` and ``layer_norm_forward`` / ``layer_norm_backward``
+  (``training.py``), ``token_logprobs``, ``token_logprobs_grad`` and
+  ``token_logprobs_backward`` (``logits.py``).
 """
 
 from __future__ import annotations
@@ -36,7 +40,16 @@ import torch
 from torch import Tensor
 
 from . import _lib
-from .logits import distill_loss, distill_loss_backward, distill_loss_grad, top_logits  # noqa: F401
+from .logits import (  # noqa: F401
+    distill_loss,
+    distill_loss_backward,
+    distill_loss_grad,
+    token_logprobs,
+    token_logprobs_backward,
+    token_logprobs_grad,
+    top_logits,
+)
+from .training import embed, embed_backward, layer_norm_backward, layer_norm_forward  # noqa: F401
 
 N = 64
 

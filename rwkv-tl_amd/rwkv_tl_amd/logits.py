@@ -1,11 +1,14 @@
-"""Operators between a large model and a small one of the same vocabulary, on
-rows of logits (no counterpart in the reference).
+"""Operators on rows of logits: between a large model and a small one of the same
+vocabulary, and the output end of a training step (no counterpart in the reference).
 
 * ``top_logits``: what a teacher hands on of each row: its largest logits, their
   token ids, and the row's log-sum-exp.
 * ``distill_loss`` / ``distill_loss_grad``: the divergence of a student's
   distribution from a teacher's top logits, alone or with its gradient in the
   same pass. ``torch.ops.rwkv_tl.distill_loss`` is the differentiable form.
+* ``token_logprobs`` / ``token_logprobs_grad``: the log probability of a given token of
+  each row, the row's entropy, its most likely alternatives, or the gradient in the same
+  pass. ``torch.ops.rwkv_tl.token_logprobs`` is the differentiable form.
 * ``verify_draft``: drafted tokens against the target model's probabilities,
   from given random numbers (speculative sampling).
 
@@ -185,6 +188,97 @@ def distill_loss_backward(grad_loss: Tensor, logits: Tensor, top_val: Tensor, to
                           temperature: float) -> Tensor:
     """Gradient of ``distill_loss`` to ``logits`` under ``grad_loss`` float32 ``[...]``."""
     return _distill(logits, top_val, top_idx, lse, temperature, grad_loss, False, True)[1]
+
+
+def _check_rows(logits: Tensor, tokens: Tensor, temperature: float) -> tuple[int, float]:
+    """The logits' dtype code and the temperature."""
+    code = _check_logits(logits, "logits")
+    if not isinstance(tokens, Tensor) or tokens.dtype is not torch.int64 or tokens.shape != logits.shape[:-1]:
+        raise ValueError(f"tokens must be int64 {tuple(logits.shape[:-1])}")
+    _same_device(logits, tokens)
+    return code, _temperature(temperature)
+
+
+def token_logprobs(logits: Tensor, tokens: Tensor, k: int = 0, *, temperature: float = 1.0) -> tuple[Tensor, ...]:
+    """Log probabilities of given tokens, with entropy and alternatives: of each row of
+    ``logits [..., V]``, with ``q = softmax(logits / temperature)``, ``log q`` of the row's
+    token (``tokens [...]`` int64) and the entropy ``-sum q log q``.
+
+    Returns ``(logprob [...], entropy [...])`` float32, and for ``k`` from 1 to
+    min(V, 256) also ``(top_logprob [..., k]`` float32, ``top_index [..., k]`` int64``)``:
+    the k most likely tokens in descending order, ties by the lowest id.
+
+    An id outside ``0..V-1`` (say -1) makes its row a padded one: logprob and entropy 0,
+    alternatives -inf and -1, whatever its logits hold. A row of -inf alone has logprobs
+    -inf and entropy 0; a NaN or +inf makes its row NaN. Without autograd;
+    ``torch.ops.rwkv_tl.token_logprobs`` is the differentiable form."""
+    code, temperature = _check_rows(logits, tokens, temperature)
+    V = logits.shape[-1]
+    if not isinstance(k, int) or not 0 <= k <= min(V, MAX_TOP):
+        raise ValueError(f"k must be in 0..{min(V, MAX_TOP)}, got {k}")
+    lead = logits.shape[:-1]
+    with _lib.device_of(logits):
+        x, N, ld = _rows(logits)
+        dev = x.device
+        logp, entropy = _empty(lead, torch.float32, dev), _empty(lead, torch.float32, dev)
+        top = idx = None
+        if k:
+            top = torch.empty(*lead, k, dtype=torch.float32, device=dev)
+            idx = torch.empty(*lead, k, dtype=torch.int64, device=dev)
+        if N:
+            t = tokens.contiguous()
+            rc = _lib.load().rwkv7_token_logprobs(
+                x.data_ptr(), code, ld, N, V, t.data_ptr(), temperature, k, logp.data_ptr(), entropy.data_ptr(), _lib.ptr(top),
+                _lib.ptr(idx), _lib.stream_of(x),
+            )
+            _lib.check(rc, "rwkv7_token_logprobs")
+    return (logp, entropy, top, idx) if k else (logp, entropy)
+
+
+def _token_grad(logits, tokens, temperature, scale, entropy_scale, want: bool):
+    code, temperature = _check_rows(logits, tokens, temperature)
+    shape = logits.shape
+    lead, V = shape[:-1], shape[-1]
+    rows = [s if isinstance(s, Tensor) else None for s in (scale, entropy_scale)]
+    for s, name in zip(rows, ("scale", "entropy_scale")):
+        if s is not None and (s.shape != lead or s.dtype is not torch.float32):
+            raise ValueError(f"{name} must be float32 {tuple(lead)}")
+    _same_device(logits, *rows)
+    one = [1.0 if r is not None else float(s) for r, s in zip(rows, (scale, entropy_scale))]
+    with _lib.device_of(logits):
+        dev = logits.device
+        logp, entropy = (_empty(lead, torch.float32, dev), _empty(lead, torch.float32, dev)) if want else (None, None)
+        grad = torch.empty(*shape, dtype=logits.dtype, device=dev)
+        x, N, ld = _rows(logits)
+        if N:
+            t = tokens.contiguous()
+            s, h = (None if r is None else r.contiguous() for r in rows)
+            rc = _lib.load().rwkv7_token_logprobs_grad(
+                x.data_ptr(), code, ld, N, V, t.data_ptr(), temperature, _lib.ptr(s), one[0], _lib.ptr(h), one[1],
+                _lib.ptr(logp), _lib.ptr(entropy), grad.data_ptr(), _lib.stream_of(x),
+            )
+            _lib.check(rc, "rwkv7_token_logprobs_grad")
+    return logp, entropy, grad
+
+
+def token_logprobs_grad(logits: Tensor, tokens: Tensor, *, temperature: float = 1.0, scale: Tensor | float = 1.0,
+                        entropy_scale: Tensor | float = 0.0) -> tuple[Tensor, Tensor, Tensor]:
+    """``token_logprobs`` and ``scale`` times the gradient of the log probability plus
+    ``entropy_scale`` times that of the entropy, to ``logits``, in one pass over them:
+    ``(logprob [...], entropy [...]`` float32, ``grad [..., V]`` of the logits' dtype``)``.
+    The scales: numbers, or float32 ``[...]`` (each row's weight in the loss, -1 / rows
+    for a mean cross entropy, and a loss scale), each / temperature within float32.
+    Padded rows, rows of -inf alone and rows with both scales 0 have gradient 0. For
+    ``logits.backward(grad)``."""
+    return _token_grad(logits, tokens, temperature, scale, entropy_scale, True)
+
+
+def token_logprobs_backward(grad_logprob: Tensor | None, grad_entropy: Tensor | None, logits: Tensor, tokens: Tensor,
+                            temperature: float) -> Tensor:
+    """Gradient of ``token_logprobs`` to ``logits`` under ``grad_logprob`` and
+    ``grad_entropy`` float32 ``[...]`` (None: zeros)."""
+    zero = lambda g: 0.0 if g is None else g  # noqa: E731
+    return _token_grad(logits, tokens, temperature, zero(grad_logprob), zero(grad_entropy), False)[2]
 
 
 def _strides(x: Tensor, V: int) -> Tensor:

@@ -30,6 +30,7 @@ import torch
 from torch import Tensor
 
 from . import kernels as K
+from . import training as T
 
 NAMESPACE = "rwkv_tl"
 
@@ -156,6 +157,58 @@ LOGITS_OPS: dict[str, tuple[str, Callable, Callable]] = {
 }
 
 
+# The two ends and the norms of a training step (no counterpart in the reference).
+# ``embed`` is differentiable to its table, ``layer_norm`` to its three tensors,
+# ``token_logprobs`` to the logits; each once.
+def _norm_meta(x, *_):
+    stat = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    return x.new_empty(x.shape), stat, torch.empty_like(stat)
+
+
+def _rows_meta(logits, *_):
+    row = logits.new_empty(logits.shape[:-1], dtype=torch.float32)
+    return row, torch.empty_like(row)
+
+
+STEP_OPS: dict[str, tuple[str, Callable, Callable]] = {
+    "embed": (
+        "(Tensor weight, Tensor tokens, float scale=1.0) -> Tensor",
+        lambda weight, tokens, scale=1.0: K.embed(weight, tokens, scale=scale),
+        lambda weight, tokens, *_: weight.new_empty(*tokens.shape, weight.shape[1]),
+    ),
+    "embed_backward": (
+        "(Tensor grad, Tensor tokens, int vocab, float scale=1.0) -> Tensor",
+        lambda grad, tokens, vocab, scale=1.0: K.embed_backward(grad, tokens, vocab, scale=scale),
+        lambda grad, tokens, vocab, *_: grad.new_empty(vocab, grad.shape[-1]),
+    ),
+    "layer_norm": (
+        "(Tensor x, Tensor weight, Tensor bias, float eps=1e-05) -> Tensor",
+        lambda x, weight, bias, eps=1e-5: T.norm(x, weight, bias, eps),
+        lambda x, *_: x.new_empty(x.shape),
+    ),
+    "layer_norm_forward": (
+        "(Tensor x, Tensor weight, Tensor bias, float eps=1e-05) -> (Tensor, Tensor, Tensor)",
+        lambda x, weight, bias, eps=1e-5: K.layer_norm_forward(x, weight, bias, eps=eps),
+        _norm_meta,
+    ),
+    "layer_norm_backward": (
+        "(Tensor grad_y, Tensor x, Tensor weight, Tensor mean, Tensor rstd) -> (Tensor, Tensor, Tensor)",
+        K.layer_norm_backward,
+        lambda grad_y, x, weight, *_: (x.new_empty(x.shape), weight.new_empty(weight.shape), weight.new_empty(weight.shape)),
+    ),
+    "token_logprobs": (
+        "(Tensor logits, Tensor tokens, float temperature=1.0) -> (Tensor, Tensor)",
+        lambda logits, tokens, temperature=1.0: K.token_logprobs(logits, tokens, temperature=temperature),
+        _rows_meta,
+    ),
+    "token_logprobs_backward": (
+        "(Tensor? grad_logprob, Tensor? grad_entropy, Tensor logits, Tensor tokens, float temperature) -> Tensor",
+        K.token_logprobs_backward,
+        lambda grad_logprob, grad_entropy, logits, *_: logits.new_empty(logits.shape),
+    ),
+}
+
+
 def _plain(x: Tensor) -> bool:
     """Whether a call on ``x`` may go straight to the kernel: no tracing, no
     dispatch mode that wants to see the operator, no batch of tensors in one (that of
@@ -202,6 +255,78 @@ def _distill_autograd(logits, top_val, top_idx, lse=None, temperature=1.0):
     return _DistillLoss.apply(logits, top_val, top_idx, lse, temperature)
 
 
+def _op(name: str, direct: Callable, plain: bool, *args):
+    """The kernel itself, or the operator below autograd (for tracing and batched tensors)."""
+    if plain:
+        return direct(*args)
+    with torch._C._AutoDispatchBelowAutograd():
+        return getattr(torch.ops.rwkv_tl, name)(*args)
+
+
+def _backward_op(name: str, direct: Callable, grad: Tensor, *args):
+    # (a gradient that is to be differentiated goes through the operator, which refuses)
+    plain = _plain(grad) and not torch.is_grad_enabled()
+    return (direct if plain else getattr(torch.ops.rwkv_tl, name))(*args)
+
+
+class _Embed(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, weight, tokens, scale):
+        ctx.save_for_backward(tokens)
+        ctx.vocab, ctx.scale = weight.shape[0], scale
+        return _op("embed", STEP_OPS["embed"][1], _plain(weight), weight, tokens, scale)
+
+    @staticmethod
+    def backward(ctx, grad):
+        args = (grad, *ctx.saved_tensors, ctx.vocab, ctx.scale)
+        return _backward_op("embed_backward", STEP_OPS["embed_backward"][1], grad, *args), None, None
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        y, mean, rstd = _op("layer_norm_forward", STEP_OPS["layer_norm_forward"][1], _plain(x), x, weight, bias, eps)
+        ctx.save_for_backward(x, weight, mean, rstd)
+        return y
+
+    @staticmethod
+    def backward(ctx, grad):
+        return *_backward_op("layer_norm_backward", K.layer_norm_backward, grad, grad, *ctx.saved_tensors), None
+
+
+class _TokenLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, temperature):
+        ctx.save_for_backward(logits, tokens)
+        ctx.temperature = temperature
+        ctx.set_materialize_grads(False)
+        return _op("token_logprobs", STEP_OPS["token_logprobs"][1], _plain(logits), logits, tokens, temperature)
+
+    @staticmethod
+    def backward(ctx, grad_logprob, grad_entropy):
+        some = grad_logprob if grad_logprob is not None else grad_entropy
+        if some is None:
+            return None, None, None
+        args = (grad_logprob, grad_entropy, *ctx.saved_tensors, ctx.temperature)
+        return _backward_op("token_logprobs_backward", K.token_logprobs_backward, some, *args), None, None
+
+
+def _once(name: str):
+    """The Autograd kernel of a gradient: it has none of its own."""
+
+    class Gradient(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, *args):
+            with torch._C._AutoDispatchBelowAutograd():
+                return getattr(torch.ops.rwkv_tl, name)(*args)
+
+        @staticmethod
+        def backward(ctx, *_):
+            raise NotImplementedError(f"{name.removesuffix('_backward')} has no second derivative")
+
+    return Gradient.apply
+
+
 def _dplr_seq_setup(ctx, inputs, output) -> None:
     ctx.save_for_backward(*inputs)
 
@@ -221,7 +346,7 @@ def register() -> None:
     global _registered
     if _registered:
         return
-    for name, (schema, cuda, meta) in {**OPS, **TRAIN_OPS, **LOGITS_OPS}.items():
+    for name, (schema, cuda, meta) in {**OPS, **TRAIN_OPS, **LOGITS_OPS, **STEP_OPS}.items():
         qual = f"{NAMESPACE}::{name}"
         torch.library.define(qual, schema)
         torch.library.impl(qual, "CUDA")(cuda)
@@ -231,6 +356,13 @@ def register() -> None:
     )
     torch.library.impl(f"{NAMESPACE}::distill_loss", "Autograd")(_distill_autograd)
     torch.library.impl(f"{NAMESPACE}::distill_loss_backward", "Autograd")(_DistillLossBackward.apply)
+    for name, autograd in (
+        ("embed", lambda weight, tokens, scale=1.0: _Embed.apply(weight, tokens, scale)),
+        ("layer_norm", lambda x, weight, bias, eps=1e-5: _LayerNorm.apply(x, weight, bias, eps)),
+        ("token_logprobs", lambda logits, tokens, temperature=1.0: _TokenLogprobs.apply(logits, tokens, temperature)),
+    ):
+        torch.library.impl(f"{NAMESPACE}::{name}", "Autograd")(autograd)
+        torch.library.impl(f"{NAMESPACE}::{name}_backward", "Autograd")(_once(f"{name}_backward"))
     _registered = True
 
 
