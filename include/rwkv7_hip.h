@@ -531,16 +531,15 @@ int rwkv7_verify(const void *target, int64_t target_b, int64_t target_r, const v
 
 /* out[i, :] = scale * weight[tokens[i], :], N rows of C values; an id outside
  * 0 .. V-1 (a padded position) gives a row of zeros. weight [V, ldw], out [N, C]
- * of the same type. N < 2^26 - 3, V <= 2^20, C <= 65536. */
+ * of the same type. N < 2^24, V <= 2^20, C <= 65536. */
 int rwkv7_embed(const void *weight, int32_t dtype, int64_t ldw, const int64_t *tokens, float scale, void *out,
                 int64_t N, int32_t V, int32_t C, void *stream);
 
 /* Its gradient to the table: grad_weight[v, :] = scale * the sum of the rows i of
  * grad [N, ldg] with tokens[i] = v, zeros where there is none; every row of
  * grad_weight [V, C] is written. Sums in 32 bits, the same bits every time. The
- * workspace is needed (its size not 0) for N > 64; it need not be cleared, and serves
- * one call in flight. Sizes as rwkv7_embed's. */
-int64_t rwkv7_embed_backward_workspace_bytes(int64_t N, int32_t V, int32_t C);
+ * workspace need not be cleared, and serves one call in flight. Sizes as rwkv7_embed's. */
+int64_t rwkv7_embed_backward_workspace_bytes(int32_t dtype, int64_t N, int32_t V, int32_t C);
 int rwkv7_embed_backward(const void *grad, int32_t dtype, int64_t ldg, const int64_t *tokens, float scale,
                          void *grad_weight, int64_t N, int32_t V, int32_t C, void *workspace, int64_t workspace_bytes,
                          void *stream);

@@ -5,23 +5,74 @@
 // The sums are in 32 bits, each token's rows added up in an order that the tokens
 // alone decide: the same call gives the same bits.
 //
-// Gradient. The table's rows belong to G workgroups, row v to workgroup v % G (frequent
-// tokens have neighbouring ids). Each counts the tokens of its rows, and reads the
-// tokens once more for their positions. Rows of up to 64 positions are summed by a wave
-// each, their positions brought into order first by counting; rows without any are
-// written as zeros by the waves that are free. The positions of a row with more go, in
-// order, to a list in the workspace, in units of about 64 that a second launch sums,
-// four waves a unit; the unit that arrives last at its row adds up the units' sums.
-//
-// Bound by the table's own bytes, written once; nothing is cleared first.
-#include "row_parts.h"
+// Gradient, two launches. The first sorts the positions by token, and beside that fills
+// the table with zeros: V C values, most of what the call has to move, which hide the
+// sort's latency (the rows that the second launch writes are so written twice: one in
+// twelve of 65536 for 16384 tokens).
+//   Sort: the table's rows belong to G workgroups, row v to workgroup v % G (frequent
+//   tokens have neighbouring ids). Each counts the tokens of its rows and those of the
+//   workgroups before it, which gives its range of the list of positions, and reads the
+//   tokens once more for the positions. Those of a row of up to 64 are put in order by
+//   counting the lesser ones; of a row with more, they are met in order.
+// The second launch goes through the sorted list, eight positions a workgroup and what
+// else belongs to the rows that begin there, so that eight rows are always in flight. A
+// row of more than 32 positions is cut into units; the one that arrives last adds up
+// the units' sums.
+#include "logits_rows.h"
 #include "rwkv7_kernels.h"
 
 namespace rwkv7 {
 namespace {
 
-constexpr int64_t kEmbedMaxN = (1 << 26) - 4;  // (a grid has fewer than 2^32 threads)
+constexpr int64_t kEmbedMaxN = (1 << 24) - 1;  // (a grid has fewer than 2^32 threads)
 constexpr int kEmbedMaxV = 1 << 20, kEmbedMaxC = 65536;
+
+// A thread's piece of a row: E values, 16 bytes or (rows shorter than that) one value. The
+// last piece of a row ends with it, over the one before where E does not divide C: both
+// have the same values there. Rows may start at any element.
+template <int FMT, int E>
+RWKV7_DEV int piece_at(int b, int C) {
+  return min(E * b, C - E);
+}
+template <int FMT, int E>
+struct Piece {
+  uint32_t w[E == 1 ? 1 : 4];
+  RWKV7_DEV void load(const char *p) {
+    if constexpr (E > 1) __builtin_memcpy(w, p, 16);
+    else if constexpr (FMT == 1) w[0] = *reinterpret_cast<const uint32_t *>(p);
+    else w[0] = *reinterpret_cast<const uint16_t *>(p);
+  }
+  RWKV7_DEV void get(float (&f)[E]) const {
+    if constexpr (FMT == 1) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) f[e] = __uint_as_float(w[e]);
+    } else if constexpr (E == 1) {
+      f[0] = F16T<FMT == 2>::to_f((uint16_t)w[0]);
+    } else {
+      F16T<FMT == 2>::to_f8(make_uint4(w[0], w[1], w[2], w[3]), f);
+    }
+  }
+};
+template <int FMT, int E>
+RWKV7_DEV void store_piece(char *p, const float (&f)[E]) {
+  if constexpr (E == 1) {
+    store_logit<FMT>(p, 0, f[0]);
+  } else if constexpr (FMT == 1) {
+    __builtin_memcpy(p, f, 16);
+  } else {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      w[i] = (uint32_t)F16T<FMT == 2>::from_f(f[2 * i]) | ((uint32_t)F16T<FMT == 2>::from_f(f[2 * i + 1]) << 16);
+    __builtin_memcpy(p, w, 16);
+  }
+}
+template <int FMT>
+constexpr int kWide = FMT == 1 ? 4 : 8;
+template <int E>
+int pieces(int C) {
+  return (C + E - 1) / E;
+}
 
 struct EmbedArgs {
   const void *w;
@@ -33,8 +84,8 @@ struct EmbedArgs {
   float scale;
 };
 
-// A wave per row and 64 eights of it.
-template <int FMT>
+// A wave per row.
+template <int FMT, int E>
 __global__ __launch_bounds__(256) void embed_kernel(EmbedArgs g) {
   const int lane = threadIdx.x & 63;
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -44,31 +95,38 @@ __global__ __launch_bounds__(256) void embed_kernel(EmbedArgs g) {
   const char *src = static_cast<const char *>(g.w) + (there ? id : 0) * g.ldw * kLogitBytes<FMT>;
   char *dst = static_cast<char *>(g.out) + row * g.C * kLogitBytes<FMT>;
 #pragma unroll 4
-  for (int b = lane; b < (g.C + 7) / 8; b += kWave) {
-    const int n = part_len(b, g.C);
-    float f[8] = {};
+  for (int b = lane; E * b < g.C; b += kWave) {
+    const int at = piece_at<FMT, E>(b, g.C) * kLogitBytes<FMT>;
+    float f[E] = {};
     if (there) {
-      load_part_f<FMT>(f, src, b, n);
+      Piece<FMT, E> x;
+      x.load(src + at);
+      x.get(f);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] *= g.scale;
+      for (int e = 0; e < E; ++e) f[e] *= g.scale;
     }
-    store_part<FMT>(dst, b, n, f);
+    store_piece<FMT, E>(dst + at, f);
   }
 }
 
 // ---- gradient -----------------------------------------------------------------
 
-constexpr int kOwnThreads = 1024, kOwnWaves = kOwnThreads / kWave;
-constexpr int kOwnRows = 256;  // rows of a workgroup at most
-constexpr int kFew = 64;       // positions that a wave sums by itself
-constexpr int kUnit = 64;      // positions of a unit of a longer row, while these make no more than
-constexpr int kMaxUnits = 256; // units a row
-constexpr int kCols = 512;     // columns of a unit's workgroup
+constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / kWave;
+constexpr int kSortRows = 256;   // rows of a workgroup at most (8 bits beside a position's 24)
+constexpr int kFew = 64;         // positions of a row that are ordered by counting
+constexpr int kUnit = 32;        // positions of a unit, while a row has no more units than
+constexpr int kMaxUnits = 128;
+constexpr int kRun = 8;          // positions of the list, and rows in flight, of a workgroup
+constexpr int kJoin = 4;         // units' sums in flight
+constexpr int kFillGroups = 1024;
+constexpr int kHeld = 16;        // tokens that a thread of the sort keeps, where there are no more
 
+// What begins at a position of the list.
 struct Unit {
-  int row;           // -1: none
-  int start, count;  // of the list of positions
-  int first, units;  // the row's first unit and how many it has
+  int row;    // -1: nothing does
+  int count;  // positions
+  int at;     // which of its row's units this is, and 2^16 times how many it has
+  int slot;   // of the row's first unit
 };
 
 struct EmbedGradArgs {
@@ -79,26 +137,37 @@ struct EmbedGradArgs {
   int64_t N;
   int V, C, log_g;
   float scale;
-  // for N > kFew
   int *order;    // [N]
-  Unit *table;   // [slots]
-  int *arrived;  // [slots][column blocks]
-  float *part;   // [slots][C]
-  int slots, blocks;
+  Unit *table;   // [N]
+  int *arrived;  // [slots][column blocks]: units that have arrived, at a row's first slot
+  float *part;   // [slots][columns, whole workgroups]: sums of the units of rows that have several
+  int blocks;
 };
 
-struct OwnLds {
-  int count[kOwnRows];
-  int at[kOwnRows];       // of a row of few: where its next position goes
-  int few[kOwnRows];      // rows of 1 .. kFew positions, then (from the end) those of none
-  int hot[kOwnRows];      // rows of more
-  int n_few, n_none, n_hot, next, less;
-  int wave[kOwnWaves];
-  uint32_t list[kOwnRows * kFew];
+// A row of several units (33 positions or more) has a slot for each, behind those of the rows before it: no more
+// than one for every 16 positions.
+RWKV7_DEV int first_slot(int start) { return (start + 15) / 16; }
+inline int64_t slots(int64_t N) { return (N + 15) / 16; }
+
+// Positions of a unit of a row of c > 0.
+RWKV7_DEV int unit_len(int c) {
+  const int units = min((c + kUnit - 1) / kUnit, kMaxUnits);
+  return (c + units - 1) / units;
+}
+
+struct SortLds {
+  int count[kSortRows];
+  int at[kSortRows];    // of a row's positions in the list
+  int few[kSortRows];   // of a row of few: in `keys`
+  int next[kSortRows];  // where its next one goes there
+  int hot[kSortRows];   // rows of more than kFew
+  int n_hot, less;
+  int wave[kSortWaves];
+  uint32_t keys[kSortRows * kFew];  // row and position
 };
 
-// Exclusive sum over the first kOwnRows threads (four waves) of the workgroup.
-RWKV7_DEV int own_scan(int v, int *wave, int &total) {
+// Exclusive sum over the first kSortRows threads (four waves) of the workgroup.
+RWKV7_DEV int sort_scan(int v, int *wave, int &total) {
   const int t = threadIdx.x, lane = t & 63, wv = t >> 6;
   int inc = v;
 #pragma unroll
@@ -112,223 +181,277 @@ RWKV7_DEV int own_scan(int v, int *wave, int &total) {
   int before = 0;
   total = 0;
 #pragma unroll
-  for (int i = 0; i < kOwnRows / kWave; ++i) {
+  for (int i = 0; i < kSortRows / kWave; ++i) {
     before += i < wv ? wave[i] : 0;
     total += wave[i];
   }
   return before + inc - v;
 }
 
-template <int FMT>
-RWKV7_DEV void add_eight(float (&acc)[8], const Chunk<FMT> &x) {
-  float f[8];
-  x.get(f);
-#pragma unroll
-  for (int e = 0; e < 8; ++e) acc[e] += f[e];
+RWKV7_DEV void fill_zeros(char *out, int64_t bytes, int group) {
+  const int64_t n16 = bytes / 16, step = (int64_t)kFillGroups * kSortThreads;
+  const uint32_t zero[4] = {0u, 0u, 0u, 0u};
+#pragma unroll 4
+  for (int64_t i = (int64_t)group * kSortThreads + threadIdx.x; i < n16; i += step) __builtin_memcpy(out + 16 * i, zero, 16);
+  if (group == 0 && threadIdx.x < bytes % 16) out[16 * n16 + threadIdx.x] = 0;
 }
 
-template <int FMT>
-__global__ __launch_bounds__(kOwnThreads) void embed_grad_kernel(EmbedGradArgs a) {
-  __shared__ OwnLds s;
+// HELD: each thread has its tokens in registers after the first pass. (Each trip to memory beside the fill's
+// stores takes 2 us or more.)
+template <int ELEM, bool HELD>
+__global__ __launch_bounds__(kSortThreads, 8) void embed_sort_kernel(EmbedGradArgs a) {
+  __shared__ SortLds s;
   const int t = threadIdx.x, lane = t & 63, wv = t >> 6, g = blockIdx.x, G = 1 << a.log_g;
-  const int rows = g < a.V ? ((a.V - 1 - g) >> a.log_g) + 1 : 0;  // <= kOwnRows
-  if (t < kOwnRows) s.count[t] = 0;
-  if (t == 0) s.n_few = s.n_none = s.n_hot = s.next = s.less = 0;
+  if (g >= G) {
+    fill_zeros(static_cast<char *>(a.out), (int64_t)a.V * a.C * ELEM, g - G);
+    return;
+  }
+  const int rows = g < a.V ? ((a.V - 1 - g) >> a.log_g) + 1 : 0;  // <= kSortRows
+  if (t < kSortRows) s.count[t] = 0;
+  if (t == 0) s.n_hot = s.less = 0;
   __syncthreads();
+
+  // Wave w has the w-th range of the tokens, 64 at a time: f(position, the token's row
+  // here or -1) for each.
+  const int N = (int)a.N, span = ((N + kSortWaves - 1) / kSortWaves + kWave - 1) / kWave * kWave;
+  const int i0 = wv * span, i1 = min(N, i0 + span);
+  auto row_of = [&](int64_t id) { return id >= 0 && id < a.V && ((int)id & (G - 1)) == g ? (int)id >> a.log_g : -1; };
+  int held[HELD ? kHeld : 1];
+  auto each = [&](auto f) {
+    if constexpr (HELD) {
+#pragma unroll
+      for (int k = 0; k < kHeld; ++k)
+        if (i0 + k * kWave < i1) f(i0 + k * kWave + lane, held[k]);
+    } else {
+#pragma unroll 4
+      for (int i = i0; i < i1; i += kWave) f(i + lane, i + lane < i1 ? row_of(a.tokens[i + lane]) : -1);
+    }
+  };
 
   // how often each row's token occurs, and how many tokens belong to workgroups before
   int less = 0;
-#pragma unroll 4
-  for (int64_t i = t; i < a.N; i += kOwnThreads) {
-    const int64_t id = a.tokens[i];
-    if (id >= 0 && id < a.V) {
-      const int owner = (int)id & (G - 1);
-      if (owner == g) atomicAdd(&s.count[(int)id >> a.log_g], 1);
-      less += owner < g;
-    }
-  }
-  if (a.slots) {
-    less = (int)(wave_sum_d((double)less));
-    if (lane == 0) atomicAdd(&s.less, less);
-  }
-  __syncthreads();
-  const int c = t < rows ? s.count[t] : 0;
-  int few_total, all;
-  const int few_at = own_scan(c <= kFew ? c : 0, s.wave, few_total);
-  const int all_at = own_scan(c, s.wave, all);
-  if (t < rows) {
-    s.at[t] = few_at;
-    if (c == 0) s.few[kOwnRows - 1 - atomicAdd(&s.n_none, 1)] = t;
-    else if (c <= kFew) s.few[atomicAdd(&s.n_few, 1)] = t;
-    else s.hot[atomicAdd(&s.n_hot, 1)] = t;
-  }
-  __syncthreads();
-
-  // the rows of few positions: these in any order, sorted below
-#pragma unroll 4
-  for (int64_t i = t; i < a.N; i += kOwnThreads) {
-    const int64_t id = a.tokens[i];
-    if (id >= 0 && id < a.V && ((int)id & (G - 1)) == g) {
-      const int r = (int)id >> a.log_g;
-      if (s.count[r] <= kFew) s.list[atomicAdd(&s.at[r], 1)] = (uint32_t)i;
-    }
-  }
-
-  // the units of the others. A workgroup's tokens are its range of the list; a row of c
-  // has no more than c / 32 units, so that its units have a range of the table likewise.
-  if (a.slots) {
-    const int base = s.less, slot0 = (base + 31) / 32;
-    int slot1 = (base + all + 31) / 32;
-    if (g == G - 1) slot1 = a.slots;
-    const bool hot = t < rows && c > kFew;
-    const int units = hot ? min((c + kUnit - 1) / kUnit, kMaxUnits) : 0, per = hot ? (c + units - 1) / units : 0;
-    int used;
-    const int first = own_scan(units, s.wave, used) + slot0;
-    for (int u = 0; u < units; ++u) {
-      const int from = min(u * per, c), to = min(from + per, c);
-      a.table[first + u] = {(t << a.log_g) + g, base + all_at + from, to - from, first, units};
-    }
-    for (int i = slot0 + used + t; i < slot1; i += kOwnThreads) a.table[i].row = -1;
-    for (int64_t i = (int64_t)slot0 * a.blocks + t; i < (int64_t)(slot0 + used) * a.blocks; i += kOwnThreads) a.arrived[i] = 0;
-    // their positions in order: each wave a range of the tokens, first counted
-    if (t < rows) s.at[t] = c > kFew ? base + all_at : s.at[t];
-    __syncthreads();
-    const int64_t span = ((a.N + kOwnWaves - 1) / kOwnWaves + kWave - 1) / kWave * kWave;
-    const int64_t i0 = wv * span, i1 = min(a.N, i0 + span);
-    for (int h = 0; h < s.n_hot; ++h) {
-      const int r = s.hot[h];
-      const int64_t want = ((int64_t)r << a.log_g) + g;
-      int n = 0;
-#pragma unroll 4
-      for (int64_t i = i0; i < i1; i += kWave) n += __popcll(__ballot(i + lane < i1 && a.tokens[min(i + lane, a.N - 1)] == want));
-      __syncthreads();
-      if (lane == 0) s.wave[wv] = n;
-      __syncthreads();
-      int at = s.at[r];
-      for (int i = 0; i < wv; ++i) at += s.wave[i];
-      if (n > 0) {
-#pragma unroll 4
-        for (int64_t i = i0; i < i1; i += kWave) {
-          const bool is = i + lane < i1 && a.tokens[min(i + lane, a.N - 1)] == want;
-          const u64 m = __ballot(is);
-          if (is) a.order[at + __popcll(m & ((1ull << lane) - 1))] = (int)(i + lane);
-          at += __popcll(m);
-        }
-      }
-    }
-  }
-  __syncthreads();
-
-  // a row at a time, to whichever wave is free: first those with positions
-  const int n_few = s.n_few, n_rows = n_few + s.n_none, n8 = (a.C + 7) / 8;
-  for (;;) {
-    int k = lane == 0 ? atomicAdd(&s.next, 1) : 0;
-    k = __builtin_amdgcn_readfirstlane(k);
-    if (k >= n_rows) break;
-    const int r = s.few[k < n_few ? k : kOwnRows - 1 - (k - n_few)];
-    char *dst = static_cast<char *>(a.out) + (((int64_t)r << a.log_g) + g) * a.C * kLogitBytes<FMT>;
-    if (k >= n_few) {
-      const float zero[8] = {};
-      for (int b = lane; b < n8; b += kWave) store_part<FMT>(dst, b, part_len(b, a.C), zero);
-      continue;
-    }
-    const int n = __builtin_amdgcn_readfirstlane(s.count[r]), at = __builtin_amdgcn_readfirstlane(s.at[r]) - n;
-    uint32_t pos = lane < n ? s.list[at + lane] : ~0u;
-    if (n > 1) {
-      int rank = 0;
-      for (int j = 0; j < n; ++j) rank += (uint32_t)__builtin_amdgcn_readlane((int)pos, j) < pos;
-      if (lane < n) s.list[at + rank] = pos;
-      __builtin_amdgcn_wave_barrier();
-      pos = lane < n ? s.list[at + lane] : 0u;
-    }
-    for (int b = lane; b < (n8 + kWave - 1) / kWave * kWave; b += kWave) {
-      const int len = part_len(b, a.C);
-      float acc[8] = {};
-#pragma unroll 8
-      for (int j = 0; j < n; ++j) {
-        const uint32_t p = (uint32_t)__builtin_amdgcn_readlane((int)pos, j);
-        Chunk<FMT> x;
-        load_part(x, static_cast<const char *>(a.dy) + p * a.ldg * kLogitBytes<FMT>, b, len);
-        add_eight(acc, x);
+  auto count = [&](int64_t id) {
+    const int r = row_of(id);
+    if (r >= 0) atomicAdd(&s.count[r], 1);
+    less += id >= 0 && id < a.V && ((int)id & (G - 1)) < g;
+    return r;
+  };
+  if constexpr (HELD) {
+#pragma unroll
+    for (int k0 = 0; k0 < kHeld; k0 += 8) {
+      int64_t id[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int i = i0 + (k0 + k) * kWave + lane;
+        id[k] = i < i1 ? a.tokens[i] : -1;
       }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) acc[e] *= a.scale;
-      store_part<FMT>(dst, b, len, acc);
+      for (int k = 0; k < 8; ++k) held[k0 + k] = count(id[k]);
     }
+  } else {
+#pragma unroll 8
+    for (int i = i0 + lane; i < i1; i += kWave) count(a.tokens[i]);
+  }
+  less = (int)wave_sum_d((double)less);
+  if (lane == 0) atomicAdd(&s.less, less);
+  __syncthreads();
+  const int c = t < rows ? s.count[t] : 0;
+  int all, n_few;
+  const int at = sort_scan(c, s.wave, all) + s.less;
+  const int few = sort_scan(c <= kFew ? c : 0, s.wave, n_few);
+  if (t < rows) s.at[t] = at, s.few[t] = s.next[t] = few;
+  if (c > kFew) s.hot[atomicAdd(&s.n_hot, 1)] = t;
+  if (c > kUnit)
+    for (int b = 0; b < a.blocks; ++b) a.arrived[(int64_t)first_slot(at) * a.blocks + b] = 0;
+  if (g == G - 1)
+    for (int i = s.less + all + t; i < N; i += kSortThreads) a.table[i].row = -1;
+  __syncthreads();
+
+  each([&](int i, int r) {
+    if (r >= 0 && s.count[r] <= kFew) s.keys[atomicAdd(&s.next[r], 1)] = ((uint32_t)r << 24) | (uint32_t)i;
+  });
+  __syncthreads();
+  // the i-th position of row r
+  auto put = [&](int r, int i, int pos) {
+    const int count = s.count[r], start = s.at[r], per = unit_len(count), units = (count + per - 1) / per;
+    Unit u = {-1, 0, 0, 0};
+    if (i % per == 0) u = {(r << a.log_g) + g, min(per, count - i), i / per | (units << 16), first_slot(start)};
+    a.order[start + i] = pos;
+    a.table[start + i] = u;
+  };
+  for (int i = t; i < n_few; i += kSortThreads) {
+    const uint32_t key = s.keys[i];
+    const int r = key >> 24, from = s.few[r], n = s.count[r];
+    int rank = 0;
+    for (int j = from; j < from + n; ++j) rank += s.keys[j] < key;
+    put(r, rank, (int)(key & 0xffffffu));
+  }
+  // rows of more: each wave's range of the tokens, first counted
+  for (int h = 0; h < s.n_hot; ++h) {
+    const int r = s.hot[h];
+    int n = 0;
+    each([&](int, int own) { n += __popcll(__ballot(own == r)); });
+    __syncthreads();
+    if (lane == 0) s.wave[wv] = n;
+    __syncthreads();
+    int to = 0;
+    for (int i = 0; i < wv; ++i) to += s.wave[i];
+    if (n > 0)
+      each([&](int i, int own) {
+        const u64 m = __ballot(own == r);
+        if (own == r) put(r, to + __popcll(m & ((1ull << lane) - 1)), i);
+        to += __popcll(m);
+      });
   }
 }
 
-// A unit's 512 columns: wave w sums the positions w, w + 4, ..; the waves' sums, and the
-// units', are added in order.
-template <int FMT>
-__global__ __launch_bounds__(256) void embed_unit_kernel(EmbedGradArgs a) {
-  __shared__ float sum[4][kCols];
-  __shared__ bool last;
-  const Unit u = a.table[blockIdx.x];
-  if (u.row < 0) return;
-  const int t = threadIdx.x, lane = t & 63, wv = t >> 6, b = blockIdx.y * (kCols / 8) + lane, len = part_len(b, a.C);
-  float acc[8] = {};
-  if (len > 0) {
-#pragma unroll 8
-    for (int j = wv; j < u.count; j += 4) {
-      const int64_t p = a.order[u.start + j];
-      Chunk<FMT> x;
-      load_part(x, static_cast<const char *>(a.dy) + p * a.ldg * kLogitBytes<FMT>, b, len);
-      add_eight(acc, x);
+// The units that begin at eight positions of the list: each thread a piece of the
+// columns, all positions one after the other.
+template <int FMT, int E>
+__global__ __launch_bounds__(256) void embed_sum_kernel(EmbedGradArgs a) {
+  __shared__ Unit s_unit[kRun];
+  __shared__ bool s_last;
+  static_assert(kRun < kUnit / 2);
+  const int t = threadIdx.x, lane = t & 63, b = blockIdx.y * blockDim.x + t;
+  const bool some = E * b < a.C;
+  const int col = (some ? piece_at<FMT, E>(b, a.C) : 0) * kLogitBytes<FMT>;
+  const int p0 = blockIdx.x * kRun, there = min((int64_t)kRun, a.N - p0);
+  Unit own = {-1, 0, 0, 0};
+  if (lane < there) own = a.table[p0 + lane];
+  const uint32_t begin = (uint32_t)__ballot(own.row >= 0);
+  if (begin == 0u) return;  // (the same for all waves)
+  if (t < kRun) s_unit[t] = own;
+  const int from = __builtin_ctz(begin), last_at = 31 - __builtin_clz(begin);
+  const int n = last_at - from + __builtin_amdgcn_readlane(own.count, last_at);  // <= kRun - 1 + kUnit positions,
+  const int pos = a.order[p0 + from + min(lane, n - 1)];                         // or one long unit's: 64 at a time
+  __syncthreads();
+  const char *dy = static_cast<const char *>(a.dy);
+  float acc[E] = {};
+
+  auto uniform = [](int v) { return __builtin_amdgcn_readfirstlane(v); };  // (every lane has the same)
+  auto put = [&](int row) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] *= a.scale;
+    if (some) store_piece<FMT, E>(static_cast<char *>(a.out) + row * (int64_t)a.C * kLogitBytes<FMT> + col, acc);
+  };
+  Piece<FMT, E> x[kRun];
+  auto load = [&](int lanes, int j, int to) {
+    asm volatile("" : "+v"(lanes));  // (has arrived here: else each readlane below waits for the rows before it)
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) {
+      x[i] = {};
+      if (j + i < to) x[i].load(dy + (int64_t)__builtin_amdgcn_readlane(lanes, j + i) * a.ldg * kLogitBytes<FMT> + col);
+    }
+  };
+  auto add = [&](const Piece<FMT, E> &p) {
+    float f[E];
+    p.get(f);
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] += f[e];
+  };
+
+  // the first eight, where units begin; then what is left of the last one. (One of several
+  // of its row has 17 positions or more: it can only be the last.)
+  load(pos, 0, n);
+  int at = from;
+#pragma unroll
+  for (int i = 0; i < kRun; ++i) {
+    if (i > 0 && from + i < kRun && ((begin >> (from + i)) & 1u)) {
+      put(uniform(s_unit[at].row));
+      at = from + i;
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] = 0.f;
+    }
+    add(x[i]);
+  }
+  for (int j = kRun; j < n; j += kRun) {
+    int lanes = pos;
+    if (j >= kWave) lanes = a.order[p0 + from + min(j / kWave * kWave + lane, n - 1)];
+    load(lanes, j % kWave, min(n - j / kWave * kWave, kWave));
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) add(x[i]);
+  }
+  const Unit u = {uniform(s_unit[at].row), 0, uniform(s_unit[at].at), uniform(s_unit[at].slot)};
+  const int units = u.at >> 16;
+  if (units > 1) {
+    // The sums as the units' threads have them: value e of all threads side by side.
+    const int64_t unit_size = (int64_t)a.blocks * blockDim.x * E;
+    float *part = a.part + u.slot * unit_size + (int64_t)blockIdx.y * blockDim.x * E + t;
+    // stored past the caches of this XCD, acknowledged before the count goes up
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      __hip_atomic_store(part + (u.at & 0xffff) * unit_size + e * blockDim.x, acc[e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (t == 0)
+      s_last = __hip_atomic_fetch_add(a.arrived + (int64_t)u.slot * a.blocks + blockIdx.y, 1, __ATOMIC_RELAXED,
+                                      __HIP_MEMORY_SCOPE_AGENT) == units - 1;
+    __syncthreads();
+    if (!s_last) return;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0.f;
+    for (int i = 0; i < units; i += kJoin) {
+      float p[kJoin][E];
+#pragma unroll
+      for (int k = 0; k < kJoin; ++k)
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          p[k][e] = __hip_atomic_load(part + min(i + k, units - 1) * unit_size + e * blockDim.x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+      for (int k = 0; k < kJoin; ++k)
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] += i + k < units ? p[k][e] : 0.f;
     }
   }
-#pragma unroll
-  for (int e = 0; e < 8; ++e) sum[wv][8 * lane + e] = acc[e];
-  __syncthreads();
-  const int64_t col0 = (int64_t)blockIdx.y * kCols + 2 * t;
-  float v[2];
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    v[e] = (sum[0][2 * t + e] + sum[1][2 * t + e]) + (sum[2][2 * t + e] + sum[3][2 * t + e]);
-    // stored past the caches of this XCD, acknowledged before the count goes up
-    if (col0 + e < a.C)
-      __hip_atomic_store(a.part + (int64_t)blockIdx.x * a.C + col0 + e, v[e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  }
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
-  if (t == 0)
-    last = __hip_atomic_fetch_add(a.arrived + (int64_t)u.first * a.blocks + blockIdx.y, 1, __ATOMIC_RELAXED,
-                                  __HIP_MEMORY_SCOPE_AGENT) == u.units - 1;
-  __syncthreads();
-  if (!last) return;
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    if (col0 + e >= a.C) break;
-    const float *p = a.part + (int64_t)u.first * a.C + col0 + e;
-    float total = 0.f;
-#pragma unroll 8
-    for (int i = 0; i < u.units; ++i)
-      total += __hip_atomic_load(p + (int64_t)i * a.C, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    store_logit<FMT>(a.out, u.row * (int64_t)a.C + col0 + e, total * a.scale);
-  }
+  put(u.row);
 }
 
 int log_groups(int V) {
   int l = 8;
-  while ((int64_t)kOwnRows << l < V) ++l;
+  while ((int64_t)kSortRows << l < V) ++l;
   return l;
+}
+
+// f(FMT, E) for a type and width
+template <class F>
+void with_pieces(int dtype, int C, F f) {
+  using std::integral_constant;
+  auto width = [&](auto fmt) {
+    constexpr int FMT = decltype(fmt)::value;
+    if (C >= kWide<FMT>) f(fmt, integral_constant<int, kWide<FMT>>());
+    else f(fmt, integral_constant<int, 1>());
+  };
+  if (dtype == 0) width(integral_constant<int, 0>());
+  else if (dtype == 1) width(integral_constant<int, 1>());
+  else width(integral_constant<int, 2>());
+}
+
+// The sums' workgroups: a piece a thread, up to 256 threads.
+struct SumShape {
+  int threads, blocks, columns;
+};
+SumShape sum_shape(int dtype, int C) {
+  SumShape s;
+  with_pieces(dtype, C, [&](auto, auto e) {
+    constexpr int E = decltype(e)::value;
+    const int n = (pieces<E>(C) + kWave - 1) / kWave * kWave;
+    s.threads = n < 256 ? n : 256;
+    s.blocks = (n + s.threads - 1) / s.threads;
+    s.columns = s.blocks * s.threads * E;
+  });
+  return s;
 }
 
 struct GradSpace {
   int64_t table, arrived, order, part, bytes;
-  int slots, blocks;
 };
-GradSpace grad_space(int64_t N, int C) {
-  GradSpace s = {};
-  if (N <= kFew) return s;  // no row has more
+GradSpace grad_space(int64_t N, int C, int dtype) {
   auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
-  s.slots = (int)((N + 31) / 32);
-  s.blocks = (C + kCols - 1) / kCols;
-  s.table = 0;
-  s.arrived = s.table + up(s.slots * (int64_t)sizeof(Unit));
-  s.order = s.arrived + up((int64_t)s.slots * s.blocks * 4);
+  GradSpace s = {};
+  s.arrived = s.table + up(N * (int64_t)sizeof(Unit));
+  s.order = s.arrived + up(slots(N) * sum_shape(dtype, C).blocks * 4);
   s.part = s.order + up(N * 4);
-  s.bytes = s.part + (int64_t)s.slots * C * 4;
+  s.bytes = s.part + slots(N) * sum_shape(dtype, C).columns * 4;
   return s;
 }
 
@@ -346,50 +469,46 @@ extern "C" int rwkv7_embed(const void *weight, int32_t dtype, int64_t ldw, const
   if (!sizes_ok(N, V, C) || ldw < C) return RWKV7_ESHAPE;
   const EmbedArgs g = {weight, ldw, tokens, out, N, V, C, scale};
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  const int grid = (int)((N + 3) / 4);
-  switch (dtype) {
-    case 0: embed_kernel<0><<<grid, 256, 0, st>>>(g); break;
-    case 1: embed_kernel<1><<<grid, 256, 0, st>>>(g); break;
-    default: embed_kernel<2><<<grid, 256, 0, st>>>(g); break;
-  }
+  with_pieces(dtype, C, [&](auto f, auto e) {
+    embed_kernel<decltype(f)::value, decltype(e)::value><<<(int)((N + 3) / 4), 256, 0, st>>>(g);
+  });
   RWKV7_CHECK_LAUNCH();
   return RWKV7_OK;
 }
 
-extern "C" int64_t rwkv7_embed_backward_workspace_bytes(int64_t N, int32_t V, int32_t C) {
+extern "C" int64_t rwkv7_embed_backward_workspace_bytes(int32_t dtype, int64_t N, int32_t V, int32_t C) {
   using namespace rwkv7;
-  return sizes_ok(N, V, C) ? grad_space(N, C).bytes : 0;
+  return sizes_ok(N, V, C) && dtype >= 0 && dtype <= 2 ? grad_space(N, C, dtype).bytes : 0;
 }
 
 extern "C" int rwkv7_embed_backward(const void *grad, int32_t dtype, int64_t ldg, const int64_t *tokens, float scale,
                                     void *grad_weight, int64_t N, int32_t V, int32_t C, void *workspace,
                                     int64_t workspace_bytes, void *stream) {
   using namespace rwkv7;
-  if (!grad || !tokens || !grad_weight || dtype < 0 || dtype > 2) return RWKV7_EINVAL;
+  if (!grad || !tokens || !grad_weight || !workspace || dtype < 0 || dtype > 2) return RWKV7_EINVAL;
   if (!sizes_ok(N, V, C) || ldg < C) return RWKV7_ESHAPE;
-  const GradSpace s = grad_space(N, C);
-  if (s.bytes && !workspace) return RWKV7_EINVAL;
+  const GradSpace s = grad_space(N, C, dtype);
   if (workspace_bytes < s.bytes) return RWKV7_EWORKSPACE;
   char *ws = static_cast<char *>(workspace);
-  const int l = log_groups(V);
-  const EmbedGradArgs a = {grad, ldg, tokens, grad_weight, N, V, C, l, scale, reinterpret_cast<int *>(ws + s.order),
+  const SumShape shape = sum_shape(dtype, C);
+  const EmbedGradArgs a = {grad, ldg, tokens, grad_weight, N, V, C, log_groups(V), scale, reinterpret_cast<int *>(ws + s.order),
                            reinterpret_cast<Unit *>(ws + s.table), reinterpret_cast<int *>(ws + s.arrived),
-                           reinterpret_cast<float *>(ws + s.part), s.slots, s.blocks};
+                           reinterpret_cast<float *>(ws + s.part), shape.blocks};
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  switch (dtype) {
-    case 0: embed_grad_kernel<0><<<1 << l, kOwnThreads, 0, st>>>(a); break;
-    case 1: embed_grad_kernel<1><<<1 << l, kOwnThreads, 0, st>>>(a); break;
-    default: embed_grad_kernel<2><<<1 << l, kOwnThreads, 0, st>>>(a); break;
+  const int groups = (1 << a.log_g) + kFillGroups;
+  const bool held = N <= kHeld * kSortThreads;
+  if (dtype == 1) {
+    if (held) embed_sort_kernel<4, true><<<groups, kSortThreads, 0, st>>>(a);
+    else embed_sort_kernel<4, false><<<groups, kSortThreads, 0, st>>>(a);
+  } else {
+    if (held) embed_sort_kernel<2, true><<<groups, kSortThreads, 0, st>>>(a);
+    else embed_sort_kernel<2, false><<<groups, kSortThreads, 0, st>>>(a);
   }
   RWKV7_CHECK_LAUNCH();
-  if (s.slots) {
-    const dim3 grid(s.slots, s.blocks);
-    switch (dtype) {
-      case 0: embed_unit_kernel<0><<<grid, 256, 0, st>>>(a); break;
-      case 1: embed_unit_kernel<1><<<grid, 256, 0, st>>>(a); break;
-      default: embed_unit_kernel<2><<<grid, 256, 0, st>>>(a); break;
-    }
-    RWKV7_CHECK_LAUNCH();
-  }
+  const dim3 grid((unsigned)((N + kRun - 1) / kRun), shape.blocks);
+  with_pieces(dtype, C, [&](auto f, auto e) {
+    embed_sum_kernel<decltype(f)::value, decltype(e)::value><<<grid, shape.threads, 0, st>>>(a);
+  });
+  RWKV7_CHECK_LAUNCH();
   return RWKV7_OK;
 }

@@ -218,7 +218,7 @@ def _declare(lib: ctypes.CDLL) -> None:
         "rwkv7_verify": (ctypes.c_int, [vp, i64, i64, vp, i64, i64, i32, vp, vp, vp, i32, i32, i32, f64, f64, vp, vp, vp,
                                         i64, vp]),
         "rwkv7_embed": (ctypes.c_int, [vp, i32, i64, vp, f32, vp, i64, i32, i32, vp]),
-        "rwkv7_embed_backward_workspace_bytes": (i64, [i64, i32, i32]),
+        "rwkv7_embed_backward_workspace_bytes": (i64, [i32, i64, i32, i32]),
         "rwkv7_embed_backward": (ctypes.c_int, [vp, i32, i64, vp, f32, vp, i64, i32, i32, vp, i64, vp]),
         "rwkv7_layer_norm_forward": (ctypes.c_int, [vp, i32, i64, vp, vp, i32, f64, vp, vp, vp, i64, i32, vp]),
         "rwkv7_layer_norm_backward_workspace_bytes": (i64, [i32, i64, i32]),

@@ -24,7 +24,7 @@ from . import _lib
 from .logits import LOGIT_DTYPES as DTYPES
 from .logits import _empty, _rows, _same_device
 
-MAX_TOKENS = 2**26 - 4  # positions of one call of embed
+MAX_TOKENS = 2**24 - 1  # positions of one call of embed
 MAX_VOCAB = 1 << 20  # rows of an embedding table
 MAX_WIDTH = 65536  # its columns
 MAX_CHANNELS = 16384  # of layer_norm
@@ -89,8 +89,8 @@ def embed(weight: Tensor, tokens: Tensor, *, scale: float = 1.0) -> Tensor:
 
 
 @lru_cache(maxsize=64)
-def _embed_bytes(N: int, V: int, C: int) -> int:
-    return _lib.load().rwkv7_embed_backward_workspace_bytes(N, V, C)
+def _embed_bytes(code: int, N: int, V: int, C: int) -> int:
+    return _lib.load().rwkv7_embed_backward_workspace_bytes(code, N, V, C)
 
 
 def embed_backward(grad: Tensor, tokens: Tensor, vocab: int, *, scale: float = 1.0) -> Tensor:
@@ -112,10 +112,10 @@ def embed_backward(grad: Tensor, tokens: Tensor, vocab: int, *, scale: float = 1
         if N:
             g, _, ld = _rows(grad)
             t = tokens.contiguous()
-            nb = _embed_bytes(N, vocab, C)
-            ws = torch.empty(nb, dtype=torch.uint8, device=grad.device) if nb else None
+            nb = _embed_bytes(code, N, vocab, C)
+            ws = torch.empty(nb, dtype=torch.uint8, device=grad.device)
             rc = _lib.load().rwkv7_embed_backward(
-                g.data_ptr(), code, ld, t.data_ptr(), scale, out.data_ptr(), N, vocab, C, _lib.ptr(ws), nb, _lib.stream_of(g)
+                g.data_ptr(), code, ld, t.data_ptr(), scale, out.data_ptr(), N, vocab, C, ws.data_ptr(), nb, _lib.stream_of(g)
             )
             _lib.check(rc, "rwkv7_embed_backward")
         else:

@@ -92,18 +92,18 @@ def test_c_entries_refuse_before_any_launch():
         return lib.rwkv7_embed(w, dt, ld, tok, 1.0, out, N, V, C, None)
 
     assert emb(w=None) == emb(tok=None) == emb(out=None) == emb(dt=-1) == emb(dt=3) == EINVAL
-    assert emb(ld=7) == emb(N=0) == emb(N=2**26 - 3) == emb(V=0) == emb(V=2**20 + 1) == emb(C=0) == ESHAPE
+    assert emb(ld=7) == emb(N=0) == emb(N=2**24) == emb(V=0) == emb(V=2**20 + 1) == emb(C=0) == ESHAPE
     assert emb(C=65537, ld=65537) == ESHAPE
 
     size = lib.rwkv7_embed_backward_workspace_bytes
-    assert size(64, 16, 8) == 0 < size(65, 16, 8) and size(0, 16, 8) == size(65, 0, 8) == size(2**26, 16, 8) == 0
+    assert 0 < size(0, 1, 16, 8) < size(0, 65, 16, 8) and size(0, 0, 16, 8) == size(0, 65, 0, 8) == size(0, 2**24, 16, 8) == 0
 
     def embg(g=p, dt=0, ld=8, tok=p, out=p, N=65, V=16, C=8, ws=p, nb=None):
-        return lib.rwkv7_embed_backward(g, dt, ld, tok, 1.0, out, N, V, C, ws, size(65, 16, 8) if nb is None else nb, None)
+        return lib.rwkv7_embed_backward(g, dt, ld, tok, 1.0, out, N, V, C, ws, size(0, 65, 16, 8) if nb is None else nb, None)
 
     assert embg(g=None) == embg(tok=None) == embg(out=None) == embg(dt=3) == embg(ws=None) == EINVAL
     assert embg(ld=7) == embg(N=0) == embg(V=0) == embg(V=2**20 + 1) == embg(C=0) == ESHAPE
-    assert embg(nb=size(65, 16, 8) - 1) == EWORKSPACE
+    assert embg(nb=size(0, 65, 16, 8) - 1) == EWORKSPACE
 
     def norm(x=p, dt=0, ld=8, w=p, b=p, wt=1, eps=1e-5, y=p, m=p, r=p, N=3, C=8):
         return lib.rwkv7_layer_norm_forward(x, dt, ld, w, b, wt, eps, y, m, r, N, C, None)
