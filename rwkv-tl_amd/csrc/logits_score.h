@@ -29,73 +29,116 @@ RWKV7_DEV double one_minus_exp(double y) {
   return 1.0 - (y == y ? exp2_d(1.4426950408889634 * y) : y);
 }
 
+// RowMax by halves in pairs for bfloat16 too, as whole numbers: the largest of these is
+// the largest logit where one is positive, and else the least is. Where a NaN that
+// counts as positive is among them it is not, and the caller takes RowMax.
+template <int FMT>
+struct PairMax : RowMax<FMT> {
+  RWKV7_DEV bool clean() const { return true; }
+};
+template <>
+struct PairMax<2> {
+  typedef short short2v __attribute__((ext_vector_type(2)));
+  short2v most = {-32768, -32768}, least = {32767, 32767};
+  RWKV7_DEV void add(const Chunk<2> &x) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const short2v v = __builtin_bit_cast(short2v, x.w[i]);
+      most = __builtin_elementwise_max(most, v);
+      least = __builtin_elementwise_min(least, v);
+    }
+  }
+  RWKV7_DEV bool clean() const { return max(most[0], most[1]) <= 0x7f80; }
+  RWKV7_DEV float value() const {
+    const short m = max(most[0], most[1]), l = min(least[0], least[1]);
+    return m >= 0 ? b2f((uint16_t)m) : l > -128 ? -kInf : b2f((uint16_t)l);  // (0xff80 is -inf; NaN beyond)
+  }
+};
+
 struct ScoreLds {
   float m[kMaxWaves], S[kMaxWaves], T[kMaxWaves];
   int n[kMaxWaves];
 };
 
-// What a wave has of the row beside the largest logits: S' and T' about M as
-// ExpScale::with() forms its exponents, which lie `at` (their own value at M) above y.
+// What the waves have of the row: S', T' and n about M as score_arg() forms the exponents,
+// which lie `at` (their own value at M) above y.
 struct RowSums {
   double S, T, n, at;
   float M;
 };
 
-// The exponent of an element, and of M, in 32 bits; F: with()'s far.
-template <bool FAR>
-RWKV7_DEV float score_arg(const ExpScale &sc, float x, float M, float R) {
-  return FAR ? (x - M) * sc.kf : fmaf(x, sc.kf, -R);
+// The exponent of an element, and of M (ref: M, or 0 for none), in 32 bits.
+RWKV7_DEV float near_arg(const ExpScale &sc, float x, float ref) { return fmaf(x, sc.kf, -(ref * sc.kf)); }
+RWKV7_DEV float score_arg(const ExpScale &sc, float x, float ref) {
+  return sc.near(ref) ? near_arg(sc, x, ref) : (x - ref) * sc.kf;
 }
 
 // Sums of a wave's row about M (wave-uniform, the largest of all waves, `own` this
-// wave's largest). A masked element's exponent, -inf, is taken as -1000: 0 times it
-// is 0. A NaN among the logits makes S NaN; M is the largest of the others.
+// wave's largest). A NaN among the logits makes S NaN; M is the largest of the others.
+// Where a logit is masked, T comes out NaN by 0 times -inf: then, and far from 0 (see
+// ExpScale), the sums are formed from memory, a chunk at a time, with exponents no less
+// than -1000. That is one instruction in nine for every logit of the others.
 template <int THREADS, bool SKIP, int FMT>
-RWKV7_DEV void score_row(Chunk<FMT> (&x)[kRowChunks], uint32_t n8, float tail, const ExpScale &sc, float M, float own,
-                         float &S, float &T, int &n) {
+RWKV7_DEV void score_row(Chunk<FMT> (&x)[kRowChunks], const void *src, uint32_t n8, float tail, const ExpScale &sc, float M,
+                         float own, float &S, float &T, int &n) {
+  const float ref = uniform_f(ExpScale::ref(M));
+  const bool holds = own == M;  // (wave-uniform)
   S = T = 0.f;
   n = 0;
-  const float ref = uniform_f(ExpScale::ref(M));
-  auto sums = [&](auto far, auto most) {
-    constexpr bool kFar = decltype(far)::value, kMost = decltype(most)::value;
-    const float R = ref * sc.kf;
-    auto add = [&](float v, float &s, float &t) {
-      const float y = score_arg<kFar>(sc, v, ref, R);
-      float e = __builtin_amdgcn_exp2f(y);
-      if (kMost) {
-        const bool is = v == M;
-        n += is;
-        e = is ? 0.f : e;
-      }
-      s += e;
-      t = fmaf(e, fmaxf(y, -1000.f), t);
-    };
-    add(tail, S, T);
+  auto add = [&](auto most, auto arg, float v, float &s, float &t) {
+    const float y = arg(v);
+    float e = __builtin_amdgcn_exp2f(y);
+    if (decltype(most)::value) {
+      const bool is = v == M;
+      n += is;
+      e = is ? 0.f : e;
+    }
+    s += e;
+    t = fmaf(e, y, t);
+  };
+  auto chunk = [&](auto most, auto arg, const Chunk<FMT> &c) {
+    float f[kRowChunk], s[2] = {0.f, 0.f}, t[2] = {0.f, 0.f};
+    c.get(f);
+#pragma unroll
+    for (int e = 0; e < kRowChunk; ++e) add(most, arg, f[e], s[e & 1], t[e & 1]);
+    S += s[0] + s[1];
+    T += t[0] + t[1];
+  };
+  const bool near = sc.near(M), has_tail = threadIdx.x < kRowChunk && !(tail == -kInf);
+  auto fast = [&](auto most) {
+    auto arg = [&](float v) { return near_arg(sc, v, ref); };
+    if (has_tail) add(most, arg, tail, S, T);
 #pragma unroll
     for (int c = 0; c < kRowChunks; ++c) {
       if (SKIP && c > 0 && c * THREADS >= (int)n8) break;
-      float f[kRowChunk];
-      if (kMost) x[c].opaque();  // (else what both arms unpack alike would go before them, a row's worth)
-      x[c].template get<kFar>(f);
-      float s[2] = {0.f, 0.f}, t[2] = {0.f, 0.f};
-#pragma unroll
-      for (int e = 0; e < kRowChunk; ++e) add(f[e], s[e & 1], t[e & 1]);
-      S += s[0] + s[1];
-      T += t[0] + t[1];
+      Chunk<FMT> y = x[c];
+      if (decltype(most)::value) y.opaque();  // (else what both arms unpack alike would go before them, a row's worth)
+      if (c * THREADS + (int)threadIdx.x < (int)n8) chunk(most, arg, y);
     }
   };
-  const bool holds = own == M, near = sc.near(M);  // (wave-uniform)
   if (near) {
-    if (holds) sums(BoolConst<false>(), BoolConst<true>());
-    else sums(BoolConst<false>(), BoolConst<false>());
-  } else {
-    if (holds) sums(BoolConst<true>(), BoolConst<true>());
-    else sums(BoolConst<true>(), BoolConst<false>());
+    if (holds) fast(BoolConst<true>());
+    else fast(BoolConst<false>());
+    const float2 st = wave_sum2(S, T);
+    S = st.x;
+    T = st.y;
   }
-  const float2 st = wave_sum2(S, T);
-  S = st.x;
-  T = st.y;
-  if (holds) n = (int)wave_sum((float)n);
+  if (!near || (T != T && S == S)) {
+    S = T = 0.f;
+    n = 0;
+    auto arg = [&](float v) { return fmaxf(score_arg(sc, v, ref), v == v ? -1000.f : v); };
+    if (has_tail) add(BoolConst<true>(), arg, tail, S, T);
+#pragma unroll 1
+    for (uint32_t b = threadIdx.x; b < n8; b += THREADS) {
+      Chunk<FMT> y;
+      y.load_whole(src, b);
+      chunk(BoolConst<true>(), arg, y);
+    }
+    const float2 st = wave_sum2(S, T);
+    S = st.x;
+    T = st.y;
+  }
+  n = holds ? (int)wave_sum((float)n) : 0;
 }
 
 // The waves joined, by one wave. (A count of 2^24 or less is a float.)
@@ -108,7 +151,7 @@ RWKV7_DEV RowSums join_sums(const ScoreLds &s, const ExpScale &sc, float M, int 
   r.n = uniform_d(wave_sum_d(in ? (double)s.n[lane] : 0.0));
   r.M = M;
   const float ref = ExpScale::ref(M);
-  r.at = sc.near(M) ? (double)score_arg<false>(sc, ref, ref, ref * sc.kf) : 0.0;
+  r.at = (double)score_arg(sc, ref, ref);
   return r;
 }
 
@@ -125,7 +168,7 @@ RWKV7_DEV RowScore row_score(const RowSums &r) {
   o.none = r.M == -kInf && r.S == 0.0;
   const double up = exp2_d(-r.at), S1 = r.S * up, T1 = up * (r.T - r.at * r.S), S = r.n + S1;
   // (NaN among the logits makes the sum NaN)
-  o.log_S = S == S && r.M < kInf ? log_n_plus(r.n, S1) : __builtin_nan("");
+  o.log_S = o.none ? 0.0 : S == S && r.M < kInf ? log_n_plus(r.n, S1) : __builtin_nan("");
   o.H = o.none ? 0.0 : o.log_S - kLn2 * T1 * rcp_d(S);
   o.total = S * exp2_d(r.at);
   o.log_total = o.log_S + kLn2 * r.at;

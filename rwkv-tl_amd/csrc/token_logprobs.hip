@@ -78,21 +78,30 @@ __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : 8) void token_kernel(TokenA
   const float xt = tail >= 0 ? load_logit<FMT>(src, tail) : -kInf;
   const float zx = load_logit<FMT>(src, id);
 
-  RowMax<FMT> most;
+  auto largest = [&](auto most) {
 #pragma unroll
-  for (int c = 0; c < kRowChunks; ++c) {
-    if (!GRAD && c > 0 && c * THREADS >= (int)n8) break;
-    most.add(x[c]);
+    for (int c = 0; c < kRowChunks; ++c) {
+      if (!GRAD && c > 0 && c * THREADS >= (int)n8) break;
+      most.add(x[c]);
+    }
+    opaque_row(x);
+    return most;
+  };
+  float own;
+  if constexpr (GRAD) {  // (bound by its bytes, and short of registers)
+    own = wave_max(fmaxf(largest(RowMax<FMT>()).value(), xt));
+  } else {
+    const PairMax<FMT> pairs = largest(PairMax<FMT>());
+    own = wave_max(fmaxf(pairs.value(), xt));
+    if (__ballot(!pairs.clean())) own = wave_max(fmaxf(largest(RowMax<FMT>()).value(), xt));
   }
-  const float own = wave_max(fmaxf(most.value(), xt));
-  opaque_row(x);
   if (lane == 0) s.s.m[wv] = own;
   __syncthreads();
   const float M = uniform_f(wave_max(lane < kWaves ? s.s.m[lane] : -kInf));
 
   float S, T;
   int n;
-  score_row<THREADS, !GRAD>(x, n8, xt, g.sc, M, own, S, T, n);
+  score_row<THREADS, !GRAD>(x, src, n8, xt, g.sc, M, own, S, T, n);
   if (lane == 0) s.s.S[wv] = S, s.s.T[wv] = T, s.s.n[wv] = n;
   if (GRAD) opaque_row(x);
   __syncthreads();
@@ -121,35 +130,44 @@ __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : 8) void token_kernel(TokenA
   if (base == 0.f && slope == 0.f) {  // a row that counts for nothing: zeros, not 0 * NaN
     zero_grad<FMT, THREADS>(dst, V);
   } else {
-    const float ref = ExpScale::ref(M);
-    auto put = [&](auto far, auto flat) {
-      constexpr bool kFar = decltype(far)::value, kFlat = decltype(flat)::value;
-      const float R = ref * g.sc.kf;
+    const float ref = uniform_f(ExpScale::ref(M));
+    // (an exponent of -inf, a masked logit's, is taken as -1000: 0 times it is 0)
+    auto sloped = [&](float y) { return __builtin_amdgcn_exp2f(y) * fmaf(slope, fmaxf(y, -1000.f), base); };
+    auto put = [&](auto flat) {
+      constexpr bool kFlat = decltype(flat)::value;
       auto one = [&](float v) {
-        const float y = score_arg<kFar>(g.sc, v, ref, R), e = __builtin_amdgcn_exp2f(y);
-        return kFlat ? e * base : e * fmaf(slope, fmaxf(y, -1000.f), base);
+        const float y = near_arg(g.sc, v, ref);
+        return kFlat ? __builtin_amdgcn_exp2f(y) * base : sloped(y);
       };
 #pragma unroll
       for (int c = 0; c < kRowChunks; ++c) {
         if (c > 0 && c * THREADS >= (int)n8) break;
         float f[kRowChunk];
         if (!kFlat) x[c].opaque();
-        x[c].template get<kFar>(f);
+        x[c].get(f);
 #pragma unroll
         for (int e = 0; e < kRowChunk; ++e) f[e] = one(f[e]);
         const uint32_t b = c * THREADS + t;
         if ((c + 1) * THREADS <= (int)n8) store_chunk<FMT>(dst, b, f);
         else if (b < n8) store_chunk<FMT>(dst, b, f);
       }
-      if (tail >= 0) store_logit<FMT>(dst, tail, one(xt));
     };
     if (g.sc.near(M)) {
-      if (slope == 0.f) put(BoolConst<false>(), BoolConst<true>());
-      else put(BoolConst<false>(), BoolConst<false>());
-    } else {
-      if (slope == 0.f) put(BoolConst<true>(), BoolConst<true>());
-      else put(BoolConst<true>(), BoolConst<false>());
+      if (slope == 0.f) put(BoolConst<true>());
+      else put(BoolConst<false>());
+    } else {  // far from 0, from memory
+#pragma unroll 1
+      for (uint32_t b = t; b < n8; b += THREADS) {
+        Chunk<FMT> y;
+        float f[kRowChunk];
+        y.load_whole(src, b);
+        y.get(f);
+#pragma unroll
+        for (int e = 0; e < kRowChunk; ++e) f[e] = sloped(score_arg(g.sc, f[e], ref));
+        store_chunk<FMT>(dst, b, f);
+      }
     }
+    if (tail >= 0) store_logit<FMT>(dst, tail, sloped(score_arg(g.sc, xt, ref)));
   }
   __syncthreads();  // the row's own stores come before the token's
   if (t == 0 && !zero) store_logit<FMT>(dst, id, (float)grad_x);

@@ -51,6 +51,7 @@ struct TopArgs {
 };
 
 constexpr int kBins = 256;
+constexpr int kFewMaxima = 4;   // lanes' maxima that are found one after the other
 constexpr int kGroups = 4;      // maxima a lane keeps: of its chunks c, c % 4
 // Lowest bit of a floor that is decided: the formats' last, f32's to 2^-15 of a value.
 template <int FMT>
@@ -152,14 +153,17 @@ RWKV7_DEV int select_digit(const char *src, int V, int &need, TopLds &s, D digit
 }
 
 struct NoLds {};
+template <int THREADS>
 struct TopScoreLds : ScoreLds {
   double log_S;
+  float zx;                        // the token's logit
+  uint32_t own[kGroups][THREADS];  // the lanes' maxima wait here while the row is summed: registers are short
 };
 
 template <int FMT, int THREADS, bool SCORE>
 __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : THREADS == 256 ? 7 : 8) void top_kernel(TopArgs g) {
   __shared__ TopLds s;
-  __shared__ std::conditional_t<SCORE, TopScoreLds, NoLds> sco;
+  __shared__ std::conditional_t<SCORE, TopScoreLds<THREADS>, NoLds> sco;
   constexpr int kWaves = THREADS / kWave;
   const int t = threadIdx.x, lane = t & 63, wv = t >> 6, V = g.V, k = g.k;
   const uint32_t n8 = (uint32_t)V / kRowChunk;
@@ -185,20 +189,44 @@ __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : THREADS == 256 ? 7 : 8) voi
   // the lane's largest, by groups of chunks (-inf also for none: a floor may be
   // too low, never too high)
   uint32_t own[kGroups];
-  float m = -kInf;
-  {
-    RowMax<FMT> most[kGroups];
+  float m;
+  auto lanes_most = [&](auto most0) {
+    decltype(most0) most[kGroups];
 #pragma unroll
     for (int c = 0; c < kRowChunks; ++c) most[c % kGroups].add(x[c]);
+    m = -kInf;
+    bool clean = true;
 #pragma unroll
     for (int i = 0; i < kGroups; ++i) {
       const float mg = i == 0 ? fmaxf(most[0].value(), xt) : most[i].value();
       own[i] = mg > -kInf ? top_key(mg) : 0u;
       m = fmaxf(m, mg);
+      if constexpr (SCORE) clean = clean && most[i].clean();
     }
+    return clean;
+  };
+  if constexpr (SCORE) {
+    if (__ballot(!lanes_most(PairMax<FMT>()))) {
+      opaque_row(x);
+      struct Exact : RowMax<FMT> {
+        RWKV7_DEV bool clean() const { return true; }
+      };
+      lanes_most(Exact());
+    }
+  } else {
+    lanes_most(RowMax<FMT>());
   }
   opaque_row(x);
   auto wave_floor = [&](int r) {
+    if (r <= kFewMaxima) {  // one after the other
+      float rest = m, most;
+      do {
+        most = wave_max(rest);
+        r -= __popcll(__ballot(rest == most));
+        rest = rest == most ? -kInf : rest;
+      } while (r > 0 && most > -kInf);
+      return most > -kInf ? top_key(most) : 0u;
+    }
     const uint32_t lo = own[0] > own[1] ? own[0] : own[1], hi = own[2] > own[3] ? own[2] : own[3], one[1] = {lo > hi ? lo : hi};
     return r > 16 ? rth_key<kFloorLow<FMT>>(own, r) : rth_key<kFloorLow<FMT>>(one, r);
   };
@@ -212,23 +240,27 @@ __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : THREADS == 256 ? 7 : 8) voi
   m = wave_max(m);
   if constexpr (SCORE) {
     if (lane == 0) s.m[wv] = m;
+    if (t == 0) sco.zx = zx;
+#pragma unroll
+    for (int i = 0; i < kGroups; ++i) sco.own[i][t] = own[i];
     __syncthreads();
     const float M = uniform_f(wave_max(lane < kWaves ? s.m[lane] : -kInf));
     float S, T;
     int n;
-    score_row<THREADS, true>(x, n8, xt, g.sc, M, m, S, T, n);
+    score_row<THREADS, true>(x, src, n8, xt, g.sc, M, m, S, T, n);
     opaque_row(x);
     if (lane == 0) sco.S[wv] = S, sco.T[wv] = T, sco.n[wv] = n;
+#pragma unroll
+    for (int i = 0; i < kGroups; ++i) own[i] = sco.own[i][t];
   } else {
     const float sum = sum_row<THREADS, true, true>(x, src, n8, xt, g.sc, m, [](int, Chunk<FMT> &) {});
     if (lane == 0) s.m[wv] = m, s.sum[wv] = sum;
   }
   __syncthreads();
   if constexpr (SCORE) {
-    if (wv == kWaves - 1) {  // (the alternatives read log_S barriers later)
-      const float M = uniform_f(wave_max(lane < kWaves ? s.m[lane] : -kInf));
-      const RowScore r = row_score(join_sums<kWaves>(sco, g.sc, M, lane));
-      if (lane == 0) sco.log_S = r.log_S, g.logp[row] = (float)log_prob(r, g.a, zx, M), g.entropy[row] = (float)r.H;
+    if (wv == kWaves - 1) {  // (the alternatives read log_S barriers later; the rest of it waits for the end)
+      const double log_S = row_score(join_sums<kWaves>(sco, g.sc, uniform_f(wave_max(lane < kWaves ? s.m[lane] : -kInf)), lane)).log_S;
+      if (lane == 0) sco.log_S = log_S;
     }
   }
 
@@ -267,6 +299,7 @@ __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : THREADS == 256 ? 7 : 8) voi
 #pragma unroll
     for (int c = 0; c < kRowChunks; ++c) {
       if (c > 0 && c * THREADS >= (int)n8) break;
+      if (SCORE && !__ballot(own[c % kGroups] >= fl)) continue;  // (few alternatives: most waves have none in most chunks)
       float v[kRowChunk];
       x[c].get(v);
 #pragma unroll
@@ -306,8 +339,8 @@ __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : THREADS == 256 ? 7 : 8) voi
     n = k;
   }
 
-  // keys from `low` up, in bins of 2^shift, the highest first
   const float mm = wave_max(lane < kWaves ? s.m[lane] : -kInf);
+  // keys from `low` up, in bins of 2^shift, the highest first
   const uint32_t low = fl, range = max(top_key(mm), 1u) - low;
   const int shift = max(0, 24 - __clz((int)(range | 1u)));
   auto bin_of = [&](u64 c) { return kBins - 1 - (int)(((uint32_t)(c >> 32) - low) >> shift); };
@@ -343,7 +376,12 @@ __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : THREADS == 256 ? 7 : 8) voi
       else static_cast<uint16_t *>(g.val)[row * k + rank] = reinterpret_cast<const uint16_t *>(src)[id];
     }
   }
-  if (!SCORE && wv == 0) {
+  if constexpr (SCORE) {
+    if (wv == kWaves - 1) {
+      const RowScore r = row_score(join_sums<kWaves>(sco, g.sc, mm, lane));
+      if (lane == 0) g.logp[row] = (float)log_prob(r, g.a, sco.zx, mm), g.entropy[row] = (float)r.H;
+    }
+  } else if (wv == 0) {
     const float mw = lane < kWaves ? s.m[lane] : -kInf;
     const double S = wave_sum_d(lane < kWaves ? (double)s.sum[lane] * g.sc.part(mw, mm) : 0.0);
     // (S is 0 where there is nothing but -inf)
