@@ -86,15 +86,10 @@ __global__ __launch_bounds__(kNormThreads<WAVES>) void norm_kernel(NormArgs g) {
   const int t = threadIdx.x % T, C = g.C;
   const float inv = 1.f / (float)C;
   int n[NC], turn = 0;
-  float w[NC][8], b[NC][8];
 #pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    n[c] = part_len(c * T + t, C);
-    load_part_f<WFMT>(w[c], g.w, c * T + t, n[c]);
-    load_part_f<WFMT>(b[c], g.b, c * T + t, n[c]);
-  }
+  for (int c = 0; c < NC; ++c) n[c] = part_len(c * T + t, C);
 #pragma unroll 1
-  for (int64_t row = (int64_t)blockIdx.x * kNormRows<WAVES> + threadIdx.x / T; row < g.N;
+  for (int64_t row = (int64_t)blockIdx.x * kNormRows<WAVES> + __builtin_amdgcn_readfirstlane(threadIdx.x / T); row < g.N;
        row += (int64_t)gridDim.x * kNormRows<WAVES>) {
     const char *src = static_cast<const char *>(g.x) + row * g.ldx * kLogitBytes<FMT>;
     char *dst = static_cast<char *>(g.y) + row * C * kLogitBytes<FMT>;
@@ -146,10 +141,12 @@ __global__ __launch_bounds__(kNormThreads<WAVES>) void norm_kernel(NormArgs g) {
     const float rs = (float)r;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      float d[8];
+      float d[8], w[8], b[8];  // (from the CU's L1, which holds them: in registers they cost the row's own waves)
+      load_part_f<WFMT>(w, g.w, c * T + t, n[c]);
+      load_part_f<WFMT>(b, g.b, c * T + t, n[c]);
       diff(c, s, m, d);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) d[e] = fmaf((d[e] - shift) * rs, w[c][e], b[c][e]);
+      for (int e = 0; e < 8; ++e) d[e] = fmaf((d[e] - shift) * rs, w[e], b[e]);
       store_part<FMT>(dst, c * T + t, n[c], d);
     }
     if (t == 0 && g.mean) {
@@ -163,7 +160,7 @@ template <int FMT, int WFMT, int WAVES, int NC>
 __global__ __launch_bounds__(kNormThreads<WAVES>) void norm_grad_kernel(NormGradArgs g) {
   __shared__ RowReduce<WAVES, 3> red;
   constexpr int T = WAVES * kWave, kRows = kNormRows<WAVES>;
-  const int t = threadIdx.x % T, sub = threadIdx.x / T, C = g.C;
+  const int t = threadIdx.x % T, sub = __builtin_amdgcn_readfirstlane(threadIdx.x / T), C = g.C;
   const float inv = 1.f / (float)C;
   int n[NC], turn = 0;
   float w[NC][8], dw[NC][8], db[NC][8];
@@ -174,15 +171,29 @@ __global__ __launch_bounds__(kNormThreads<WAVES>) void norm_grad_kernel(NormGrad
 #pragma unroll
     for (int e = 0; e < 8; ++e) dw[c][e] = db[c][e] = 0.f;
   }
-#pragma unroll 1
-  for (int64_t row = (int64_t)blockIdx.x * kRows + sub; row < g.N; row += (int64_t)gridDim.x * kRows) {
+  // the next row is on its way while one is worked on (but of 8 and 16 waves, which have no registers for it)
+  constexpr bool kAhead = WAVES <= 4;
+  Chunk<FMT> xn[NC], yn[NC];
+  float rstd_n, mean_n;
+  auto fetch = [&](int64_t row) {
     const char *xs = static_cast<const char *>(g.x) + row * g.ldx * kLogitBytes<FMT>;
     const char *ys = static_cast<const char *>(g.dy) + row * g.lddy * kLogitBytes<FMT>;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) load_part(xn[c], xs, c * T + t, n[c]), load_part(yn[c], ys, c * T + t, n[c]);
+    rstd_n = g.rstd[row], mean_n = g.mean[row];
+  };
+  const int64_t step = (int64_t)gridDim.x * kRows;
+  int64_t row = (int64_t)blockIdx.x * kRows + sub;
+  if (kAhead && row < g.N) fetch(row);
+#pragma unroll 1
+  for (; row < g.N; row += step) {
+    if (!kAhead) fetch(row);
     char *dst = static_cast<char *>(g.dx) + row * C * kLogitBytes<FMT>;
     Chunk<FMT> x[NC], y[NC];
 #pragma unroll
-    for (int c = 0; c < NC; ++c) load_part(x[c], xs, c * T + t, n[c]), load_part(y[c], ys, c * T + t, n[c]);
-    const float rstd = g.rstd[row], mean = g.mean[row];
+    for (int c = 0; c < NC; ++c) x[c] = xn[c], y[c] = yn[c];
+    const float rstd = rstd_n, mean = mean_n;
+    if (kAhead && row + step < g.N) fetch(row + step);
     const float s = rstd < 0x1p-50f ? kFarScale : 1.f, m = mean * s, rs = rstd * (1.f / s);
     float a[3] = {0.f, 0.f, 0.f};  // sums of g, g (x - m) and x - m
 #pragma unroll
@@ -224,29 +235,35 @@ __global__ __launch_bounds__(kNormThreads<WAVES>) void norm_grad_kernel(NormGrad
       store_part<FMT>(dst, c * T + t, n[c], d);
     }
   }
-  // the workgroup's sums, its rows' waves one after the other
+  // the workgroup's sums: its waves' added by one wave a chunk
   float *part = g.part + (int64_t)blockIdx.x * 2 * C;
   if constexpr (kRows > 1) {
-    __shared__ float sum[2][NC * 8][T];
-    for (int i = 0; i < kRows; ++i) {
-      if (sub == i) {
+    static_assert(NC <= kRows);
+    __shared__ float sum[2][kRows][NC * 8][T];
 #pragma unroll
-        for (int c = 0; c < NC; ++c)
+    for (int c = 0; c < NC; ++c)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            float *p = &sum[0][8 * c + e][t], *q = &sum[1][8 * c + e][t];
-            if (i > 0) dw[c][e] += *p, db[c][e] += *q;
-            if (i < kRows - 1) *p = dw[c][e], *q = db[c][e];
-          }
+      for (int e = 0; e < 8; ++e) sum[0][sub][8 * c + e][t] = dw[c][e], sum[1][sub][8 * c + e][t] = db[c][e];
+    __syncthreads();
+    if (sub >= NC) return;
+    const int len = part_len(sub * T + t, C);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        v[e] = sum[k][0][8 * sub + e][t];
+#pragma unroll
+        for (int i = 1; i < kRows; ++i) v[e] += sum[k][i][8 * sub + e][t];
       }
-      __syncthreads();
+      store_part<1>(part + k * C, sub * T + t, len, v);
     }
-    if (sub != kRows - 1) return;
-  }
+  } else {
 #pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    store_part<1>(part, c * T + t, n[c], dw[c]);
-    store_part<1>(part + C, c * T + t, n[c], db[c]);
+    for (int c = 0; c < NC; ++c) {
+      store_part<1>(part, c * T + t, n[c], dw[c]);
+      store_part<1>(part + C, c * T + t, n[c], db[c]);
+    }
   }
 }
 
@@ -273,12 +290,10 @@ __global__ __launch_bounds__(kSumWaves *kWave) void norm_sum_kernel(const float 
   else static_cast<uint16_t *>(out)[at] = f_to_u16((float)a, fmt == 2);
 }
 
-constexpr int64_t kGradBlocks = 512;
-inline int rows_at_once(int dtype, int C) { return C <= (dtype == 1 ? 1024 : 2048) ? 4 : 1; }
+// Workgroups of the gradient: as many as a CU holds, their sums [2][C] each being written and read once more.
 inline int64_t grad_blocks(int dtype, int64_t N, int C) {
-  const int r = rows_at_once(dtype, C);
-  const int64_t n = (N + r - 1) / r;
-  return n < kGradBlocks ? n : kGradBlocks;
+  const int64_t n = C <= (dtype == 1 ? 1024 : 2048) ? (N + kNormRows<1> - 1) / kNormRows<1> : N, most = C <= 8192 ? 512 : 256;
+  return n < most ? n : most;
 }
 
 // f(WAVES, NC) for rows of C channels
@@ -322,13 +337,12 @@ extern "C" int rwkv7_layer_norm_forward(const void *x, int32_t dtype, int64_t ld
   if (!(eps >= 1e-30 && eps <= 1e30)) return RWKV7_EINVAL;
   if (N < 1 || C < 1 || C > kNormMaxC || ldx < C) return RWKV7_ESHAPE;
   const NormArgs g = {x, weight, bias, ldx, y, mean, rstd, N, C, eps};
-  const int64_t n = (N + rows_at_once(dtype, C) - 1) / rows_at_once(dtype, C);
-  const int grid = (int)(n < 1024 ? n : 1024);
   with_types(dtype, weight_dtype, [&](auto f, auto wf) {
     with_shape<decltype(f)::value>(C, [&](auto waves, auto nc) {
       constexpr int W = decltype(waves)::value;
+      const int64_t n = (N + kNormRows<W> - 1) / kNormRows<W>;
       norm_kernel<decltype(f)::value, decltype(wf)::value, W, decltype(nc)::value>
-          <<<grid, kNormThreads<W>, 0, static_cast<hipStream_t>(stream)>>>(g);
+          <<<(int)(n < (1 << 20) ? n : 1 << 20), kNormThreads<W>, 0, static_cast<hipStream_t>(stream)>>>(g);
     });
   });
   RWKV7_CHECK_LAUNCH();
