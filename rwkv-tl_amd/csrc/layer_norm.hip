@@ -126,8 +126,9 @@ __global__ __launch_bounds__(kNormThreads<WAVES>) void norm_kernel(NormArgs g) {
       for (int c = 0; c < NC; ++c) {
         float d[8];
         diff(c, s, m, d);
+        a[0] += ((d[0] + d[1]) + (d[2] + d[3])) + ((d[4] + d[5]) + (d[6] + d[7]));
 #pragma unroll
-        for (int e = 0; e < 8; ++e) a[0] += d[e], a[1] = fmaf(d[e], d[e], a[1]);
+        for (int e = 0; e < 8; ++e) a[1] = fmaf(d[e], d[e], a[1]);
       }
       row_reduce(red, turn, a);
       shift = a[0] * inv;

@@ -263,9 +263,10 @@ struct BoolConst {
 struct ExpScale {
   float kf;    // a log2(e) in float
   double k;    // the same in 64 bits
+  double more; // k / kf - 1
   static ExpScale of(double a) {
     const double k = a * 1.4426950408889634;
-    return {(float)k, k};
+    return {(float)k, k, k / (double)(float)k - 1.0};
   }
   // m: -inf for none, which any finite reference serves
   static RWKV7_DEV float ref(float m) { return m > -kInf ? m : 0.f; }

@@ -64,6 +64,7 @@ struct ScoreLds {
 // which lie `at` (their own value at M) above y.
 struct RowSums {
   double S, T, n, at;
+  double slope;  // ln 2 times what log2(e) / temperature has over its float, of itself
   float M;
 };
 
@@ -152,27 +153,38 @@ RWKV7_DEV RowSums join_sums(const ScoreLds &s, const ExpScale &sc, float M, int 
   r.M = M;
   const float ref = ExpScale::ref(M);
   r.at = (double)score_arg(sc, ref, ref);
+  r.slope = kLn2 * sc.more;
   return r;
 }
 
 struct RowScore {
   double log_S;  // log sum exp(a (z - M))
   double H;
-  double total;  // sum of the exponents' powers as score_arg forms them, and its logarithm
-  double log_total;
   bool none;     // every logit is -inf
 };
 
 RWKV7_DEV RowScore row_score(const RowSums &r) {
   RowScore o;
   o.none = r.M == -kInf && r.S == 0.0;
-  const double up = exp2_d(-r.at), S1 = r.S * up, T1 = up * (r.T - r.at * r.S), S = r.n + S1;
+  // The exponents' factor is a float, 1.3e-8 less than log2(e): at a mean exponent of -10 a
+  // bias of 1e-7 in S, which T makes up for. (H would need a third sum; its two terms are
+  // left as they are together, off by that 1.3e-8 times the variance of log q.)
+  const double up = exp2_d(-r.at), T1 = up * (r.T - r.at * r.S), more = r.slope * T1;
+  const double S1 = fma(r.S, up, more), S = r.n + S1, mean = T1 * rcp_d(S - more);
   // (NaN among the logits makes the sum NaN)
   o.log_S = o.none ? 0.0 : S == S && r.M < kInf ? log_n_plus(r.n, S1) : __builtin_nan("");
-  o.H = o.none ? 0.0 : o.log_S - kLn2 * T1 * rcp_d(S);
-  o.total = S * exp2_d(r.at);
-  o.log_total = o.log_S + kLn2 * r.at;
+  o.H = o.none ? 0.0 : o.log_S - (kLn2 + r.slope) * mean;
   return o;
+}
+
+// For the gradient, without a logarithm: the sum of the powers as score_arg() forms them, and
+// H less its logarithm, which is the sums' quotient alone. (total is NaN where log_S is.)
+struct RowCentre {
+  double total, centre;
+};
+RWKV7_DEV RowCentre row_centre(const RowSums &r) {
+  const double one = exp2_frac(r.at), T1 = r.T - r.at * r.S, S = fma(r.n, one, r.S);  // (|at| <= 2^-4)
+  return {r.M < kInf ? fma(r.slope, T1, S) : __builtin_nan(""), -(kLn2 + r.slope) * T1 * rcp_d(S) - kLn2 * r.at};
 }
 
 // log q of a logit

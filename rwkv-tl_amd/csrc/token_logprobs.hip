@@ -106,26 +106,34 @@ __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : 8) void token_kernel(TokenA
   if (GRAD) opaque_row(x);
   __syncthreads();
 
-  double grad_x = 0.0;
-  bool zero = false;
-  if (wv == 0) {
+  // What the row's gradient needs of the sums, by one wave that the others wait for (no
+  // more than that: beside the row there are no registers for it, and a spilled one is a
+  // trip to memory); all else when the row is stored.
+  if (GRAD && wv == 0) {
+    const RowSums r = join_sums<kWaves>(s.s, g.sc, M, lane);
+    const bool zero = (up == 0.f && up_h == 0.f) || (M == -kInf && r.S == 0.0);
+    // log q = ln 2 y - log total
+    const RowCentre o = row_centre(r);
+    const double f = -g.a * rcp_d(o.total), base = f * ((double)up + (double)up_h * o.centre), slope = f * kLn2 * (double)up_h;
+    if (lane == 0) s.base = zero ? 0.f : (float)base, s.slope = zero ? 0.f : (float)slope;
+  }
+  if (GRAD) __syncthreads();
+  auto outputs = [&]() {  // by one wave
     const RowScore r = row_score(join_sums<kWaves>(s.s, g.sc, M, lane));
     const double lp = log_prob(r, g.a, zx, M);
     if (lane == 0 && g.logp) g.logp[row] = (float)lp;
     if (lane == 0 && g.entropy) g.entropy[row] = (float)r.H;
-    if (GRAD) {
-      zero = r.none || (up == 0.f && up_h == 0.f);
-      const double f = g.a * rcp_d(r.total);
-      const double q = lp > -__builtin_inf() ? exp2_d(1.4426950408889634 * lp) : lp == lp ? 0.0 : lp;
-      grad_x = g.a * ((double)up * one_minus_exp(lp) - (q != 0.0 ? q * (double)up_h * (lp + r.H) : 0.0));
-      if (lane == 0) {
-        s.base = zero ? 0.f : (float)(-f * ((double)up + (double)up_h * (r.H - r.log_total)));
-        s.slope = zero ? 0.f : (float)(-f * kLn2 * (double)up_h);
-      }
+    if (GRAD && !(r.none || (up == 0.f && up_h == 0.f))) {
+      double grad = g.a * (double)up * one_minus_exp(lp);
+      if (up_h != 0.f && lp != -__builtin_inf())  // (NaN stays NaN)
+        grad -= g.a * (double)up_h * (lp == lp ? exp2_d(1.4426950408889634 * lp) : lp) * (lp + r.H);
+      if (lane == 0) store_logit<FMT>(dst, id, (float)grad);
     }
+  };
+  if (!GRAD) {
+    if (wv == 0) outputs();
+    return;
   }
-  if (!GRAD) return;
-  __syncthreads();
   const float base = uniform_f(s.base), slope = uniform_f(s.slope);
   if (base == 0.f && slope == 0.f) {  // a row that counts for nothing: zeros, not 0 * NaN
     zero_grad<FMT, THREADS>(dst, V);
@@ -170,7 +178,7 @@ __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : 8) void token_kernel(TokenA
     if (tail >= 0) store_logit<FMT>(dst, tail, sloped(score_arg(g.sc, xt, ref)));
   }
   __syncthreads();  // the row's own stores come before the token's
-  if (t == 0 && !zero) store_logit<FMT>(dst, id, (float)grad_x);
+  if (wv == 0) outputs();
 }
 
 template <int FMT, int THREADS>

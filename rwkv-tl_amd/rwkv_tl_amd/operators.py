@@ -255,18 +255,16 @@ def _distill_autograd(logits, top_val, top_idx, lse=None, temperature=1.0):
     return _DistillLoss.apply(logits, top_val, top_idx, lse, temperature)
 
 
-def _op(name: str, direct: Callable, plain: bool, *args):
-    """The kernel itself, or the operator below autograd (for tracing and batched tensors)."""
-    if plain:
-        return direct(*args)
+def _below(op: Callable, *args):
+    """The operator below autograd (for tracing and batched tensors)."""
     with torch._C._AutoDispatchBelowAutograd():
-        return getattr(torch.ops.rwkv_tl, name)(*args)
+        return op(*args)
 
 
-def _backward_op(name: str, direct: Callable, grad: Tensor, *args):
-    # (a gradient that is to be differentiated goes through the operator, which refuses)
-    plain = _plain(grad) and not torch.is_grad_enabled()
-    return (direct if plain else getattr(torch.ops.rwkv_tl, name))(*args)
+def _direct(grad: Tensor) -> bool:
+    """Whether a gradient goes straight to its kernel (one that is to be differentiated goes
+    through the operator, which refuses)."""
+    return _plain(grad) and not torch.is_grad_enabled()
 
 
 class _Embed(torch.autograd.Function):
@@ -274,24 +272,28 @@ class _Embed(torch.autograd.Function):
     def forward(ctx, weight, tokens, scale):
         ctx.save_for_backward(tokens)
         ctx.vocab, ctx.scale = weight.shape[0], scale
-        return _op("embed", STEP_OPS["embed"][1], _plain(weight), weight, tokens, scale)
+        return K.embed(weight, tokens, scale=scale) if _plain(weight) else _below(torch.ops.rwkv_tl.embed, weight, tokens, scale)
 
     @staticmethod
     def backward(ctx, grad):
-        args = (grad, *ctx.saved_tensors, ctx.vocab, ctx.scale)
-        return _backward_op("embed_backward", STEP_OPS["embed_backward"][1], grad, *args), None, None
+        f = T.embed_backward_checked if _direct(grad) else torch.ops.rwkv_tl.embed_backward
+        return f(grad, *ctx.saved_tensors, ctx.vocab, ctx.scale), None, None
 
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        y, mean, rstd = _op("layer_norm_forward", STEP_OPS["layer_norm_forward"][1], _plain(x), x, weight, bias, eps)
+        if _plain(x):
+            y, mean, rstd = K.layer_norm_forward(x, weight, bias, eps=eps)
+        else:
+            y, mean, rstd = _below(torch.ops.rwkv_tl.layer_norm_forward, x, weight, bias, eps)
         ctx.save_for_backward(x, weight, mean, rstd)
         return y
 
     @staticmethod
     def backward(ctx, grad):
-        return *_backward_op("layer_norm_backward", K.layer_norm_backward, grad, grad, *ctx.saved_tensors), None
+        f = T.layer_norm_backward_checked if _direct(grad) else torch.ops.rwkv_tl.layer_norm_backward
+        return *f(grad, *ctx.saved_tensors), None
 
 
 class _TokenLogprobs(torch.autograd.Function):
@@ -300,15 +302,17 @@ class _TokenLogprobs(torch.autograd.Function):
         ctx.save_for_backward(logits, tokens)
         ctx.temperature = temperature
         ctx.set_materialize_grads(False)
-        return _op("token_logprobs", STEP_OPS["token_logprobs"][1], _plain(logits), logits, tokens, temperature)
+        if _plain(logits):
+            return K.token_logprobs(logits, tokens, temperature=temperature)
+        return _below(torch.ops.rwkv_tl.token_logprobs, logits, tokens, temperature)
 
     @staticmethod
     def backward(ctx, grad_logprob, grad_entropy):
         some = grad_logprob if grad_logprob is not None else grad_entropy
         if some is None:
             return None, None, None
-        args = (grad_logprob, grad_entropy, *ctx.saved_tensors, ctx.temperature)
-        return _backward_op("token_logprobs_backward", K.token_logprobs_backward, some, *args), None, None
+        f = K.token_logprobs_backward if _direct(some) else torch.ops.rwkv_tl.token_logprobs_backward
+        return f(grad_logprob, grad_entropy, *ctx.saved_tensors, ctx.temperature), None, None
 
 
 def _once(name: str):

@@ -97,8 +97,8 @@ def embed_backward(grad: Tensor, tokens: Tensor, vocab: int, *, scale: float = 1
     """Gradient of ``embed`` to its table: ``[vocab, C]`` of the type of ``grad [..., C]``,
     ``scale`` times the sum of each token's rows (in 32 bits, rounded once), zeros
     where there is none."""
-    code = _check(grad, "grad")
-    N = _check_tokens(tokens)
+    _check(grad, "grad")
+    _check_tokens(tokens)
     if grad.ndim != tokens.ndim + 1 or grad.shape[:-1] != tokens.shape:
         raise ValueError(f"grad must be [{', '.join(map(str, (*tokens.shape, 'C')))}], got {tuple(grad.shape)}")
     C = grad.shape[-1]
@@ -107,6 +107,12 @@ def embed_backward(grad: Tensor, tokens: Tensor, vocab: int, *, scale: float = 1
     _check_table(vocab, C)
     scale = _factor(scale)
     _same_device(grad, tokens)
+    return embed_backward_checked(grad, tokens, vocab, scale)
+
+
+def embed_backward_checked(grad: Tensor, tokens: Tensor, vocab: int, scale: float) -> Tensor:
+    """``embed_backward`` of what autograd hands on: shapes, types and device are the forward pass's."""
+    code, N, C = DTYPES[grad.dtype], tokens.numel(), grad.shape[-1]
     with _lib.device_of(grad):
         out = torch.empty(vocab, C, dtype=grad.dtype, device=grad.device)
         if N:
@@ -181,14 +187,21 @@ def _norm_bytes(code: int, N: int, C: int) -> int:
 def layer_norm_backward(grad_y: Tensor, x: Tensor, weight: Tensor, mean: Tensor, rstd: Tensor) -> tuple[Tensor, Tensor, Tensor]:
     """Gradients of ``layer_norm_forward`` to ``(x, weight, bias)`` under ``grad_y [..., C]`` of
     x's type, from the input and the statistics that the forward pass returned."""
-    code, wcode = _check_norm(x, weight, None)
-    lead, C = x.shape[:-1], x.shape[-1]
+    _check_norm(x, weight, None)
+    lead = x.shape[:-1]
     if grad_y.shape != x.shape or grad_y.dtype is not x.dtype:
         raise ValueError(f"grad_y must be {x.dtype} {tuple(x.shape)}, got {grad_y.dtype} {tuple(grad_y.shape)}")
     for t, name in ((mean, "mean"), (rstd, "rstd")):
         if t.shape != lead or t.dtype is not torch.float32:
             raise ValueError(f"{name} must be float32 {tuple(lead)}, got {t.dtype} {tuple(t.shape)}")
     _same_device(x, grad_y, weight, mean, rstd)
+    return layer_norm_backward_checked(grad_y, x, weight, mean, rstd)
+
+
+def layer_norm_backward_checked(grad_y: Tensor, x: Tensor, weight: Tensor, mean: Tensor, rstd: Tensor):
+    """``layer_norm_backward`` of what autograd hands on: shapes, types and device are the forward pass's."""
+    code, wcode = DTYPES[x.dtype], DTYPES[weight.dtype]
+    lead, C = x.shape[:-1], x.shape[-1]
     with _lib.device_of(x):
         dev = x.device
         gx = torch.empty(*lead, C, dtype=x.dtype, device=dev)
