@@ -18,6 +18,16 @@
 // else belongs to the rows that begin there, so that eight rows are always in flight. A
 // row of more than 32 positions is cut into units; the one that arrives last adds up
 // the units' sums.
+//
+// Measured (kernel trace, us; tokens with frequencies of 1 / rank; a large copy moves 5.09
+// TB/s here, a large fill 6.9-7.9). 8192 tokens x 1024 of 65536 bf16: sort and fill 20
+// (6.7 TB/s), sums 11; 16384 x 2048: 40 and 36, the second beside the first's lines on their
+// way from the caches; 509 x 768 of 20011 f32: 12 and 5. Sort alone 6.5 for one token, 13
+// for 16384; past those that its threads hold (16384) 2.2 per 1024. Lookup of 16384 x 2048
+// bf16 28 (4.8 TB/s), of 16 2.8. Tried: a wave a row in the sort's workgroups, zeros and sums
+// included (the table's rows of 16384 x 2048: 179; the longest rows' chains bound it);
+// units of 64 positions (sums of 8192 x 1024 10.0 -> 11.9); the sums of a unit stored 32
+// bytes a thread (27 instead of 10: each 4-byte store past the caches is a trip of its own).
 #include "logits_rows.h"
 #include "rwkv7_kernels.h"
 
@@ -118,7 +128,7 @@ constexpr int kUnit = 32;        // positions of a unit, while a row has no more
 constexpr int kMaxUnits = 128;
 constexpr int kRun = 8;          // positions of the list, and rows in flight, of a workgroup
 constexpr int kJoin = 4;         // units' sums in flight
-constexpr int kFillGroups = 1024;
+constexpr int kFillGroups = 1024, kFillBytes = 1 << 16;  // workgroups of the fill at most, and bytes of each at least
 constexpr int kHeld = 16;        // tokens that a thread of the sort keeps, where there are no more
 
 // What begins at a position of the list.
@@ -161,6 +171,7 @@ struct SortLds {
   int few[kSortRows];   // of a row of few: in `keys`
   int next[kSortRows];  // where its next one goes there
   int hot[kSortRows];   // rows of more than kFew
+  int per[kSortRows];   // and the length of their units
   int n_hot, less;
   int wave[kSortWaves];
   uint32_t keys[kSortRows * kFew];  // row and position
@@ -188,8 +199,8 @@ RWKV7_DEV int sort_scan(int v, int *wave, int &total) {
   return before + inc - v;
 }
 
-RWKV7_DEV void fill_zeros(char *out, int64_t bytes, int group) {
-  const int64_t n16 = bytes / 16, step = (int64_t)kFillGroups * kSortThreads;
+RWKV7_DEV void fill_zeros(char *out, int64_t bytes, int group, int groups) {
+  const int64_t n16 = bytes / 16, step = (int64_t)groups * kSortThreads;
   const uint32_t zero[4] = {0u, 0u, 0u, 0u};
 #pragma unroll 4
   for (int64_t i = (int64_t)group * kSortThreads + threadIdx.x; i < n16; i += step) __builtin_memcpy(out + 16 * i, zero, 16);
@@ -203,7 +214,7 @@ __global__ __launch_bounds__(kSortThreads, 8) void embed_sort_kernel(EmbedGradAr
   __shared__ SortLds s;
   const int t = threadIdx.x, lane = t & 63, wv = t >> 6, g = blockIdx.x, G = 1 << a.log_g;
   if (g >= G) {
-    fill_zeros(static_cast<char *>(a.out), (int64_t)a.V * a.C * ELEM, g - G);
+    fill_zeros(static_cast<char *>(a.out), (int64_t)a.V * a.C * ELEM, g - G, gridDim.x - G);
     return;
   }
   const int rows = g < a.V ? ((a.V - 1 - g) >> a.log_g) + 1 : 0;  // <= kSortRows
@@ -260,7 +271,10 @@ __global__ __launch_bounds__(kSortThreads, 8) void embed_sort_kernel(EmbedGradAr
   const int at = sort_scan(c, s.wave, all) + s.less;
   const int few = sort_scan(c <= kFew ? c : 0, s.wave, n_few);
   if (t < rows) s.at[t] = at, s.few[t] = s.next[t] = few;
-  if (c > kFew) s.hot[atomicAdd(&s.n_hot, 1)] = t;
+  if (c > kFew) {
+    s.hot[atomicAdd(&s.n_hot, 1)] = t;
+    s.per[t] = unit_len(c);
+  }
   if (c > kUnit)
     for (int b = 0; b < a.blocks; ++b) a.arrived[(int64_t)first_slot(at) * a.blocks + b] = 0;
   if (g == G - 1)
@@ -271,20 +285,16 @@ __global__ __launch_bounds__(kSortThreads, 8) void embed_sort_kernel(EmbedGradAr
     if (r >= 0 && s.count[r] <= kFew) s.keys[atomicAdd(&s.next[r], 1)] = ((uint32_t)r << 24) | (uint32_t)i;
   });
   __syncthreads();
-  // the i-th position of row r
-  auto put = [&](int r, int i, int pos) {
-    const int count = s.count[r], start = s.at[r], per = unit_len(count), units = (count + per - 1) / per;
-    Unit u = {-1, 0, 0, 0};
-    if (i % per == 0) u = {(r << a.log_g) + g, min(per, count - i), i / per | (units << 16), first_slot(start)};
-    a.order[start + i] = pos;
-    a.table[start + i] = u;
-  };
   for (int i = t; i < n_few; i += kSortThreads) {
     const uint32_t key = s.keys[i];
-    const int r = key >> 24, from = s.few[r], n = s.count[r];
+    const int r = key >> 24, from = s.few[r], n = s.count[r], start = s.at[r];
     int rank = 0;
     for (int j = from; j < from + n; ++j) rank += s.keys[j] < key;
-    put(r, rank, (int)(key & 0xffffffu));
+    const int units = n > kUnit ? 2 : 1, per = n > kUnit ? (n + 1) / 2 : n;  // (no more: kFew is two units)
+    Unit u = {-1, 0, 0, 0};
+    if (rank == 0 || rank == per) u = {(r << a.log_g) + g, rank == 0 ? per : n - per, (rank != 0) | (units << 16), first_slot(start)};
+    a.order[start + rank] = (int)(key & 0xffffffu);
+    a.table[start + rank] = u;
   }
   // rows of more: each wave's range of the tokens, first counted
   for (int h = 0; h < s.n_hot; ++h) {
@@ -294,13 +304,22 @@ __global__ __launch_bounds__(kSortThreads, 8) void embed_sort_kernel(EmbedGradAr
     __syncthreads();
     if (lane == 0) s.wave[wv] = n;
     __syncthreads();
-    int to = 0;
+    int to = 0;  // the row's positions so far
     for (int i = 0; i < wv; ++i) to += s.wave[i];
+    const int total = s.count[r], start = s.at[r], per = s.per[r], units = (total + per - 1) / per;
+    int unit = (to + per - 1) / per, begin = unit * per;  // the next unit and where it begins
     if (n > 0)
       each([&](int i, int own) {
         const u64 m = __ballot(own == r);
-        if (own == r) put(r, to + __popcll(m & ((1ull << lane) - 1)), i);
+        const int rank = to + __popcll(m & ((1ull << lane) - 1));
         to += __popcll(m);
+        Unit u = {-1, 0, 0, 0};
+        for (; begin < to; begin += per, ++unit)  // (of 64 positions three units at most begin at one)
+          if (rank == begin) u = {(r << a.log_g) + g, min(per, total - begin), unit | (units << 16), first_slot(start)};
+        if (own == r) {
+          a.order[start + rank] = i;
+          a.table[start + rank] = u;
+        }
       });
   }
 }
@@ -311,7 +330,7 @@ template <int FMT, int E>
 __global__ __launch_bounds__(256) void embed_sum_kernel(EmbedGradArgs a) {
   __shared__ Unit s_unit[kRun];
   __shared__ bool s_last;
-  static_assert(kRun < kUnit / 2);
+  static_assert(kRun < kUnit / 2 && kFew <= 2 * kUnit);
   const int t = threadIdx.x, lane = t & 63, b = blockIdx.y * blockDim.x + t;
   const bool some = E * b < a.C;
   const int col = (some ? piece_at<FMT, E>(b, a.C) : 0) * kLogitBytes<FMT>;
@@ -495,7 +514,8 @@ extern "C" int rwkv7_embed_backward(const void *grad, int32_t dtype, int64_t ldg
                            reinterpret_cast<Unit *>(ws + s.table), reinterpret_cast<int *>(ws + s.arrived),
                            reinterpret_cast<float *>(ws + s.part), shape.blocks};
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  const int groups = (1 << a.log_g) + kFillGroups;
+  const int64_t fill = ((int64_t)V * C * logit_bytes(dtype) + kFillBytes - 1) / kFillBytes;
+  const int groups = (1 << a.log_g) + (int)(fill < kFillGroups ? fill : kFillGroups);
   const bool held = N <= kHeld * kSortThreads;
   if (dtype == 1) {
     if (held) embed_sort_kernel<4, true><<<groups, kSortThreads, 0, st>>>(a);

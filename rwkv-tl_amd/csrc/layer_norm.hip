@@ -8,6 +8,12 @@
 // to 2048 16-bit or 1024 32-bit channels (no barrier), a workgroup beyond, and a wave
 // takes several rows with the weight in registers.
 //
+// Measured (kernel trace, us; a large copy moves 5.09 TB/s here). Forward: 16384 x 2048 bf16 30.5
+// (4.4 TB/s), 4096 x 2048 10.3, 7 x 2048 f16 4.0. Gradient and the joining of its
+// workgroups' sums: 16384 x 2048 bf16 35.0 + 4.8 (5.1 TB/s with both), f32 74 + 4.8 (5.1),
+// 4096 x 2048 bf16 13.8 + 4.0, 331 x 1001 f32 5.8 + 3.8, 1024 x 16384 bf16 26.8 + 6.4. Without
+// the next row on its way the first took 45.8; with workgroups of 8 waves 39 (256 of them) or 44.
+//
 // Statistics in 32 bits about a first mean, whose own rounding (what is left of the
 // differences' mean) is taken out again: a row whose mean is many times its deviation
 // keeps its differences. The gradient does the same about the mean it is given. Rows

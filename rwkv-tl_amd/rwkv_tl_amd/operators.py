@@ -213,7 +213,7 @@ def _plain(x: Tensor) -> bool:
     """Whether a call on ``x`` may go straight to the kernel: no tracing, no
     dispatch mode that wants to see the operator, no batch of tensors in one (that of
     ``torch.autograd.grad(..., is_grads_batched=True)``, which has no storage)."""
-    return type(x) is Tensor and x.is_cuda and not torch._C._len_torch_dispatch_stack() and torch._C._has_storage(x)
+    return type(x) in (Tensor, torch.nn.Parameter) and x.is_cuda and not torch._C._len_torch_dispatch_stack() and torch._C._has_storage(x)
 
 
 class _DistillLoss(torch.autograd.Function):

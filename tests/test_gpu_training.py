@@ -164,6 +164,18 @@ def test_embed_gradient_adds_whole_numbers_exactly(cuda):
     assert torch.equal(K.embed_backward(dy.to(cuda), t.to(cuda), V).cpu(), want)
 
 
+def test_embed_gradient_of_the_largest_table(cuda):
+    """2^20 rows: sixteen times the workgroups, rows far apart."""
+    g = _gen(18)
+    V, C = 2**20, 5
+    t = torch.cat([torch.randint(0, V, (3000,), generator=g), torch.tensor([0, V - 1, V, -1]), torch.full((200,), V - 4097)])
+    dy = torch.randint(-8, 9, (t.numel(), C), generator=g).float()
+    want = torch.zeros(V + 1, C).index_add_(0, torch.where((t >= 0) & (t < V), t, V), dy)[:V]
+    assert torch.equal(K.embed_backward(dy.to(cuda), t.to(cuda), V).cpu(), want)
+    w = torch.randn(V, C, generator=g)
+    assert torch.equal(K.embed(w.to(cuda), t[:3002].to(cuda)).cpu(), w[t[:3002]])
+
+
 @DTYPES
 def test_embed_gradient_layouts(cuda, dtype):
     g = _gen(5)
@@ -380,6 +392,10 @@ def test_autograd(cuda, dtype):
     gx, gw, gb = K.layer_norm_backward(dy, x.detach(), ln[0].detach(), m, r)
     assert torch.equal(y, y0)
     assert torch.equal(got[0], K.embed_backward(gx, t, 50, scale=1.5)) and torch.equal(got[1], gw) and torch.equal(got[2], gb)
+    # parameters, as modules have them
+    params = [torch.nn.Parameter(v.detach()) for v in (w, *ln)]
+    again = torch.autograd.grad(ops.layer_norm(ops.embed(params[0], t, 1.5), *params[1:], 1e-4), params, dy)
+    assert all(torch.equal(a, b) for a, b in zip(again, got))
     # one of the inputs alone, and none
     assert torch.equal(torch.autograd.grad(ops.layer_norm(x.detach(), ln[0].detach(), ln[1], 1e-4), ln[1], dy)[0], gb)
     with torch.no_grad():
@@ -394,6 +410,26 @@ def test_autograd(cuda, dtype):
         y = ops.layer_norm(x, *ln)
         (a,) = torch.autograd.grad((y.float() ** 2).sum(), x, create_graph=True)
         torch.autograd.grad(a.float().sum(), ln[0])
+
+
+def test_traced(cuda):
+    """Through torch.compile, whole and with its gradients: the operators, not their kernels, are traced."""
+    g = _gen(19)
+    w = torch.randn(60, 64, generator=g).to(cuda).requires_grad_()
+    ln = [torch.randn(64, generator=g).to(cuda).requires_grad_() for _ in range(2)]
+    t = _tokens(g, 30, 60).to(cuda)
+
+    def f(w, a, b, t):
+        x = ops.layer_norm(ops.embed(w, t, 1.5), a, b)
+        lp, H = ops.token_logprobs(x @ w.t(), t)
+        return lp.sum() + 0.1 * H.sum()
+
+    want = f(w, *ln, t)
+    grads = torch.autograd.grad(want, (w, *ln))
+    got = torch.compile(f, backend="aot_eager", fullgraph=True)(w, *ln, t)
+    assert torch.equal(got, want)
+    for a, b in zip(torch.autograd.grad(got, (w, *ln)), grads):
+        assert torch.allclose(a, b, rtol=1e-6, atol=1e-6)  # (the table's two gradients are added in either order)
 
 
 def test_gradients_match_differences(cuda):
