@@ -9,7 +9,7 @@
 // is or is +inf, -inf if all are.
 //
 // Selection. Each wave finds the r-th largest of its lanes' maxima, r = ceil(k /
-// waves), by ballots; the least of them over the waves is a floor that k logits
+// waves), one after the other or by ballots; the least of them over the waves is a floor that k logits
 // of the row reach, and few more: each wave has r lanes with a logit from
 // there up. (From r = 17 of four maxima a lane; where a mask leaves a wave without
 // r of them, by the waves that have 64.) The logits from the floor up are gathered
@@ -25,7 +25,9 @@
 // logit (maxima, exponentials, comparisons). 509 x 65536 bf16, k 64, 20, 3.3 TB/s: one
 // round of two rows a CU, each a chain of load, floor, sum, gather and ranking. One row
 // 9.1; 257 x 20011 f32 12.5 (back to back in a graph 9.9); 2000 x 65536 f32, k 64, back
-// to back 125, 4.2 TB/s.
+// to back 125, 4.2 TB/s. With scores: 2039 x 65536 bf16, k 5, 69, f16 66 (without them 56, the
+// sums alone in token_logprobs.hip 48); one row, k 20, 11.0. There, few candidates ranked
+// each against all, to save the bins' barriers, took 13.0.
 #include "logits_score.h"
 #include "rwkv7_kernels.h"
 
