@@ -124,7 +124,7 @@ __global__ __launch_bounds__(256) void embed_kernel(EmbedArgs g) {
 constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / kWave;
 constexpr int kSortRows = 256;   // rows of a workgroup at most (8 bits beside a position's 24)
 constexpr int kFew = 64;         // positions of a row that are ordered by counting
-constexpr int kUnit = 32;        // positions of a unit, while a row has no more units than
+constexpr int kUnit = 32;        // positions of a unit at most, while a row has no more units than
 constexpr int kMaxUnits = 128;
 constexpr int kRun = 8;          // positions of the list, and rows in flight, of a workgroup
 constexpr int kJoin = 4;         // units' sums in flight
@@ -159,11 +159,11 @@ struct EmbedGradArgs {
 RWKV7_DEV int first_slot(int start) { return (start + 15) / 16; }
 inline int64_t slots(int64_t N) { return (N + 15) / 16; }
 
-// Positions of a unit of a row of c > 0.
-RWKV7_DEV int unit_len(int c) {
-  const int units = min((c + kUnit - 1) / kUnit, kMaxUnits);
-  return (c + units - 1) / units;
-}
+// A row of c > kUnit positions has units_of(c) units of c / units, rounded down or up: 16 at
+// least, so that behind one that begins among a workgroup's eight no other does.
+RWKV7_DEV int units_of(int c) { return min((c + kUnit - 1) / kUnit, kMaxUnits); }
+RWKV7_DEV int unit_start(int c, int units, int unit) { return (int)((uint32_t)unit * (uint32_t)c / (uint32_t)units); }
+static_assert((uint64_t)kMaxUnits * kEmbedMaxN < 1ull << 32);
 
 struct SortLds {
   int count[kSortRows];
@@ -171,7 +171,6 @@ struct SortLds {
   int few[kSortRows];   // of a row of few: in `keys`
   int next[kSortRows];  // where its next one goes there
   int hot[kSortRows];   // rows of more than kFew
-  int per[kSortRows];   // and the length of their units
   int n_hot, less;
   int wave[kSortWaves];
   uint32_t keys[kSortRows * kFew];  // row and position
@@ -271,10 +270,7 @@ __global__ __launch_bounds__(kSortThreads, 8) void embed_sort_kernel(EmbedGradAr
   const int at = sort_scan(c, s.wave, all) + s.less;
   const int few = sort_scan(c <= kFew ? c : 0, s.wave, n_few);
   if (t < rows) s.at[t] = at, s.few[t] = s.next[t] = few;
-  if (c > kFew) {
-    s.hot[atomicAdd(&s.n_hot, 1)] = t;
-    s.per[t] = unit_len(c);
-  }
+  if (c > kFew) s.hot[atomicAdd(&s.n_hot, 1)] = t;
   if (c > kUnit)
     for (int b = 0; b < a.blocks; ++b) a.arrived[(int64_t)first_slot(at) * a.blocks + b] = 0;
   if (g == G - 1)
@@ -290,7 +286,7 @@ __global__ __launch_bounds__(kSortThreads, 8) void embed_sort_kernel(EmbedGradAr
     const int r = key >> 24, from = s.few[r], n = s.count[r], start = s.at[r];
     int rank = 0;
     for (int j = from; j < from + n; ++j) rank += s.keys[j] < key;
-    const int units = n > kUnit ? 2 : 1, per = n > kUnit ? (n + 1) / 2 : n;  // (no more: kFew is two units)
+    const int units = n > kUnit ? 2 : 1, per = n / units;  // (no more: kFew is two units)
     Unit u = {-1, 0, 0, 0};
     if (rank == 0 || rank == per) u = {(r << a.log_g) + g, rank == 0 ? per : n - per, (rank != 0) | (units << 16), first_slot(start)};
     a.order[start + rank] = (int)(key & 0xffffffu);
@@ -306,16 +302,22 @@ __global__ __launch_bounds__(kSortThreads, 8) void embed_sort_kernel(EmbedGradAr
     __syncthreads();
     int to = 0;  // the row's positions so far
     for (int i = 0; i < wv; ++i) to += s.wave[i];
-    const int total = s.count[r], start = s.at[r], per = s.per[r], units = (total + per - 1) / per;
-    int unit = (to + per - 1) / per, begin = unit * per;  // the next unit and where it begins
+    const int total = s.count[r], start = s.at[r], units = units_of(total);
+    int unit = (int)(((uint32_t)to * (uint32_t)units + total - 1) / (uint32_t)total);  // the next unit, and where
+    int begin = unit_start(total, units, unit);                                        // it begins and ends
+    int end = unit_start(total, units, unit + 1);
     if (n > 0)
       each([&](int i, int own) {
         const u64 m = __ballot(own == r);
         const int rank = to + __popcll(m & ((1ull << lane) - 1));
         to += __popcll(m);
         Unit u = {-1, 0, 0, 0};
-        for (; begin < to; begin += per, ++unit)  // (of 64 positions three units at most begin at one)
-          if (rank == begin) u = {(r << a.log_g) + g, min(per, total - begin), unit | (units << 16), first_slot(start)};
+        while (begin < to) {  // (of 64 positions four units at most begin at one; begin is total behind the last)
+          if (rank == begin) u = {(r << a.log_g) + g, end - begin, unit | (units << 16), first_slot(start)};
+          ++unit;
+          begin = end;
+          end = unit_start(total, units, unit + 1);
+        }
         if (own == r) {
           a.order[start + rank] = i;
           a.table[start + rank] = u;
@@ -330,7 +332,7 @@ template <int FMT, int E>
 __global__ __launch_bounds__(256) void embed_sum_kernel(EmbedGradArgs a) {
   __shared__ Unit s_unit[kRun];
   __shared__ bool s_last;
-  static_assert(kRun < kUnit / 2 && kFew <= 2 * kUnit);
+  static_assert(kRun <= kUnit / 2 && kFew <= 2 * kUnit);
   const int t = threadIdx.x, lane = t & 63, b = blockIdx.y * blockDim.x + t;
   const bool some = E * b < a.C;
   const int col = (some ? piece_at<FMT, E>(b, a.C) : 0) * kLogitBytes<FMT>;
@@ -370,7 +372,7 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(EmbedGradArgs a) {
   };
 
   // the first eight, where units begin; then what is left of the last one. (One of several
-  // of its row has 17 positions or more: it can only be the last.)
+  // of its row has 16 positions or more: it can only be the last.)
   load(pos, 0, n);
   int at = from;
 #pragma unroll

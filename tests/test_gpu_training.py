@@ -154,6 +154,22 @@ def test_embed_gradient_counts(cuda, counts, step):
     _embed_grad_close(K.embed_backward(dy.to(cuda), t.to(cuda), V), dy, t, V, 1.0)
 
 
+@pytest.mark.parametrize("counts", [[993, 2, 1], [4097, 3, 1], [5000, 1, 1, 1], "all"], ids=str)
+@pytest.mark.parametrize("step", [1, 256], ids=["neighbours", "one workgroup"])
+def test_embed_gradient_units_before_short_rows(cuda, counts, step):
+    """Rows of every length that is cut, each before one of a single position: a row's last part is never taken for a row."""
+    g = _gen(step, 20)
+    if counts == "all":
+        counts = [c for n in (range(33, 1100) if step == 1 else range(33, 200)) for c in (n, 1)]
+    ids = torch.arange(len(counts)) * step
+    t = torch.repeat_interleave(ids, torch.tensor(counts))
+    t = t[torch.randperm(t.numel(), generator=g)]
+    V = int(ids[-1]) + 1
+    dy = torch.randint(-8, 9, (t.numel(), 8), generator=g).float()
+    want = torch.zeros(V, 8).index_add_(0, t, dy)
+    assert torch.equal(K.embed_backward(dy.to(cuda), t.to(cuda), V).cpu(), want)
+
+
 def test_embed_gradient_adds_whole_numbers_exactly(cuda):
     """Sums of whole numbers have one value whatever their order: no row is left out or taken twice."""
     g = _gen(4)
