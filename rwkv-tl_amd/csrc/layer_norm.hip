@@ -8,11 +8,12 @@
 // to 2048 16-bit or 1024 32-bit channels (no barrier), a workgroup beyond, and a wave
 // takes several rows with the weight in registers.
 //
-// Measured (kernel trace, us; a large copy moves 5.09 TB/s here). Forward: 16384 x 2048 bf16 30.5
-// (4.4 TB/s), 4096 x 2048 10.3, 7 x 2048 f16 4.0. Gradient and the joining of its
-// workgroups' sums: 16384 x 2048 bf16 35.0 + 4.8 (5.1 TB/s with both), f32 74 + 4.8 (5.1),
-// 4096 x 2048 bf16 13.8 + 4.0, 331 x 1001 f32 5.8 + 3.8, 1024 x 16384 bf16 26.8 + 6.4. Without
+// Measured (kernel trace, us; a large copy moves 5.09 TB/s here). Forward: 16384 x 2048 bf16 26.5
+// (5.1 TB/s), 4096 x 2048 9.9, 7 x 2048 f16 3.5. Gradient and the joining of its
+// workgroups' sums: 16384 x 2048 bf16 34.6 + 4.6 (5.1 TB/s with both), f32 75 + 4.8 (5.1),
+// 4096 x 2048 bf16 13.0 + 3.9, 331 x 1001 f32 5.9 + 3.8, 1024 x 16384 bf16 25.2 + 6.1. Without
 // the next row on its way the first took 45.8; with workgroups of 8 waves 39 (256 of them) or 44.
+// The forward pass forced into the registers of 5, 6 or 8 waves a SIMD spills: 50, 70, 97.
 //
 // Statistics in 32 bits about a first mean, whose own rounding (what is left of the
 // differences' mean) is taken out again: a row whose mean is many times its deviation
@@ -85,7 +86,11 @@ constexpr int kNormThreads = WAVES == 1 ? 256 : WAVES * kWave;
 template <int WAVES>
 constexpr int kNormRows = kNormThreads<WAVES> / (WAVES * kWave);  // rows of a workgroup at a time
 
-template <int FMT, int WFMT, int WAVES, int NC>
+// EIGHTS: C is a multiple of 8, so that no thread has a part of an eight: its selects and
+// addresses cost registers (94 for 110 at 2048 16-bit channels, five waves a SIMD for
+// four) and a test before each load. Forward of 16384 x 2048 bf16 26.5 with, 34 without;
+// of 7 x 2048 f16 3.5 and 4.1, its gradient 4.5 and 5.5.
+template <int FMT, int WFMT, int WAVES, int NC, bool EIGHTS>
 __global__ __launch_bounds__(kNormThreads<WAVES>) void norm_kernel(NormArgs g) {
   __shared__ RowReduce<WAVES, 2> red;
   constexpr int T = WAVES * kWave;
@@ -101,7 +106,7 @@ __global__ __launch_bounds__(kNormThreads<WAVES>) void norm_kernel(NormArgs g) {
     char *dst = static_cast<char *>(g.y) + row * C * kLogitBytes<FMT>;
     Chunk<FMT> x[NC];
 #pragma unroll
-    for (int c = 0; c < NC; ++c) load_part(x[c], src, c * T + t, n[c]);
+    for (int c = 0; c < NC; ++c) load_part<FMT, EIGHTS>(x[c], src, c * T + t, n[c]);
     auto diff = [&](int c, float s, float m, float (&d)[8]) {  // x s - m, 0 where there is no x
       x[c].get(d);
 #pragma unroll
@@ -109,7 +114,7 @@ __global__ __launch_bounds__(kNormThreads<WAVES>) void norm_kernel(NormArgs g) {
       if (n[c] < 8) {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          if (e >= n[c]) d[e] = 0.f;
+          if (EIGHTS || e >= n[c]) d[e] = 0.f;
       }
     };
     float s, m, shift, var;
@@ -149,12 +154,12 @@ __global__ __launch_bounds__(kNormThreads<WAVES>) void norm_kernel(NormArgs g) {
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       float d[8], w[8], b[8];  // (from the CU's L1, which holds them: in registers they cost the row's own waves)
-      load_part_f<WFMT>(w, g.w, c * T + t, n[c]);
-      load_part_f<WFMT>(b, g.b, c * T + t, n[c]);
+      load_part_f<WFMT, EIGHTS>(w, g.w, c * T + t, n[c]);
+      load_part_f<WFMT, EIGHTS>(b, g.b, c * T + t, n[c]);
       diff(c, s, m, d);
 #pragma unroll
       for (int e = 0; e < 8; ++e) d[e] = fmaf((d[e] - shift) * rs, w[e], b[e]);
-      store_part<FMT>(dst, c * T + t, n[c], d);
+      store_part<FMT, EIGHTS>(dst, c * T + t, n[c], d);
     }
     if (t == 0 && g.mean) {
       g.mean[row] = (m + shift) * (1.f / s);
@@ -163,7 +168,7 @@ __global__ __launch_bounds__(kNormThreads<WAVES>) void norm_kernel(NormArgs g) {
   }
 }
 
-template <int FMT, int WFMT, int WAVES, int NC>
+template <int FMT, int WFMT, int WAVES, int NC, bool EIGHTS>
 __global__ __launch_bounds__(kNormThreads<WAVES>) void norm_grad_kernel(NormGradArgs g) {
   __shared__ RowReduce<WAVES, 3> red;
   constexpr int T = WAVES * kWave, kRows = kNormRows<WAVES>;
@@ -174,7 +179,7 @@ __global__ __launch_bounds__(kNormThreads<WAVES>) void norm_grad_kernel(NormGrad
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
     n[c] = part_len(c * T + t, C);
-    load_part_f<WFMT>(w[c], g.w, c * T + t, n[c]);
+    load_part_f<WFMT, EIGHTS>(w[c], g.w, c * T + t, n[c]);
 #pragma unroll
     for (int e = 0; e < 8; ++e) dw[c][e] = db[c][e] = 0.f;
   }
@@ -186,7 +191,10 @@ __global__ __launch_bounds__(kNormThreads<WAVES>) void norm_grad_kernel(NormGrad
     const char *xs = static_cast<const char *>(g.x) + row * g.ldx * kLogitBytes<FMT>;
     const char *ys = static_cast<const char *>(g.dy) + row * g.lddy * kLogitBytes<FMT>;
 #pragma unroll
-    for (int c = 0; c < NC; ++c) load_part(xn[c], xs, c * T + t, n[c]), load_part(yn[c], ys, c * T + t, n[c]);
+    for (int c = 0; c < NC; ++c) {
+      load_part<FMT, EIGHTS>(xn[c], xs, c * T + t, n[c]);
+      load_part<FMT, EIGHTS>(yn[c], ys, c * T + t, n[c]);
+    }
     rstd_n = g.rstd[row], mean_n = g.mean[row];
   };
   const int64_t step = (int64_t)gridDim.x * kRows;
@@ -213,7 +221,7 @@ __global__ __launch_bounds__(kNormThreads<WAVES>) void norm_grad_kernel(NormGrad
       if (n[c] < 8) {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          if (e >= n[c]) d[e] = 0.f;
+          if (EIGHTS || e >= n[c]) d[e] = 0.f;
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -239,7 +247,7 @@ __global__ __launch_bounds__(kNormThreads<WAVES>) void norm_grad_kernel(NormGrad
         db[c][e] += q[e];
         d[e] = rstd * fmaf(-xh, c2, fmaf(q[e], w[c][e], -c1));
       }
-      store_part<FMT>(dst, c * T + t, n[c], d);
+      store_part<FMT, EIGHTS>(dst, c * T + t, n[c], d);
     }
   }
   // the workgroup's sums: its waves' added by one wave a chunk
@@ -263,13 +271,13 @@ __global__ __launch_bounds__(kNormThreads<WAVES>) void norm_grad_kernel(NormGrad
 #pragma unroll
         for (int i = 1; i < kRows; ++i) v[e] += sum[k][i][8 * sub + e][t];
       }
-      store_part<1>(part + k * C, sub * T + t, len, v);
+      store_part<1, EIGHTS>(part + k * C, sub * T + t, len, v);
     }
   } else {
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      store_part<1>(part, c * T + t, n[c], dw[c]);
-      store_part<1>(part + C, c * T + t, n[c], db[c]);
+      store_part<1, EIGHTS>(part, c * T + t, n[c], dw[c]);
+      store_part<1, EIGHTS>(part + C, c * T + t, n[c], db[c]);
     }
   }
 }
@@ -303,11 +311,13 @@ inline int64_t grad_blocks(int dtype, int64_t N, int C) {
   return n < most ? n : most;
 }
 
-// f(WAVES, NC) for rows of C channels
+// f(WAVES, NC, EIGHTS) for rows of C channels
 template <int FMT, class F>
 void with_shape(int C, F f) {
   using std::integral_constant;
-#define RWKV7_SHAPE(W, N) f(integral_constant<int, W>(), integral_constant<int, N>())
+#define RWKV7_SHAPE(W, N)                                                                   \
+  C % 8 == 0 ? f(integral_constant<int, W>(), integral_constant<int, N>(), std::true_type()) \
+             : f(integral_constant<int, W>(), integral_constant<int, N>(), std::false_type())
   if (C <= 512) RWKV7_SHAPE(1, 1);
   else if (C <= 1024) RWKV7_SHAPE(1, 2);
   else if (C <= 2048) {
@@ -345,10 +355,10 @@ extern "C" int rwkv7_layer_norm_forward(const void *x, int32_t dtype, int64_t ld
   if (N < 1 || C < 1 || C > kNormMaxC || ldx < C) return RWKV7_ESHAPE;
   const NormArgs g = {x, weight, bias, ldx, y, mean, rstd, N, C, eps};
   with_types(dtype, weight_dtype, [&](auto f, auto wf) {
-    with_shape<decltype(f)::value>(C, [&](auto waves, auto nc) {
+    with_shape<decltype(f)::value>(C, [&](auto waves, auto nc, auto eights) {
       constexpr int W = decltype(waves)::value;
       const int64_t n = (N + kNormRows<W> - 1) / kNormRows<W>;
-      norm_kernel<decltype(f)::value, decltype(wf)::value, W, decltype(nc)::value>
+      norm_kernel<decltype(f)::value, decltype(wf)::value, W, decltype(nc)::value, decltype(eights)::value>
           <<<(int)(n < (1 << 20) ? n : 1 << 20), kNormThreads<W>, 0, static_cast<hipStream_t>(stream)>>>(g);
     });
   });
@@ -376,9 +386,10 @@ extern "C" int rwkv7_layer_norm_backward(const void *grad_y, int64_t ldg, const 
   const int G = (int)grad_blocks(dtype, N, C);
   const hipStream_t st = static_cast<hipStream_t>(stream);
   with_types(dtype, weight_dtype, [&](auto f, auto wf) {
-    with_shape<decltype(f)::value>(C, [&](auto waves, auto nc) {
+    with_shape<decltype(f)::value>(C, [&](auto waves, auto nc, auto eights) {
       constexpr int W = decltype(waves)::value;
-      norm_grad_kernel<decltype(f)::value, decltype(wf)::value, W, decltype(nc)::value><<<G, kNormThreads<W>, 0, st>>>(g);
+      norm_grad_kernel<decltype(f)::value, decltype(wf)::value, W, decltype(nc)::value, decltype(eights)::value>
+          <<<G, kNormThreads<W>, 0, st>>>(g);
     });
   });
   RWKV7_CHECK_LAUNCH();

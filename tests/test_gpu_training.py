@@ -283,6 +283,16 @@ def test_layer_norm(cuda, dtype, wdtype, N, C):
     _check_norm_grad(cuda, x, w, b, dy)
 
 
+@pytest.mark.parametrize("dtype,wdtype", [(H, H), (B16, F), (F, F)], ids=str)
+@pytest.mark.parametrize("C", [520, 1000, 1032, 2040, 2056, 4088, 4104, 8184, 8200, 16376])
+def test_layer_norm_whole_eights_of_some_threads(cuda, dtype, wdtype, C):
+    """Multiples of 8 channels that leave threads without any, in rows of any alignment."""
+    x, w, b, dy = _norm_inputs(_gen(C, 11), 5, C, dtype, wdtype)
+    x, dy = (torch.cat((v, v[:, :3]), 1)[:, 3:] for v in (x, dy))  # rows of C + 3, from the fourth channel
+    _check_norm(cuda, x, w, b)
+    _check_norm_grad(cuda, x, w, b, dy)
+
+
 @pytest.mark.parametrize("eps", [1e-12, 1e-5, 64e-5, 3.0, 1e6])
 def test_layer_norm_eps(cuda, eps):
     x, w, b, dy = _norm_inputs(_gen(7), 6, 300, F, F)
