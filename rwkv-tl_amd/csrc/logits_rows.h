@@ -116,7 +116,14 @@ struct Chunk {
   }
 };
 
-// The largest of some chunks' logits, NaN left out: halves in pairs.
+// From here on a NaN is left out of the wave's maxima and medians whichever it is. As a
+// wave starts (IEEE mode, bit 9 of MODE), one with a signalling NaN is NaN, and the next
+// maximum drops that, and with it every logit before: the largest was then not the
+// largest. (bfloat16 and float32; halves are quiet once converted.)
+RWKV7_DEV void leave_out_nans() { __builtin_amdgcn_s_setreg(1 | 9 << 6, 0); }
+
+// The largest of some chunks' logits, NaN left out (of signalling ones: see
+// leave_out_nans): halves in pairs.
 template <int FMT>
 struct RowMax {
   float m = -kInf;

@@ -167,6 +167,7 @@ __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : THREADS == 256 ? 7 : 8) voi
   __shared__ TopLds s;
   __shared__ std::conditional_t<SCORE, TopScoreLds<THREADS>, NoLds> sco;
   constexpr int kWaves = THREADS / kWave;
+  leave_out_nans();
   const int t = threadIdx.x, lane = t & 63, wv = t >> 6, V = g.V, k = g.k;
   const uint32_t n8 = (uint32_t)V / kRowChunk;
   const int64_t row = g.row0 + blockIdx.x;
@@ -342,10 +343,11 @@ __global__ __launch_bounds__(THREADS, FMT == 1 ? 4 : THREADS == 256 ? 7 : 8) voi
   }
 
   const float mm = wave_max(lane < kWaves ? s.m[lane] : -kInf);
-  // keys from `low` up, in bins of 2^shift, the highest first
+  // keys from `low` up, in bins of 2^shift, the highest first (and what is above mm, if it
+  // were not the largest, with those: no logit may lead outside the bins)
   const uint32_t low = fl, range = max(top_key(mm), 1u) - low;
   const int shift = max(0, 24 - __clz((int)(range | 1u)));
-  auto bin_of = [&](u64 c) { return kBins - 1 - (int)(((uint32_t)(c >> 32) - low) >> shift); };
+  auto bin_of = [&](u64 c) { return kBins - 1 - (int)min(((uint32_t)(c >> 32) - low) >> shift, (uint32_t)(kBins - 1)); };
 #pragma unroll 1
   for (int i = t; i < n; i += THREADS) {  // (from here on by their keys)
     const u64 c = s.cand[i], own = ((u64)top_key(__uint_as_float((uint32_t)(c >> 32))) << 32) | (uint32_t)c;
