@@ -167,6 +167,7 @@ template <int FMT, bool GREEDY>
 __global__ __launch_bounds__(kVerThreads) void verify_stats_kernel(VerifyArgs a) {
   __shared__ float s_m[kVerWaves];
   __shared__ double s_sum[kVerWaves];
+  leave_out_nans();
   const int t = threadIdx.x, lane = t & 63, wv = t >> 6, V = a.V, g = blockIdx.x;
   const int r = blockIdx.y, nt = a.B * (a.K + 1);
   const bool tgt = r < nt;
@@ -470,6 +471,7 @@ template <int FMT, int CH>
 __global__ __launch_bounds__(kVerThreads) void verify_draw_kernel(VerifyArgs a) {
   __shared__ DecideLds s;
   __shared__ bool s_last;
+  leave_out_nans();
   const int t = threadIdx.x, lane = t & 63, wv = t >> 6, V = a.V, g = blockIdx.x, b = blockIdx.y;
   decide<FMT>(a, b, s);
   const Decision d = s.d;
