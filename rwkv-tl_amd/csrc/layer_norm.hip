@@ -148,7 +148,8 @@ __global__ __launch_bounds__(kNormThreads<WAVES>) void norm_kernel(NormArgs g) {
     stats(1.f);
     if (!(var < 0x1p100f)) stats(kFarScale);  // (the same for every lane of the row)
     const double v = (double)var + g.eps * (double)s * (double)s;
-    double r = (double)__builtin_amdgcn_rsqf((float)v);
+    // (in 64 bits: of a row of one value that is taken times 2^-72, v is eps 2^-144 alone, which float32 has not)
+    double r = __builtin_amdgcn_rsq(v);
     r = r * fma(-0.5 * v * r, r, 1.5);
     const float rs = (float)r;
 #pragma unroll
