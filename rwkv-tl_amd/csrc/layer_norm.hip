@@ -17,8 +17,10 @@
 //
 // Statistics in 32 bits about a first mean, whose own rounding (what is left of the
 // differences' mean) is taken out again: a row whose mean is many times its deviation
-// keeps its differences. The gradient does the same about the mean it is given. Rows
-// whose squares pass 2^100 are taken times 2^-72.
+// keeps its differences. Where that rounding is more than about four times the deviation
+// (rows of one value far from 0, or nearly), the differences are formed once more about
+// the corrected mean. The gradient takes the rounding of the mean it is given out alike.
+// Rows whose squares pass 2^100 are taken times 2^-72.
 #include "row_parts.h"
 #include "rwkv7_kernels.h"
 
@@ -129,21 +131,30 @@ __global__ __launch_bounds__(kNormThreads<WAVES>) void norm_kernel(NormArgs g) {
       }
       row_reduce(red, turn, a);
       m = a[0] * inv;
-      // (one value: the compiler joins this product and some of the differences in an fma,
-      // and two m of a row of one value are a deviation to an eps of 1e-12)
-      asm volatile("" : "+v"(m));
-      a[0] = a[1] = 0.f;
+      // Where a fifteenth part or less of the mean square about m is deviation (m is rounded: a
+      // few steps of float32), once more about the corrected mean: else the variance is
+      // what rounding leaves of m's error, 0 too, and the error comes out as a deviation.
+#pragma unroll 1
+      for (int turns = 0; turns < 2; ++turns) {
+        // (one value: the compiler joins this product and some of the differences in an fma,
+        // and two m of a row of one value are a deviation to an eps of 1e-12)
+        asm volatile("" : "+v"(m));
+        a[0] = a[1] = 0.f;
 #pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        float d[8];
-        diff(c, s, m, d);
-        a[0] += ((d[0] + d[1]) + (d[2] + d[3])) + ((d[4] + d[5]) + (d[6] + d[7]));
+        for (int c = 0; c < NC; ++c) {
+          float d[8];
+          diff(c, s, m, d);
+          a[0] += ((d[0] + d[1]) + (d[2] + d[3])) + ((d[4] + d[5]) + (d[6] + d[7]));
 #pragma unroll
-        for (int e = 0; e < 8; ++e) a[1] = fmaf(d[e], d[e], a[1]);
+          for (int e = 0; e < 8; ++e) a[1] = fmaf(d[e], d[e], a[1]);
+        }
+        row_reduce(red, turn, a);
+        shift = a[0] * inv;
+        const float square = a[1] * inv;
+        var = fmaxf(fmaf(-shift, shift, square), 0.f) + 0.f * a[1];  // (NaN and inf stay)
+        if (turns > 0 || !(var < 0.0625f * square)) break;           // (the same for every lane of the row)
+        m += shift;
       }
-      row_reduce(red, turn, a);
-      shift = a[0] * inv;
-      var = fmaxf(fmaf(-shift, shift, a[1] * inv), 0.f) + 0.f * a[1];  // (NaN and inf stay)
     };
     stats(1.f);
     if (!(var < 0x1p100f)) stats(kFarScale);  // (the same for every lane of the row)

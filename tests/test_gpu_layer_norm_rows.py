@@ -63,3 +63,63 @@ def test_rows_of_one_value_whose_sum_passes_float32(cuda, dtype, C):
     _check_one_value(cuda, [3e38, -3e38, torch.finfo(dtype).max, torch.finfo(dtype).min], C, dtype)
     _check_one_value(cuda, [3e38, torch.finfo(dtype).min], C, dtype, 1e-30)
     _check_one_value(cuda, [3e38, torch.finfo(dtype).min], C, dtype, 1e6)
+
+def _exact_rows(units, size):
+    """Rows of size * (2^23 + units), size a power of two: float32 neighbours, with what float64 has of them exactly."""
+    x = ((2.0**23 + units.double()) * size).float()
+    assert torch.equal(x.double(), (2.0**23 + units.double()) * size)
+    near = units.double() - units[:, 2:3].double()
+    d = (near - near.mean(-1, keepdim=True)) * size
+    return x, d, (d * d).mean(-1)
+
+
+@pytest.mark.parametrize("dtype", [H, B16, F], ids=str)
+@pytest.mark.parametrize("C", [41, 110, 165, 427, 660, 1473, 1699, 1857, 2606, 7680, 8186, 12729, 13141, 14030, 15688, 16113])
+def test_rows_of_one_value(cuda, dtype, C):
+    """Also where the row's first mean is some roundings beside the value: those are no deviation."""
+    far = [float(torch.tensor(2.0**k * f)) for k in range(10, 76 if dtype is not H else 15) for f in (1.0, 1.171875, 1.7265625)]
+    near = [0.0, -0.0, 0.1, -1.0, 3.3, 1000.1]
+    if dtype is F:  # a few of those whose first mean was off
+        far += [27381108.0, 1298594200.0, 4706949700000.0, 2334959000000.0, 2.7584979e17, 1.3984066e19, 4.9142143e13, 2.5621844e16,
+                4.7746643e20, 1.1452193e16, 4.3576782e18, 2.4010826e17, 13705251000000.0, 1.590149e11, 8.714119e18]
+    _check_one_value(cuda, far + near, C, dtype)
+    _check_one_value(cuda, near, C, dtype, 1e-12)
+
+
+@pytest.mark.parametrize("C", [3, 100, 770, 1001, 2040, 5001, 9999, 16384])
+@pytest.mark.parametrize("size", [2.0**-20, 1.0, 2.0**30, 2.0**60])
+def test_rows_of_neighbouring_values(cuda, C, size):
+    """Deviations of a step of float32 and less: from one value that is a step beside the others to several steps.
+
+    The mean that the differences are formed about is the row's to half a step; or its rounding e is no more than four
+    times the deviation D, f = e / D: then too. A sum is within 54 U, say 56 U with the factor 1 / C, of its terms':
+    the mean of the differences within 56 U sqrt(1 + f^2) D, the variance within 3 times 56 U (1 + f^2) of itself and the
+    reciprocal deviation within 84 U (1 + f^2) and its own 2 U. A normalised value so within U (86 (1 + f^2) |xh| +
+    57 sqrt(1 + f^2)), U of the difference; the gradient's sums about the stored mean, half a step from the row's, alike."""
+    g = _gen(C, 2)
+    units = torch.stack([torch.zeros(C), torch.zeros(C), torch.zeros(C), torch.randint(0, 2, (C,), generator=g).float(),
+                         torch.randint(-1, 2, (C,), generator=g).float(), torch.randint(-40, 41, (C,), generator=g).float()])
+    units[0, 0], units[1, C // 2], units[2, C - 1], units[3, 0], units[3, 1] = 1, -1, 5, 0, 1
+    units[4, :2], units[5, :2] = torch.tensor([0.0, 1.0]), torch.tensor([-9.0, 9.0])
+    units += torch.tensor([0.0, 1234567.0, 3.0, 4000000.0, 77.0, 50.0])[:, None]
+    x, d, var = _exact_rows(units, size)
+    w, b, dy = torch.randn(C, generator=g), torch.randn(C, generator=g), torch.randn(6, C, generator=g)
+    y, mean, rstd = K.layer_norm_forward(x.to(cuda), w.to(cuda), b.to(cuda))
+    r = (var + 1e-5) ** -0.5
+    f2 = (1 + torch.maximum(0.2501 * size**2 / var, torch.tensor(16.0).double()))[:, None]
+    xh = d * r[:, None]
+    xerr = U * (86 * f2 * xh.abs() + 58 * f2.sqrt())
+    _within(rstd, r, (86 * U * f2[:, 0]) * r)
+    _within(mean, x[:, 0].double() - d[:, 0], 0.501 * size)
+    _within(y, xh * w.double() + b.double(), w.double().abs() * xerr + 2 * U * (xh * w.double()).abs() + 2 * U * b.double().abs())
+    gx, gw, gb = K.layer_norm_backward(dy.to(cuda), x.to(cuda), w.to(cuda), mean, rstd)
+    q = dy.double() * w.double()
+    c1, c2 = q.mean(-1, keepdim=True), (q * xh).mean(-1, keepdim=True)
+    want = r[:, None] * (q - c1 - xh * c2)
+    qm, a = q.abs().mean(-1, keepdim=True), xh.abs()
+    c2err = U * (q.abs() * 2 * (86 * f2 * a + 58 * f2.sqrt())).mean(-1, keepdim=True) + 57 * U * f2.sqrt() * qm
+    bound = 4 * U * q.abs() + 60 * U * qm + a * c2err + c2.abs() * xerr + 3 * U * (a * c2.abs())
+    _within(gx, want, r[:, None] * bound + (88 * U * f2) * want.abs())
+    ad = dy.double().abs()
+    _within(gw, (dy.double() * xh).sum(0), (ad * xerr).sum(0) + 14 * U * (ad * a).sum(0))
+    _within(gb, dy.double().sum(0), 14 * U * ad.sum(0))
