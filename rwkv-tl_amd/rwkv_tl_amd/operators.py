@@ -308,10 +308,11 @@ class _TokenLogprobs(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad_logprob, grad_entropy):
-        some = grad_logprob if grad_logprob is not None else grad_entropy
-        if some is None:
+        some = [g for g in (grad_logprob, grad_entropy) if g is not None]
+        if not some:
             return None, None, None
-        f = K.token_logprobs_backward if _direct(some) else torch.ops.rwkv_tl.token_logprobs_backward
+        # (one of the two may be a batch, the other not)
+        f = K.token_logprobs_backward if all(map(_direct, some)) else torch.ops.rwkv_tl.token_logprobs_backward
         return f(grad_logprob, grad_entropy, *ctx.saved_tensors, ctx.temperature), None, None
 
 
