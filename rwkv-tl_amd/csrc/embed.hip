@@ -13,7 +13,10 @@
 //   tokens have neighbouring ids). Each counts the tokens of its rows and those of the
 //   workgroups before it, which gives its range of the list of positions, and reads the
 //   tokens once more for the positions. Those of a row of up to 64 are put in order by
-//   counting the lesser ones; of a row with more, they are met in order.
+//   counting the lesser ones. Of rows with more, the second pass counts each wave's share
+//   and a third, if there is such a row, meets the positions in order: three passes
+//   however many there are (with two for each, 2^20 tokens of 8192 ids took 26 ms, 2^22 of
+//   65536 461; now 1.15 and 5.0).
 // The second launch goes through the sorted list, eight positions a workgroup and what
 // else belongs to the rows that begin there, so that eight rows are always in flight. A
 // row of more than 32 positions is cut into units; the one that arrives last adds up
@@ -23,7 +26,7 @@
 // TB/s here, a large fill 6.9-7.9). 8192 tokens x 1024 of 65536 bf16: sort and fill 20
 // (6.7 TB/s), sums 11; 16384 x 2048: 40 and 36, the second beside the first's lines on their
 // way from the caches; 509 x 768 of 20011 f32: 12 and 5. Sort alone 6.5 for one token, 13
-// for 16384; past those that its threads hold (16384) 2.2 per 1024. Lookup of 16384 x 2048
+// for 16384; past those that its threads hold (16384) it reads them again. Lookup of 16384 x 2048
 // bf16 28 (4.8 TB/s), of 16 2.8. Tried: a wave a row in the sort's workgroups, zeros and sums
 // included (the table's rows of 16384 x 2048: 179; the longest rows' chains bound it);
 // units of 64 positions (sums of 8192 x 1024 10.0 -> 11.9); the sums of a unit stored 32
@@ -169,11 +172,14 @@ struct SortLds {
   int count[kSortRows];
   int at[kSortRows];    // of a row's positions in the list
   int few[kSortRows];   // of a row of few: in `keys`
-  int next[kSortRows];  // where its next one goes there
+  int next[kSortRows];  // where its next one goes there; of a row of more its counters there
   int hot[kSortRows];   // rows of more than kFew
   int n_hot, less;
   int wave[kSortWaves];
-  uint32_t keys[kSortRows * kFew];  // row and position
+  // Row and position of those of rows of few; and behind them, a word left out, for each row of
+  // more a counter of each wave (16 words for the 64 that the row has not taken).
+  uint32_t keys[kSortRows * kFew];
+  static_assert(kSortWaves < kFew);
 };
 
 // Exclusive sum over the first kSortRows threads (four waves) of the workgroup.
@@ -270,7 +276,13 @@ __global__ __launch_bounds__(kSortThreads, 8) void embed_sort_kernel(EmbedGradAr
   const int at = sort_scan(c, s.wave, all) + s.less;
   const int few = sort_scan(c <= kFew ? c : 0, s.wave, n_few);
   if (t < rows) s.at[t] = at, s.few[t] = s.next[t] = few;
-  if (c > kFew) s.hot[atomicAdd(&s.n_hot, 1)] = t;
+  if (c > kFew) {
+    const int h = atomicAdd(&s.n_hot, 1);
+    s.hot[h] = t;
+    s.next[t] = n_few + 1 + h * kSortWaves;
+#pragma unroll
+    for (int w = 0; w < kSortWaves; ++w) s.keys[s.next[t] + w] = 0u;
+  }
   if (c > kUnit)
     for (int b = 0; b < a.blocks; ++b) a.arrived[(int64_t)first_slot(at) * a.blocks + b] = 0;
   if (g == G - 1)
@@ -278,7 +290,9 @@ __global__ __launch_bounds__(kSortThreads, 8) void embed_sort_kernel(EmbedGradAr
   __syncthreads();
 
   each([&](int i, int r) {
-    if (r >= 0 && s.count[r] <= kFew) s.keys[atomicAdd(&s.next[r], 1)] = ((uint32_t)r << 24) | (uint32_t)i;
+    if (r < 0) return;
+    if (s.count[r] <= kFew) s.keys[atomicAdd(&s.next[r], 1)] = ((uint32_t)r << 24) | (uint32_t)i;
+    else atomicAdd(&s.keys[s.next[r] + wv], 1u);
   });
   __syncthreads();
   for (int i = t; i < n_few; i += kSortThreads) {
@@ -292,37 +306,44 @@ __global__ __launch_bounds__(kSortThreads, 8) void embed_sort_kernel(EmbedGradAr
     a.order[start + rank] = (int)(key & 0xffffffu);
     a.table[start + rank] = u;
   }
-  // rows of more: each wave's range of the tokens, first counted
-  for (int h = 0; h < s.n_hot; ++h) {
-    const int r = s.hot[h];
-    int n = 0;
-    each([&](int, int own) { n += __popcll(__ballot(own == r)); });
-    __syncthreads();
-    if (lane == 0) s.wave[wv] = n;
-    __syncthreads();
-    int to = 0;  // the row's positions so far
-    for (int i = 0; i < wv; ++i) to += s.wave[i];
-    const int total = s.count[r], start = s.at[r], units = units_of(total);
-    int unit = (int)(((uint32_t)to * (uint32_t)units + total - 1) / (uint32_t)total);  // the next unit, and where
-    int begin = unit_start(total, units, unit);                                        // it begins and ends
-    int end = unit_start(total, units, unit + 1);
-    if (n > 0)
-      each([&](int i, int own) {
-        const u64 m = __ballot(own == r);
-        const int rank = to + __popcll(m & ((1ull << lane) - 1));
-        to += __popcll(m);
-        Unit u = {-1, 0, 0, 0};
-        while (begin < to) {  // (of 64 positions four units at most begin at one; begin is total behind the last)
-          if (rank == begin) u = {(r << a.log_g) + g, end - begin, unit | (units << 16), first_slot(start)};
-          ++unit;
-          begin = end;
-          end = unit_start(total, units, unit + 1);
-        }
-        if (own == r) {
-          a.order[start + rank] = i;
-          a.table[start + rank] = u;
-        }
-      });
+  if (s.n_hot == 0) return;
+  // rows of more, all in one pass: each wave's place in the list for each, and from there
+  // its range of the tokens in order
+  if (t < s.n_hot) {
+    const int r = s.hot[t];
+    uint32_t *const to = s.keys + s.next[r];
+    uint32_t place = (uint32_t)s.at[r];
+#pragma unroll
+    for (int w = 0; w < kSortWaves; ++w) {
+      const uint32_t n = to[w];
+      to[w] = place;
+      place += n;
+    }
+  }
+  __syncthreads();
+  each([&](int i, int r) {
+    const int of = r >= 0 ? s.next[r] : 0;  // (no row of few has come further than n_few)
+    u64 left = __ballot(of > n_few);
+    while (left) {  // a row of the 64 tokens' a turn
+      const int row = __builtin_amdgcn_readlane(of, __builtin_ctzll(left));
+      const u64 m = __ballot(of == row);
+      const uint32_t first = s.keys[row + wv];
+      if (of == row) {
+        const uint32_t place = first + __popcll(m & ((1ull << lane) - 1));
+        a.order[place] = i;
+        a.table[place].row = -1;
+      }
+      s.keys[row + wv] = first + __popcll(m);  // (by every lane, so that each reads what it wrote)
+      left &= ~m;
+    }
+  });
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();  // the units' entries come after the positions' own
+  for (int i = t; i < s.n_hot * kMaxUnits; i += kSortThreads) {
+    const int r = s.hot[i / kMaxUnits], unit = i % kMaxUnits, total = s.count[r], start = s.at[r], units = units_of(total);
+    if (unit >= units) continue;
+    const int begin = unit_start(total, units, unit), end = unit_start(total, units, unit + 1);
+    a.table[start + begin] = {(r << a.log_g) + g, end - begin, unit | (units << 16), first_slot(start)};
   }
 }
 
