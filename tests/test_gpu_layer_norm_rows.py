@@ -123,3 +123,32 @@ def test_rows_of_neighbouring_values(cuda, C, size):
     ad = dy.double().abs()
     _within(gw, (dy.double() * xh).sum(0), (ad * xerr).sum(0) + 14 * U * (ad * a).sum(0))
     _within(gb, dy.double().sum(0), 14 * U * ad.sum(0))
+
+def _rows_of_a_wave(dtype, N, C):
+    """How many rows a wave of the gradient takes: four waves a workgroup have a row each up to 2048 16-bit or 1024 32-bit
+    channels, a workgroup has one beyond; 512 workgroups, 256 above 8192 channels."""
+    at_once = 4 if C <= (1024 if dtype is F else 2048) else 1
+    groups = min(-(-N // at_once), 512 if C <= 8192 else 256)
+    return -(-N // (groups * at_once))
+
+
+@pytest.mark.parametrize("dtype,wdtype", [(H, H), (B16, F), (F, F)], ids=str)
+@pytest.mark.parametrize("N,C", [(9000, 72), (5000, 1030), (1500, 2056), (1200, 4096), (1100, 8192), (700, 8200), (600, 16384)])
+def test_weight_gradients_of_many_rows(cuda, dtype, wdtype, N, C):
+    """Rows added up in a wave's registers, then the waves of a workgroup, then the workgroups in 64 bits.
+
+    R rows of a wave and three more waves: R + 3 roundings, U of the terms each, and the errors of the normalised values,
+    U (86 |xh| + 58) (the first mean is off by 54 U of mean |x|, nothing beside the deviation here); then half a step."""
+    g = _gen(N, C, 3)
+    x = (torch.randn(N, C, generator=g) * (torch.randn(C, generator=g) * 0.6).exp() + torch.randn(C, generator=g)).to(dtype)
+    dy, w, b = torch.randn(N, C, generator=g).to(dtype), (1 + 0.2 * torch.randn(C, generator=g)).to(wdtype), torch.zeros(C, dtype=wdtype)
+    _, mean, rstd = K.layer_norm_forward(x.to(cuda), w.to(cuda), b.to(cuda))
+    _, gw, gb = K.layer_norm_backward(dy.to(cuda), x.to(cuda), w.to(cuda), mean, rstd)
+    d = x.double() - x.double().mean(-1, keepdim=True)
+    xh = d * ((d * d).mean(-1, keepdim=True) + 1e-5) ** -0.5
+    R, ad = _rows_of_a_wave(dtype, N, C), dy.double().abs()
+    assert R > 1
+    for got, want, terms, err in ((gw, (dy.double() * xh).sum(0), (ad * xh.abs()).sum(0), (ad * U * (86 * xh.abs() + 58)).sum(0)),
+                                  (gb, dy.double().sum(0), ad.sum(0), 0.0)):
+        half = torch.finfo(wdtype).eps / 2 * want.abs() + (2.0**-25 if wdtype is H else 0.0)
+        _within(got, want, (R + 3) * U * terms + err + half + U * want.abs())
