@@ -73,3 +73,35 @@ def test_the_time_follows_the_tokens(cuda):
 
     rare, often = best(65536), best(8192)
     assert often < 5 * rare, f"{often} ms for frequent rows, {rare} ms for rare ones"
+
+
+@pytest.mark.parametrize("ids", [1, 3, 60000])
+def test_the_most_tokens_of_a_call(cuda, ids):
+    """2^24 - 1 of them: all one, of three ids, and 280 of each id. (Sums of at most 2^24 whole numbers of at most 1.)"""
+    N = 2**24 - 1
+    g = torch.Generator(device=cuda).manual_seed(ids)
+    t = torch.randint(0, ids, (N,), generator=g, device=cuda) * (1 if ids > 3 else 256)
+    dy = torch.randint(-1, 2, (N, 2), generator=g, device=cuda).float()
+    V = int(t.max()) + 2
+    got = K.embed_backward(dy, t, V)
+    want = torch.stack([torch.bincount(t, dy[:, c].double(), minlength=V) for c in range(2)], 1)
+    assert torch.equal(got.double(), want)
+
+
+def test_a_table_past_2_to_the_32_bytes(cuda):
+    """Rows of the table, looked up and filled, past 32 bits of elements."""
+    V, C = 150001, 16500
+    w = torch.zeros(V, C, dtype=H, device=cuda)
+    ids = torch.tensor([0, 65535, 65536, 130149, 130151, V - 1, -1, V], device=cuda)
+    w[ids[:6], 7] = torch.arange(1.0, 7.0, device=cuda).half()
+    out = K.embed(w, ids)
+    assert out[:, 7].tolist() == [1, 2, 3, 4, 5, 6, 0, 0] and int((out != 0).sum()) == 6
+    del w
+    t = ids.repeat_interleave(torch.tensor([1, 70, 2, 40, 1, 200, 3, 3], device=cuda))
+    dy = torch.zeros(t.numel(), C, dtype=H, device=cuda)
+    dy[:, 0], dy[:, C - 1] = 1, 2
+    grad = K.embed_backward(dy, t, V)
+    assert grad[ids[:6], 0].tolist() == [1, 70, 2, 40, 1, 200] and grad[ids[:6], C - 1].tolist() == [2, 140, 4, 80, 2, 400]
+    rest = grad.view(torch.int16)
+    rest[ids[:6, None], torch.tensor([0, C - 1], device=cuda)] = 0
+    assert all(not bool(part.any()) for part in rest.split(20000))
