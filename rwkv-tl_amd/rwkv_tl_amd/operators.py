@@ -316,8 +316,9 @@ class _TokenLogprobs(torch.autograd.Function):
         return f(grad_logprob, grad_entropy, *ctx.saved_tensors, ctx.temperature), None, None
 
 
-def _once(name: str):
-    """The Autograd kernel of a gradient: it has none of its own."""
+def _no_gradient(name: str, why: str):
+    """The Autograd kernel of an operator without a gradient: a backward pass that reaches it raises
+    (torch's own, for want of one, warns and leaves the gradients out)."""
 
     class Gradient(torch.autograd.Function):
         @staticmethod
@@ -327,7 +328,7 @@ def _once(name: str):
 
         @staticmethod
         def backward(ctx, *_):
-            raise NotImplementedError(f"{name.removesuffix('_backward')} has no second derivative")
+            raise NotImplementedError(why)
 
     return Gradient.apply
 
@@ -367,7 +368,12 @@ def register() -> None:
         ("token_logprobs", lambda logits, tokens, temperature=1.0: _TokenLogprobs.apply(logits, tokens, temperature)),
     ):
         torch.library.impl(f"{NAMESPACE}::{name}", "Autograd")(autograd)
-        torch.library.impl(f"{NAMESPACE}::{name}_backward", "Autograd")(_once(f"{name}_backward"))
+        torch.library.impl(f"{NAMESPACE}::{name}_backward", "Autograd")(
+            _no_gradient(f"{name}_backward", f"{name} has no second derivative")
+        )
+    torch.library.impl(f"{NAMESPACE}::layer_norm_forward", "Autograd")(
+        _no_gradient("layer_norm_forward", "layer_norm_forward has no gradient: layer_norm is the differentiable form")
+    )
     _registered = True
 
 
