@@ -25,9 +25,12 @@
 // Measured (kernel trace, us; tokens with frequencies of 1 / rank; a large copy moves 5.09
 // TB/s here, a large fill 6.9-7.9). 8192 tokens x 1024 of 65536 bf16: sort and fill 20
 // (6.7 TB/s), sums 11; 16384 x 2048: 40 and 36, the second beside the first's lines on their
-// way from the caches; 509 x 768 of 20011 f32: 12 and 5. Sort alone 6.5 for one token, 13
-// for 16384; past those that its threads hold (16384) it reads them again. Lookup of 16384 x 2048
-// bf16 28 (4.8 TB/s), of 16 2.8. Tried: a wave a row in the sort's workgroups, zeros and sums
+// way from the caches; 509 x 768 of 20011 f32: 12 and 5. Sort alone 6.7 for one token, 14
+// for 16384; past those that its threads hold (16384) it reads them again, about 1 for every
+// 1024 (65536: 57, 2^20: 1080, and 685 with no row of more than 64). 16384 x 2048 of one
+// id: 45-51 and 120 (128 units of 128 positions, on half of the CUs), half of them one id 47
+// and 54. Lookup of 16384 x 2048 bf16 28 (4.8 TB/s), of the same ids again 17, f32 36; of 16
+// 2.8. Tried: a wave a row in the sort's workgroups, zeros and sums
 // included (the table's rows of 16384 x 2048: 179; the longest rows' chains bound it);
 // units of 64 positions (sums of 8192 x 1024 10.0 -> 11.9); the sums of a unit stored 32
 // bytes a thread (27 instead of 10: each 4-byte store past the caches is a trip of its own).

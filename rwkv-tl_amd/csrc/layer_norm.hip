@@ -5,13 +5,14 @@
 //   dw = sum over rows of dy xh, db = sum over rows of dy
 //
 // Bytes bound both passes (x, y; x, dy, dx): a row stays in registers, one wave a row up
-// to 2048 16-bit or 1024 32-bit channels (no barrier), a workgroup beyond, and a wave
-// takes several rows with the weight in registers.
+// to 2048 16-bit or 1024 32-bit channels (no barrier), a workgroup beyond. The forward pass
+// has a wave (or workgroup) for each row, weight and bias from the CU's L1; a wave of the
+// gradient takes several rows with the weight in registers.
 //
 // Measured (kernel trace, us; a large copy moves 5.09 TB/s here). Forward: 16384 x 2048 bf16 26.5
-// (5.1 TB/s), 4096 x 2048 9.9, 7 x 2048 f16 3.5. Gradient and the joining of its
+// (5.1 TB/s), f32 40, 4096 x 2048 9.9, f32 15, 1024 x 16384 19, f32 31, 7 x 2048 f16 3.5. Gradient and the joining of its
 // workgroups' sums: 16384 x 2048 bf16 34.6 + 4.6 (5.1 TB/s with both), f32 75 + 4.8 (5.1),
-// 4096 x 2048 bf16 13.0 + 3.9, 331 x 1001 f32 5.9 + 3.8, 1024 x 16384 bf16 25.2 + 6.1. Without
+// 4096 x 2048 bf16 13.0 + 3.9, f32 20 + 3.9, 331 x 1001 f32 5.9 + 3.8, 1024 x 16384 bf16 25.2 + 6.1, f32 48 + 6.4. Without
 // the next row on its way the first took 45.8; with workgroups of 8 waves 39 (256 of them) or 44.
 // The forward pass forced into the registers of 5, 6 or 8 waves a SIMD spills: 50, 70, 97.
 //
@@ -89,7 +90,7 @@ template <int WAVES>
 constexpr int kNormRows = kNormThreads<WAVES> / (WAVES * kWave);  // rows of a workgroup at a time
 
 // EIGHTS: C is a multiple of 8, so that no thread has a part of an eight: its selects and
-// addresses cost registers (94 for 110 at 2048 16-bit channels, five waves a SIMD for
+// addresses cost registers (94 for 108 at 2048 16-bit channels, five waves a SIMD for
 // four) and a test before each load. Forward of 16384 x 2048 bf16 26.5 with, 34 without;
 // of 7 x 2048 f16 3.5 and 4.1, its gradient 4.5 and 5.5.
 template <int FMT, int WFMT, int WAVES, int NC, bool EIGHTS>
@@ -131,9 +132,9 @@ __global__ __launch_bounds__(kNormThreads<WAVES>) void norm_kernel(NormArgs g) {
       }
       row_reduce(red, turn, a);
       m = a[0] * inv;
-      // Where a fifteenth part or less of the mean square about m is deviation (m is rounded: a
-      // few steps of float32), once more about the corrected mean: else the variance is
-      // what rounding leaves of m's error, 0 too, and the error comes out as a deviation.
+      // Where a sixteenth or less of the mean square about m is deviation (m is rounded: a few
+      // steps of float32), once more about the corrected mean: else the variance is what
+      // rounding leaves of m's error, 0 too, and the error comes out as a deviation.
 #pragma unroll 1
       for (int turns = 0; turns < 2; ++turns) {
         // (one value: the compiler joins this product and some of the differences in an fma,
@@ -195,7 +196,8 @@ __global__ __launch_bounds__(kNormThreads<WAVES>) void norm_grad_kernel(NormGrad
 #pragma unroll
     for (int e = 0; e < 8; ++e) dw[c][e] = db[c][e] = 0.f;
   }
-  // the next row is on its way while one is worked on (but of 8 and 16 waves, which have no registers for it)
+  // the next row is on its way while one is worked on (but of 8 and 16 waves, which have no registers for it: 16 waves
+  // have 128 each, and without it spill 19 of them in float32, and 2 in 16 bits where C is no multiple of 8)
   constexpr bool kAhead = WAVES <= 4;
   Chunk<FMT> xn[NC], yn[NC];
   float rstd_n, mean_n;

@@ -14,8 +14,9 @@
 // stored over the row's after a barrier.
 //
 // Bytes bound it. Measured (kernel trace, us; a large copy moves 5.09 TB/s here): 2039 x 65536 bf16 48
-// (5.6 TB/s), 2000 x 65536 f32 108 (4.9, one workgroup on a CU); with the gradient 4096 x 65536
-// bf16 201 and f16 199 (5.4), 2000 x 65536 f32 231 (4.5), with that of the entropy 2048 x 65536 bf16
+// (5.6 TB/s), with a masked end 96 and with all but 300 masked 105 (-inf: the sums once more, from
+// memory), 2000 x 65536 f32 108 (4.9, one workgroup on a CU); with the gradient 4096 x 65536
+// bf16 201 and f16 199 (5.4), masked alike 303 and 320, 2000 x 65536 f32 231 (4.5), with that of the entropy 2048 x 65536 bf16
 // 102; one row 6.6 and 10.8, 331 x 20011 f32 9.1 and 14.3, chains of load, maximum, sum and
 // join. With the logarithms and the token's own gradient before the row's, where a wave
 // that holds the row has no registers for them, 4096 x 65536 bf16 took 228-245.

@@ -26,7 +26,10 @@
 // round of two rows a CU, each a chain of load, floor, sum, gather and ranking. One row
 // 9.1; 257 x 20011 f32 12.5 (back to back in a graph 9.9); 2000 x 65536 f32, k 64, back
 // to back 125, 4.2 TB/s. With scores: 2039 x 65536 bf16, k 5, 69, f16 66 (without them 56, the
-// sums alone in token_logprobs.hip 48); one row, k 20, 11.0. There, few candidates ranked
+// sums alone in token_logprobs.hip 48), k 20 67, k 50 71, k 256 77, 2000 x 65536 f32 140 (k 200 163); one
+// row, k 20, 11.0. A masked end (-inf) costs the sums a second pass, 117 for 64 at k 5 (without
+// scores 55 and 55); where masks leave the waves fewer logits than the floor needs, all
+// but 300, the passes that count keys take 740-780. There, few candidates ranked
 // each against all, to save the bins' barriers, took 13.0.
 #include "logits_score.h"
 #include "rwkv7_kernels.h"

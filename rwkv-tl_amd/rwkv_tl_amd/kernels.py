@@ -381,7 +381,8 @@ def fused_lerp1_copy(x, prev, w, x_copy):
 
 
 def layer_norm(x: Tensor, weight: Tensor, bias: Tensor) -> Tensor:
-    """LayerNorm over the last dim, eps 1e-5; returns f32 (``weight.py:14-15``)."""
+    """LayerNorm over the last dim, eps 1e-5; returns f32 (``weight.py:14-15``): inference's, without a gradient.
+    Training's, in x's type, are ``layer_norm_forward`` and ``torch.ops.rwkv_tl.layer_norm``."""
     _dev(x)
     C = x.shape[-1]
     _need(x.dtype in (torch.float16, torch.bfloat16, torch.float32), "x must be f16, bf16 or f32")

@@ -4,7 +4,8 @@ counterpart in the reference, whose training is a plan, ``TODO.md:46-54``).
 * ``embed`` / ``embed_backward``: rows of an embedding table times a factor, and the
   table's gradient.
 * ``layer_norm_forward`` / ``layer_norm_backward``: LayerNorm (``weight.py:14-15``) in
-  its input's type that keeps its statistics, and its gradients.
+  its input's type that keeps its statistics, and its gradients. (``kernels.layer_norm``
+  is inference's: float32 out, eps 1e-5, no gradient.)
 
 ``torch.ops.rwkv_tl.embed`` and ``torch.ops.rwkv_tl.layer_norm`` are the differentiable
 forms. (The output end is ``token_logprobs`` in ``logits.py``.) Tensors are float16,
